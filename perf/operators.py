@@ -237,11 +237,13 @@ def _prepare_verify(case, seed):
 
 
 def _caches(case, blocks, seed):
-    """K and V caches of every layer, views of one allocation: [layers, 2, blocks, page, kv_heads, 128]."""
+    """K and V caches of every layer, views of one allocation [layers, 2, blocks, page, kv_heads, 128], and the handle
+    that a program makes of its caches once."""
     all_layers = torch.empty(case["layers"], 2, blocks, PAGE, case["kv_heads"], DIM, dtype=torch.bfloat16,
                              device="cuda")
     all_layers.normal_(generator=_generator(seed))
-    return all_layers, [x[0] for x in all_layers], [x[1] for x in all_layers]
+    handle = _package().CacheLayers([x[0] for x in all_layers], [x[1] for x in all_layers]) if own else None
+    return all_layers, handle
 
 
 def _prepare_compact(case, seed):
@@ -260,8 +262,8 @@ def _prepare_compact(case, seed):
     for i in range(b):
         path[i, 0] = 0
         path[i, 1:1 + accepted[i]] = np.sort(rng.permutation(np.arange(1, nodes[i]))[:accepted[i]])
-    whole, ks, vs = _caches(case, blocks, seed)
-    return dict(op="compact", case=case, whole=whole, ks=ks, vs=vs, table=torch.from_numpy(table).cuda(),
+    whole, layers = _caches(case, blocks, seed)
+    return dict(op="compact", case=case, whole=whole, layers=layers, table=torch.from_numpy(table).cuda(),
                 cu_q=_cu(nodes), lens=torch.from_numpy((ctx + nodes).astype(np.int32)).cuda(),
                 path=torch.from_numpy(path).cuda(), counts=torch.from_numpy((accepted + 1).astype(np.int32)).cuda(),
                 blocks=blocks, new_lens=torch.zeros(b, dtype=torch.int32, device="cuda"))
@@ -271,9 +273,9 @@ def _prepare_copy(case, seed):
     rng, pairs = np.random.RandomState(seed % (2 ** 31)), case["pairs"]
     blocks = 2 * pairs + 3
     order = rng.permutation(blocks)
-    whole, ks, vs = _caches(case, blocks, seed)
+    whole, layers = _caches(case, blocks, seed)
     rows = None if case["whole"] else torch.from_numpy(_copy_rows(case).astype(np.int32)).cuda()
-    return dict(op="copy", case=case, whole=whole, ks=ks, vs=vs, blocks=blocks, rows=rows,
+    return dict(op="copy", case=case, whole=whole, layers=layers, blocks=blocks, rows=rows,
                 src=torch.from_numpy(order[:pairs].astype(np.int32)).cuda(),
                 dst=torch.from_numpy(order[pairs:2 * pairs].astype(np.int32)).cuda())
 
@@ -311,13 +313,13 @@ def _own_verify(st):
 
 
 def _own_compact(st):
-    _package().cache_compact_paths(st["ks"], st["vs"], st["cu_q"], st["lens"], st["table"], st["path"],
-                                   st["counts"], st["new_lens"])
+    _package().cache_compact_paths(st["layers"], st["cu_q"], st["lens"], st["table"], st["path"], st["counts"],
+                                   st["new_lens"])
     return st["whole"], st["new_lens"]
 
 
 def _own_copy(st):
-    _package().cache_copy_pages(st["ks"], st["vs"], st["src"], st["dst"], st["rows"])
+    _package().cache_copy_pages(st["layers"], st["src"], st["dst"], st["rows"])
     return st["whole"]
 
 
