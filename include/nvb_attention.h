@@ -160,6 +160,68 @@ int nvb_peer_buffer_open(const void* ipc_handle, void** ptr);
 int nvb_peer_buffer_close(void* ptr);
 int nvb_peer_buffer_free(void* ptr);
 
+/* Attention of drafted trees over the paged cache, for steps that verify
+ * several drafted tokens of a sequence at once (no counterpart in the
+ * reference, which decodes one token per sequence and step).
+ *
+ * Sequence b's queries [cu_q[b], cu_q[b + 1]) are the n nodes of its tree in
+ * any order; the last n of its kv_lens[b] keys are the same nodes' keys, in
+ * the same order, and the keys before them (ctx = kv_lens[b] - n) are visible
+ * to every node. tree_mask [total_q, mask_words] says which nodes a node sees:
+ * bit (t & 63) of word t / 64 of row i is set where node i attends to node t
+ * (itself and its ancestors; nvbh_tree_mask builds it from parents). Where a
+ * chain's mask is given this is causal attention.
+ *
+ *  - max_q bounds every sequence's nodes (at most 64 * mask_words, mask_words
+ *    in [1, 16]), max_k its kv_lens. Sequences without nodes, and rows of q
+ *    and out at and behind cu_q[batch], are left alone.
+ *  - lse (may be null) is [total_q, q_heads]. A node that sees no key has
+ *    output 0 and lse -inf; so has a sequence with kv_lens < n or longer than
+ *    its table.
+ *  - num_splits > 1 cuts every sequence's keys into that many ranges with
+ *    partials in lse_accum [num_splits, total_q, q_heads] and out_accum
+ *    [num_splits, total_q, q_heads, 128] (FP32); calls that may overlap need
+ *    their own. nvb_tree_num_splits gives the count for a GPU of num_sms SMs.
+ *  - a key that a node does not see has no part in its result, whatever
+ *    values the cache holds there (infinities and NaN too).
+ *  - page ids outside [0, num_blocks) mask their tokens.
+ * Other limits as nvb_paged_fwd_ex; batch at most 65535. */
+int nvb_paged_tree_fwd(void* stream, const void* q, const void* k, const void* v, void* out,
+                       const int* cu_q, const int* kv_lens, const int* block_table,
+                       const uint64_t* tree_mask, int mask_words, int batch, int total_q, int max_q,
+                       int max_k, int q_heads, int kv_heads, int block_size, int table_stride,
+                       int num_splits, float* lse, float* lse_accum, float* out_accum,
+                       int num_blocks);
+int nvb_tree_num_splits(int batch, int max_q, int q_heads, int kv_heads, int max_k, int num_sms);
+
+/* Copies within the cache over all layers at once (no counterpart in the
+ * reference). k_layers and v_layers are HOST arrays of `layers` device
+ * pointers, each a cache [num_blocks, block_size, kv_heads, head_dim] BF16;
+ * they are read during the call. At most 1024 layers, 64 in one launch.
+ *
+ * nvb_cache_copy_pages copies page src_pages[i] to page dst_pages[i] for each
+ * of `pairs` pairs (device arrays), the first rows[i] tokens of it where rows
+ * is not null: the pages that forked sequences must not share
+ * (nvbh_pool_fork). Pairs with a page outside [0, num_blocks) are skipped.
+ * Pairs run in any order: no page may be the target of two pairs, nor the
+ * target of one and the source of another.
+ *
+ * nvb_cache_compact_paths keeps the accepted path of a verified tree: with
+ * ctx = kv_lens[b] - n as in nvb_paged_tree_fwd, the K and V rows at position
+ * ctx + path[b, d] move to position ctx + d for d in [1, counts[b]), and
+ * new_kv_lens[b] = ctx + counts[b] (path and counts as nvbe_layer_verify
+ * writes them: strictly increasing from path[b, 0] = 0; path_stride is the
+ * row length of path). The pages written must not be shared with another
+ * sequence of the batch. */
+int nvb_cache_copy_pages(void* stream, void* const* k_layers, void* const* v_layers, int layers,
+                         const int* src_pages, const int* dst_pages, const int* rows, int pairs,
+                         int kv_heads, int head_dim, int block_size, int num_blocks);
+int nvb_cache_compact_paths(void* stream, void* const* k_layers, void* const* v_layers, int layers,
+                            const int* cu_q, const int* kv_lens, const int* block_table,
+                            const int* path, const int* counts, int* new_kv_lens, int batch,
+                            int path_stride, int kv_heads, int head_dim, int block_size,
+                            int table_stride, int num_blocks);
+
 /* Thread-local message for the last failing call on this thread
  * (kernels/flash_native/flash_native.cu:15, kernels/kernels.cu:28). */
 const char* nvb_last_error(void);

@@ -268,6 +268,51 @@ int nvbe_sample_partitions(int vocab);
 int nvbe_layer_sample(void* stream, const void* logits, const float* temperatures, const uint64_t* seeds, int* out,
                       float* partial_scores, int* partial_indices, int rows, int vocab);
 
+/* Verification of drafted tokens against the target's probabilities, beside
+ * nvbe_layer_sample (no counterpart in the reference, which decodes one token
+ * per step). Rows [cu_q[b], cu_q[b + 1]) are the nodes of sequence b's tree,
+ * parents before children: its first row is the last committed token (the
+ * root), tokens[r] is node r's token and parents[r] its parent's place in the
+ * sequence (smaller than its own; nodes without a valid one are never
+ * reached). A chain has parents -1, 0, 1, ...
+ *
+ *   logits, draft_logits  [rows, vocab] BF16: the target's logits after each
+ *     node, and the draft's that the node's children were drawn from (only
+ *     rows of nodes with children are read). draft_logits may be null: drafts
+ *     without probabilities, as looked up in the prompt.
+ *   temperatures [batch], uniforms [rows] in [0, 1), seeds [rows]
+ *
+ * From the root on, the current node's children are tested in row order. With
+ * P = softmax(logits / T) and Q = softmax(draft_logits / T), a child with
+ * token t is accepted where its uniform is below a = min(1, P(t) / Q(t)) and
+ * becomes the current node. A rejected one leaves P = max(P - Q, 0) / sum
+ * (unchanged where that sum is 0) and Q without t, renormalised, to its next
+ * sibling (drafts of one node are drawn without replacement). Without
+ * draft_logits Q is 1 at t. Once a node's children are all rejected the next
+ * token is drawn from the P that is left, with the sampler's Gumbel stream
+ * of the node's seed; where nothing was rejected it is the token that
+ * nvbe_layer_sample draws. T = 0: a child is accepted where its token is the
+ * argmax of logits (the lowest index of equal ones), which is the next token
+ * otherwise. NaN logits have probability 0, tokens outside [0, vocab) too.
+ *
+ *   path [batch, max_q]: nodes of the accepted path, the root (0) first
+ *   counts [batch]: nodes on the path = tokens emitted
+ *   out_tokens [batch, max_q]: the path's tokens behind the root, then the
+ *     next token
+ *   accept_prob [rows]: a of each child, tested as if its parent had been
+ *     reached; 0 for the root and for children behind an accepted sibling
+ *
+ * Entries behind counts are -1; a sequence without rows has counts 0. Rows at
+ * and behind cu_q[batch] are neither read nor written. max_q bounds the nodes
+ * of a sequence (at most 1024). `workspace`: 16-byte aligned,
+ * nvbe_verify_workspace_bytes(rows) bytes, written before it is read; calls
+ * that may overlap need one each. Allocates nothing and can be captured. */
+size_t nvbe_verify_workspace_bytes(int rows);
+int nvbe_layer_verify(void* stream, const void* logits, const void* draft_logits, const int* tokens,
+                      const int* parents, const float* uniforms, const uint64_t* seeds, const float* temperatures,
+                      const int* cu_q, int* out_tokens, int* path, int* counts, float* accept_prob, int rows,
+                      int batch, int max_q, int vocab, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -122,6 +122,31 @@ void nvbh_pool_clear_cache(NvbhBlockPool* pool);
  * hash collision (src/runtime/tests.rs:213-234 does the same in Rust). */
 void nvbh_pool_force_hash_entry(NvbhBlockPool* pool, const uint32_t* prefix, size_t n, int block);
 
+/* Forks a sequence of `tokens` tokens held in `blocks` (no counterpart in the
+ * reference): child (num_blocks entries) shares the full pages, each retained
+ * once more, and gets a new page for a partly filled last one, whose tokens
+ * the caller copies on the device (nvb_cache_copy_pages: *copy_src to
+ * *copy_dst, *copy_rows tokens; *copy_rows = 0 where there is none to copy).
+ * *child_blocks = pages of the child. On failure (an unreferenced page, no
+ * free one, too few pages for the tokens) the pool is unchanged. */
+int nvbh_pool_fork(NvbhBlockPool* pool, const int32_t* blocks, size_t num_blocks, size_t tokens,
+                   size_t block_size, int32_t* child, size_t* child_blocks, int32_t* copy_src,
+                   int32_t* copy_dst, size_t* copy_rows);
+/* Releases the pages that a sequence cut to `tokens` tokens does not need any
+ * more (drafts that were rejected), the last first; *num_blocks becomes the
+ * number it keeps and the released entries of blocks -1. */
+int nvbh_pool_truncate(NvbhBlockPool* pool, int32_t* blocks, size_t* num_blocks, size_t tokens,
+                       size_t block_size);
+
+/* Ancestor masks of drafted trees for nvb_paged_tree_fwd: rows [cu_q[s],
+ * cu_q[s + 1]) are the nodes of tree s, parents[r] the place in it of r's
+ * parent (smaller than its own; -1 for a node without one, which the first
+ * has to be). mask is [rows, words] (row r sees itself and its ancestors);
+ * depth (may be null) [rows] counts the ancestors, so that a node's position
+ * is its context plus its depth. */
+int nvbh_tree_mask(const int32_t* parents, const int32_t* cu_q, size_t sequences, size_t words,
+                   uint64_t* mask, int32_t* depth);
+
 /* One sequence's slice of a forward pass (the reference's Segment plus the
  * sequence fields make_batch reads, src/runtime.rs:355-358, 728-777). */
 typedef struct NvbhSegment {

@@ -49,6 +49,10 @@ def _declare(lib):
         "nvb_clear_device_error": [],
         "nvb_paged_decode_gather": [_P] * 8 + [c_int] * 8 + [_P] * 4 + [c_int, c_int, ctypes.c_uint],
         "nvb_paged_decode_gather_capturable": [_P] * 8 + [c_int] * 8 + [_P] * 5 + [c_int, c_int],
+        "nvb_paged_tree_fwd": [_P] * 9 + [c_int] * 10 + [_P] * 3 + [c_int],
+        "nvb_tree_num_splits": [c_int] * 6,
+        "nvb_cache_copy_pages": [_P] * 3 + [c_int] + [_P] * 3 + [c_int] * 5,
+        "nvb_cache_compact_paths": [_P] * 3 + [c_int] + [_P] * 6 + [c_int] * 7,
         "nvb_peer_buffer_create": [ctypes.c_size_t, ctypes.POINTER(c_void_p), _P],
         "nvb_peer_buffer_open": [_P, ctypes.POINTER(c_void_p)],
         "nvb_peer_buffer_close": [_P],
@@ -127,6 +131,24 @@ def _distinct(output, inputs, name):
         a0, a1 = _span(t)
         if o0 < a1 and a0 < o1:
             raise NvbError(f"{name} aliases an input or another output")
+
+
+def _exact(t, shape, dtype, name):
+    """_tensor with the shape itself, on the current device (the kernels run there)."""
+    import torch
+
+    if t is None:
+        raise NvbError(f"{name} is required")
+    if not t.is_cuda:
+        raise NvbError(f"{name} must be a CUDA tensor")
+    if t.dtype != dtype:
+        raise NvbError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise NvbError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise NvbError(f"{name} must be contiguous")
+    if t.device.index != torch.cuda.current_device():
+        raise NvbError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
 def num_splits(batch, q_heads, kv_heads, max_k, num_sms):
@@ -264,6 +286,145 @@ def paged_fwd(q, k, v, out, cu_q, kv_lens, block_table, *, batch, max_q, max_k, 
                                 _ptr(kv_lens), _ptr(block_table), batch, total_q, max_q, max_k, q_heads,
                                 kv_heads, block_size, table_stride, num_splits, _ptr(lse), _ptr(lse_accum),
                                 _ptr(out_accum), num_blocks))
+
+
+def tree_num_splits(batch, max_q, q_heads, kv_heads, max_k, num_sms=None):
+    """Split count of paged_tree_fwd for a GPU of num_sms SMs (default: the current device's)."""
+    if num_sms is None:
+        import torch
+
+        num_sms = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
+    return library().nvb_tree_num_splits(batch, max_q, q_heads, kv_heads, max_k, num_sms)
+
+
+def tree_scratch(num_splits_, total_q, q_heads, device):
+    """Caller-owned FP32 scratch (lse_accum, out_accum) of paged_tree_fwd; (None, None) for one split."""
+    return splitkv_scratch(num_splits_, total_q, q_heads, device) if num_splits_ > 1 else (None, None)
+
+
+def paged_tree_fwd(q, k, v, out, cu_q, kv_lens, block_table, tree_mask, *, batch, max_q, max_k, q_heads, kv_heads,
+                   block_size, table_stride, num_blocks, num_splits=1, lse=None, lse_accum=None, out_accum=None,
+                   stream=None, check=True):
+    """Attention of drafted trees over the paged cache (nvb_paged_tree_fwd).
+
+    Queries cu_q[b]..cu_q[b + 1] are sequence b's nodes, whose keys are the
+    last of its kv_lens[b] keys in the same order; tree_mask [total_q, words]
+    int64 has bit t % 64 of word t // 64 set where a node attends to node t
+    (host.tree_mask). The keys before the tree are visible to all. lse, where
+    given, is [total_q, q_heads].
+    """
+    import torch
+
+    total_q, words = q.shape[0], tree_mask.shape[-1]
+    if check:
+        bf16, i32, f32 = torch.bfloat16, torch.int32, torch.float32
+        for t, nm in ((q, "q"), (out, "out")):
+            _exact(t, (total_q, q_heads, 128), bf16, nm)
+        for t, nm in ((k, "k"), (v, "v")):
+            _exact(t, (num_blocks, block_size, kv_heads, 128), bf16, nm)
+        _exact(cu_q, (batch + 1,), i32, "cu_q")
+        _exact(kv_lens, (batch,), i32, "kv_lens")
+        _exact(block_table, (batch, table_stride), i32, "block_table")
+        _exact(tree_mask, (total_q, words), torch.int64, "tree_mask")
+        outputs = [out]
+        if lse is not None:
+            _exact(lse, (total_q, q_heads), f32, "lse")
+            outputs.append(lse)
+        if num_splits > 1:
+            _exact(lse_accum, (num_splits, total_q, q_heads), f32, "lse_accum")
+            _exact(out_accum, (num_splits, total_q, q_heads, 128), f32, "out_accum")
+            outputs += [lse_accum, out_accum]
+        taken = [q, k, v, cu_q, kv_lens, block_table, tree_mask]
+        for o in outputs:
+            _distinct(o, taken, "output")
+            taken.append(o)
+    _check(library().nvb_paged_tree_fwd(_stream(stream), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(cu_q),
+                                        _ptr(kv_lens), _ptr(block_table), _ptr(tree_mask), words, batch, total_q,
+                                        max_q, max_k, q_heads, kv_heads, block_size, table_stride, num_splits,
+                                        _ptr(lse), _ptr(lse_accum), _ptr(out_accum), num_blocks))
+
+
+class CacheLayers:
+    """The K and V caches of a model's layers ([num_blocks, block_size,
+    kv_heads, head_dim] BF16 each), checked once, for the copies below. Keeps
+    the tensors alive."""
+
+    def __init__(self, k_caches, v_caches):
+        import torch
+
+        k_caches, v_caches = list(k_caches), list(v_caches)
+        if not k_caches or len(k_caches) != len(v_caches):
+            raise NvbError(f"{len(k_caches)} K caches and {len(v_caches)} V caches")
+        if k_caches[0].dim() != 4:
+            raise NvbError("a cache must be [num_blocks, block_size, kv_heads, head_dim]")
+        self.shape = tuple(k_caches[0].shape)
+        for i, (k, v) in enumerate(zip(k_caches, v_caches)):
+            _exact(k, self.shape, torch.bfloat16, f"k_caches[{i}]")
+            _exact(v, self.shape, torch.bfloat16, f"v_caches[{i}]")
+        spans = sorted(_span(t) for t in k_caches + v_caches)
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise NvbError("two caches overlap")
+        self.layers = len(k_caches)
+        self.extent = (spans[0][0], spans[-1][1])
+        self.device = k_caches[0].device
+        self._tensors = k_caches + v_caches
+        self._k = (c_void_p * self.layers)(*[t.data_ptr() for t in k_caches])
+        self._v = (c_void_p * self.layers)(*[t.data_ptr() for t in v_caches])
+
+    def _apart(self, tensors):
+        import torch
+
+        if self.device.index != torch.cuda.current_device():
+            raise NvbError(f"the caches are on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
+        for t in tensors:
+            a0, a1 = _span(t)
+            if a0 < self.extent[1] and self.extent[0] < a1 and any(
+                    a0 < s[1] and s[0] < a1 for s in map(_span, self._tensors)):
+                raise NvbError("an argument lies in a cache")
+
+
+def cache_copy_pages(layers, src, dst, rows=None, *, stream=None):
+    """Copies page src[i] to page dst[i] in every cache of `layers` (a
+    CacheLayers), its first rows[i] tokens where rows is given
+    (nvb_cache_copy_pages). src, dst and rows are int32 CUDA tensors; no page
+    may be the target of two pairs, nor a target and a source."""
+    import torch
+
+    num_blocks, block_size, kv_heads, head_dim = layers.shape
+    pairs = src.numel()
+    arguments = [src, dst] + ([rows] if rows is not None else [])
+    for t, nm in zip(arguments, ("src", "dst", "rows")):
+        _exact(t, (pairs,), torch.int32, nm)
+    layers._apart(arguments)
+    _check(library().nvb_cache_copy_pages(_stream(stream), layers._k, layers._v, layers.layers, _ptr(src), _ptr(dst),
+                                          _ptr(rows), pairs, kv_heads, head_dim, block_size, num_blocks))
+
+
+def cache_compact_paths(layers, cu_q, kv_lens, block_table, path, counts, new_kv_lens, *, stream=None):
+    """Moves the K and V rows of each sequence's accepted path (path and counts
+    of model.layer_verify) together behind its context, in every cache of
+    `layers` (a CacheLayers), and writes the lengths that are left to
+    new_kv_lens (nvb_cache_compact_paths)."""
+    import torch
+
+    num_blocks, block_size, kv_heads, head_dim = layers.shape
+    batch = kv_lens.numel()
+    if path.dim() != 2 or block_table.dim() != 2:
+        raise NvbError("path and block_table must have a row for each sequence")
+    i32 = torch.int32
+    _exact(cu_q, (batch + 1,), i32, "cu_q")
+    _exact(kv_lens, (batch,), i32, "kv_lens")
+    _exact(block_table, (batch, block_table.shape[1]), i32, "block_table")
+    _exact(path, (batch, path.shape[1]), i32, "path")
+    _exact(counts, (batch,), i32, "counts")
+    _exact(new_kv_lens, (batch,), i32, "new_kv_lens")
+    inputs = [cu_q, kv_lens, block_table, path, counts]
+    _distinct(new_kv_lens, inputs, "new_kv_lens")
+    layers._apart(inputs + [new_kv_lens])
+    _check(library().nvb_cache_compact_paths(_stream(stream), layers._k, layers._v, layers.layers, _ptr(cu_q),
+                                             _ptr(kv_lens), _ptr(block_table), _ptr(path), _ptr(counts),
+                                             _ptr(new_kv_lens), batch, path.shape[1], kv_heads, head_dim, block_size,
+                                             block_table.shape[1], num_blocks))
 
 
 def attention(q, kcache, vcache, positions, seq_indices, tables, out, *, rows, q_heads, kv_heads, head_dim,

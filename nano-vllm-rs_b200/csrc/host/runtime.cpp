@@ -319,6 +319,72 @@ void nvbh_pool_clear_cache(NvbhBlockPool* p) {
   }
 }
 
+int nvbh_pool_fork(NvbhBlockPool* p, const int32_t* blocks, size_t num_blocks, size_t tokens, size_t block_size,
+                   int32_t* child, size_t* child_blocks, int32_t* copy_src, int32_t* copy_dst, size_t* copy_rows) {
+  g_error[0] = 0;
+  if (!p || block_size == 0 || !child_blocks || !copy_src || !copy_dst || !copy_rows ||
+      (num_blocks && (!blocks || !child)))
+    return fail("invalid fork arguments");
+  const size_t full = tokens / block_size, part = tokens % block_size, need = full + (part ? 1 : 0);
+  if (need > num_blocks) return fail("the sequence's pages do not hold its tokens");
+  for (size_t i = 0; i < need; ++i)
+    if (nvbh_pool_references(p, blocks[i]) == 0) return fail("a page of the sequence is not in use");
+  int fresh = -1;
+  if (part) {
+    // the sequence's own pages are referenced, so none of them is taken
+    fresh = nvbh_pool_allocate(p);
+    if (fresh < 0) return fail("no free page for the fork");
+  }
+  for (size_t i = 0; i < full; ++i) {
+    p->blocks[size_t(blocks[i])].references += 1;
+    p->touch(blocks[i]);
+    child[i] = blocks[i];
+  }
+  *copy_src = part ? blocks[full] : -1;
+  if (part) child[full] = fresh;
+  *child_blocks = need;
+  *copy_dst = fresh;
+  *copy_rows = part;
+  return 0;
+}
+
+int nvbh_pool_truncate(NvbhBlockPool* p, int32_t* blocks, size_t* num_blocks, size_t tokens, size_t block_size) {
+  g_error[0] = 0;
+  if (!p || block_size == 0 || !num_blocks || (*num_blocks && !blocks)) return fail("invalid truncate arguments");
+  const size_t need = tokens / block_size + (tokens % block_size ? 1 : 0);
+  if (need > *num_blocks) return fail("the sequence's pages do not hold its tokens");
+  for (size_t i = need; i < *num_blocks; ++i)
+    if (nvbh_pool_references(p, blocks[i]) == 0) return fail("a page of the sequence is not in use");
+  for (size_t i = *num_blocks; i > need; --i) {
+    nvbh_pool_release(p, blocks[i - 1]);
+    blocks[i - 1] = -1;
+  }
+  *num_blocks = need;
+  return 0;
+}
+
+int nvbh_tree_mask(const int32_t* parents, const int32_t* cu_q, size_t sequences, size_t words, uint64_t* mask,
+                   int32_t* depth) {
+  g_error[0] = 0;
+  if (!cu_q || words == 0 || (sequences && (!parents || !mask))) return fail("invalid tree mask arguments");
+  if (cu_q[0] != 0) return fail("cu_q must start at 0");
+  for (size_t s = 0; s < sequences; ++s) {
+    if (cu_q[s + 1] < cu_q[s]) return fail("cu_q must not decrease");
+    const size_t begin = size_t(cu_q[s]), n = size_t(cu_q[s + 1]) - begin;
+    if (n > 64 * words) return fail("a tree has more nodes than its mask has bits");
+    for (size_t i = 0; i < n; ++i) {
+      const int32_t parent = parents[begin + i];
+      if (parent < -1 || parent >= (long long)i || (i == 0 && parent != -1))
+        return fail("a node's parent must come before it");
+      uint64_t* row = mask + (begin + i) * words;
+      for (size_t w = 0; w < words; ++w) row[w] = parent < 0 ? 0 : mask[(begin + size_t(parent)) * words + w];
+      row[i / 64] |= uint64_t(1) << (i % 64);
+      if (depth) depth[begin + i] = parent < 0 ? 0 : depth[begin + size_t(parent)] + 1;
+    }
+  }
+  return 0;
+}
+
 void nvbh_pool_force_hash_entry(NvbhBlockPool* p, const uint32_t* prefix, size_t n, int block) {
   p->by_hash[prefix_hash(prefix, n)].push_back(block);
 }

@@ -108,6 +108,34 @@ cudaError_t once_per_context(unsigned* seen, F&& init) {
   return e;
 }
 
+// Copies within the cache over all layers (cache_ops.cu); at most this many
+// layers in one launch (their pointers are kernel parameters).
+constexpr int kCacheLayers = 64;
+// vec16: rows and caches are made of aligned 16-byte vectors.
+cudaError_t launch_copy_pages(cudaStream_t stream, void* const* k, void* const* v, int layers, bool vec16,
+                              const int* src, const int* dst, const int* rows, int pairs, int row_bytes,
+                              int block_size, int num_blocks);
+cudaError_t launch_compact_paths(cudaStream_t stream, void* const* k, void* const* v, int layers, bool vec16,
+                                 const int* cu_q, const int* kv_lens, const int* tables, const int* path,
+                                 const int* counts, int* new_lens, int batch, int path_stride, int row_bytes,
+                                 int block_size, int table_stride, int num_blocks, bool write_lens);
+
+// Attention of drafted trees over the paged cache (tree.cu).
+struct TreeParams {
+  const __nv_bfloat16* q;    // [total_q, qh, 128]
+  __nv_bfloat16* out;        // [total_q, qh, 128]
+  const int* cu_q;           // [batch + 1]
+  const int* kv_lens;        // [batch], the tree's nodes included
+  const int* block_table;    // [batch, table_stride]
+  const unsigned long long* mask;  // [total_q, mask_words]
+  float* lse;                // [total_q, qh] or null
+  float* lse_accum;          // [splits, total_q, qh]      (splits > 1)
+  float* out_accum;          // [splits, total_q, qh, 128] (splits > 1)
+  int batch, total_q, max_q, qh, kvh, block_size, table_stride, num_blocks, num_splits, mask_words;
+  float scale_log2;
+};
+cudaError_t launch_tree(const TreeParams& p, const void* k, const void* v, cudaStream_t stream);
+
 // Native-form attention for head dimensions other than 128 (generic.cu).
 cudaError_t launch_generic_attention(const void* q, const void* k, const void* v, void* out, const int* positions,
                                      const int* seq_indices, const int* tables, int rows, int qh, int kvh, int dim,

@@ -1,5 +1,6 @@
-// Gumbel-max score arithmetic shared by the sampler (sample.cu) and the
-// decode GEMM's sampling epilogue (gemm.cu), so both pick the same token from
+// Gumbel-max score arithmetic shared by the sampler (sample.cu), the
+// decode GEMM's sampling epilogue (gemm.cu) and the verification of drafted
+// tokens (verify.cu), so all pick the same token from
 // the same BF16 logits. The reference's stream and arithmetic
 // (kernels/kernels.cu:371-377, 413-431): for temperature T > 0 and seed s,
 // token v scores logit / T - logf(-logf(u)), u = ((x >> 41) + 0.5) / 2^23,
@@ -38,12 +39,17 @@ __device__ __forceinline__ void warp_best(float& score, int& index) {
   }
 }
 
-__device__ __forceinline__ float gumbel_score(float logit, float temperature, uint64_t seed, int token) {
-  if (!(temperature > 0.0f)) return logit;
+// logf(-logf(u)): what a token's score loses to its Gumbel noise.
+__device__ __forceinline__ float gumbel_log(uint64_t seed, int token) {
   const uint64_t x = splitmix64(seed ^ (uint64_t(token) * 0xd2b74407b1ce6e93ULL));
   // x >> 41 has 23 bits: its 32-bit conversion is exact, like the 64-bit one.
   const float u = __fmul_rn(__fadd_rn(float(uint32_t(x >> 41)), 0.5f), 1.0f / 8388608.0f);
-  return __fsub_rn(__fdiv_rn(logit, temperature), logf(-logf(u)));
+  return logf(-logf(u));
+}
+
+__device__ __forceinline__ float gumbel_score(float logit, float temperature, uint64_t seed, int token) {
+  if (!(temperature > 0.0f)) return logit;
+  return __fsub_rn(__fdiv_rn(logit, temperature), gumbel_log(seed, token));
 }
 
 }  // namespace sample_math

@@ -82,6 +82,10 @@ def library():
         L.nvbh_pool_clear_cache.restype = None
         L.nvbh_pool_force_hash_entry.argtypes = [P, P, c_size, ctypes.c_int]
         L.nvbh_pool_force_hash_entry.restype = None
+        L.nvbh_pool_fork.argtypes = [P, P, c_size, c_size, c_size, P, ctypes.POINTER(c_size), P, P,
+                                     ctypes.POINTER(c_size)]
+        L.nvbh_pool_truncate.argtypes = [P, P, ctypes.POINTER(c_size), c_size, c_size]
+        L.nvbh_tree_mask.argtypes = [P, P, c_size, c_size, P, P]
         L.nvbh_make_batch.argtypes = [ctypes.POINTER(NvbhSegment), c_size, c_size, ctypes.c_uint64,
                                       ctypes.POINTER(NvbhBatchOut)]
         L.nvbh_sampling_seed.argtypes = [ctypes.c_uint64] * 3
@@ -214,6 +218,24 @@ class BlockPool:
         t = self._toks(prefix)
         library().nvbh_pool_publish(self.h, block, _p(t), t.size)
 
+    def fork(self, blocks, tokens, block_size):
+        """(child's pages, None or (source page, target page, tokens to copy)):
+        a fork of a sequence of `tokens` tokens in `blocks` (nvbh_pool_fork)."""
+        b = _arr(blocks, np.int32)
+        child = np.zeros(max(1, b.size), np.int32)
+        count, rows = c_size(0), c_size(0)
+        src, dst = ctypes.c_int32(-1), ctypes.c_int32(-1)
+        _check(library().nvbh_pool_fork(self.h, _p(b), b.size, tokens, block_size, _p(child), ctypes.byref(count),
+                                        ctypes.byref(src), ctypes.byref(dst), ctypes.byref(rows)))
+        return child[:count.value].tolist(), ((src.value, dst.value, rows.value) if rows.value else None)
+
+    def truncate(self, blocks, tokens, block_size):
+        """The pages a sequence cut to `tokens` tokens keeps; the others are released (nvbh_pool_truncate)."""
+        b = _arr(blocks, np.int32).copy()
+        count = c_size(b.size)
+        _check(library().nvbh_pool_truncate(self.h, _p(b), ctypes.byref(count), tokens, block_size))
+        return b[:count.value].tolist()
+
     def available(self):
         return library().nvbh_pool_available(self.h)
 
@@ -273,6 +295,20 @@ def make_batch(segments, block_size, seed, is_decode=False) -> Batch:
                  block_tables=out["block_tables"][:n * co.table_stride].tolist(), table_stride=co.table_stride,
                  last_token_indices=out["last"][:k].tolist(), temperatures=out["temps"][:k].tolist(),
                  seeds=[int(x) for x in out["seeds"][:k]], is_decode=is_decode)
+
+
+def tree_mask(parents, cu_q, words=None):
+    """(mask [rows, words] int64, depth [rows] int32) of drafted trees for
+    paged_tree_fwd: parents[r] is the place of row r's parent in its own tree,
+    -1 for a root (nvbh_tree_mask)."""
+    p, cu = _arr(parents, np.int32), _arr(cu_q, np.int32)
+    if cu.ndim != 1 or cu.size < 1 or p.ndim != 1 or p.size < int(cu[-1]):
+        raise HostError("cu_q must end at the number of parents at most")
+    n = int(np.diff(cu).max(initial=1))
+    words = max(1, (n + 63) // 64) if words is None else int(words)
+    mask, depth = np.zeros((p.size, max(words, 0)), np.int64), np.zeros(p.size, np.int32)
+    _check(library().nvbh_tree_mask(_p(p), _p(cu), cu.size - 1, words, _p(mask), _p(depth)))
+    return mask, depth
 
 
 def sampling_seed(base, request_id, generated):

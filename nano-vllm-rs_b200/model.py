@@ -76,6 +76,9 @@ def library():
         L.nvbe_layer_gemm_sample.argtypes = [P, P, P, P, I, I, I, P, P, P, P, P]
         L.nvbe_sample_partitions.argtypes = [I]
         L.nvbe_layer_sample.argtypes = [P] * 7 + [I, I]
+        L.nvbe_verify_workspace_bytes.argtypes = [I]
+        L.nvbe_verify_workspace_bytes.restype = ctypes.c_size_t
+        L.nvbe_layer_verify.argtypes = [P] * 13 + [I] * 4 + [P, ctypes.c_size_t]
         _lib = L
     return _lib
 
@@ -233,6 +236,13 @@ class Qwen3Model:
         return tuple(torch.as_tensor(_DeviceArray(p.value, shape, "<i2"), device=dev).view(torch.bfloat16)
                      for p in (k, v))
 
+    def cache_layers(self):
+        """The caches of every layer, for cache_copy_pages and cache_compact_paths (used before close())."""
+        from . import CacheLayers
+
+        pairs = [self.kv_cache(i) for i in range(self.config.num_hidden_layers)]
+        return CacheLayers([k for k, _ in pairs], [v for _, v in pairs])
+
     def close(self):
         if getattr(self, "_handle", None):
             library().nvbe_model_destroy(self._handle)
@@ -333,3 +343,56 @@ def layer_sample(logits, temperatures, seeds, out, stream=None):
     pi = torch.empty(rows * parts, dtype=torch.int32, device=logits.device)
     _check(library().nvbe_layer_sample(_s(stream), _p(logits), _p(temperatures), _p(seeds), _p(out), _p(ps), _p(pi),
                                        rows, vocab))
+
+
+def verify_workspace_bytes(rows):
+    return library().nvbe_verify_workspace_bytes(rows)
+
+
+def layer_verify(logits, draft_logits, tokens, parents, uniforms, seeds, temperatures, cu_q, out_tokens, path, counts,
+                 accept_prob, stream=None, workspace=None):
+    """nvbe_layer_verify: accepts drafted tokens against the target's
+    probabilities (softmax of logits / temperature) and draws the token behind
+    them. Rows cu_q[b]..cu_q[b + 1] are sequence b's tree, its root (the last
+    committed token) first; draft_logits None: drafts without probabilities.
+    out_tokens and path are [batch, max_q] int32, counts [batch] int32 and
+    accept_prob [rows] FP32; seeds are int64 (or uint64) words. `workspace` (a
+    CUDA uint8 tensor of verify_workspace_bytes(rows)) is allocated per call
+    when not given."""
+    import torch
+
+    if logits.dim() != 2 or out_tokens.dim() != 2 or temperatures.dim() != 1:
+        raise ValueError("logits must be [rows, vocab], out_tokens [batch, max_q] and temperatures [batch]")
+    (rows, vocab), (batch, max_q) = logits.shape, out_tokens.shape
+    i32, f32 = torch.int32, torch.float32
+    seed_type = seeds.dtype if seeds.dtype == torch.uint64 else torch.int64
+    device = torch.cuda.current_device()
+    wanted = [("logits", logits, (rows, vocab), torch.bfloat16), ("tokens", tokens, (rows,), i32),
+              ("parents", parents, (rows,), i32), ("uniforms", uniforms, (rows,), f32),
+              ("seeds", seeds, (rows,), seed_type), ("temperatures", temperatures, (batch,), f32),
+              ("cu_q", cu_q, (batch + 1,), i32), ("out_tokens", out_tokens, (batch, max_q), i32),
+              ("path", path, (batch, max_q), i32), ("counts", counts, (batch,), i32),
+              ("accept_prob", accept_prob, (rows,), f32)]
+    if draft_logits is not None:
+        wanted.append(("draft_logits", draft_logits, (rows, vocab), torch.bfloat16))
+    if workspace is not None:
+        wanted.append(("workspace", workspace, (workspace.numel(),), torch.uint8))
+    for name, t, shape, dtype in wanted:
+        if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device.index != device \
+                or not t.is_cuda:
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} on cuda:{device}")
+    written = ("out_tokens", "path", "counts", "accept_prob", "workspace")
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name) for name, t, _, _ in wanted)
+    end, held = 0, False
+    for a, z, name in spans:  # what is written overlaps nothing
+        if a < end and (held or name in written):
+            raise ValueError(f"{name} overlaps another argument")
+        if z > end:
+            end, held = z, name in written
+    ws = workspace
+    if ws is None:
+        ws = torch.empty(max(16, verify_workspace_bytes(rows)), dtype=torch.uint8, device=logits.device)
+    _check(library().nvbe_layer_verify(_s(stream), _p(logits), _p(draft_logits) if draft_logits is not None else None,
+                                       _p(tokens), _p(parents), _p(uniforms), _p(seeds), _p(temperatures), _p(cu_q),
+                                       _p(out_tokens), _p(path), _p(counts), _p(accept_prob), rows, batch, max_q,
+                                       vocab, _p(ws), ws.numel()))
