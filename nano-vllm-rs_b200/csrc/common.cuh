@@ -30,6 +30,7 @@ enum DeviceError : int {
   kErrBadPage = 5,            // reserved: a page id outside [0, num_blocks)
   kErrPrefillAlign = 6,       // prefill: dynamic shared memory base not usable for the tile layout
   kErrGatherWait = 7,         // multi-GPU gather: a peer's completion flag did not arrive in time
+  kErrTreeWait = 8,           // a wait of the tree attention gave up
 };
 
 constexpr long long kWaitCycles = 4000000000LL;

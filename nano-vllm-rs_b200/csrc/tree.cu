@@ -8,67 +8,502 @@
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(q_i k_j / sqrt(128)) over
 //   j < ctx and over j = ctx + t where bit t of mask[i] is set.
-#include "internal.cuh"
+//
+// Tensor-core kernel: a CTA takes 128 rows of one (sequence, kv head) and one
+// range of its keys. Rows pack the GQA group, row r = (node r / G, head
+// r % G), so every K/V tile serves all nodes and heads of the group. Per tile
+// of 64 keys
+//
+//   S = Q K^T   tcgen05.mma M=128 N=64 K=128, Q from TMEM, K from shared memory
+//   P = exp2(S * scale * log2 e - m), one thread a row, written back over S
+//   O += P V    tcgen05.mma M=128 N=128 K=64, P from TMEM, V from shared memory
+//
+// What bounds it: HBM for trees of up to 128 rows, each K/V byte read once. A
+// tile is 32 KB of K and V, 740 ns of an SM's share of HBM bandwidth (~1,350
+// cycles); its MMAs take 512 cycles and its 128 x 64 exponentials 512 of the
+// MUFU unit. Its steps follow each other, so two CTAs share an SM (256 TMEM
+// columns each: Q 64, S/P 64, O 128) and one's softmax runs beside the other's
+// MMAs. Keeping Q in TMEM leaves the shared memory to the ring of K and V
+// tiles, loaded by TMA in the order K0 V0 K1 V1 ...
+//
+// Roles: warp 0 loads, warp 1 owns TMEM and issues the MMAs, warps 2-5 hold
+// the rows (a warp whose 32 rows are all past the last node only waits). S_j
+// is issued once PV_j-1 has completed, so S_j's commit also says that O may be
+// rescaled, and the chain needs one barrier each way.
+//
+// Keys that a node does not see get probability 0; their V rows must not hold
+// infinities or NaN, as 0 times those is not 0. V rows of keys that nobody
+// sees (behind the sequence, bad pages) are zeroed in shared memory. A tree
+// key may be seen by some rows and not by others: its non-finite elements are
+// zeroed too, and added at the end to the rows that see the key.
+#include "combine.cuh"
+#include "prefill_common.cuh"
 
 namespace nvb {
 
 namespace tree_detail {
 
-constexpr float kLn2 = 0.693147180559945309f;
-constexpr int kWarps = 8;
+using namespace prefill_common;
 
-// One warp per (node, query head): a lane holds four dimensions.
-__global__ void __launch_bounds__(kWarps * 32)
-    tree_kernel(const TreeParams p, const __nv_bfloat16* __restrict__ kc, const __nv_bfloat16* __restrict__ vc) {
-  const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int item = blockIdx.x * kWarps + warp;
+constexpr int kRows = 128;              // rows of a CTA (TMEM lanes)
+constexpr int kKeys = 64;               // keys of a tile
+constexpr int kHalf = kKeys * 128;      // 64 rows x 64 BF16 (one swizzled half)
+constexpr int kTileBytes = 2 * kHalf;   // K or V tile 64 x 128 BF16
+constexpr int kSlots = 7;               // ring slots shared by K and V tiles
+constexpr int kThreads = 192;
+constexpr int kTmemCols = 256;
+constexpr int kSCol = 64, kOCol = 128;  // Q at 0
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kRescaleLog2 = 8.0f;    // the maximum in use moves when it grew by 2^8 (P <= 2^8)
+
+enum Bar { kFull = 0, kEmpty = kFull + kSlots, kQReady = kEmpty + kSlots, kSFull, kPFull, kODone, kDrain, kNumBars };
+constexpr int kTmemSlotOff = kNumBars * 8;
+constexpr int kFlagOff = kTmemSlotOff + 4;
+constexpr int kHeadBytes = 1024;  // tiles start at the next 1 KB boundary
+static_assert(kFlagOff + 4 <= kHeadBytes, "barrier block must fit below the first 1 KB boundary");
+constexpr int kSmemBytes = kHeadBytes + kSlots * kTileBytes;  // two CTAs an SM: at most 113 KB each
+
+// kind::f16, FP32 accumulate, BF16 A (from TMEM) and B, M = 128.
+constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
+constexpr uint32_t kIdescS = kIdesc | ((uint32_t(kKeys) >> 3) << 17);       // B K-major (keys)
+constexpr uint32_t kIdescPV = kIdesc | ((128u >> 3) << 17) | (1u << 16);    // B MN-major (dims contiguous)
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+  return mbar_wait(bar, parity, kErrTreeWait);
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait(bar, parity));
+}
+
+// Bits [t, t + 64) of a row's mask; bits outside it are 0.
+__device__ __forceinline__ unsigned long long mask_window(const unsigned long long* row, int words, int t) {
+  const int w = t >> 6, s = t & 63;  // t < 0 rounds down
+  const unsigned long long lo = w >= 0 && w < words ? row[w] : 0ull;
+  if (s == 0) return lo;
+  const unsigned long long hi = w + 1 >= 0 && w + 1 < words ? row[w + 1] : 0ull;
+  return (lo >> s) | (hi << (64 - s));
+}
+
+__device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {  // 0xffff in each BF16 that is inf or NaN
+  return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+
+__global__ void __launch_bounds__(kThreads, 2)
+    tree_kernel(const TreeParams p, const FastDiv fd_group, const FastDiv fd_bs, const int row_tiles,
+                const __nv_bfloat16* __restrict__ vcache, const __grid_constant__ CUtensorMap kmap,
+                const __grid_constant__ CUtensorMap vmap) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + kTmemSlotOff);
+  int* bad_v = reinterpret_cast<int*>(smem_raw + kFlagOff);
+  const uint32_t raw_addr = smem_addr(smem_raw), sbase = raw_addr + kHeadBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // Row tiles of one key range are neighbours: they read its K and V together.
+  int cta = blockIdx.x;
+  const int tile = cta % row_tiles;
+  cta /= row_tiles;
+  const int split = cta % p.num_splits;
+  cta /= p.num_splits;
+  const int kvhead = cta % p.kvh, b = cta / p.kvh;
+  const int group = p.qh / p.kvh;
+
+  // The kernel before this one has completed, its writes are visible.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int begin = p.cu_q[b], n = min(p.cu_q[b + 1], p.total_q) - begin;
-  const int node = item / p.qh, head = item - node * p.qh;
-  if (begin < 0 || node >= min(n, p.max_q)) return;
+  const int row0 = tile * kRows, rows = min(n, p.max_q) * group - row0;
+  if (begin < 0 || rows <= 0) return;
   const int len = p.kv_lens[b], ctx = len - n;
   const bool valid = ctx >= 0 && (long long)len <= (long long)p.table_stride * p.block_size;
-  const long long row = begin + node;
-  const uint2 qw = *reinterpret_cast<const uint2*>(p.q + (row * p.qh + head) * 128 + lane * 4);
-  const float q0 = bf16lo(qw.x), q1 = bf16hi(qw.x), q2 = bf16lo(qw.y), q3 = bf16hi(qw.y);
-  const int* table = p.block_table + (long long)b * p.table_stride;
-  float m = -INFINITY, l = 0.0f, a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
-  for (int key = 0; valid && key < len; ++key) {
-    const int page = table[key / p.block_size];
-    if (page < 0 || page >= p.num_blocks) continue;
-    const int t = key - ctx;
-    if (t >= 0 && (t >= 64 * p.mask_words || !((p.mask[row * p.mask_words + (t >> 6)] >> (t & 63)) & 1))) continue;
-    const long long at =
-        (((long long)page * p.block_size + key % p.block_size) * p.kvh + head / (p.qh / p.kvh)) * 128 + lane * 4;
-    const uint2 kw = *reinterpret_cast<const uint2*>(kc + at), vw = *reinterpret_cast<const uint2*>(vc + at);
-    float s = q0 * bf16lo(kw.x) + q1 * bf16hi(kw.x) + q2 * bf16lo(kw.y) + q3 * bf16hi(kw.y);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s *= p.scale_log2;
-    const float mn = fmaxf(m, s);
-    const float alpha = m == -INFINITY ? 0.0f : exp2f(m - mn), w = exp2f(s - mn);
-    m = mn;
-    l = l * alpha + w;
-    a0 = a0 * alpha + w * bf16lo(vw.x);
-    a1 = a1 * alpha + w * bf16hi(vw.x);
-    a2 = a2 * alpha + w * bf16lo(vw.y);
-    a3 = a3 * alpha + w * bf16hi(vw.y);
+  const int tiles_total = valid ? (len + kKeys - 1) / kKeys : 0;
+  const int per_split = (tiles_total + p.num_splits - 1) / p.num_splits;
+  const int t0 = split * per_split, ntiles = max(0, min(t0 + per_split, tiles_total) - t0);
+
+  // This thread's row (warps 2-5): its TMEM lane, node and output place.
+  const int r = (warp & 3) * 32 + lane;
+  const bool row_ok = warp >= 2 && r < rows;
+  const int node = fd_group.div(row_ok ? row0 + r : 0), head = kvhead * group + (row0 + r - node * group);
+  const long long item = (long long)(begin + node) * p.qh + head;  // of [total_q, qh]
+  const long long partial = (long long)split * p.total_q * p.qh + item;
+
+  if (ntiles == 0 || (sbase & 1023u) != 0) {
+    if (ntiles != 0 && threadIdx.x == 0) record_error(kErrPrefillAlign);
+    if (row_ok) {
+      if (p.num_splits > 1) {
+        p.lse_accum[partial] = -INFINITY;  // the combine reads no output of such a split
+      } else {
+        for (int d = 0; d < 128; d += 8) *reinterpret_cast<uint4*>(p.out + item * 128 + d) = make_uint4(0, 0, 0, 0);
+        if (p.lse) p.lse[item] = -INFINITY;
+      }
+    }
+    return;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint2 o;
-  o.x = pack_bf16x2(a0 * inv, a1 * inv);
-  o.y = pack_bf16x2(a2 * inv, a3 * inv);
-  *reinterpret_cast<uint2*>(p.out + (row * p.qh + head) * 128 + lane * 4) = o;
-  if (lane == 0 && p.lse) p.lse[row * p.qh + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+
+  const int active = (min(rows, kRows) + 31) / 32;  // warps with rows
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&bars[kFull + s], 1);
+      mbar_init(&bars[kEmpty + s], 1);
+    }
+    mbar_init(&bars[kQReady], active);
+    mbar_init(&bars[kSFull], 1);
+    mbar_init(&bars[kPFull], active);
+    mbar_init(&bars[kODone], 1);
+    mbar_init(&bars[kDrain], 1);
+    *bad_v = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int* table = p.block_table + (long long)b * p.table_stride;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------- producer
+    if (lane == 0) {
+      tma_prefetch_desc(&kmap);
+      tma_prefetch_desc(&vmap);
+      int issued = 0;
+      for (int i = 0; i < 2 * ntiles; ++i) {
+        const int key0 = (t0 + (i >> 1)) * kKeys, logical = fd_bs.div(key0), slot = i % kSlots;
+        const int page = table[logical];
+        // released by the MMA that read the slot's last load: S of a K tile, PV of a V tile
+        if (i >= kSlots && !wait(&bars[kEmpty + slot], ((i / kSlots) + 1) & 1)) break;
+        if (page_ok(page, p.num_blocks)) {
+          const CUtensorMap* map = (i & 1) ? &vmap : &kmap;
+          unsigned char* dst = smem_raw + kHeadBytes + slot * kTileBytes;
+          const int trow = page * p.block_size + (key0 - logical * p.block_size);
+          mbar_arrive_expect_tx(&bars[kFull + slot], kTileBytes);
+          tma_load_3d(dst, map, &bars[kFull + slot], 0, kvhead, trow);
+          tma_load_3d(dst + kHalf, map, &bars[kFull + slot], 64, kvhead, trow);
+        } else {
+          mbar_arrive(&bars[kFull + slot]);
+        }
+        issued = i + 1;
+      }
+      // Every copy has landed before the CTA may exit (on the normal path its readers have waited for it).
+      for (int i = max(0, issued - kSlots); i < issued; ++i)
+        if (!wait(&bars[kFull + i % kSlots], (i / kSlots) & 1)) break;
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      const uint64_t kd = sw128_desc(sbase, 16, 1024), vd = sw128_desc(sbase, kHalf, 1024);
+      const uint32_t k_lo = uint32_t(kd), k_hi = uint32_t(kd >> 32), v_lo = uint32_t(vd), v_hi = uint32_t(vd >> 32);
+      bool alive = wait(&bars[kQReady], 0);
+      for (int j = 0; j < ntiles && alive; ++j) {
+        const int ki = 2 * j, ks = ki % kSlots, vi = 2 * j + 1, vs = vi % kSlots;
+        alive = wait(&bars[kFull + ks], (ki / kSlots) & 1);
+        // S_j goes where P_j-1 was: PV_j-1, whose commit released V_j-1's slot, has read it
+        if (alive && j > 0) alive = wait(&bars[kEmpty + (vi - 2) % kSlots], ((vi - 2) / kSlots) & 1);
+        if (!alive) break;
+        tc_fence_after();
+        const uint32_t kb = k_lo + uint32_t(ks * (kTileBytes >> 4));
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_ts(tmem + kSCol, tmem + kk * 8, kb + uint32_t(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4), k_hi, kIdescS,
+                  kk > 0 ? 1u : 0u);
+        umma_commit(&bars[kSFull]);
+        umma_commit(&bars[kEmpty + ks]);
+        alive = wait(&bars[kPFull], j & 1) && wait(&bars[kFull + vs], (vi / kSlots) & 1);
+        if (!alive) break;
+        tc_fence_after();
+        const uint32_t vb = v_lo + uint32_t(vs * (kTileBytes >> 4));
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys: 8 packed columns of P, 2048 bytes of V rows
+          umma_ts(tmem + kOCol, tmem + kSCol + kk * 8, vb + kk * 128, v_hi, kIdescPV, (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&bars[kEmpty + vs]);
+      }
+      if (alive) umma_commit(&bars[kODone]);
+      // every MMA completes before TMEM is freed
+      umma_commit(&bars[kDrain]);
+      wait(&bars[kDrain], 0);
+    }
+  } else if ((warp & 3) < active) {
+    // ---------------------------------------------- softmax and epilogue
+    const int part = warp & 3;  // place among the warps with rows
+    const uint32_t lane_base = tmem + (uint32_t(part * 32) << 16);
+    {
+      uint32_t q[64];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const uint4 w = row_ok ? *reinterpret_cast<const uint4*>(p.q + item * 128 + c * 8) : make_uint4(0, 0, 0, 0);
+        q[4 * c] = w.x;
+        q[4 * c + 1] = w.y;
+        q[4 * c + 2] = w.z;
+        q[4 * c + 3] = w.w;
+      }
+      tmem_st32(lane_base, *reinterpret_cast<const uint32_t(*)[32]>(q));
+      tmem_st32(lane_base + 32, *reinterpret_cast<const uint32_t(*)[32]>(q + 32));
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kQReady]);
+    }
+    const unsigned long long* mask = p.mask + (long long)(begin + node) * p.mask_words;
+    const float sl2 = p.scale_log2;
+    float m_used = -INFINITY, l = 0.0f;
+    bool alive = true;
+    for (int j = 0; j < ntiles; ++j) {
+      const int key0 = (t0 + j) * kKeys;
+      const bool ok = page_ok(table[fd_bs.div(key0)], p.num_blocks);
+      const bool plain = ok && key0 + kKeys <= ctx;  // every row sees every key
+      unsigned long long seen = ~0ull;
+      if (!plain) {
+        const int real = ok ? min(kKeys, len - key0) : 0;  // keys of the sequence
+        const int t = key0 - ctx;
+        seen = mask_window(mask, p.mask_words, t);
+        if (t < 0) seen |= t > -64 ? ~0ull >> (64 + t) : ~0ull;  // context keys
+        seen &= real > 0 ? ~0ull >> (64 - real) : 0ull;
+        // V rows of the tile that may not meet a probability of 0
+        const int vi = 2 * j + 1, vs = vi % kSlots;
+        if (!wait_warp(&bars[kFull + vs], (vi / kSlots) & 1)) {
+          alive = false;
+          break;
+        }
+        const uint32_t vbase = sbase + vs * kTileBytes;
+        for (int key = part * 32 + lane; key < kKeys; key += 32 * active) {
+          if (key >= real) {
+            for (int c = 0; c < 8; ++c) {
+              st_shared_zero16(vbase + key * 128 + c * 16);
+              st_shared_zero16(vbase + kHalf + key * 128 + c * 16);
+            }
+          } else if (key + t >= 0) {
+            uint4* row = reinterpret_cast<uint4*>(smem_raw + kHeadBytes + vs * kTileBytes + key * 128);
+            for (int c = 0; c < 16; ++c) {  // (c + lane) & 7: the lanes' rows are a bank row apart
+              uint4* at = row + (c >> 3) * (kHalf / 16) + ((c + lane) & 7);
+              uint4 w = *at;
+              const uint32_t x = nonfinite_halves(w.x), y = nonfinite_halves(w.y), z = nonfinite_halves(w.z),
+                             u = nonfinite_halves(w.w);
+              if (x | y | z | u) {
+                *at = make_uint4(w.x & ~x, w.y & ~y, w.z & ~z, w.w & ~u);
+                *bad_v = 1;
+              }
+            }
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      if (!wait_warp(&bars[kSFull], j & 1)) {
+        alive = false;
+        break;
+      }
+      tc_fence_after();
+      float s[64];
+      {
+        uint32_t a0[32], a1[32];
+        tmem_ld32(lane_base + kSCol, a0);
+        tmem_ld32(lane_base + kSCol + 32, a1);
+        tmem_ld_wait();
+        reg_fence(a0);
+        reg_fence(a1);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          s[c] = __uint_as_float(a0[c]);
+          s[32 + c] = __uint_as_float(a1[c]);
+        }
+      }
+      if (!plain) {
+        const uint32_t lo = uint32_t(seen), hi = uint32_t(seen >> 32);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          if (!(lo >> c & 1u)) s[c] = -INFINITY;
+          if (!(hi >> c & 1u)) s[32 + c] = -INFINITY;
+        }
+      }
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c < 60; c += 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], s[c + i], s[c + 4 + i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], s[60 + i]);
+      const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+      // The maximum in use moves only when the row's grew by more than 2^8 (or with its first key): O is seldom
+      // rescaled, and P <= 2^8 divides out at the end.
+      float alpha = 1.0f;
+      if (m_tile > m_used + kRescaleLog2 || (m_used == -INFINITY && m_tile > -INFINITY)) {
+        alpha = fast_exp2(m_used - m_tile);  // 0 with the first key
+        m_used = m_tile;
+      }
+      const float nm = m_used == -INFINITY ? 0.0f : -m_used;
+      float sum[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+      uint32_t pk[32];
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        fma2(s[c], s[c + 1], s[c], s[c + 1], sl2, sl2, nm, nm);
+        s[c] = fast_exp2(s[c]);
+        s[c + 1] = fast_exp2(s[c + 1]);
+        const int k = (c >> 1) & 3;
+        add2(sum[2 * k], sum[2 * k + 1], sum[2 * k], sum[2 * k + 1], s[c], s[c + 1]);
+        // BF16 for the tensor core (V's type): half a step of each probability. The sum keeps their FP32 values.
+        pk[c >> 1] = pack_bf16x2(s[c], s[c + 1]);
+      }
+      tmem_st32(lane_base + kSCol, pk);
+      l = l * alpha + (((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7])));
+      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          uint32_t o[32];
+          tmem_ld32(lane_base + kOCol + 32 * h, o);
+          tmem_ld_wait();
+          reg_fence(o);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+          tmem_st32(lane_base + kOCol + 32 * h, o);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kPFull]);
+    }
+    if (alive && wait_warp(&bars[kODone], 0)) {
+      tc_fence_after();
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // NaN stays NaN
+      const float lse = l == 0.0f ? -INFINITY : (m_used + fast_log2(l)) * kLn2;
+      const bool mend = *reinterpret_cast<volatile int*>(bad_v) != 0;
+      for (int h = 0; h < 4; ++h) {
+        uint32_t o[32];
+        tmem_ld32(lane_base + kOCol + 32 * h, o);
+        tmem_ld_wait();
+        reg_fence(o);
+        float f[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) f[c] = __uint_as_float(o[c]) * inv;
+        if (mend && row_ok) {  // what the tree keys' V rows held beside numbers
+          for (int t = max(0, t0 * kKeys - ctx); t < min(n, (t0 + ntiles) * kKeys - ctx); ++t) {
+            if (!(mask_window(mask, p.mask_words, t) & 1)) continue;
+            const int page = table[fd_bs.div(ctx + t)];
+            if (!page_ok(page, p.num_blocks)) continue;
+            const __nv_bfloat16* row =
+                vcache + (((long long)page * p.block_size + (ctx + t - fd_bs.div(ctx + t) * p.block_size)) * p.kvh +
+                          kvhead) * 128 + 32 * h;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              const float x = __bfloat162float(row[c]);
+              if (!isfinite(x)) f[c] += x;
+            }
+          }
+        }
+        if (row_ok && p.num_splits == 1) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 8)
+            *reinterpret_cast<uint4*>(p.out + item * 128 + 32 * h + c) =
+                make_uint4(pack_bf16x2(f[c], f[c + 1]), pack_bf16x2(f[c + 2], f[c + 3]),
+                           pack_bf16x2(f[c + 4], f[c + 5]), pack_bf16x2(f[c + 6], f[c + 7]));
+        } else if (row_ok) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            *reinterpret_cast<float4*>(p.out_accum + partial * 128 + 32 * h + c) =
+                make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
+        }
+      }
+      if (row_ok) {
+        if (p.num_splits > 1)
+          p.lse_accum[partial] = lse;
+        else if (p.lse)
+          p.lse[item] = lse;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// Joins the splits of each (node, head): W warps share one (combine.cuh).
+template <int W>
+__global__ void __launch_bounds__(combine_detail::kCombineThreads)
+    tree_combine_kernel(const TreeParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % W;
+  const long long item = (long long)blockIdx.x * (combine_detail::kCombineThreads / 32 / W) + warp / W;
+  const long long stride = (long long)p.total_q * p.qh;
+  // rows behind the last sequence have no partials and keep what they hold
+  const bool live = item < (long long)min(p.cu_q[p.batch], p.total_q) * p.qh;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float total = 0.0f, mx = -INFINITY;
+  bool nan = false;
+  if (live) {
+    combine_detail::combine_share<W>(p.lse_accum, p.out_accum, item, stride, p.num_splits, sub, lane, acc, total, mx);
+    for (int s = lane; s < p.num_splits; s += 32) nan |= isnan(p.lse_accum[s * stride + item]);
+    nan = __any_sync(0xffffffffu, nan);
+  }
+  combine_detail::combine_gather_shares<W>(acc, total, warp, lane, sub);
+  if (!live || sub != 0) return;
+  // a maximum over splits passes over NaN: a NaN score's row is NaN throughout
+  const float inv = nan ? NAN : (total == 0.0f ? 0.0f : 1.0f / total);
+  uint2 packed;
+  packed.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+  packed.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(p.out + item * 128 + lane * 4) = packed;
+  if (lane == 0 && p.lse) p.lse[item] = nan ? NAN : (total == 0.0f ? -INFINITY : mx + __logf(total));
 }
 
 }  // namespace tree_detail
 
 cudaError_t launch_tree(const TreeParams& p, const void* k, const void* v, cudaStream_t stream) {
   using namespace tree_detail;
-  const dim3 grid(unsigned((p.max_q * p.qh + kWarps - 1) / kWarps), unsigned(p.batch));
-  tree_kernel<<<grid, kWarps * 32, 0, stream>>>(p, static_cast<const __nv_bfloat16*>(k),
-                                                static_cast<const __nv_bfloat16*>(v));
-  return cudaGetLastError();
+  CUtensorMap kmap, vmap;
+  {
+    const uint64_t dims[3] = {128, uint64_t(p.kvh), uint64_t(p.num_blocks) * uint64_t(p.block_size)};
+    const uint64_t strides[2] = {256, uint64_t(p.kvh) * 256};
+    const uint32_t box[3] = {64, 1, uint32_t(kKeys)};
+    if (make_map_3d(k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, &kmap)) return cudaErrorInvalidValue;
+    if (make_map_3d(v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, &vmap)) return cudaErrorInvalidValue;
+  }
+  static unsigned configured[kContextSlots] = {};
+  cudaError_t e = once_per_context(configured, [] {
+    cudaError_t r = cudaFuncSetAttribute(tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (r != cudaSuccess) return r;
+    return cudaFuncSetAttribute(tree_kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                cudaSharedmemCarveoutMaxShared);
+  });
+  if (e != cudaSuccess) return e;
+  const int group = p.qh / p.kvh;
+  const int row_tiles = (p.max_q * group + kRows - 1) / kRows;
+  const long long grid = (long long)p.batch * p.kvh * p.num_splits * row_tiles;
+  if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+  // Programmatic dependents: launched while the kernel before them ends; they wait for it before any global access.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, tree_kernel, p, FastDiv::make(group), FastDiv::make(p.block_size), row_tiles,
+                         static_cast<const __nv_bfloat16*>(v), kmap, vmap);
+  if (e != cudaSuccess || p.num_splits == 1) return e;
+  const int warps = combine_detail::combine_warps(p.num_splits);
+  const long long items = (long long)p.total_q * p.qh, per = combine_detail::kCombineThreads / 32 / warps;
+  cfg.gridDim = dim3(unsigned((items + per - 1) / per));
+  cfg.blockDim = dim3(combine_detail::kCombineThreads);
+  cfg.dynamicSmemBytes = 0;
+  switch (warps) {
+    case 1: return cudaLaunchKernelEx(&cfg, tree_combine_kernel<1>, p);
+    case 2: return cudaLaunchKernelEx(&cfg, tree_combine_kernel<2>, p);
+    case 4: return cudaLaunchKernelEx(&cfg, tree_combine_kernel<4>, p);
+    default: return cudaLaunchKernelEx(&cfg, tree_combine_kernel<8>, p);
+  }
 }
 
 }  // namespace nvb
@@ -79,7 +514,13 @@ int nvb_tree_num_splits(int batch, int max_q, int q_heads, int kv_heads, int max
   if (batch <= 0 || max_q <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || max_k <= 0 ||
       num_sms <= 0 || num_sms > 1024)
     return 0;
-  return 1;
+  const long long tiles = ((long long)max_q * (q_heads / kv_heads) + 127) / 128;  // row tiles of a kv head
+  const long long work = (long long)batch * kv_heads * tiles;
+  long long splits = 2LL * num_sms / work;             // two resident CTAs an SM
+  const long long by_len = (max_k + 255) / 256;        // at least 256 keys a split
+  if (splits > by_len) splits = by_len;
+  if (splits > 128) splits = 128;
+  return splits < 1 ? 1 : int(splits);
 }
 
 int nvb_paged_tree_fwd(void* stream, const void* q, const void* k, const void* v, void* out, const int* cu_q,
