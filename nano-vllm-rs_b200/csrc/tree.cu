@@ -14,29 +14,33 @@
 // r % G), so every K/V tile serves all nodes and heads of the group. Per tile
 // of 64 keys
 //
-//   S = Q K^T   tcgen05.mma M=128 N=64 K=128, Q from TMEM, K from shared memory
+//   S = Q K^T   tcgen05.mma M=128 N=64 K=128, Q and K from shared memory
 //   P = exp2(S * scale * log2 e - m), one thread a row, written back over S
 //   O += P V    tcgen05.mma M=128 N=128 K=64, P from TMEM, V from shared memory
 //
 // What bounds it: HBM for trees of up to 128 rows, each K/V byte read once. A
 // tile is 32 KB of K and V, 740 ns of an SM's share of HBM bandwidth (~1,350
-// cycles); its MMAs take 512 cycles and its 128 x 64 exponentials 512 of the
-// MUFU unit. Its steps follow each other, so two CTAs share an SM (256 TMEM
-// columns each: Q 64, S/P 64, O 128) and one's softmax runs beside the other's
-// MMAs. Keeping Q in TMEM leaves the shared memory to the ring of K and V
-// tiles, loaded by TMA in the order K0 V0 K1 V1 ...
+// cycles); its MMAs take ~640 cycles (S reads 48 KB of operands, at 128 bytes
+// a cycle) and its 128 x 64 exponentials 512 of the MUFU unit. S has two
+// buffers, so S_j+1 is computed while the rows work on S_j, and two CTAs share
+// an SM (256 TMEM columns each: S/P twice 64, O 128).
 //
-// Roles: warp 0 loads, warp 1 owns TMEM and issues the MMAs, warps 2-5 hold
-// the rows (a warp whose 32 rows are all past the last node only waits). S_j
-// is issued once PV_j-1 has completed, so S_j's commit also says that O may be
-// rescaled, and the chain needs one barrier each way.
+// Roles: warp 0 loads K and V tiles by TMA into one ring in the order of their
+// use (K0 K1 V0 K2 V1 ...), warp 1 owns TMEM and issues the MMAs, warps 2-5
+// hold the rows (a warp whose 32 rows are all past the last node only waits).
+//
+// Split keys: the CTAs of a cluster take equal ranges of a sequence's tiles.
+// At the end each leaves its rows of O, their maxima and sums in its shared
+// memory, and each joins every C-th row from all of them (distributed shared
+// memory), so a launch of up to 8 splits writes no partials and needs no
+// second kernel. More splits (few sequences, long contexts) are several
+// clusters a sequence, whose joined rows go through lse_accum / out_accum.
 //
 // Keys that a node does not see get probability 0; their V rows must not hold
 // infinities or NaN, as 0 times those is not 0. V rows of keys that nobody
 // sees (behind the sequence, bad pages) are zeroed in shared memory. A tree
 // key may be seen by some rows and not by others: its non-finite elements are
 // zeroed too, and added at the end to the rows that see the key.
-#include "combine.cuh"
 #include "prefill_common.cuh"
 
 namespace nvb {
@@ -49,24 +53,58 @@ constexpr int kRows = 128;              // rows of a CTA (TMEM lanes)
 constexpr int kKeys = 64;               // keys of a tile
 constexpr int kHalf = kKeys * 128;      // 64 rows x 64 BF16 (one swizzled half)
 constexpr int kTileBytes = 2 * kHalf;   // K or V tile 64 x 128 BF16
-constexpr int kSlots = 7;               // ring slots shared by K and V tiles
+constexpr int kQHalf = kRows * 128;     // Q: 128 rows x 64 BF16, twice
+constexpr int kSlots = 5;               // ring slots shared by K and V tiles
 constexpr int kThreads = 192;
+constexpr int kMaxCluster = 8;          // CTAs that join through shared memory
 constexpr int kTmemCols = 256;
-constexpr int kSCol = 64, kOCol = 128;  // Q at 0
+constexpr int kOCol = 128;              // S/P buffers at 0 and 64
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kRescaleLog2 = 8.0f;    // the maximum in use moves when it grew by 2^8 (P <= 2^8)
 
-enum Bar { kFull = 0, kEmpty = kFull + kSlots, kQReady = kEmpty + kSlots, kSFull, kPFull, kODone, kDrain, kNumBars };
+// kSFull, kPFull: one per S buffer. A warp may be a tile ahead of another one,
+// so the arrivals of two tiles in a row must not meet in one barrier.
+enum Bar { kFull = 0, kEmpty = kFull + kSlots, kQReady = kEmpty + kSlots, kSFull, kPFull = kSFull + 2,
+           kPVDone = kPFull + 2, kODone, kDrain, kNumBars };
 constexpr int kTmemSlotOff = kNumBars * 8;
 constexpr int kFlagOff = kTmemSlotOff + 4;
+constexpr int kSumRow = 132 * 4;  // bytes of a row of O in the ring at the join: 4 banks apart from the next
 constexpr int kHeadBytes = 1024;  // tiles start at the next 1 KB boundary
+constexpr int kStatsOff = kHeadBytes;  // float2 [128] where Q was: a row's maximum in use and sum, for the join
 static_assert(kFlagOff + 4 <= kHeadBytes, "barrier block must fit below the first 1 KB boundary");
-constexpr int kSmemBytes = kHeadBytes + kSlots * kTileBytes;  // two CTAs an SM: at most 113 KB each
+static_assert(kRows * kSumRow <= kSlots * kTileBytes, "the ring holds the rows of O at the join");
+constexpr int kRingOff = kHeadBytes + 2 * kQHalf;
+constexpr int kSmemBytes = kRingOff + kSlots * kTileBytes;  // two CTAs an SM: at most 113 KB each
 
-// kind::f16, FP32 accumulate, BF16 A (from TMEM) and B, M = 128.
+// Place of tile j's K and V (of n tiles) in the order of the loads.
+__device__ __forceinline__ int k_place(int j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ int v_place(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
+
+// kind::f16, FP32 accumulate, BF16 A and B, M = 128, A K-major (Q) or from TMEM (P).
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
 constexpr uint32_t kIdescS = kIdesc | ((uint32_t(kKeys) >> 3) << 17);       // B K-major (keys)
 constexpr uint32_t kIdescPV = kIdesc | ((128u >> 3) << 17) | (1u << 16);    // B MN-major (dims contiguous)
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+// Every thread of every CTA of the cluster; orders their shared memory accesses.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
   return mbar_wait(bar, parity, kErrTreeWait);
@@ -100,12 +138,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t raw_addr = smem_addr(smem_raw), sbase = raw_addr + kHeadBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // Row tiles of one key range are neighbours: they read its K and V together.
+  // Splits are neighbours (a cluster's CTAs among them), then the row tiles, which read the same K and V.
   int cta = blockIdx.x;
-  const int tile = cta % row_tiles;
-  cta /= row_tiles;
   const int split = cta % p.num_splits;
   cta /= p.num_splits;
+  const int tile = cta % row_tiles;
+  cta /= row_tiles;
   const int kvhead = cta % p.kvh, b = cta / p.kvh;
   const int group = p.qh / p.kvh;
 
@@ -113,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int begin = p.cu_q[b], n = min(p.cu_q[b + 1], p.total_q) - begin;
   const int row0 = tile * kRows, rows = min(n, p.max_q) * group - row0;
-  if (begin < 0 || rows <= 0) return;
+  if (begin < 0 || rows <= 0) return;  // all of a cluster
   const int len = p.kv_lens[b], ctx = len - n;
   const bool valid = ctx >= 0 && (long long)len <= (long long)p.table_stride * p.block_size;
   const int tiles_total = valid ? (len + kKeys - 1) / kKeys : 0;
@@ -123,22 +161,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   // This thread's row (warps 2-5): its TMEM lane, node and output place.
   const int r = (warp & 3) * 32 + lane;
   const bool row_ok = warp >= 2 && r < rows;
-  const int node = fd_group.div(row_ok ? row0 + r : 0), head = kvhead * group + (row0 + r - node * group);
-  const long long item = (long long)(begin + node) * p.qh + head;  // of [total_q, qh]
-  const long long partial = (long long)split * p.total_q * p.qh + item;
-
-  if (ntiles == 0 || (sbase & 1023u) != 0) {
-    if (ntiles != 0 && threadIdx.x == 0) record_error(kErrPrefillAlign);
-    if (row_ok) {
-      if (p.num_splits > 1) {
-        p.lse_accum[partial] = -INFINITY;  // the combine reads no output of such a split
-      } else {
-        for (int d = 0; d < 128; d += 8) *reinterpret_cast<uint4*>(p.out + item * 128 + d) = make_uint4(0, 0, 0, 0);
-        if (p.lse) p.lse[item] = -INFINITY;
-      }
-    }
-    return;
-  }
+  const int node = fd_group.div(row_ok ? row0 + r : 0);
+  const bool work = ntiles > 0 && (sbase & 1023u) == 0;
+  if (ntiles > 0 && !work && threadIdx.x == 0) record_error(kErrPrefillAlign);
 
   const int active = (min(rows, kRows) + 31) / 32;  // warps with rows
   if (threadIdx.x == 0) {
@@ -147,14 +172,17 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(&bars[kEmpty + s], 1);
     }
     mbar_init(&bars[kQReady], active);
-    mbar_init(&bars[kSFull], 1);
-    mbar_init(&bars[kPFull], active);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars[kSFull + s], 1);
+      mbar_init(&bars[kPFull + s], active);
+    }
+    mbar_init(&bars[kPVDone], 1);
     mbar_init(&bars[kODone], 1);
     mbar_init(&bars[kDrain], 1);
     *bad_v = 0;
     fence_barrier_init();
   }
-  if (warp == 1) {
+  if (work && warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                  "r"(kTmemCols)
                  : "memory");
@@ -166,20 +194,25 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem = *tmem_slot;
   const int* table = p.block_table + (long long)b * p.table_stride;
 
-  if (warp == 0) {
+  float2* stats = reinterpret_cast<float2*>(smem_raw + kStatsOff);
+  if (!work) {
+    if (threadIdx.x < kRows) stats[threadIdx.x] = make_float2(-INFINITY, 0.0f);
+  } else if (warp == 0) {
     // ---------------------------------------------------------- producer
     if (lane == 0) {
       tma_prefetch_desc(&kmap);
       tma_prefetch_desc(&vmap);
       int issued = 0;
       for (int i = 0; i < 2 * ntiles; ++i) {
-        const int key0 = (t0 + (i >> 1)) * kKeys, logical = fd_bs.div(key0), slot = i % kSlots;
+        const bool is_v = i > 0 && ((i & 1) == 0 || i == 2 * ntiles - 1);
+        const int j = i == 0 ? 0 : (i == 2 * ntiles - 1 ? ntiles - 1 : (is_v ? i / 2 - 1 : (i + 1) / 2));
+        const int key0 = (t0 + j) * kKeys, logical = fd_bs.div(key0), slot = i % kSlots;
         const int page = table[logical];
         // released by the MMA that read the slot's last load: S of a K tile, PV of a V tile
         if (i >= kSlots && !wait(&bars[kEmpty + slot], ((i / kSlots) + 1) & 1)) break;
         if (page_ok(page, p.num_blocks)) {
-          const CUtensorMap* map = (i & 1) ? &vmap : &kmap;
-          unsigned char* dst = smem_raw + kHeadBytes + slot * kTileBytes;
+          const CUtensorMap* map = is_v ? &vmap : &kmap;
+          unsigned char* dst = smem_raw + kRingOff + slot * kTileBytes;
           const int trow = page * p.block_size + (key0 - logical * p.block_size);
           mbar_arrive_expect_tx(&bars[kFull + slot], kTileBytes);
           tma_load_3d(dst, map, &bars[kFull + slot], 0, kvhead, trow);
@@ -196,30 +229,39 @@ __global__ void __launch_bounds__(kThreads, 2)
   } else if (warp == 1) {
     // -------------------------------------------------------- MMA issuer
     if (lane == 0) {
-      const uint64_t kd = sw128_desc(sbase, 16, 1024), vd = sw128_desc(sbase, kHalf, 1024);
-      const uint32_t k_lo = uint32_t(kd), k_hi = uint32_t(kd >> 32), v_lo = uint32_t(vd), v_hi = uint32_t(vd >> 32);
+      const uint32_t ring = raw_addr + kRingOff;
+      const uint64_t qd = sw128_desc(sbase, 16, 1024), kd = sw128_desc(ring, 16, 1024),
+                     vd = sw128_desc(ring, kHalf, 1024);
+      const uint32_t q_lo = uint32_t(qd), q_hi = uint32_t(qd >> 32), k_lo = uint32_t(kd), k_hi = uint32_t(kd >> 32),
+                     v_lo = uint32_t(vd), v_hi = uint32_t(vd >> 32);
       bool alive = wait(&bars[kQReady], 0);
-      for (int j = 0; j < ntiles && alive; ++j) {
-        const int ki = 2 * j, ks = ki % kSlots, vi = 2 * j + 1, vs = vi % kSlots;
-        alive = wait(&bars[kFull + ks], (ki / kSlots) & 1);
-        // S_j goes where P_j-1 was: PV_j-1, whose commit released V_j-1's slot, has read it
-        if (alive && j > 0) alive = wait(&bars[kEmpty + (vi - 2) % kSlots], ((vi - 2) / kSlots) & 1);
-        if (!alive) break;
-        tc_fence_after();
-        const uint32_t kb = k_lo + uint32_t(ks * (kTileBytes >> 4));
+      for (int j = -1; j < ntiles && alive; ++j) {
+        if (j + 1 < ntiles) {  // S_j+1, beside the rows' work on S_j
+          const int ki = k_place(j + 1), ks = ki % kSlots, buf = (j + 1) & 1;
+          alive = wait(&bars[kFull + ks], (ki / kSlots) & 1);
+          // its buffer held P_j-1: PV_j-1 must have read it
+          if (alive && j >= 1) alive = wait(&bars[kPVDone], (j - 1) & 1);
+          if (!alive) break;
+          tc_fence_after();
+          const uint32_t kb = k_lo + uint32_t(ks * (kTileBytes >> 4));
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_ts(tmem + kSCol, tmem + kk * 8, kb + uint32_t(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4), k_hi, kIdescS,
-                  kk > 0 ? 1u : 0u);
-        umma_commit(&bars[kSFull]);
-        umma_commit(&bars[kEmpty + ks]);
-        alive = wait(&bars[kPFull], j & 1) && wait(&bars[kFull + vs], (vi / kSlots) & 1);
+          for (int kk = 0; kk < 8; ++kk)
+            umma_ss(tmem + buf * kKeys, q_lo + uint32_t(((kk >> 2) * kQHalf + (kk & 3) * 32) >> 4), q_hi,
+                    kb + uint32_t(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4), k_hi, kIdescS, kk > 0 ? 1u : 0u);
+          umma_commit(&bars[kSFull + buf]);
+          umma_commit(&bars[kEmpty + ks]);
+        }
+        if (j < 0) continue;
+        const int vi = v_place(j, ntiles), vs = vi % kSlots, buf = j & 1;
+        alive = wait(&bars[kPFull + buf], (j >> 1) & 1) && wait(&bars[kFull + vs], (vi / kSlots) & 1);
         if (!alive) break;
         tc_fence_after();
         const uint32_t vb = v_lo + uint32_t(vs * (kTileBytes >> 4));
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys: 8 packed columns of P, 2048 bytes of V rows
-          umma_ts(tmem + kOCol, tmem + kSCol + kk * 8, vb + kk * 128, v_hi, kIdescPV, (j > 0 || kk > 0) ? 1u : 0u);
+          umma_ts(tmem + kOCol, tmem + buf * kKeys + kk * 8, vb + kk * 128, v_hi, kIdescPV,
+                  (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&bars[kPVDone]);
         umma_commit(&bars[kEmpty + vs]);
       }
       if (alive) umma_commit(&bars[kODone]);
@@ -228,23 +270,21 @@ __global__ void __launch_bounds__(kThreads, 2)
       wait(&bars[kDrain], 0);
     }
   } else if ((warp & 3) < active) {
-    // ---------------------------------------------- softmax and epilogue
+    // ------------------------------------------------------------ softmax
     const int part = warp & 3;  // place among the warps with rows
     const uint32_t lane_base = tmem + (uint32_t(part * 32) << 16);
     {
-      uint32_t q[64];
+      // this row of Q, K-major and 128-byte swizzled (rows past the last node stay as they are: their lanes' results
+      // are dropped)
+      if (row_ok) {
+        const int head = kvhead * group + (row0 + r - node * group);
+        const __nv_bfloat16* q = p.q + ((long long)(begin + node) * p.qh + head) * 128;
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const uint4 w = row_ok ? *reinterpret_cast<const uint4*>(p.q + item * 128 + c * 8) : make_uint4(0, 0, 0, 0);
-        q[4 * c] = w.x;
-        q[4 * c + 1] = w.y;
-        q[4 * c + 2] = w.z;
-        q[4 * c + 3] = w.w;
+        for (int c = 0; c < 16; ++c)
+          *reinterpret_cast<uint4*>(smem_raw + kHeadBytes + (c >> 3) * kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+              *reinterpret_cast<const uint4*>(q + c * 8);
       }
-      tmem_st32(lane_base, *reinterpret_cast<const uint32_t(*)[32]>(q));
-      tmem_st32(lane_base + 32, *reinterpret_cast<const uint32_t(*)[32]>(q + 32));
-      tmem_st_wait();
-      tc_fence_before();
+      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[kQReady]);
     }
@@ -264,12 +304,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (t < 0) seen |= t > -64 ? ~0ull >> (64 + t) : ~0ull;  // context keys
         seen &= real > 0 ? ~0ull >> (64 - real) : 0ull;
         // V rows of the tile that may not meet a probability of 0
-        const int vi = 2 * j + 1, vs = vi % kSlots;
+        const int vi = v_place(j, ntiles), vs = vi % kSlots;
         if (!wait_warp(&bars[kFull + vs], (vi / kSlots) & 1)) {
           alive = false;
           break;
         }
-        const uint32_t vbase = sbase + vs * kTileBytes;
+        const uint32_t vbase = raw_addr + kRingOff + vs * kTileBytes;
         for (int key = part * 32 + lane; key < kKeys; key += 32 * active) {
           if (key >= real) {
             for (int c = 0; c < 8; ++c) {
@@ -277,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               st_shared_zero16(vbase + kHalf + key * 128 + c * 16);
             }
           } else if (key + t >= 0) {
-            uint4* row = reinterpret_cast<uint4*>(smem_raw + kHeadBytes + vs * kTileBytes + key * 128);
+            uint4* row = reinterpret_cast<uint4*>(smem_raw + kRingOff + vs * kTileBytes + key * 128);
             for (int c = 0; c < 16; ++c) {  // (c + lane) & 7: the lanes' rows are a bank row apart
               uint4* at = row + (c >> 3) * (kHalf / 16) + ((c + lane) & 7);
               uint4 w = *at;
@@ -292,16 +332,17 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         fence_proxy_async_smem();
       }
-      if (!wait_warp(&bars[kSFull], j & 1)) {
+      if (!wait_warp(&bars[kSFull + (j & 1)], (j >> 1) & 1)) {
         alive = false;
         break;
       }
       tc_fence_after();
+      const uint32_t scol = lane_base + (j & 1) * kKeys;
       float s[64];
       {
         uint32_t a0[32], a1[32];
-        tmem_ld32(lane_base + kSCol, a0);
-        tmem_ld32(lane_base + kSCol + 32, a1);
+        tmem_ld32(scol, a0);
+        tmem_ld32(scol + 32, a1);
         tmem_ld_wait();
         reg_fence(a0);
         reg_fence(a1);
@@ -349,9 +390,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         // BF16 for the tensor core (V's type): half a step of each probability. The sum keeps their FP32 values.
         pk[c >> 1] = pack_bf16x2(s[c], s[c + 1]);
       }
-      tmem_st32(lane_base + kSCol, pk);
+      tmem_st32(scol, pk);
       l = l * alpha + (((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7])));
       if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+        // PV_j-1 must be done with O (PV_j waits for this P; PV_j-2 completed before S_j was issued)
+        if (!wait_warp(&bars[kPVDone], (j - 1) & 1)) {
+          alive = false;
+          break;
+        }
+        tc_fence_after();
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
           uint32_t o[32];
@@ -366,12 +413,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kPFull]);
+      if (lane == 0) mbar_arrive(&bars[kPFull + (j & 1)]);
     }
-    if (alive && wait_warp(&bars[kODone], 0)) {
+    // A barrier of its own: behind the last P, kPVDone may pass two phases before a slow warp looks at it.
+    alive = alive && wait_warp(&bars[kODone], 0);
+    stats[r] = alive ? make_float2(m_used, l) : make_float2(-INFINITY, 0.0f);
+    if (alive) {
       tc_fence_after();
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // NaN stays NaN
-      const float lse = l == 0.0f ? -INFINITY : (m_used + fast_log2(l)) * kLn2;
       const bool mend = *reinterpret_cast<volatile int*>(bad_v) != 0;
       for (int h = 0; h < 4; ++h) {
         uint32_t o[32];
@@ -380,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         reg_fence(o);
         float f[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) f[c] = __uint_as_float(o[c]) * inv;
+        for (int c = 0; c < 32; ++c) f[c] = __uint_as_float(o[c]);
         if (mend && row_ok) {  // what the tree keys' V rows held beside numbers
           for (int t = max(0, t0 * kKeys - ctx); t < min(n, (t0 + ntiles) * kKeys - ctx); ++t) {
             if (!(mask_window(mask, p.mask_words, t) & 1)) continue;
@@ -396,63 +444,140 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
         }
-        if (row_ok && p.num_splits == 1) {
+        // every copy into the ring has landed and been read
+        float4* dst = reinterpret_cast<float4*>(smem_raw + kRingOff + r * kSumRow + h * 128);
 #pragma unroll
-          for (int c = 0; c < 32; c += 8)
-            *reinterpret_cast<uint4*>(p.out + item * 128 + 32 * h + c) =
-                make_uint4(pack_bf16x2(f[c], f[c + 1]), pack_bf16x2(f[c + 2], f[c + 3]),
-                           pack_bf16x2(f[c + 4], f[c + 5]), pack_bf16x2(f[c + 6], f[c + 7]));
-        } else if (row_ok) {
-#pragma unroll
-          for (int c = 0; c < 32; c += 4)
-            *reinterpret_cast<float4*>(p.out_accum + partial * 128 + 32 * h + c) =
-                make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
-        }
-      }
-      if (row_ok) {
-        if (p.num_splits > 1)
-          p.lse_accum[partial] = lse;
-        else if (p.lse)
-          p.lse[item] = lse;
+        for (int c = 0; c < 32; c += 4) dst[c / 4] = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (work && warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
+
+  // ---------------------------------------------------------------- join
+  // A warp a row, a lane four dimensions: sum_s 2^(m_s - max) O_s over the
+  // cluster's CTAs s, divided by the same sum of their row sums.
+  cluster_sync();
+  {
+    const int size = int(cluster_size()), rank = int(cluster_rank());
+    const uint32_t stats_addr = raw_addr + kStatsOff, rows_addr = raw_addr + kRingOff;
+    for (int row = rank + size * warp; row < min(rows, kRows); row += size * (kThreads / 32)) {
+      float m = -INFINITY, sum = 0.0f;
+      if (lane < size)
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(m), "=f"(sum)
+                     : "r"(peer_addr(stats_addr + row * 8, lane)));
+      float mx = sum == 0.0f ? -INFINITY : m;
+#pragma unroll
+      for (int off = 4; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+      // a range without a seen key has no part; one whose scores are all NaN has no maximum, its sum is NaN
+      float w = sum == 0.0f ? 0.0f : (m == -INFINITY ? NAN : fast_exp2(m - mx));
+      float total = w * sum;
+      mx = __shfl_sync(0xffffffffu, mx, 0);  // lanes 0-7 agree
+#pragma unroll
+      for (int off = 4; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+      total = __shfl_sync(0xffffffffu, total, 0);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 v[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const float ws = __shfl_sync(0xffffffffu, w, s);
+        v[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s < size && ws != 0.0f)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w)
+                       : "r"(peer_addr(rows_addr + row * kSumRow + lane * 16, s)));
+      }
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const float ws = __shfl_sync(0xffffffffu, w, s);
+        if (s >= size || ws == 0.0f) continue;
+        acc.x = fmaf(ws, v[s].x, acc.x);
+        acc.y = fmaf(ws, v[s].y, acc.y);
+        acc.z = fmaf(ws, v[s].z, acc.z);
+        acc.w = fmaf(ws, v[s].w, acc.w);
+      }
+      const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // NaN stays NaN
+      const float lse = total == 0.0f ? -INFINITY : (mx + fast_log2(total)) * kLn2;
+      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      const int at = fd_group.div(row0 + row);
+      const long long item = (long long)(begin + at) * p.qh + kvhead * group + (row0 + row - at * group);
+      if (p.num_splits == size) {
+        *reinterpret_cast<uint2*>(p.out + item * 128 + lane * 4) =
+            make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+        if (lane == 0 && p.lse) p.lse[item] = lse;
+      } else {
+        const long long partial = (long long)(split / size) * p.total_q * p.qh + item;
+        *reinterpret_cast<float4*>(p.out_accum + partial * 128 + lane * 4) = acc;
+        if (lane == 0) p.lse_accum[partial] = lse;
+      }
+    }
+  }
+  cluster_sync();  // nobody leaves while its shared memory is read
 }
 
-// Joins the splits of each (node, head): W warps share one (combine.cuh).
-template <int W>
-__global__ void __launch_bounds__(combine_detail::kCombineThreads)
-    tree_combine_kernel(const TreeParams p) {
+// Joins the clusters' parts of each (node, head), a warp an item and a lane four
+// dimensions. The LSEs and rows of eight parts are loaded together and the
+// running maximum moves with them, so that an item costs one round trip to L2
+// for eight parts: what bounds it is the latency of that.
+constexpr int kCombineWarps = 4;
+constexpr int kCombineBatch = 8;
+
+__global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const TreeParams p, const int parts) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % W;
-  const long long item = (long long)blockIdx.x * (combine_detail::kCombineThreads / 32 / W) + warp / W;
+  const int lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
   const long long stride = (long long)p.total_q * p.qh;
+  if (item >= stride) return;
   // rows behind the last sequence have no partials and keep what they hold
-  const bool live = item < (long long)min(p.cu_q[p.batch], p.total_q) * p.qh;
+  const bool live = item < (long long)p.cu_q[p.batch] * p.qh;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float total = 0.0f, mx = -INFINITY;
-  bool nan = false;
-  if (live) {
-    combine_detail::combine_share<W>(p.lse_accum, p.out_accum, item, stride, p.num_splits, sub, lane, acc, total, mx);
-    for (int s = lane; s < p.num_splits; s += 32) nan |= isnan(p.lse_accum[s * stride + item]);
-    nan = __any_sync(0xffffffffu, nan);
+  for (int s0 = 0; s0 < parts; s0 += kCombineBatch) {
+    float ls[kCombineBatch];
+    float4 v[kCombineBatch];
+#pragma unroll
+    for (int u = 0; u < kCombineBatch; ++u) {
+      ls[u] = -INFINITY;
+      if (s0 + u < parts) {
+        ls[u] = p.lse_accum[(s0 + u) * stride + item];
+        v[u] = *reinterpret_cast<const float4*>(p.out_accum + ((s0 + u) * stride + item) * 128 + lane * 4);
+      }
+    }
+    float m = mx;
+#pragma unroll
+    for (int u = 0; u < kCombineBatch; ++u) m = fmaxf(m, ls[u]);
+    const float a = mx == m ? 1.0f : __expf(mx - m);  // 0 with the first split that saw a key
+    mx = m;
+    total *= a;
+    acc.x *= a;
+    acc.y *= a;
+    acc.z *= a;
+    acc.w *= a;
+#pragma unroll
+    for (int u = 0; u < kCombineBatch; ++u) {
+      if (ls[u] == -INFINITY) continue;  // saw no key: its row was not written
+      // a NaN score's split: the maximum passes over it, its row is NaN throughout
+      const float w = isnan(ls[u]) ? NAN : __expf(ls[u] - mx);
+      total += w;
+      acc.x = fmaf(w, v[u].x, acc.x);
+      acc.y = fmaf(w, v[u].y, acc.y);
+      acc.z = fmaf(w, v[u].z, acc.z);
+      acc.w = fmaf(w, v[u].w, acc.w);
+    }
   }
-  combine_detail::combine_gather_shares<W>(acc, total, warp, lane, sub);
-  if (!live || sub != 0) return;
-  // a maximum over splits passes over NaN: a NaN score's row is NaN throughout
-  const float inv = nan ? NAN : (total == 0.0f ? 0.0f : 1.0f / total);
+  if (!live) return;
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   uint2 packed;
   packed.x = pack_bf16x2(acc.x * inv, acc.y * inv);
   packed.y = pack_bf16x2(acc.z * inv, acc.w * inv);
   *reinterpret_cast<uint2*>(p.out + item * 128 + lane * 4) = packed;
-  if (lane == 0 && p.lse) p.lse[item] = nan ? NAN : (total == 0.0f ? -INFINITY : mx + __logf(total));
+  if (lane == 0 && p.lse) p.lse[item] = total == 0.0f ? -INFINITY : mx + __logf(total);
 }
 
 }  // namespace tree_detail
@@ -479,31 +604,34 @@ cudaError_t launch_tree(const TreeParams& p, const void* k, const void* v, cudaS
   const int row_tiles = (p.max_q * group + kRows - 1) / kRows;
   const long long grid = (long long)p.batch * p.kvh * p.num_splits * row_tiles;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+  // The largest cluster whose size divides the splits.
+  int cluster = 1;
+  for (int c = 2; c <= kMaxCluster; ++c)
+    if (p.num_splits % c == 0) cluster = c;
   // Programmatic dependents: launched while the kernel before them ends; they wait for it before any global access.
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(grid));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   e = cudaLaunchKernelEx(&cfg, tree_kernel, p, FastDiv::make(group), FastDiv::make(p.block_size), row_tiles,
                          static_cast<const __nv_bfloat16*>(v), kmap, vmap);
-  if (e != cudaSuccess || p.num_splits == 1) return e;
-  const int warps = combine_detail::combine_warps(p.num_splits);
-  const long long items = (long long)p.total_q * p.qh, per = combine_detail::kCombineThreads / 32 / warps;
-  cfg.gridDim = dim3(unsigned((items + per - 1) / per));
-  cfg.blockDim = dim3(combine_detail::kCombineThreads);
+  if (e != cudaSuccess || p.num_splits == cluster) return e;
+  const long long items = (long long)p.total_q * p.qh;
+  cfg.gridDim = dim3(unsigned((items + kCombineWarps - 1) / kCombineWarps));
+  cfg.blockDim = dim3(kCombineWarps * 32);
   cfg.dynamicSmemBytes = 0;
-  switch (warps) {
-    case 1: return cudaLaunchKernelEx(&cfg, tree_combine_kernel<1>, p);
-    case 2: return cudaLaunchKernelEx(&cfg, tree_combine_kernel<2>, p);
-    case 4: return cudaLaunchKernelEx(&cfg, tree_combine_kernel<4>, p);
-    default: return cudaLaunchKernelEx(&cfg, tree_combine_kernel<8>, p);
-  }
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, tree_combine_kernel, p, p.num_splits / cluster);
 }
 
 }  // namespace nvb
