@@ -64,15 +64,18 @@ constexpr float kRescaleLog2 = 8.0f;    // the maximum in use moves when it grew
 
 // kSFull, kPFull: one per S buffer. A warp may be a tile ahead of another one,
 // so the arrivals of two tiles in a row must not meet in one barrier.
-enum Bar { kFull = 0, kEmpty = kFull + kSlots, kQReady = kEmpty + kSlots, kSFull, kPFull = kSFull + 2,
+enum Bar { kFull = 0, kEmpty = kFull + kSlots, kSFull = kEmpty + kSlots, kPFull = kSFull + 2,
            kPVDone = kPFull + 2, kODone, kDrain, kNumBars };
 constexpr int kTmemSlotOff = kNumBars * 8;
 constexpr int kFlagOff = kTmemSlotOff + 4;
+constexpr int kOutRow = 272;      // bytes of a row of the output in the ring
 constexpr int kSumRow = 132 * 4;  // bytes of a row of O in the ring at the join: 4 banks apart from the next
 constexpr int kHeadBytes = 1024;  // tiles start at the next 1 KB boundary
 constexpr int kStatsOff = kHeadBytes;  // float2 [128] where Q was: a row's maximum in use and sum, for the join
+constexpr int kFactorOff = kStatsOff + kRows * 8;  // float [rows of a CTA][cluster]
+static_assert(kFactorOff + kRows * kMaxCluster * 4 <= kHeadBytes + 2 * kQHalf, "the join's tables fit where Q was");
 static_assert(kFlagOff + 4 <= kHeadBytes, "barrier block must fit below the first 1 KB boundary");
-static_assert(kRows * kSumRow <= kSlots * kTileBytes, "the ring holds the rows of O at the join");
+static_assert(kRows * kSumRow <= kSlots * kTileBytes && kOutRow <= kSumRow, "the ring holds the rows of O at the join");
 constexpr int kRingOff = kHeadBytes + 2 * kQHalf;
 constexpr int kSmemBytes = kRingOff + kSlots * kTileBytes;  // two CTAs an SM: at most 113 KB each
 
@@ -122,8 +125,13 @@ __device__ __forceinline__ unsigned long long mask_window(const unsigned long lo
   return (lo >> s) | (hi << (64 - s));
 }
 
-__device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {  // 0xffff in each BF16 that is inf or NaN
-  return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+// Whether a pair of BF16 holds an infinity or NaN: an exponent of all ones carries into the sign's place.
+__device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
+  return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) {  // such halves as 0
+  return w & ~(((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u));
 }
 
 __global__ void __launch_bounds__(kThreads, 2)
@@ -147,16 +155,34 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int kvhead = cta % p.kvh, b = cta / p.kvh;
   const int group = p.qh / p.kvh;
 
-  // The kernel before this one has completed, its writes are visible.
+  // Set-up that needs no input runs beside the end of the kernel before this one.
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&bars[kFull + s], 1);
+      mbar_init(&bars[kEmpty + s], 1);
+    }
+    for (int s = 0; s < 2; ++s) mbar_init(&bars[kSFull + s], 1);
+    mbar_init(&bars[kPVDone], 1);
+    mbar_init(&bars[kODone], 1);
+    mbar_init(&bars[kDrain], 1);
+    *bad_v = 0;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // That kernel has completed, its writes are visible.
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int begin = p.cu_q[b], n = min(p.cu_q[b + 1], p.total_q) - begin;
-  const int row0 = tile * kRows, rows = min(n, p.max_q) * group - row0;
-  if (begin < 0 || rows <= 0) return;  // all of a cluster
-  const int len = p.kv_lens[b], ctx = len - n;
+  const int begin = p.cu_q[b], next = p.cu_q[b + 1], len = p.kv_lens[b];
+  const int n = min(next, p.total_q) - begin, ctx = len - n;
+  const int row0 = tile * kRows, rows = begin < 0 ? 0 : min(n, p.max_q) * group - row0;  // none for all of a cluster
   const bool valid = ctx >= 0 && (long long)len <= (long long)p.table_stride * p.block_size;
   const int tiles_total = valid ? (len + kKeys - 1) / kKeys : 0;
   const int per_split = (tiles_total + p.num_splits - 1) / p.num_splits;
-  const int t0 = split * per_split, ntiles = max(0, min(t0 + per_split, tiles_total) - t0);
+  const int t0 = split * per_split, ntiles = rows > 0 ? max(0, min(t0 + per_split, tiles_total) - t0) : 0;
+  const int* table = p.block_table + (long long)b * p.table_stride;
 
   // This thread's row (warps 2-5): its TMEM lane, node and output place.
   const int r = (warp & 3) * 32 + lane;
@@ -167,32 +193,29 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   const int active = (min(rows, kRows) + 31) / 32;  // warps with rows
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSlots; ++s) {
-      mbar_init(&bars[kFull + s], 1);
-      mbar_init(&bars[kEmpty + s], 1);
-    }
-    mbar_init(&bars[kQReady], active);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars[kSFull + s], 1);
-      mbar_init(&bars[kPFull + s], active);
-    }
-    mbar_init(&bars[kPVDone], 1);
-    mbar_init(&bars[kODone], 1);
-    mbar_init(&bars[kDrain], 1);
-    *bad_v = 0;
+    for (int s = 0; s < 2; ++s) mbar_init(&bars[kPFull + s], max(active, 1));
     fence_barrier_init();
   }
-  if (work && warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  int page0 = -1;
+  if (work && threadIdx.x == 0) page0 = table[fd_bs.div(t0 * kKeys)];
+  if (work && row_ok) {
+    // this row of Q, K-major and 128-byte swizzled (rows past the last node stay as they are: their lanes' results
+    // are dropped)
+    const int head = kvhead * group + (row0 + r - node * group);
+    const __nv_bfloat16* q = p.q + ((long long)(begin + node) * p.qh + head) * 128;
+    uint4 w[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) w[c] = *reinterpret_cast<const uint4*>(q + c * 8);
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      *reinterpret_cast<uint4*>(smem_raw + kHeadBytes + (c >> 3) * kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+          w[c];
+    fence_proxy_async_smem();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int* table = p.block_table + (long long)b * p.table_stride;
 
   float2* stats = reinterpret_cast<float2*>(smem_raw + kStatsOff);
   if (!work) {
@@ -202,12 +225,15 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (lane == 0) {
       tma_prefetch_desc(&kmap);
       tma_prefetch_desc(&vmap);
-      int issued = 0;
+      int issued = 0, page = page0, last = fd_bs.div(t0 * kKeys);
       for (int i = 0; i < 2 * ntiles; ++i) {
         const bool is_v = i > 0 && ((i & 1) == 0 || i == 2 * ntiles - 1);
         const int j = i == 0 ? 0 : (i == 2 * ntiles - 1 ? ntiles - 1 : (is_v ? i / 2 - 1 : (i + 1) / 2));
         const int key0 = (t0 + j) * kKeys, logical = fd_bs.div(key0), slot = i % kSlots;
-        const int page = table[logical];
+        if (logical != last) {
+          page = table[logical];
+          last = logical;
+        }
         // released by the MMA that read the slot's last load: S of a K tile, PV of a V tile
         if (i >= kSlots && !wait(&bars[kEmpty + slot], ((i / kSlots) + 1) & 1)) break;
         if (page_ok(page, p.num_blocks)) {
@@ -234,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                      vd = sw128_desc(ring, kHalf, 1024);
       const uint32_t q_lo = uint32_t(qd), q_hi = uint32_t(qd >> 32), k_lo = uint32_t(kd), k_hi = uint32_t(kd >> 32),
                      v_lo = uint32_t(vd), v_hi = uint32_t(vd >> 32);
-      bool alive = wait(&bars[kQReady], 0);
+      bool alive = true;
       for (int j = -1; j < ntiles && alive; ++j) {
         if (j + 1 < ntiles) {  // S_j+1, beside the rows' work on S_j
           const int ki = k_place(j + 1), ks = ki % kSlots, buf = (j + 1) & 1;
@@ -273,21 +299,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     // ------------------------------------------------------------ softmax
     const int part = warp & 3;  // place among the warps with rows
     const uint32_t lane_base = tmem + (uint32_t(part * 32) << 16);
-    {
-      // this row of Q, K-major and 128-byte swizzled (rows past the last node stay as they are: their lanes' results
-      // are dropped)
-      if (row_ok) {
-        const int head = kvhead * group + (row0 + r - node * group);
-        const __nv_bfloat16* q = p.q + ((long long)(begin + node) * p.qh + head) * 128;
-#pragma unroll
-        for (int c = 0; c < 16; ++c)
-          *reinterpret_cast<uint4*>(smem_raw + kHeadBytes + (c >> 3) * kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
-              *reinterpret_cast<const uint4*>(q + c * 8);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kQReady]);
-    }
     const unsigned long long* mask = p.mask + (long long)(begin + node) * p.mask_words;
     const float sl2 = p.scale_log2;
     float m_used = -INFINITY, l = 0.0f;
@@ -296,41 +307,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int key0 = (t0 + j) * kKeys;
       const bool ok = page_ok(table[fd_bs.div(key0)], p.num_blocks);
       const bool plain = ok && key0 + kKeys <= ctx;  // every row sees every key
+      const int real = ok ? min(kKeys, len - key0) : 0;  // keys of the sequence
       unsigned long long seen = ~0ull;
       if (!plain) {
-        const int real = ok ? min(kKeys, len - key0) : 0;  // keys of the sequence
         const int t = key0 - ctx;
         seen = mask_window(mask, p.mask_words, t);
         if (t < 0) seen |= t > -64 ? ~0ull >> (64 + t) : ~0ull;  // context keys
         seen &= real > 0 ? ~0ull >> (64 - real) : 0ull;
-        // V rows of the tile that may not meet a probability of 0
-        const int vi = v_place(j, ntiles), vs = vi % kSlots;
-        if (!wait_warp(&bars[kFull + vs], (vi / kSlots) & 1)) {
-          alive = false;
-          break;
-        }
-        const uint32_t vbase = raw_addr + kRingOff + vs * kTileBytes;
-        for (int key = part * 32 + lane; key < kKeys; key += 32 * active) {
-          if (key >= real) {
-            for (int c = 0; c < 8; ++c) {
-              st_shared_zero16(vbase + key * 128 + c * 16);
-              st_shared_zero16(vbase + kHalf + key * 128 + c * 16);
-            }
-          } else if (key + t >= 0) {
-            uint4* row = reinterpret_cast<uint4*>(smem_raw + kRingOff + vs * kTileBytes + key * 128);
-            for (int c = 0; c < 16; ++c) {  // (c + lane) & 7: the lanes' rows are a bank row apart
-              uint4* at = row + (c >> 3) * (kHalf / 16) + ((c + lane) & 7);
-              uint4 w = *at;
-              const uint32_t x = nonfinite_halves(w.x), y = nonfinite_halves(w.y), z = nonfinite_halves(w.z),
-                             u = nonfinite_halves(w.w);
-              if (x | y | z | u) {
-                *at = make_uint4(w.x & ~x, w.y & ~y, w.z & ~z, w.w & ~u);
-                *bad_v = 1;
-              }
-            }
-          }
-        }
-        fence_proxy_async_smem();
       }
       if (!wait_warp(&bars[kSFull + (j & 1)], (j >> 1) & 1)) {
         alive = false;
@@ -370,11 +353,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
       // The maximum in use moves only when the row's grew by more than 2^8 (or with its first key): O is seldom
       // rescaled, and P <= 2^8 divides out at the end.
-      float alpha = 1.0f;
-      if (m_tile > m_used + kRescaleLog2 || (m_used == -INFINITY && m_tile > -INFINITY)) {
-        alpha = fast_exp2(m_used - m_tile);  // 0 with the first key
-        m_used = m_tile;
-      }
+      const bool grew = m_tile > m_used + kRescaleLog2;
+      const float alpha = grew ? fast_exp2(m_used - m_tile) : 1.0f;  // 0 with the first key
+      m_used = grew ? m_tile : m_used;
       const float nm = m_used == -INFINITY ? 0.0f : -m_used;
       float sum[8];
 #pragma unroll
@@ -410,6 +391,29 @@ __global__ void __launch_bounds__(kThreads, 2)
           tmem_st32(lane_base + kOCol + 32 * h, o);
         }
       }
+      if (!plain) {
+        // V rows of the tile that may not meet a probability of 0
+        const int vi = v_place(j, ntiles), vs = vi % kSlots;
+        if (!wait_warp(&bars[kFull + vs], (vi / kSlots) & 1)) {
+          alive = false;
+          break;
+        }
+        // 16-byte piece i of the tile's rows: the halves of a row are kHalf apart
+        unsigned char* vt = smem_raw + kRingOff + vs * kTileBytes;
+        auto piece = [&](int i) {
+          return reinterpret_cast<uint4*>(vt + ((i >> 3) & 1) * kHalf + (i >> 4) * 128 + (i & 7) * 16);
+        };
+        for (int i = 16 * real + part * 32 + lane; i < 16 * kKeys; i += 32 * active) *piece(i) = make_uint4(0, 0, 0, 0);
+        for (int i = 16 * max(0, ctx - key0) + part * 32 + lane; i < 16 * real; i += 32 * active) {
+          const uint4 w = *piece(i);
+          if (nonfinite(w.x) | nonfinite(w.y) | nonfinite(w.z) | nonfinite(w.w)) {
+            *piece(i) = make_uint4(finite_part(w.x), finite_part(w.y), finite_part(w.z), finite_part(w.w));
+            *bad_v = 1;
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      __syncwarp();  // the lanes of the loops above meet again before the warp-wide TMEM instructions
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -417,106 +421,154 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     // A barrier of its own: behind the last P, kPVDone may pass two phases before a slow warp looks at it.
     alive = alive && wait_warp(&bars[kODone], 0);
-    stats[r] = alive ? make_float2(m_used, l) : make_float2(-INFINITY, 0.0f);
-    if (alive) {
-      tc_fence_after();
-      const bool mend = *reinterpret_cast<volatile int*>(bad_v) != 0;
-      for (int h = 0; h < 4; ++h) {
-        uint32_t o[32];
-        tmem_ld32(lane_base + kOCol + 32 * h, o);
-        tmem_ld_wait();
-        reg_fence(o);
-        float f[32];
+    tc_fence_after();
+    const bool whole = p.num_splits == 1;  // no other range: this warp writes its rows itself
+    const float inv = !whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);  // NaN stays NaN
+    if (!whole) stats[r] = alive ? make_float2(m_used, l) : make_float2(-INFINITY, 0.0f);
+    const bool mend = *reinterpret_cast<volatile int*>(bad_v) != 0;
+    for (int h = 0; h < 4 && alive; ++h) {
+      uint32_t o[32];
+      tmem_ld32(lane_base + kOCol + 32 * h, o);
+      tmem_ld_wait();
+      reg_fence(o);
+      float f[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) f[c] = __uint_as_float(o[c]);
-        if (mend && row_ok) {  // what the tree keys' V rows held beside numbers
-          for (int t = max(0, t0 * kKeys - ctx); t < min(n, (t0 + ntiles) * kKeys - ctx); ++t) {
-            if (!(mask_window(mask, p.mask_words, t) & 1)) continue;
-            const int page = table[fd_bs.div(ctx + t)];
-            if (!page_ok(page, p.num_blocks)) continue;
-            const __nv_bfloat16* row =
-                vcache + (((long long)page * p.block_size + (ctx + t - fd_bs.div(ctx + t) * p.block_size)) * p.kvh +
-                          kvhead) * 128 + 32 * h;
+      for (int c = 0; c < 32; ++c) f[c] = __uint_as_float(o[c]) * inv;
+      if (mend && row_ok) {  // what the tree keys' V rows held beside numbers
+        for (int t = max(0, t0 * kKeys - ctx); t < min(n, (t0 + ntiles) * kKeys - ctx); ++t) {
+          if (!(mask_window(mask, p.mask_words, t) & 1)) continue;
+          const int page = table[fd_bs.div(ctx + t)];
+          if (!page_ok(page, p.num_blocks)) continue;
+          const __nv_bfloat16* row =
+              vcache + (((long long)page * p.block_size + (ctx + t - fd_bs.div(ctx + t) * p.block_size)) * p.kvh +
+                        kvhead) * 128 + 32 * h;
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const float x = __bfloat162float(row[c]);
-              if (!isfinite(x)) f[c] += x;
-            }
+          for (int c = 0; c < 32; ++c) {
+            const float x = __bfloat162float(row[c]);
+            if (!isfinite(x)) f[c] += x;
           }
         }
-        // every copy into the ring has landed and been read
+      }
+      __syncwarp();  // the rows' loops are of different lengths, the next TMEM load is the warp's
+      // into the ring, whose copies have all landed and been read
+      if (whole) {
+        uint4* dst = reinterpret_cast<uint4*>(smem_raw + kRingOff + r * kOutRow + h * 64);
+#pragma unroll
+        for (int c = 0; c < 32; c += 8)
+          dst[c / 8] = make_uint4(pack_bf16x2(f[c], f[c + 1]), pack_bf16x2(f[c + 2], f[c + 3]),
+                                  pack_bf16x2(f[c + 4], f[c + 5]), pack_bf16x2(f[c + 6], f[c + 7]));
+      } else {
         float4* dst = reinterpret_cast<float4*>(smem_raw + kRingOff + r * kSumRow + h * 128);
 #pragma unroll
         for (int c = 0; c < 32; c += 4) dst[c / 4] = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
+      }
+    }
+    if (whole) {
+      // 16 lanes a row, so that every store is of whole lines
+      __syncwarp();
+      for (int i = 0; i < 32; i += 2) {
+        const int row = part * 32 + i + (lane >> 4);
+        if (row >= min(rows, kRows)) break;
+        const int at = fd_group.div(row0 + row);
+        const long long item = (long long)(begin + at) * p.qh + kvhead * group + (row0 + row - at * group);
+        const uint4 w = alive ? *reinterpret_cast<const uint4*>(smem_raw + kRingOff + row * kOutRow + (lane & 15) * 16)
+                              : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(p.out + item * 128 + (lane & 15) * 8) = w;
+      }
+      __syncwarp();
+      if (row_ok && p.lse) {
+        const int head = kvhead * group + (row0 + r - node * group);
+        p.lse[(long long)(begin + node) * p.qh + head] =
+            !alive || l == 0.0f ? -INFINITY : (m_used + fast_log2(l)) * kLn2;
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (work && warp == 1) {
+  if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
+  if (rows <= 0) return;
+  if (p.num_splits == 1) {
+    if (!work && row_ok) {  // no keys
+      const int head = kvhead * group + (row0 + r - node * group);
+      const long long item = (long long)(begin + node) * p.qh + head;
+      for (int d = 0; d < 128; d += 8) *reinterpret_cast<uint4*>(p.out + item * 128 + d) = make_uint4(0, 0, 0, 0);
+      if (p.lse) p.lse[item] = -INFINITY;
+    }
+    return;
+  }
 
   // ---------------------------------------------------------------- join
-  // A warp a row, a lane four dimensions: sum_s 2^(m_s - max) O_s over the
-  // cluster's CTAs s, divided by the same sum of their row sums.
+  // Every C-th row from the cluster's C CTAs: sum_s 2^(m_s - max) O_s over the
+  // same sum of their row sums. A thread works out a row's C factors, then
+  // each takes four dimensions of a row.
   cluster_sync();
-  {
-    const int size = int(cluster_size()), rank = int(cluster_rank());
-    const uint32_t stats_addr = raw_addr + kStatsOff, rows_addr = raw_addr + kRingOff;
-    for (int row = rank + size * warp; row < min(rows, kRows); row += size * (kThreads / 32)) {
-      float m = -INFINITY, sum = 0.0f;
-      if (lane < size)
+  const int size = int(cluster_size()), rank = int(cluster_rank());
+  const int mine = (min(rows, kRows) - rank + size - 1) / size;  // rows of this CTA
+  float* factor = reinterpret_cast<float*>(smem_raw + kFactorOff);
+  if (int(threadIdx.x) < mine) {
+    const int row = rank + size * threadIdx.x;
+    float m[kMaxCluster], sum[kMaxCluster], mx = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kMaxCluster; ++s) {
+      m[s] = -INFINITY;
+      sum[s] = 0.0f;
+      if (s < size)
         asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-                     : "=f"(m), "=f"(sum)
-                     : "r"(peer_addr(stats_addr + row * 8, lane)));
-      float mx = sum == 0.0f ? -INFINITY : m;
-#pragma unroll
-      for (int off = 4; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      // a range without a seen key has no part; one whose scores are all NaN has no maximum, its sum is NaN
-      float w = sum == 0.0f ? 0.0f : (m == -INFINITY ? NAN : fast_exp2(m - mx));
-      float total = w * sum;
-      mx = __shfl_sync(0xffffffffu, mx, 0);  // lanes 0-7 agree
-#pragma unroll
-      for (int off = 4; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-      total = __shfl_sync(0xffffffffu, total, 0);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float4 v[8];
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const float ws = __shfl_sync(0xffffffffu, w, s);
-        v[s] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (s < size && ws != 0.0f)
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w)
-                       : "r"(peer_addr(rows_addr + row * kSumRow + lane * 16, s)));
-      }
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const float ws = __shfl_sync(0xffffffffu, w, s);
-        if (s >= size || ws == 0.0f) continue;
-        acc.x = fmaf(ws, v[s].x, acc.x);
-        acc.y = fmaf(ws, v[s].y, acc.y);
-        acc.z = fmaf(ws, v[s].z, acc.z);
-        acc.w = fmaf(ws, v[s].w, acc.w);
-      }
-      const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // NaN stays NaN
-      const float lse = total == 0.0f ? -INFINITY : (mx + fast_log2(total)) * kLn2;
-      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-      const int at = fd_group.div(row0 + row);
-      const long long item = (long long)(begin + at) * p.qh + kvhead * group + (row0 + row - at * group);
-      if (p.num_splits == size) {
-        *reinterpret_cast<uint2*>(p.out + item * 128 + lane * 4) =
-            make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
-        if (lane == 0 && p.lse) p.lse[item] = lse;
-      } else {
-        const long long partial = (long long)(split / size) * p.total_q * p.qh + item;
-        *reinterpret_cast<float4*>(p.out_accum + partial * 128 + lane * 4) = acc;
-        if (lane == 0) p.lse_accum[partial] = lse;
-      }
+                     : "=f"(m[s]), "=f"(sum[s])
+                     : "r"(peer_addr(raw_addr + kStatsOff + row * 8, s)));
     }
+#pragma unroll
+    for (int s = 0; s < kMaxCluster; ++s) mx = fmaxf(mx, sum[s] == 0.0f ? -INFINITY : m[s]);
+#pragma unroll
+    for (int s = 0; s < kMaxCluster; ++s) {
+      // a range without a seen key has no part; one whose scores are all NaN has no maximum, its sum is NaN
+      m[s] = sum[s] == 0.0f ? 0.0f : (m[s] == -INFINITY ? NAN : fast_exp2(m[s] - mx));
+      total += m[s] * sum[s];
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int s = 0; s < kMaxCluster; ++s) factor[threadIdx.x * kMaxCluster + s] = m[s] == 0.0f ? 0.0f : m[s] * inv;
+    const float lse = total == 0.0f ? -INFINITY : (mx + fast_log2(total)) * kLn2;
+    const int at = fd_group.div(row0 + row);
+    const long long item = (long long)(begin + at) * p.qh + kvhead * group + (row0 + row - at * group);
+    if (p.num_splits > size)
+      p.lse_accum[(long long)(split / size) * p.total_q * p.qh + item] = lse;
+    else if (p.lse)
+      p.lse[item] = lse;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * mine; i += kThreads) {
+    const int k = i >> 5, row = rank + size * k;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f), v[kMaxCluster];
+    float f[kMaxCluster];
+#pragma unroll
+    for (int s = 0; s < kMaxCluster; ++s) {
+      f[s] = s < size ? factor[k * kMaxCluster + s] : 0.0f;
+      if (f[s] != 0.0f)  // NaN too
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w)
+                     : "r"(peer_addr(raw_addr + kRingOff + row * kSumRow + lane * 16, s)));
+    }
+#pragma unroll
+    for (int s = 0; s < kMaxCluster; ++s) {
+      if (f[s] == 0.0f) continue;
+      acc.x = fmaf(f[s], v[s].x, acc.x);
+      acc.y = fmaf(f[s], v[s].y, acc.y);
+      acc.z = fmaf(f[s], v[s].z, acc.z);
+      acc.w = fmaf(f[s], v[s].w, acc.w);
+    }
+    const int at = fd_group.div(row0 + row);
+    const long long item = (long long)(begin + at) * p.qh + kvhead * group + (row0 + row - at * group);
+    if (p.num_splits > size)
+      *reinterpret_cast<float4*>(p.out_accum + ((long long)(split / size) * p.total_q * p.qh + item) * 128 +
+                                 lane * 4) = acc;
+    else
+      *reinterpret_cast<uint2*>(p.out + item * 128 + lane * 4) =
+          make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
   }
   cluster_sync();  // nobody leaves while its shared memory is read
 }
