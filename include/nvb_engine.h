@@ -305,9 +305,9 @@ int nvbe_layer_sample(void* stream, const void* logits, const float* temperature
  * Entries behind counts are -1; a sequence without rows has counts 0. Rows at
  * and behind cu_q[batch] are neither read nor written. max_q bounds the nodes
  * of a sequence (at most 1024). `workspace`: 16-byte aligned,
- * nvbe_verify_workspace_bytes(rows) bytes, written before it is read; calls
+ * nvbe_verify_workspace_bytes(rows, batch) bytes, written before it is read; calls
  * that may overlap need one each. Allocates nothing and can be captured. */
-size_t nvbe_verify_workspace_bytes(int rows);
+size_t nvbe_verify_workspace_bytes(int rows, int batch);
 int nvbe_layer_verify(void* stream, const void* logits, const void* draft_logits, const int* tokens,
                       const int* parents, const float* uniforms, const uint64_t* seeds, const float* temperatures,
                       const int* cu_q, int* out_tokens, int* path, int* counts, float* accept_prob, int rows,

@@ -614,7 +614,9 @@ int nvbe_layer_sample(void* stream, const void* logits, const float* temperature
                  "sample launch");
 }
 
-size_t nvbe_verify_workspace_bytes(int rows) { return rows > 0 ? nvbm::verify_workspace(rows) : 0; }
+size_t nvbe_verify_workspace_bytes(int rows, int batch) {
+  return rows > 0 && batch > 0 ? nvbm::verify_workspace(rows, batch) : 0;
+}
 
 int nvbe_layer_verify(void* stream, const void* logits, const void* draft_logits, const int* tokens,
                       const int* parents, const float* uniforms, const uint64_t* seeds, const float* temperatures,
@@ -626,12 +628,12 @@ int nvbe_layer_verify(void* stream, const void* logits, const void* draft_logits
     return mfail("invalid verify arguments");
   if (max_q > nvbm::verify_max_nodes())
     return mfail("a tree has at most %d nodes (max_q %d)", nvbm::verify_max_nodes(), max_q);
-  const size_t need = nvbm::verify_workspace(rows);
+  const size_t need = nvbm::verify_workspace(rows, batch);
   if (!workspace || !aligned16(workspace) || workspace_bytes < need)
     return mfail("verify needs a 16-byte aligned workspace of %zu bytes (got %zu)", need, workspace_bytes);
   return cuda_rc(nvbm::launch_verify(static_cast<cudaStream_t>(stream), logits, draft_logits, tokens, parents,
                                      uniforms, seeds, temperatures, cu_q, out_tokens, path, counts, accept_prob,
-                                     rows, batch, max_q, vocab, workspace),
+                                     rows, batch, max_q, vocab, workspace, sm_count()),
                  "verify launch");
 }
 

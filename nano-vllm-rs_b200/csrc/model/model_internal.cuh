@@ -52,11 +52,11 @@ cudaError_t launch_sample_combine(cudaStream_t s, const float* part_score, const
 // Verification of drafted tokens (verify.cu); include/nvb_engine.h has the
 // meaning of the arguments. `ws` holds verify_workspace bytes.
 int verify_max_nodes();
-size_t verify_workspace(int rows);
+size_t verify_workspace(int rows, int batch);
 cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft, const int* tokens,
                           const int* parents, const float* uniforms, const uint64_t* seeds, const float* temps,
                           const int* cu_q, int* out_tokens, int* path, int* counts, float* accept, int rows, int batch,
-                          int max_q, int vocab, void* ws);
+                          int max_q, int vocab, void* ws, int sms);
 // The decode GEMM's device error word (1: a pipeline wait gave up), or -1.
 int gemm_decode_error();
 

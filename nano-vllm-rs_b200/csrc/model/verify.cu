@@ -14,6 +14,25 @@
 // accepted child, or the token drawn from the P that is left when all are
 // rejected, is distributed as the target's P. Without draft probabilities Q
 // is 1 at the child's token. T = 0 accepts the argmax's child.
+//
+// Two kernels. verify_nodes_kernel tests every node's children as if the node
+// had been reached, so all nodes run at once: a cluster of up to 8 CTAs reads
+// a node's two rows once (running maximum and sum, joined through distributed
+// shared memory), and once more, from L2, for each rejected child that has a
+// sibling behind it. Nodes without children are not read. What bounds it is
+// HBM; one exponential per logit takes 3/4 of the MUFU rate that goes with it.
+//
+// verify_sample_kernel follows the accepted children from the root and draws
+// the next token from the last node's row, cut over CTAs that hold 4096 tokens
+// in registers. A token's score is log P(v) plus Gumbel noise of u(v); the
+// noise takes a SplitMix64 and two logarithms, ~100 instructions in all, for
+// 152 thousand tokens a sequence. The best score of a slice with sum Z is
+// below log Z - 3 once in 10^9 times (exp(-e^3)), and a token reaches log Z - 3
+// only if 1 - u < e^3 P(v) / Z (-log u >= 1 - u). So the slice's sum is added
+// up first, the hash alone sorts out nearly all tokens, and the exact scores
+// of the ~20 that are left decide; a slice where none reached the bound scores
+// all its tokens. The slices' best meet in a 64-bit maximum (score, then the
+// lowest token), which no order of arrival changes.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -28,19 +47,28 @@ namespace {
 
 using namespace sample_math;
 
-constexpr int kThreads = 512;
-constexpr int kMaxNodes = 1024;  // of one tree (verify_max_nodes)
+constexpr int kThreads = 256;        // of a nodes CTA
+constexpr int kSampleThreads = 512;  // of a sample CTA, 8 tokens a thread
+constexpr int kMaxCluster = 8;
+constexpr int kMaxNodes = 1024;      // of one tree (verify_max_nodes)
 constexpr float kLog2e = 1.4426950408889634f;
 
 // What the first kernel leaves per row. For a node with children: its
 // statistics, accepted child and count of rejected children; for a child that
-// was rejected: the levels that its rejection adds.
+// was rejected: the level that its rejection adds.
 struct VerifyRow {
   float m_p, z_p, m_q, z_q;  // max logit and sum of exp((l - max) / T)
   float mass_q;              // child: Q's remaining sum (of its z_q) when it was tested
   float left;                // child: sum max(P - Q, 0) at its rejection, <= 0: P stayed
-  int winner;                // node: accepted child's row in its sequence, or -1
+  int winner;                // node: accepted child's place in its sequence, or -1
   int rejected;              // node: children rejected
+};
+
+// The slices' best of a sequence; zeroed by the first kernel.
+struct VerifyBest {
+  unsigned long long key;  // ordered score, then inverted token; 0: none
+  unsigned done;           // slices that have added theirs
+  unsigned unused;
 };
 
 struct VerifyParams {
@@ -57,92 +85,219 @@ struct VerifyParams {
   int* counts;      // [batch]
   float* accept;    // [rows]
   VerifyRow* ws;    // [rows]
+  VerifyBest* best;  // [batch]
   int rows, max_q, vocab;
 };
 
-// exp((l - m) / T) with c = log2(e) / T. NaN logits have no probability; an
-// infinite one takes all of it.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// exp((l - m) / T) with c = log2(e) / T. The difference of two BF16 is exact
+// in FP32 (or as good), so the argument's error is relative. NaN logits have
+// no probability; an infinite one takes all of it.
 __device__ __forceinline__ float weight(float l, float m, float c) {
   if (!(l == l)) return 0.0f;
   if (m == INFINITY) return l == INFINITY ? 1.0f : 0.0f;
-  return m == -INFINITY ? 0.0f : exp2f((l - m) * c);
+  return m == -INFINITY ? 0.0f : ex2((l - m) * c);
 }
 
 __device__ __forceinline__ float inv_temperature(float t) { return fminf(kLog2e / t, 1e38f); }
 
-__device__ __forceinline__ float block_sum(float v, float* s) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.0f;
-  for (int w = 0; w < kThreads / 32; ++w) v += s[w];
-  return v;
-}
+// ------------------------------------------------------------- rows of logits
+// A row starts at any element (odd vocabularies), so it is read in the aligned
+// 16-byte groups that cover it: group g holds elements [8 g - shift, + 8).
+// Elements outside the row read as -inf.
+struct Row {
+  const __nv_bfloat16* p;
+  int shift, groups, vocab;
+  __device__ __forceinline__ Row(const __nv_bfloat16* row, int vocab_)
+      : p(row), shift(int(reinterpret_cast<uintptr_t>(row) >> 1) & 7), groups((vocab_ + shift + 7) >> 3),
+        vocab(vocab_) {}
+};
 
-__device__ __forceinline__ float block_max(float v, float* s) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = -INFINITY;
-  for (int w = 0; w < kThreads / 32; ++w) v = fmaxf(v, s[w]);
-  return v;
-}
-
-__device__ __forceinline__ void block_best(float& score, int& index, float* s, int* si) {
-  warp_best(score, index);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) {
-    s[threadIdx.x >> 5] = score;
-    si[threadIdx.x >> 5] = index;
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int at, int vocab) {
+  if (at >= 0 && at + 8 <= vocab && (reinterpret_cast<uintptr_t>(row + at) & 15) == 0)
+    return __ldg(reinterpret_cast<const uint4*>(row + at));
+  uint64_t lo = 0, hi = 0;  // the last element first
+#pragma unroll 1
+  for (int e = at + 7; e >= at; --e) {
+    hi = (hi << 16) | (lo >> 48);
+    lo = (lo << 16) | (e >= 0 && e < vocab ? __bfloat16_as_ushort(row[e]) : 0xff80u);
   }
-  __syncthreads();
-  for (int w = 0; w < kThreads / 32; ++w)
-    if (better(s[w], si[w], score, index)) {
-      score = s[w];
-      index = si[w];
+  return make_uint4(uint32_t(lo), uint32_t(lo >> 32), uint32_t(hi), uint32_t(hi >> 32));
+}
+
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// The largest of eight logits, NaN left out (NaN where all are).
+__device__ __forceinline__ float max8(const uint4& v) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
+// Running maximum and sum of exp((l - m) / T). NaN and infinite logits make
+// the sum NaN (the caller then adds it up anew with weight()).
+struct Online {
+  float m = -INFINITY, z = 0.0f;
+  __device__ __forceinline__ void add(const uint4& v, float c) {
+    const float gm = max8(v);
+    if (gm > m) {
+      z = m == -INFINITY ? z : z * ex2((m - gm) * c);
+      m = gm;
     }
+    if (!(m > -INFINITY)) {  // nothing but -inf so far, or NaN
+      if (!(gm == gm)) z = NAN;
+      return;
+    }
+    float f[8], s0 = 0.0f, s1 = 0.0f;
+    unpack8(v, f);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      s0 += ex2((f[i] - m) * c);
+      s1 += ex2((f[i + 1] - m) * c);
+    }
+    z += s0 + s1;
+  }
+  __device__ __forceinline__ void join(float om, float oz, float c) {
+    const float nm = fmaxf(m, om);
+    // a side without a finite maximum has sum 0, or NaN to pass on
+    z = (m == nm || m == -INFINITY ? z : z * ex2((m - nm) * c)) +
+        (om == nm || om == -INFINITY ? oz : oz * ex2((om - nm) * c));
+    m = nm;
+  }
+};
+
+// ----------------------------------------------------------- CTA and cluster
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 peer_load(const float4* p, uint32_t rank) {
+  const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(p));
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(remote)
+               : "memory");
+  return v;
+}
+
+// Joins four numbers of every thread of the cluster with `op` (commutative
+// pairs of float4), in one order for all: every thread gets the same result.
+// Alternating buffers: a CTA may be one exchange ahead of another.
+struct Exchange {
+  float4 warp[2][kThreads / 32];
+  float4 cta[2];
+};
+template <class Op>
+__device__ __forceinline__ float4 exchange(float4 v, Exchange& x, int& turn, uint32_t size, Op op) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    const float4 o = make_float4(__shfl_xor_sync(0xffffffffu, v.x, off), __shfl_xor_sync(0xffffffffu, v.y, off),
+                                 __shfl_xor_sync(0xffffffffu, v.z, off), __shfl_xor_sync(0xffffffffu, v.w, off));
+    v = op(v, o);
+  }
+  const int t = turn & 1;
+  ++turn;
+  if ((threadIdx.x & 31) == 0) x.warp[t][threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = x.warp[t][0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 32; ++w) v = op(v, x.warp[t][w]);
+  if (size == 1) return v;
+  if (threadIdx.x == 0) x.cta[t] = v;
+  cluster_sync();
+  v = peer_load(&x.cta[t], 0);
+  for (uint32_t r = 1; r < size; ++r) v = op(v, peer_load(&x.cta[t], r));
+  return v;
 }
 
 // A node's children that were rejected, in order: what P has become.
 struct Levels {
-  int n;                   // rejected children
-  const int* token;        // [n]
-  const float* mass_q;     // [n]
-  const float* left;       // [n]
+  const int* token;     // [n]
+  const float* mass_q;  // [n]
+  const float* left;    // [n]
 };
 
 // P(v) after the first `n` rejections, from P's weight over its sum (p) and
-// Q's weight (q, 1 over z_q not applied).
+// Q's weight (wq).
 __device__ __forceinline__ float remaining(float p, float wq, int v, bool has_q, const Levels& lv, int n) {
   for (int i = 0; i < n; ++i) {
     if (!(lv.left[i] > 0.0f)) continue;
     if (has_q) {
       bool gone = false;
       for (int j = 0; j < i; ++j) gone |= lv.token[j] == v;
-      const float q = gone || !(lv.mass_q[i] > 0.0f) ? 0.0f : wq / lv.mass_q[i];
+      const float q = gone || !(lv.mass_q[i] > 0.0f) ? 0.0f : __fdividef(wq, lv.mass_q[i]);
       p = fmaxf(p - q, 0.0f);
     } else if (lv.token[i] == v) {
       p = 0.0f;
     }
-    p /= lv.left[i];
+    p = __fdividef(p, lv.left[i]);
   }
   return p;
 }
 
-// One CTA per node: its statistics, and its children's tests.
+struct SumOp {
+  __device__ float4 operator()(const float4& a, const float4& b) const {
+    return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+  }
+};
+struct BestOp {  // (score, index bits)
+  __device__ float4 operator()(const float4& a, const float4& b) const {
+    return better(b.x, __float_as_int(b.y), a.x, __float_as_int(a.y)) ? b : a;
+  }
+};
+struct OnlineOp {  // (m_p, z_p, m_q, z_q)
+  float c;
+  __device__ float4 operator()(const float4& a, const float4& b) const {
+    Online p, q;
+    p.m = a.x;
+    p.z = a.y;
+    q.m = a.z;
+    q.z = a.w;
+    p.join(b.x, b.y, c);
+    q.join(b.z, b.w, c);
+    return make_float4(p.m, p.z, q.m, q.z);
+  }
+};
+
+// A cluster per node: its statistics, and its children's tests.
 __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyParams p) {
-  __shared__ float s_red[kThreads / 32];
-  __shared__ int s_idx[kThreads / 32];
+  __shared__ Exchange s_x;
   __shared__ int s_child[kMaxNodes], s_token[kMaxNodes];
   __shared__ float s_mass[kMaxNodes], s_left[kMaxNodes];
   __shared__ int s_kids;
-  const int b = blockIdx.y, node = blockIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint32_t size = cluster_size(), rank = cluster_rank();
+  const int b = blockIdx.y, node = blockIdx.x / size;
   const int begin = p.cu_q[b], n = min(min(p.cu_q[b + 1], p.rows) - begin, p.max_q);
-  if (begin < 0 || node >= n) return;
+  if (node == 0 && rank == 0 && threadIdx.x == 0) p.best[b] = VerifyBest{0ull, 0u, 0u};
+  if (begin < 0 || node >= n) return;  // all of a cluster
   VerifyRow* ws = p.ws + begin;
   const int row = begin + node;
   if (threadIdx.x < 32) {
@@ -162,27 +317,47 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
   }
   __syncthreads();
   const int kids = s_kids;
-  const __nv_bfloat16* lp = p.logits + (long long)row * p.vocab;
-  const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
-  const float temperature = p.temps[b];
-  if (threadIdx.x == 0) {  // a node that is no node's child is tested by nobody
+  const bool writes = rank == 0 && threadIdx.x == 0;
+  if (writes) {  // a node that is no node's child is tested by nobody
     const int parent = p.parents[row];
     if (node == 0 || parent < 0 || parent >= node) p.accept[row] = 0.0f;
   }
-  if (kids == 0 || !(temperature > 0.0f)) {
+  if (kids == 0) {
+    if (writes) {
+      ws[node].winner = -1;
+      ws[node].rejected = 0;
+    }
+    return;
+  }
+  const Row lp(p.logits + (long long)row * p.vocab, p.vocab);
+  const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
+  const float temperature = p.temps[b];
+  // this CTA's groups
+  const int per = (lp.groups + int(size) - 1) / int(size), g0 = int(rank) * per, g1 = min(g0 + per, lp.groups);
+  int turn = 0;
+  if (!(temperature > 0.0f)) {
     float best = -INFINITY;
     int best_index = kNone;
-    if (kids)
-      for (int v = threadIdx.x; v < p.vocab; v += kThreads) {
-        const float l = __bfloat162float(lp[v]);
-        if (better(l, v, best, best_index)) {
-          best = l;
-          best_index = v;
+#pragma unroll 4
+    for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
+      const uint4 v = load8(lp.p, 8 * g - lp.shift, p.vocab);
+      if (max8(v) > best || best_index == kNone) {
+        float f[8];
+        unpack8(v, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int t = 8 * g - lp.shift + i;
+          if (t >= 0 && t < p.vocab && better(f[i], t, best, best_index)) {
+            best = f[i];
+            best_index = t;
+          }
         }
       }
-    block_best(best, best_index, s_red, s_idx);
+    }
+    const float4 top = exchange(make_float4(best, __int_as_float(best_index), 0.f, 0.f), s_x, turn, size, BestOp());
+    best_index = __float_as_int(top.y);
     if (best_index == kNone) best_index = 0;
-    if (threadIdx.x == 0) {
+    if (writes) {
       int winner = -1;
       for (int i = 0; i < kids; ++i) {
         const bool taken = winner < 0 && s_token[i] == best_index;
@@ -192,24 +367,51 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
       ws[node].winner = winner;
       ws[node].rejected = 0;
     }
+    if (size > 1) cluster_sync();  // nobody leaves while its shared memory is read
     return;
   }
   const float c = inv_temperature(temperature);
-  float m_p = -INFINITY, m_q = -INFINITY;
-  for (int v = threadIdx.x; v < p.vocab; v += kThreads) {
-    m_p = fmaxf(m_p, __bfloat162float(lp[v]));
-    if (lq) m_q = fmaxf(m_q, __bfloat162float(lq[v]));
+  float m_p, z_p, m_q, z_q;
+  {
+    Online op, oq;
+    if (lq) {
+#pragma unroll 2
+      for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
+        const int at = 8 * g - lp.shift;
+        const uint4 vp = load8(lp.p, at, p.vocab), vq = load8(lq, at, p.vocab);
+        op.add(vp, c);
+        oq.add(vq, c);
+      }
+    } else {
+#pragma unroll 4
+      for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) op.add(load8(lp.p, 8 * g - lp.shift, p.vocab), c);
+    }
+    const float4 all = exchange(make_float4(op.m, op.z, oq.m, oq.z), s_x, turn, size, OnlineOp{c});
+    m_p = all.x;
+    z_p = all.y;
+    m_q = all.z;
+    z_q = all.w;
   }
-  m_p = block_max(m_p, s_red);
-  m_q = block_max(m_q, s_red);
-  float z_p = 0.0f, z_q = 0.0f;
-  for (int v = threadIdx.x; v < p.vocab; v += kThreads) {
-    z_p += weight(__bfloat162float(lp[v]), m_p, c);
-    if (lq) z_q += weight(__bfloat162float(lq[v]), m_q, c);
+  if (!(z_p == z_p) || !(z_q == z_q) || m_p == INFINITY || m_q == INFINITY) {
+    // NaN or infinite logits: the maxima are right, the sums are taken anew
+    float2 z = make_float2(0.f, 0.f);
+    for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
+      const int at = 8 * g - lp.shift;
+      float f[8];
+      unpack8(load8(lp.p, at, p.vocab), f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z.x += weight(f[i], m_p, c);
+      if (lq) {
+        unpack8(load8(lq, at, p.vocab), f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z.y += weight(f[i], m_q, c);
+      }
+    }
+    const float4 all = exchange(make_float4(z.x, z.y, 0.f, 0.f), s_x, turn, size, SumOp());
+    z_p = all.x;
+    z_q = all.y;
   }
-  z_p = block_sum(z_p, s_red);
-  z_q = block_sum(z_q, s_red);
-  const Levels lv{0, s_token, s_mass, s_left};
+  const Levels lv{s_token, s_mass, s_left};
   int winner = -1, rejected = 0;
   float mass = z_q;
   for (int i = 0; i < kids; ++i) {
@@ -218,7 +420,7 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
     float a = 0.0f;
     if (t >= 0 && t < p.vocab && z_p > 0.0f) {
       const float wq = lq ? weight(__bfloat162float(lq[t]), m_q, c) : 0.0f;
-      const float pt = remaining(weight(__bfloat162float(lp[t]), m_p, c) / z_p, wq, t, lq != nullptr, lv, i);
+      const float pt = remaining(weight(__bfloat162float(lp.p[t]), m_p, c) / z_p, wq, t, lq != nullptr, lv, i);
       float qt = 1.0f;
       if (lq) {
         bool gone = false;
@@ -228,39 +430,60 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
       a = !(pt > 0.0f) ? 0.0f : (qt > 0.0f ? fminf(pt / qt, 1.0f) : 1.0f);
     }
     const bool taken = p.uniforms[begin + s_child[i]] < a;
-    if (threadIdx.x == 0) p.accept[begin + s_child[i]] = a;
+    if (writes) p.accept[begin + s_child[i]] = a;
     if (taken) {
       winner = s_child[i];
-      for (int j = i + 1 + threadIdx.x; j < kids; j += kThreads) p.accept[begin + s_child[j]] = 0.0f;
+      if (rank == 0)
+        for (int j = i + 1 + int(threadIdx.x); j < kids; j += kThreads) p.accept[begin + s_child[j]] = 0.0f;
       break;
     }
-    // rejected: what is left of P, and Q's sum without the rejected tokens
-    // (added up anew: a difference would cancel where the tokens had most)
+    rejected = i + 1;
     if (threadIdx.x == 0) {
       s_mass[i] = mass;
       s_left[i] = 1.0f;  // its sum is what the pass below adds up
     }
-    __syncthreads();
-    float left = 0.0f, rest = 0.0f;
-    for (int v = threadIdx.x; v < p.vocab; v += kThreads) {
-      const float wq = lq ? weight(__bfloat162float(lq[v]), m_q, c) : 0.0f;
-      left += remaining(weight(__bfloat162float(lp[v]), m_p, c) / z_p, wq, v, lq != nullptr, lv, i + 1);
-      bool gone = false;
-      for (int j = 0; j <= i; ++j) gone |= s_token[j] == v;
-      rest += gone ? 0.0f : wq;
+    if (i + 1 == kids) {  // no sibling needs the sums; the draw does without
+      if (writes) {
+        ws[s_child[i]].mass_q = mass;
+        ws[s_child[i]].left = 1.0f;
+      }
+      break;
     }
-    left = z_p > 0.0f ? block_sum(left, s_red) : 0.0f;
-    mass = block_sum(rest, s_red);
+    __syncthreads();
+    // what is left of P, and Q's sum without the rejected tokens (added up anew: a difference would cancel where the
+    // tokens had most)
+    float left = 0.0f, rest = 0.0f;
+#pragma unroll 2
+    for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
+      const int at = 8 * g - lp.shift;
+      float f[8], h[8];
+      unpack8(load8(lp.p, at, p.vocab), f);
+      if (lq) unpack8(load8(lq, at, p.vocab), h);
+      uint32_t gone = 0;
+      for (int j = 0; j <= i; ++j) {
+        const unsigned e = unsigned(s_token[j] - at);
+        if (e < 8u) gone |= 1u << e;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float wq = lq ? weight(h[e], m_q, c) : 0.0f;
+        left += remaining(__fdividef(weight(f[e], m_p, c), z_p), wq, at + e, lq != nullptr, lv, i + 1);
+        rest += gone >> e & 1u ? 0.0f : wq;
+      }
+    }
+    const float4 all = exchange(make_float4(left, rest, 0.f, 0.f), s_x, turn, size, SumOp());
+    left = z_p > 0.0f ? all.x : 0.0f;
     if (threadIdx.x == 0) {
       s_left[i] = left;
-      VerifyRow& r = ws[s_child[i]];
-      r.mass_q = s_mass[i];
-      r.left = left;
+      if (rank == 0) {
+        ws[s_child[i]].mass_q = mass;
+        ws[s_child[i]].left = left;
+      }
     }
+    mass = all.y;
     __syncthreads();
-    rejected = i + 1;
   }
-  if (threadIdx.x == 0) {
+  if (writes) {
     VerifyRow& r = ws[node];
     r.m_p = m_p;
     r.z_p = z_p;
@@ -269,106 +492,248 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
     r.winner = winner;
     r.rejected = rejected;
   }
+  if (size > 1) cluster_sync();  // nobody leaves while its shared memory is read
 }
 
-// One CTA per sequence: the accepted path, and the token behind it.
-__global__ void __launch_bounds__(kThreads) verify_sample_kernel(const VerifyParams p) {
-  __shared__ float s_red[kThreads / 32];
-  __shared__ int s_idx[kThreads / 32];
-  __shared__ int s_winner[kMaxNodes], s_token[kMaxNodes];
+// ---------------------------------------------------------------- next token
+// Scores as an integer that orders like them, then the lowest token first.
+__device__ __forceinline__ unsigned long long sort_key(float score, int token) {
+  if (!(score == score)) return 0ull;  // NaN is never it
+  const uint32_t u = __float_as_uint(score), o = u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (static_cast<unsigned long long>(o) << 32) | (0xffffffffu - uint32_t(token));
+}
+__device__ __forceinline__ float key_score(unsigned long long key) {
+  const uint32_t o = uint32_t(key >> 32);
+  return key ? __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o) : -INFINITY;
+}
+__device__ __forceinline__ unsigned long long max_key(unsigned long long a, unsigned long long b) {
+  return a > b ? a : b;
+}
+
+__device__ __forceinline__ float sample_sum(float v, float* s) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = s[threadIdx.x & 15];
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+__device__ __forceinline__ float sample_max(float v, float* s) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = s[threadIdx.x & 15];
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+__device__ __forceinline__ unsigned long long sample_key(unsigned long long v, unsigned long long* s) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v = max_key(v, __shfl_xor_sync(0xffffffffu, v, off));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = s[threadIdx.x & 15];
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) v = max_key(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+static_assert(kSampleThreads == 512, "the reductions above are over 16 warps");
+
+// CTA (slice, sequence): the accepted path, and the slice's best token.
+__global__ void __launch_bounds__(kSampleThreads) verify_sample_kernel(const VerifyParams p) {
+  __shared__ float s_red[16];
+  __shared__ unsigned long long s_key[16];
+  __shared__ int s_winner[kMaxNodes], s_path[kMaxNodes], s_token[kMaxNodes];
   __shared__ float s_mass[kMaxNodes], s_left[kMaxNodes];
-  __shared__ int s_last, s_count;
-  const int b = blockIdx.x, begin = p.cu_q[b], n = min(min(p.cu_q[b + 1], p.rows) - begin, p.max_q);
+  __shared__ int s_count, s_is_last;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int b = blockIdx.y, begin = p.cu_q[b], n = min(min(p.cu_q[b + 1], p.rows) - begin, p.max_q);
   int* tokens = p.out_tokens + (long long)b * p.max_q;
   int* path = p.path + (long long)b * p.max_q;
+  const float temperature = p.temps[b];
   if (begin < 0 || n <= 0) {
-    for (int i = threadIdx.x; i < p.max_q; i += kThreads) tokens[i] = path[i] = -1;
-    if (threadIdx.x == 0) p.counts[b] = 0;
+    if (blockIdx.x == 0) {
+      for (int i = threadIdx.x; i < p.max_q; i += kSampleThreads) tokens[i] = path[i] = -1;
+      if (threadIdx.x == 0) p.counts[b] = 0;
+    }
     return;
   }
   const VerifyRow* ws = p.ws + begin;
-  for (int i = threadIdx.x; i < n; i += kThreads) s_winner[i] = ws[i].winner;
+  for (int i = threadIdx.x; i < n; i += kSampleThreads) s_winner[i] = ws[i].winner;
   __syncthreads();
   if (threadIdx.x == 0) {
     int at = 0, count = 1;
-    path[0] = 0;
+    s_path[0] = 0;
     while (s_winner[at] > at) {
       at = s_winner[at];
-      path[count] = at;
-      tokens[count - 1] = p.tokens[begin + at];
-      ++count;
+      s_path[count++] = at;
     }
-    s_last = at;
     s_count = count;
-    p.counts[b] = count;
   }
   __syncthreads();
-  const int last = s_last, count = s_count, row = begin + last;
-  for (int i = count + threadIdx.x; i < p.max_q; i += kThreads) tokens[i] = path[i] = -1;
-  const __nv_bfloat16* lp = p.logits + (long long)row * p.vocab;
+  const int count = s_count, last = s_path[count - 1], row = begin + last;
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < p.max_q; i += kSampleThreads) {
+      path[i] = i < count ? s_path[i] : -1;
+      if (i + 1 != count) tokens[i] = i + 1 < count ? p.tokens[begin + s_path[i + 1]] : -1;
+    }
+    if (threadIdx.x == 0) p.counts[b] = count;
+  }
+  const Row lp(p.logits + (long long)row * p.vocab, p.vocab);
   const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
-  const float temperature = p.temps[b];
+  const uint64_t seed = p.seeds[row];
   const int rejected = ws[last].rejected;
-  if (threadIdx.x < 32) {  // the rejected children's levels
-    int kids = 0;
-    for (int base = last + 1; base < n && kids < rejected; base += 32) {
-      const int i = base + threadIdx.x;
-      const bool mine = i < n && p.parents[begin + i] == last;
-      const unsigned hits = __ballot_sync(0xffffffffu, mine);
-      const int at = kids + __popc(hits & ((1u << threadIdx.x) - 1u));
-      if (mine && at < rejected) {
-        s_token[at] = p.tokens[begin + i];
-        s_mass[at] = ws[i].mass_q;
-        s_left[at] = ws[i].left;
+  const int g = blockIdx.x * kSampleThreads + threadIdx.x, at = 8 * g - lp.shift;
+  // the slice's tokens, in registers from here on
+  uint4 vp = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u), vq = vp;
+  if (g < lp.groups) {
+    vp = load8(lp.p, at, p.vocab);
+    if (lq && rejected) vq = load8(lq, at, p.vocab);
+  }
+  float m_p = 0.f, z_p = 1.f, m_q = 0.f;
+  if (rejected) {
+    m_p = ws[last].m_p;
+    z_p = ws[last].z_p;
+    m_q = ws[last].m_q;
+    if (threadIdx.x < 32) {  // the rejected children's levels
+      int kids = 0;
+      for (int base = last + 1; base < n && kids < rejected; base += 32) {
+        const int i = base + threadIdx.x;
+        const bool mine = i < n && p.parents[begin + i] == last;
+        const unsigned hits = __ballot_sync(0xffffffffu, mine);
+        const int k = kids + __popc(hits & ((1u << threadIdx.x) - 1u));
+        if (mine && k < rejected) {
+          s_token[k] = p.tokens[begin + i];
+          s_mass[k] = ws[i].mass_q;
+          s_left[k] = ws[i].left;
+        }
+        kids += __popc(hits);
       }
-      kids += __popc(hits);
     }
+    __syncthreads();
+  }
+  const Levels lv{s_token, s_mass, s_left};
+  const float c = inv_temperature(temperature);
+  // P (over any common factor) of a token after `levels` rejections
+  auto probability = [&](float l, float lqv, int v, int levels) {
+    const float wq = lq ? weight(lqv, m_q, c) : 0.0f;
+    return remaining(__fdividef(weight(l, m_p, c), z_p), wq, v, lq != nullptr, lv, levels);
+  };
+  // the exact score: the sampler's where nothing was rejected
+  auto score = [&](float l, float prob, int v, int levels) {
+    if (levels == 0) return gumbel_score(l, temperature, seed, v);
+    return prob > 0.0f ? logf(prob) - gumbel_log(seed, v) : NAN;
+  };
+  float f[8], h[8], prob[8];
+  unpack8(vp, f);
+  unpack8(vq, h);
+  unsigned long long best = 0ull;
+  if (!(temperature > 0.0f)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (at + e >= 0 && at + e < p.vocab) best = max_key(best, sort_key(f[e], at + e));
+    best = sample_key(best, s_key);
+  } else {
+    // weights of the slice; where nothing was rejected they are relative to its own maximum
+    float top = 0.0f;
+    if (rejected == 0) {
+      top = sample_max(max8(vp), s_red);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) prob[e] = weight(f[e], top, c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) prob[e] = probability(f[e], h[e], at + e, rejected);
+    }
+    float z = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z += prob[e];
+    z = sample_sum(z, s_red);
+    const bool bounded = z > 0.0f && top > -INFINITY && top < INFINITY;
+    // the bound that the tokens sorted out stay below (and 1/1000 for the roundings of the scores)
+    const float least = (rejected == 0 ? __fdividef(top, temperature) : 0.0f) + logf(z) - 3.0f;
+    // (1 - u) 2^23 is the inverted hash's 23 bits plus a half; e^3 and a little for the roundings
+    const float scale = __fdividef(20.1f * 8388608.0f, z);
+    bool all = !bounded;  // then every token is scored
+    for (;;) {
+      uint64_t x = uint64_t(int64_t(at)) * 0xd2b74407b1ce6e93ULL;
+#pragma unroll
+      for (int e = 0; e < 8; ++e, x += 0xd2b74407b1ce6e93ULL) {
+        const uint32_t k = uint32_t(splitmix64(seed ^ x) >> 41);
+        if ((all || float(0x7fffffu - k) + 0.5f < prob[e] * scale) && at + e >= 0 && at + e < p.vocab)
+          best = max_key(best, sort_key(score(f[e], prob[e], at + e, rejected), at + e));
+      }
+      best = sample_key(best, s_key);
+      if (all || key_score(best) >= least + 1e-3f * (1.0f + fabsf(least))) break;
+      all = true;
+    }
+  }
+  // join the slices; the last one writes the token
+  if (threadIdx.x == 0) {
+    if (best) atomicMax(&p.best[b].key, best);
+    __threadfence();
+    s_is_last = atomicAdd(&p.best[b].done, 1u) == gridDim.x - 1;
   }
   __syncthreads();
-  const Levels lv{rejected, s_token, s_mass, s_left};
-  const float m_p = ws[last].m_p, z_p = ws[last].z_p, m_q = ws[last].m_q;
-  const float c = inv_temperature(temperature);
-  const uint64_t seed = p.seeds[row];
-  float best = -INFINITY;
-  int best_index = kNone;
-  for (int v = threadIdx.x; v < p.vocab; v += kThreads) {
-    const float l = __bfloat162float(lp[v]);
-    float score;
-    if (rejected == 0) {
-      score = gumbel_score(l, temperature, seed, v);
-    } else {
-      const float wq = lq ? weight(__bfloat162float(lq[v]), m_q, c) : 0.0f;
-      const float left = remaining(weight(l, m_p, c) / z_p, wq, v, lq != nullptr, lv, rejected);
-      if (!(left > 0.0f)) continue;
-      score = logf(left) - gumbel_log(seed, v);
+  if (!s_is_last) return;
+  __threadfence();
+  unsigned long long key = atomicMax(&p.best[b].key, 0ull);
+  // The last rejection left nothing of P: it stays what it was before it. (The sums behind the others were not 0.)
+  for (int levels = rejected - 1; key == 0ull && levels >= 0; --levels) {
+    best = 0ull;
+    for (int v = threadIdx.x; v < p.vocab; v += kSampleThreads) {
+      const float l = __bfloat162float(lp.p[v]);
+      const float pr = levels ? probability(l, lq ? __bfloat162float(lq[v]) : 0.0f, v, levels) : 0.0f;
+      best = max_key(best, sort_key(score(l, pr, v, levels), v));
     }
-    if (better(score, v, best, best_index)) {
-      best = score;
-      best_index = v;
-    }
+    key = sample_key(best, s_key);
   }
-  block_best(best, best_index, s_red, s_idx);
-  if (threadIdx.x == 0) tokens[count - 1] = best_index == kNone ? 0 : best_index;
+  if (threadIdx.x == 0) tokens[count - 1] = key ? int(0xffffffffu - uint32_t(key)) : 0;
 }
 
 }  // namespace
 
 int verify_max_nodes() { return kMaxNodes; }
 
-size_t verify_workspace(int rows) { return size_t(rows) * sizeof(VerifyRow); }
+size_t verify_workspace(int rows, int batch) {
+  return size_t(rows) * sizeof(VerifyRow) + size_t(batch) * sizeof(VerifyBest);
+}
 
 cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft, const int* tokens,
                           const int* parents, const float* uniforms, const uint64_t* seeds, const float* temps,
                           const int* cu_q, int* out_tokens, int* path, int* counts, float* accept, int rows, int batch,
-                          int max_q, int vocab, void* ws) {
-  VerifyParams p{static_cast<const __nv_bfloat16*>(logits), static_cast<const __nv_bfloat16*>(draft), tokens,
-                 parents, uniforms, seeds, temps, cu_q, out_tokens, path, counts, accept,
-                 static_cast<VerifyRow*>(ws), rows, max_q, vocab};
-  verify_nodes_kernel<<<dim3(max_q, batch), kThreads, 0, s>>>(p);
-  cudaError_t e = cudaGetLastError();
+                          int max_q, int vocab, void* ws, int sms) {
+  VerifyParams p{static_cast<const __nv_bfloat16*>(logits), static_cast<const __nv_bfloat16*>(draft), tokens, parents,
+                 uniforms, seeds, temps, cu_q, out_tokens, path, counts, accept, static_cast<VerifyRow*>(ws),
+                 reinterpret_cast<VerifyBest*>(static_cast<VerifyRow*>(ws) + rows), rows, max_q, vocab};
+  // CTAs a node: enough that the nodes fill the GPU about four times over, none with less than 4096 logits.
+  int cluster = 1;
+  while (cluster < kMaxCluster && (long long)rows * cluster < 4LL * sms && vocab >= 2 * cluster * 4096) cluster *= 2;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(max_q) * unsigned(cluster), unsigned(batch));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_nodes_kernel, p);
   if (e != cudaSuccess) return e;
-  verify_sample_kernel<<<batch, kThreads, 0, s>>>(p);
-  return cudaGetLastError();
+  cfg.gridDim = dim3(unsigned((vocab + 7 + 7) / 8 + kSampleThreads - 1) / kSampleThreads, unsigned(batch));
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, verify_sample_kernel, p);
 }
 
 }  // namespace nvbm

@@ -76,7 +76,7 @@ def library():
         L.nvbe_layer_gemm_sample.argtypes = [P, P, P, P, I, I, I, P, P, P, P, P]
         L.nvbe_sample_partitions.argtypes = [I]
         L.nvbe_layer_sample.argtypes = [P] * 7 + [I, I]
-        L.nvbe_verify_workspace_bytes.argtypes = [I]
+        L.nvbe_verify_workspace_bytes.argtypes = [I, I]
         L.nvbe_verify_workspace_bytes.restype = ctypes.c_size_t
         L.nvbe_layer_verify.argtypes = [P] * 13 + [I] * 4 + [P, ctypes.c_size_t]
         _lib = L
@@ -345,8 +345,8 @@ def layer_sample(logits, temperatures, seeds, out, stream=None):
                                        rows, vocab))
 
 
-def verify_workspace_bytes(rows):
-    return library().nvbe_verify_workspace_bytes(rows)
+def verify_workspace_bytes(rows, batch):
+    return library().nvbe_verify_workspace_bytes(rows, batch)
 
 
 def layer_verify(logits, draft_logits, tokens, parents, uniforms, seeds, temperatures, cu_q, out_tokens, path, counts,
@@ -357,7 +357,7 @@ def layer_verify(logits, draft_logits, tokens, parents, uniforms, seeds, tempera
     committed token) first; draft_logits None: drafts without probabilities.
     out_tokens and path are [batch, max_q] int32, counts [batch] int32 and
     accept_prob [rows] FP32; seeds are int64 (or uint64) words. `workspace` (a
-    CUDA uint8 tensor of verify_workspace_bytes(rows)) is allocated per call
+    CUDA uint8 tensor of verify_workspace_bytes(rows, batch)) is allocated per call
     when not given."""
     import torch
 
@@ -391,7 +391,7 @@ def layer_verify(logits, draft_logits, tokens, parents, uniforms, seeds, tempera
             end, held = z, name in written
     ws = workspace
     if ws is None:
-        ws = torch.empty(max(16, verify_workspace_bytes(rows)), dtype=torch.uint8, device=logits.device)
+        ws = torch.empty(max(16, verify_workspace_bytes(rows, batch)), dtype=torch.uint8, device=logits.device)
     _check(library().nvbe_layer_verify(_s(stream), _p(logits), _p(draft_logits) if draft_logits is not None else None,
                                        _p(tokens), _p(parents), _p(uniforms), _p(seeds), _p(temperatures), _p(cu_q),
                                        _p(out_tokens), _p(path), _p(counts), _p(accept_prob), rows, batch, max_q,

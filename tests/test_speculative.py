@@ -198,8 +198,9 @@ def test_verify_refuses_on_the_host(nvb, bad):
 
 
 def test_verify_workspace_grows_with_the_rows(nvb):
-    assert nvb.model.verify_workspace_bytes(0) == 0
-    assert 0 < nvb.model.verify_workspace_bytes(1) <= nvb.model.verify_workspace_bytes(100)
+    size = nvb.model.verify_workspace_bytes
+    assert size(0, 1) == 0 and size(1, 0) == 0
+    assert 0 < size(1, 1) < size(100, 1) < size(100, 7)
 
 
 def test_engine_header_functions_are_exported(nvb):

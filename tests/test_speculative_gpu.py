@@ -531,7 +531,7 @@ def test_verify_captured_and_on_two_streams(nvb):
     runs = []
     for case in cases:
         a, o, stream = case.args(), case.outputs(), torch.cuda.Stream()
-        ws = torch.full((nvb.model.verify_workspace_bytes(len(case.tokens)),), 0xff, dtype=torch.uint8, device="cuda")
+        ws = torch.full((nvb.model.verify_workspace_bytes(len(case.tokens), len(case.sizes)),), 0xff, dtype=torch.uint8, device="cuda")
         torch.cuda.synchronize()
         step = lambda a=a, o=o, s=stream, ws=ws: nvb.model.layer_verify(**a, **o, stream=s, workspace=ws)  # noqa: E731
         step()
@@ -718,7 +718,7 @@ def test_a_step_of_attention_verification_and_compaction(nvb, captured):
     out, lse = torch.zeros_like(a["q"]), torch.zeros(case.rows, qh, device="cuda")
     new = torch.zeros(2, dtype=torch.int32, device="cuda")
     la, oa = nvb.tree_scratch(2, case.rows, qh, "cuda")
-    ws = torch.empty(nvb.model.verify_workspace_bytes(12), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(nvb.model.verify_workspace_bytes(12, 2), dtype=torch.uint8, device="cuda")
     stream = torch.cuda.Stream()
 
     def step():
