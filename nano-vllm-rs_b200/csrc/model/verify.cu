@@ -23,16 +23,17 @@
 // HBM; one exponential per logit takes 3/4 of the MUFU rate that goes with it.
 //
 // verify_sample_kernel follows the accepted children from the root and draws
-// the next token from the last node's row, cut over CTAs that hold 4096 tokens
-// in registers. A token's score is log P(v) plus Gumbel noise of u(v); the
-// noise takes a SplitMix64 and two logarithms, ~100 instructions in all, for
-// 152 thousand tokens a sequence. The best score of a slice with sum Z is
-// below log Z - 3 once in 10^9 times (exp(-e^3)), and a token reaches log Z - 3
-// only if 1 - u < e^3 P(v) / Z (-log u >= 1 - u). So the slice's sum is added
-// up first, the hash alone sorts out nearly all tokens, and the exact scores
-// of the ~20 that are left decide; a slice where none reached the bound scores
-// all its tokens. The slices' best meet in a 64-bit maximum (score, then the
-// lowest token), which no order of arrival changes.
+// the next token from the last node's row, cut over CTAs. A token's score is
+// log P(v) plus Gumbel noise of u(v); the noise takes a SplitMix64 and two
+// logarithms, ~100 instructions in all, for 152 thousand tokens a sequence. A
+// token can only beat a score L if 1 - u < P(v) e^-L (as -log u >= 1 - u), so
+// the hash alone sorts out nearly all tokens once L is known. The best score of
+// a CTA's first 4096 tokens, of weight Z, is below log Z - 5/2 five times in
+// a million (exp(-e^2.5)): with that L the ~12 tokens that are left are scored;
+// if none reached L all of them are. Their best is the L of the CTA's other
+// tokens. What bounds it is the issue rate: ~35 instructions a token. The CTAs'
+// best meet in a 64-bit maximum (score, then the lowest token), which no
+// order of arrival changes.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -47,8 +48,9 @@ namespace {
 
 using namespace sample_math;
 
-constexpr int kThreads = 256;        // of a nodes CTA
-constexpr int kSampleThreads = 512;  // of a sample CTA, 8 tokens a thread
+constexpr int kThreads = 512;        // of a nodes CTA
+constexpr int kSampleThreads = 512;  // of a sample CTA, 8 tokens a thread and chunk
+constexpr int kMaxList = 256;        // tokens of the first chunk that may reach its bound
 constexpr int kMaxCluster = 8;
 constexpr int kMaxNodes = 1024;      // of one tree (verify_max_nodes)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -58,10 +60,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // was rejected: the level that its rejection adds.
 struct VerifyRow {
   float m_p, z_p, m_q, z_q;  // max logit and sum of exp((l - max) / T)
-  float mass_q;              // child: Q's remaining sum (of its z_q) when it was tested
-  float left;                // child: sum max(P - Q, 0) at its rejection, <= 0: P stayed
+  float over_q, over_p;      // child: its level (Levels)
   int winner;                // node: accepted child's place in its sequence, or -1
-  int rejected;              // node: children rejected
+  int rejected;              // node: children rejected; its complement where they are not regular (Levels)
 };
 
 // The slices' best of a sequence; zeroed by the first kernel.
@@ -236,29 +237,66 @@ __device__ __forceinline__ float4 exchange(float4 v, Exchange& x, int& turn, uin
   return v;
 }
 
-// A node's children that were rejected, in order: what P has become.
+// A node's children that were rejected, in order: what P has become. `regular`:
+// every rejection left something, and where there are draft probabilities
+// P(t) < Q(t) held for its token, so that t has nothing left and a Q(t) that
+// goes on being subtracted changes nothing.
 struct Levels {
-  const int* token;     // [n]
-  const float* mass_q;  // [n]
-  const float* left;    // [n]
+  const int* token;      // [n]
+  const float* over_q;   // [n]: 1 / Q's remaining sum, 0 where nothing is left of Q
+  const float* over_p;   // [n]: 1 / sum max(P - Q, 0); 0: P stayed
+  bool has_q, regular;
 };
 
-// P(v) after the first `n` rejections, from P's weight over its sum (p) and
-// Q's weight (wq).
-__device__ __forceinline__ float remaining(float p, float wq, int v, bool has_q, const Levels& lv, int n) {
+// P of eight tokens from `at` on after the first `n` rejections, in place: x
+// holds P's weights over their sum, wq Q's weights.
+__device__ __forceinline__ void remaining8(float (&x)[8], const float (&wq)[8], int at, const Levels& lv, int n) {
   for (int i = 0; i < n; ++i) {
-    if (!(lv.left[i] > 0.0f)) continue;
-    if (has_q) {
+    const float over_p = lv.over_p[i];
+    if (over_p == 0.0f) continue;
+    uint32_t gone = 0;
+    if (!lv.has_q) {
+      const unsigned e = unsigned(lv.token[i] - at);
+      if (e < 8u) gone = 1u << e;
+    } else if (!lv.regular) {
+      for (int j = 0; j < i; ++j) {
+        const unsigned e = unsigned(lv.token[j] - at);
+        if (e < 8u) gone |= 1u << e;
+      }
+    }
+    const float over_q = lv.has_q ? lv.over_q[i] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float q = wq[e] * over_q;
+      if (lv.has_q)
+        x[e] = fmaxf(x[e] - (gone >> e & 1u ? 0.0f : q), 0.0f) * over_p;
+      else
+        x[e] = gone >> e & 1u ? 0.0f : x[e] * over_p;
+    }
+  }
+}
+
+// The same of one token.
+__device__ __forceinline__ float remaining(float x, float wq, int v, const Levels& lv, int n) {
+  for (int i = 0; i < n; ++i) {
+    if (lv.over_p[i] == 0.0f) continue;
+    if (lv.has_q) {
       bool gone = false;
       for (int j = 0; j < i; ++j) gone |= lv.token[j] == v;
-      const float q = gone || !(lv.mass_q[i] > 0.0f) ? 0.0f : __fdividef(wq, lv.mass_q[i]);
-      p = fmaxf(p - q, 0.0f);
+      x = fmaxf(x - (gone ? 0.0f : wq * lv.over_q[i]), 0.0f);
     } else if (lv.token[i] == v) {
-      p = 0.0f;
+      x = 0.0f;
     }
-    p = __fdividef(p, lv.left[i]);
+    x *= lv.over_p[i];
   }
-  return p;
+  return x;
+}
+
+// Weights of eight logits: NaN and infinities only where `safe`.
+__device__ __forceinline__ void weights8(const uint4& v, float m, float c, float scale, bool safe, float (&w)[8]) {
+  unpack8(v, w);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = (safe ? weight(w[e], m, c) : ex2((w[e] - m) * c)) * scale;
 }
 
 struct SumOp {
@@ -286,20 +324,25 @@ struct OnlineOp {  // (m_p, z_p, m_q, z_q)
 };
 
 // A cluster per node: its statistics, and its children's tests.
-__global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyParams p) {
   __shared__ Exchange s_x;
   __shared__ int s_child[kMaxNodes], s_token[kMaxNodes];
-  __shared__ float s_mass[kMaxNodes], s_left[kMaxNodes];
+  __shared__ float s_lp[kMaxNodes], s_lq[kMaxNodes], s_u[kMaxNodes];  // children's logits and uniforms
+  __shared__ float s_over_q[kMaxNodes], s_over_p[kMaxNodes];
   __shared__ int s_kids;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t size = cluster_size(), rank = cluster_rank();
   const int b = blockIdx.y, node = blockIdx.x / size;
-  const int begin = p.cu_q[b], n = min(min(p.cu_q[b + 1], p.rows) - begin, p.max_q);
+  const int begin = p.cu_q[b], next = p.cu_q[b + 1];
+  const float temperature = p.temps[b];
+  const int n = min(min(next, p.rows) - begin, p.max_q);
   if (node == 0 && rank == 0 && threadIdx.x == 0) p.best[b] = VerifyBest{0ull, 0u, 0u};
   if (begin < 0 || node >= n) return;  // all of a cluster
   VerifyRow* ws = p.ws + begin;
   const int row = begin + node;
+  const Row lp(p.logits + (long long)row * p.vocab, p.vocab);
+  const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
   if (threadIdx.x < 32) {
     int kids = 0;
     for (int base = node + 1; base < n; base += 32) {
@@ -307,9 +350,13 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
       const bool mine = i < n && p.parents[begin + i] == node;
       const unsigned hits = __ballot_sync(0xffffffffu, mine);
       if (mine) {
-        const int at = kids + __popc(hits & ((1u << threadIdx.x) - 1u));
+        const int at = kids + __popc(hits & ((1u << threadIdx.x) - 1u)), t = p.tokens[begin + i];
+        const bool inside = t >= 0 && t < p.vocab;
         s_child[at] = i;
-        s_token[at] = p.tokens[begin + i];
+        s_token[at] = t;
+        s_u[at] = p.uniforms[begin + i];
+        s_lp[at] = inside ? __bfloat162float(lp.p[t]) : -INFINITY;
+        s_lq[at] = inside && lq ? __bfloat162float(lq[t]) : -INFINITY;
       }
       kids += __popc(hits);
     }
@@ -329,9 +376,6 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
     }
     return;
   }
-  const Row lp(p.logits + (long long)row * p.vocab, p.vocab);
-  const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
-  const float temperature = p.temps[b];
   // this CTA's groups
   const int per = (lp.groups + int(size) - 1) / int(size), g0 = int(rank) * per, g1 = min(g0 + per, lp.groups);
   int turn = 0;
@@ -354,6 +398,7 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
         }
       }
     }
+    __syncwarp();
     const float4 top = exchange(make_float4(best, __int_as_float(best_index), 0.f, 0.f), s_x, turn, size, BestOp());
     best_index = __float_as_int(top.y);
     if (best_index == kNone) best_index = 0;
@@ -375,7 +420,7 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
   {
     Online op, oq;
     if (lq) {
-#pragma unroll 2
+#pragma unroll 4
       for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
         const int at = 8 * g - lp.shift;
         const uint4 vp = load8(lp.p, at, p.vocab), vq = load8(lq, at, p.vocab);
@@ -386,50 +431,52 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
 #pragma unroll 4
       for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) op.add(load8(lp.p, 8 * g - lp.shift, p.vocab), c);
     }
+    __syncwarp();
     const float4 all = exchange(make_float4(op.m, op.z, oq.m, oq.z), s_x, turn, size, OnlineOp{c});
     m_p = all.x;
     z_p = all.y;
     m_q = all.z;
     z_q = all.w;
   }
-  if (!(z_p == z_p) || !(z_q == z_q) || m_p == INFINITY || m_q == INFINITY) {
-    // NaN or infinite logits: the maxima are right, the sums are taken anew
+  // NaN or infinite logits (or none but -inf): the maxima are right, the sums are taken anew
+  const bool safe = !(z_p == z_p) || !(z_q == z_q) || m_p == INFINITY || m_q == INFINITY || m_p == -INFINITY ||
+                    (lq && m_q == -INFINITY);
+  if (safe) {
     float2 z = make_float2(0.f, 0.f);
+    float f[8];
     for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
       const int at = 8 * g - lp.shift;
-      float f[8];
-      unpack8(load8(lp.p, at, p.vocab), f);
+      weights8(load8(lp.p, at, p.vocab), m_p, c, 1.0f, true, f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) z.x += weight(f[i], m_p, c);
-      if (lq) {
-        unpack8(load8(lq, at, p.vocab), f);
+      for (int i = 0; i < 8; ++i) z.x += f[i];
+      if (!lq) continue;
+      weights8(load8(lq, at, p.vocab), m_q, c, 1.0f, true, f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) z.y += weight(f[i], m_q, c);
-      }
+      for (int i = 0; i < 8; ++i) z.y += f[i];
     }
+    __syncwarp();
     const float4 all = exchange(make_float4(z.x, z.y, 0.f, 0.f), s_x, turn, size, SumOp());
     z_p = all.x;
     z_q = all.y;
   }
-  const Levels lv{s_token, s_mass, s_left};
+  const float over_z = z_p > 0.0f ? 1.0f / z_p : 0.0f;
+  Levels lv{s_token, s_over_q, s_over_p, lq != nullptr, true};
   int winner = -1, rejected = 0;
   float mass = z_q;
   for (int i = 0; i < kids; ++i) {
     // every thread works out the child's probability
     const int t = s_token[i];
-    float a = 0.0f;
-    if (t >= 0 && t < p.vocab && z_p > 0.0f) {
-      const float wq = lq ? weight(__bfloat162float(lq[t]), m_q, c) : 0.0f;
-      const float pt = remaining(weight(__bfloat162float(lp.p[t]), m_p, c) / z_p, wq, t, lq != nullptr, lv, i);
-      float qt = 1.0f;
-      if (lq) {
-        bool gone = false;
-        for (int j = 0; j < i; ++j) gone |= s_token[j] == t;
-        qt = gone || !(mass > 0.0f) ? 0.0f : wq / mass;
-      }
-      a = !(pt > 0.0f) ? 0.0f : (qt > 0.0f ? fminf(pt / qt, 1.0f) : 1.0f);
+    const float wq = lq ? weight(s_lq[i], m_q, c) : 0.0f;
+    const float pt = remaining(weight(s_lp[i], m_p, c) * over_z, wq, t, lv, i);
+    const float over_q = mass > 0.0f ? 1.0f / mass : 0.0f;
+    float qt = 1.0f;
+    if (lq) {
+      bool gone = false;
+      for (int j = 0; j < i; ++j) gone |= s_token[j] == t;
+      qt = gone ? 0.0f : wq * over_q;
     }
-    const bool taken = p.uniforms[begin + s_child[i]] < a;
+    const float a = !(pt > 0.0f) ? 0.0f : (qt > 0.0f ? fminf(pt / qt, 1.0f) : 1.0f);
+    const bool taken = s_u[i] < a;
     if (writes) p.accept[begin + s_child[i]] = a;
     if (taken) {
       winner = s_child[i];
@@ -438,14 +485,15 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
       break;
     }
     rejected = i + 1;
+    lv.regular = lv.regular && (a < 1.0f || !lq);  // a uniform of 1 or more rejects anything
     if (threadIdx.x == 0) {
-      s_mass[i] = mass;
-      s_left[i] = 1.0f;  // its sum is what the pass below adds up
+      s_over_q[i] = over_q;
+      s_over_p[i] = 1.0f;  // what the pass below adds up is its inverse
     }
     if (i + 1 == kids) {  // no sibling needs the sums; the draw does without
       if (writes) {
-        ws[s_child[i]].mass_q = mass;
-        ws[s_child[i]].left = 1.0f;
+        ws[s_child[i]].over_q = over_q;
+        ws[s_child[i]].over_p = 1.0f;
       }
       break;
     }
@@ -456,30 +504,33 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
 #pragma unroll 2
     for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
       const int at = 8 * g - lp.shift;
-      float f[8], h[8];
-      unpack8(load8(lp.p, at, p.vocab), f);
-      if (lq) unpack8(load8(lq, at, p.vocab), h);
-      uint32_t gone = 0;
-      for (int j = 0; j <= i; ++j) {
-        const unsigned e = unsigned(s_token[j] - at);
-        if (e < 8u) gone |= 1u << e;
-      }
+      float x[8], w[8];
+      weights8(load8(lp.p, at, p.vocab), m_p, c, over_z, safe, x);
+      if (lq) {
+        weights8(load8(lq, at, p.vocab), m_q, c, 1.0f, safe, w);
+        uint32_t gone = 0;
+        for (int j = 0; j <= i; ++j) {
+          const unsigned e = unsigned(s_token[j] - at);
+          if (e < 8u) gone |= 1u << e;
+        }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float wq = lq ? weight(h[e], m_q, c) : 0.0f;
-        left += remaining(__fdividef(weight(f[e], m_p, c), z_p), wq, at + e, lq != nullptr, lv, i + 1);
-        rest += gone >> e & 1u ? 0.0f : wq;
+        for (int e = 0; e < 8; ++e) rest += gone >> e & 1u ? 0.0f : w[e];
       }
+      remaining8(x, w, at, lv, i + 1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) left += x[e];
     }
+    __syncwarp();
     const float4 all = exchange(make_float4(left, rest, 0.f, 0.f), s_x, turn, size, SumOp());
-    left = z_p > 0.0f ? all.x : 0.0f;
+    const float over_p = all.x > 0.0f ? 1.0f / all.x : 0.0f;
     if (threadIdx.x == 0) {
-      s_left[i] = left;
+      s_over_p[i] = over_p;
       if (rank == 0) {
-        ws[s_child[i]].mass_q = mass;
-        ws[s_child[i]].left = left;
+        ws[s_child[i]].over_q = over_q;
+        ws[s_child[i]].over_p = over_p;
       }
     }
+    lv.regular = lv.regular && over_p > 0.0f;
     mass = all.y;
     __syncthreads();
   }
@@ -490,7 +541,7 @@ __global__ void __launch_bounds__(kThreads) verify_nodes_kernel(const VerifyPara
     r.m_q = m_q;
     r.z_q = z_q;
     r.winner = winner;
-    r.rejected = rejected;
+    r.rejected = lv.regular && !safe ? rejected : ~rejected;
   }
   if (size > 1) cluster_sync();  // nobody leaves while its shared memory is read
 }
@@ -545,19 +596,22 @@ __device__ __forceinline__ unsigned long long sample_key(unsigned long long v, u
 }
 static_assert(kSampleThreads == 512, "the reductions above are over 16 warps");
 
-// CTA (slice, sequence): the accepted path, and the slice's best token.
-__global__ void __launch_bounds__(kSampleThreads) verify_sample_kernel(const VerifyParams p) {
+// CTA (part, sequence): the accepted path, and the best of the part's tokens.
+__global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const VerifyParams p) {
   __shared__ float s_red[16];
   __shared__ unsigned long long s_key[16];
   __shared__ int s_winner[kMaxNodes], s_path[kMaxNodes], s_token[kMaxNodes];
-  __shared__ float s_mass[kMaxNodes], s_left[kMaxNodes];
-  __shared__ int s_count, s_is_last;
+  __shared__ float s_over_q[kMaxNodes], s_over_p[kMaxNodes];
+  __shared__ int s_list[kMaxList];        // tokens that may reach the bound
+  __shared__ float2 s_list_x[kMaxList];   // their logits and probabilities
+  __shared__ int s_count, s_is_last, s_listed;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int b = blockIdx.y, begin = p.cu_q[b], n = min(min(p.cu_q[b + 1], p.rows) - begin, p.max_q);
+  const int b = blockIdx.y, begin = p.cu_q[b], next = p.cu_q[b + 1];
+  const float temperature = p.temps[b];
+  const int n = min(min(next, p.rows) - begin, p.max_q);
   int* tokens = p.out_tokens + (long long)b * p.max_q;
   int* path = p.path + (long long)b * p.max_q;
-  const float temperature = p.temps[b];
   if (begin < 0 || n <= 0) {
     if (blockIdx.x == 0) {
       for (int i = threadIdx.x; i < p.max_q; i += kSampleThreads) tokens[i] = path[i] = -1;
@@ -567,6 +621,7 @@ __global__ void __launch_bounds__(kSampleThreads) verify_sample_kernel(const Ver
   }
   const VerifyRow* ws = p.ws + begin;
   for (int i = threadIdx.x; i < n; i += kSampleThreads) s_winner[i] = ws[i].winner;
+  if (threadIdx.x == 0) s_listed = 0;
   __syncthreads();
   if (threadIdx.x == 0) {
     int at = 0, count = 1;
@@ -579,6 +634,26 @@ __global__ void __launch_bounds__(kSampleThreads) verify_sample_kernel(const Ver
   }
   __syncthreads();
   const int count = s_count, last = s_path[count - 1], row = begin + last;
+  const Row lp(p.logits + (long long)row * p.vocab, p.vocab);
+  const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
+  const uint64_t seed = p.seeds[row];
+  const int stored = ws[last].rejected;
+  const bool safe = stored < 0;  // see VerifyRow
+  const int rejected = safe ? ~stored : stored;
+  const float m_p = ws[last].m_p, z_p = ws[last].z_p, m_q = ws[last].m_q;  // of nodes with children
+  // this CTA's chunks of kSampleThreads groups
+  const int chunks = (lp.groups + kSampleThreads - 1) / kSampleThreads;
+  int chunk = blockIdx.x;
+  auto load = [&](int k, uint4& vp, uint4& vq) {
+    const int g = k * kSampleThreads + int(threadIdx.x), at = 8 * g - lp.shift;
+    vp = vq = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+    if (g < lp.groups) {
+      vp = load8(lp.p, at, p.vocab);
+      if (lq && rejected) vq = load8(lq, at, p.vocab);
+    }
+  };
+  uint4 vp, vq;
+  load(chunk, vp, vq);
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < p.max_q; i += kSampleThreads) {
       path[i] = i < count ? s_path[i] : -1;
@@ -586,22 +661,7 @@ __global__ void __launch_bounds__(kSampleThreads) verify_sample_kernel(const Ver
     }
     if (threadIdx.x == 0) p.counts[b] = count;
   }
-  const Row lp(p.logits + (long long)row * p.vocab, p.vocab);
-  const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
-  const uint64_t seed = p.seeds[row];
-  const int rejected = ws[last].rejected;
-  const int g = blockIdx.x * kSampleThreads + threadIdx.x, at = 8 * g - lp.shift;
-  // the slice's tokens, in registers from here on
-  uint4 vp = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u), vq = vp;
-  if (g < lp.groups) {
-    vp = load8(lp.p, at, p.vocab);
-    if (lq && rejected) vq = load8(lq, at, p.vocab);
-  }
-  float m_p = 0.f, z_p = 1.f, m_q = 0.f;
   if (rejected) {
-    m_p = ws[last].m_p;
-    z_p = ws[last].z_p;
-    m_q = ws[last].m_q;
     if (threadIdx.x < 32) {  // the rejected children's levels
       int kids = 0;
       for (int base = last + 1; base < n && kids < rejected; base += 32) {
@@ -611,70 +671,120 @@ __global__ void __launch_bounds__(kSampleThreads) verify_sample_kernel(const Ver
         const int k = kids + __popc(hits & ((1u << threadIdx.x) - 1u));
         if (mine && k < rejected) {
           s_token[k] = p.tokens[begin + i];
-          s_mass[k] = ws[i].mass_q;
-          s_left[k] = ws[i].left;
+          s_over_q[k] = ws[i].over_q;
+          s_over_p[k] = ws[i].over_p;
         }
         kids += __popc(hits);
       }
     }
     __syncthreads();
   }
-  const Levels lv{s_token, s_mass, s_left};
-  const float c = inv_temperature(temperature);
-  // P (over any common factor) of a token after `levels` rejections
-  auto probability = [&](float l, float lqv, int v, int levels) {
-    const float wq = lq ? weight(lqv, m_q, c) : 0.0f;
-    return remaining(__fdividef(weight(l, m_p, c), z_p), wq, v, lq != nullptr, lv, levels);
-  };
+  const Levels lv{s_token, s_over_q, s_over_p, lq != nullptr, !safe};
+  const float c = inv_temperature(temperature), over_z = z_p > 0.0f ? 1.0f / z_p : 0.0f;
   // the exact score: the sampler's where nothing was rejected
   auto score = [&](float l, float prob, int v, int levels) {
     if (levels == 0) return gumbel_score(l, temperature, seed, v);
     return prob > 0.0f ? logf(prob) - gumbel_log(seed, v) : NAN;
   };
-  float f[8], h[8], prob[8];
-  unpack8(vp, f);
-  unpack8(vq, h);
   unsigned long long best = 0ull;
   if (!(temperature > 0.0f)) {
+    float f[8];
+    for (; chunk < chunks; chunk += gridDim.x) {
+      const int at = 8 * (chunk * kSampleThreads + int(threadIdx.x)) - lp.shift;
+      const uint4 v = vp;
+      if (chunk + int(gridDim.x) < chunks) load(chunk + gridDim.x, vp, vq);
+      unpack8(v, f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (at + e >= 0 && at + e < p.vocab) best = max_key(best, sort_key(f[e], at + e));
+      for (int e = 0; e < 8; ++e)
+        if (at + e >= 0 && at + e < p.vocab) best = max_key(best, sort_key(f[e], at + e));
+    }
     best = sample_key(best, s_key);
   } else {
-    // weights of the slice; where nothing was rejected they are relative to its own maximum
-    float top = 0.0f;
-    if (rejected == 0) {
-      top = sample_max(max8(vp), s_red);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) prob[e] = weight(f[e], top, c);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) prob[e] = probability(f[e], h[e], at + e, rejected);
-    }
+    // P where something was rejected; else weights relative to the first chunk's maximum
+    float top = 0.0f, w[8], x[8];
+    auto probabilities = [&](const uint4& a, const uint4& q, int at, bool careful) {
+      if (rejected == 0) {
+        weights8(a, top, c, 1.0f, careful, x);
+      } else {
+        weights8(a, m_p, c, over_z, careful, x);
+        if (lq) weights8(q, m_q, c, 1.0f, careful, w);
+        remaining8(x, w, at, lv, rejected);
+      }
+    };
+    int at = 8 * (chunk * kSampleThreads + int(threadIdx.x)) - lp.shift;
+    if (rejected == 0) top = sample_max(max8(vp), s_red);
+    probabilities(vp, vq, at, safe);
     float z = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z += prob[e];
+    for (int e = 0; e < 8; ++e) z += x[e];
     z = sample_sum(z, s_red);
-    const bool bounded = z > 0.0f && top > -INFINITY && top < INFINITY;
-    // the bound that the tokens sorted out stay below (and 1/1000 for the roundings of the scores)
-    const float least = (rejected == 0 ? __fdividef(top, temperature) : 0.0f) + logf(z) - 3.0f;
-    // (1 - u) 2^23 is the inverted hash's 23 bits plus a half; e^3 and a little for the roundings
-    const float scale = __fdividef(20.1f * 8388608.0f, z);
-    bool all = !bounded;  // then every token is scored
-    for (;;) {
-      uint64_t x = uint64_t(int64_t(at)) * 0xd2b74407b1ce6e93ULL;
+    bool careful = safe;
+    if (!(z < INFINITY)) {  // NaN or infinite logits
+      careful = true;
+      probabilities(vp, vq, at, true);
+      z = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e, x += 0xd2b74407b1ce6e93ULL) {
-        const uint32_t k = uint32_t(splitmix64(seed ^ x) >> 41);
-        if ((all || float(0x7fffffu - k) + 0.5f < prob[e] * scale) && at + e >= 0 && at + e < p.vocab)
-          best = max_key(best, sort_key(score(f[e], prob[e], at + e, rejected), at + e));
-      }
-      best = sample_key(best, s_key);
-      if (all || key_score(best) >= least + 1e-3f * (1.0f + fabsf(least))) break;
-      all = true;
+      for (int e = 0; e < 8; ++e) z += x[e];
+      z = sample_sum(z, s_red);
     }
+    const float base = rejected == 0 ? __fdividef(top, temperature) : 0.0f;  // log of the weights' unit
+    const bool bounded = z > 0.0f && top > -INFINITY && top < INFINITY;
+    float least = base + logf(z) - 2.5f;  // a score; with 1/1000 for the roundings of the scores
+    least += 1e-3f * (1.0f + fabsf(least));
+    // e^2.5 and a little; (1 - u) is the inverted hash's 23 bits and a half step
+    const float first = __fdividef(12.2f, z);
+    // 1 - u < x scale: the 23 bits as the mantissa of a number in [1, 2)
+    auto may = [&](uint64_t hash, float prob, float scale) {
+      const uint32_t k = uint32_t(hash >> 41) ^ 0x7fffffu;
+      return __uint_as_float(0x3f800000u | k) <= fmaf(prob, scale, 1.0f);
+    };
+    if (bounded) {
+      uint64_t t = uint64_t(int64_t(at)) * 0xd2b74407b1ce6e93ULL;
+#pragma unroll
+      for (int e = 0; e < 8; ++e, t += 0xd2b74407b1ce6e93ULL)
+        if (may(splitmix64(seed ^ t), x[e], first) && at + e >= 0 && at + e < p.vocab) {
+          const int i = atomicAdd(&s_listed, 1);
+          if (i < kMaxList) {
+            const uint32_t word = e < 2 ? vp.x : e < 4 ? vp.y : e < 6 ? vp.z : vp.w;
+            s_list[i] = at + e;
+            s_list_x[i] = make_float2(__uint_as_float(e & 1 ? word & 0xffff0000u : word << 16), x[e]);
+          }
+        }
+      __syncthreads();
+      for (int i = threadIdx.x; i < min(s_listed, kMaxList); i += kSampleThreads)
+        best = max_key(best, sort_key(score(s_list_x[i].x, s_list_x[i].y, s_list[i], rejected), s_list[i]));
+    }
+    best = sample_key(best, s_key);
+    if (!bounded || s_listed > kMaxList || !(key_score(best) >= least)) {
+      best = 0ull;
+      float f[8];
+      unpack8(vp, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (at + e >= 0 && at + e < p.vocab)
+          best = max_key(best, sort_key(score(f[e], x[e], at + e, rejected), at + e));
+      best = sample_key(best, s_key);
+    }
+    // The other chunks: a token is scored where it may beat the best so far.
+    while ((chunk += gridDim.x) < chunks) {
+      at = 8 * (chunk * kSampleThreads + int(threadIdx.x)) - lp.shift;
+      load(chunk, vp, vq);
+      probabilities(vp, vq, at, careful);
+      float f[8];
+      unpack8(vp, f);
+      // e^-(best - base) and a little; everything is scored where there is no finite best yet
+      const float l = key_score(best);
+      const float scale = l > -INFINITY && l < INFINITY ? __expf(base - l + 2e-3f * (1.0f + fabsf(l))) : INFINITY;
+      uint64_t t = uint64_t(int64_t(at)) * 0xd2b74407b1ce6e93ULL;
+#pragma unroll
+      for (int e = 0; e < 8; ++e, t += 0xd2b74407b1ce6e93ULL)
+        if (!(scale < INFINITY) || !(x[e] == x[e]) || may(splitmix64(seed ^ t), x[e], scale))
+          if (at + e >= 0 && at + e < p.vocab)
+            best = max_key(best, sort_key(score(f[e], x[e], at + e, rejected), at + e));
+    }
+    best = sample_key(best, s_key);
   }
-  // join the slices; the last one writes the token
+  // join the parts; the last one writes the token
   if (threadIdx.x == 0) {
     if (best) atomicMax(&p.best[b].key, best);
     __threadfence();
@@ -689,7 +799,9 @@ __global__ void __launch_bounds__(kSampleThreads) verify_sample_kernel(const Ver
     best = 0ull;
     for (int v = threadIdx.x; v < p.vocab; v += kSampleThreads) {
       const float l = __bfloat162float(lp.p[v]);
-      const float pr = levels ? probability(l, lq ? __bfloat162float(lq[v]) : 0.0f, v, levels) : 0.0f;
+      float pr = 0.0f;
+      if (levels)
+        pr = remaining(weight(l, m_p, c) * over_z, lq ? weight(__bfloat162float(lq[v]), m_q, c) : 0.0f, v, lv, levels);
       best = max_key(best, sort_key(score(l, pr, v, levels), v));
     }
     key = sample_key(best, s_key);
@@ -712,9 +824,10 @@ cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft,
   VerifyParams p{static_cast<const __nv_bfloat16*>(logits), static_cast<const __nv_bfloat16*>(draft), tokens, parents,
                  uniforms, seeds, temps, cu_q, out_tokens, path, counts, accept, static_cast<VerifyRow*>(ws),
                  reinterpret_cast<VerifyBest*>(static_cast<VerifyRow*>(ws) + rows), rows, max_q, vocab};
-  // CTAs a node: enough that the nodes fill the GPU about four times over, none with less than 4096 logits.
+  // CTAs a node: 16 thousand logits each where the nodes fill the GPU, 4 thousand where they do not.
   int cluster = 1;
-  while (cluster < kMaxCluster && (long long)rows * cluster < 4LL * sms && vocab >= 2 * cluster * 4096) cluster *= 2;
+  while (cluster < kMaxCluster && vocab >= 2 * cluster * ((long long)rows * cluster < 2LL * sms ? 4096 : 16384))
+    cluster *= 2;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -730,7 +843,12 @@ cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft,
   cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_nodes_kernel, p);
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3(unsigned((vocab + 7 + 7) / 8 + kSampleThreads - 1) / kSampleThreads, unsigned(batch));
+  // Parts of a sequence: about as many as fit the GPU at once (two CTAs an SM), at most one for each chunk. A CTA's
+  // start (the path, the levels, the first bound) costs about as much as two chunks.
+  const int chunks = ((vocab + 14) / 8 + kSampleThreads - 1) / kSampleThreads;
+  int parts = int((2LL * sms + batch - 1) / batch);
+  parts = parts < 1 ? 1 : (parts > chunks ? chunks : parts);
+  cfg.gridDim = dim3(unsigned(parts), unsigned(batch));
   cfg.blockDim = dim3(kSampleThreads);
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, verify_sample_kernel, p);
