@@ -170,13 +170,6 @@ struct Online {
     }
     z += s0 + s1;
   }
-  __device__ __forceinline__ void join(float om, float oz, float c) {
-    const float nm = fmaxf(m, om);
-    // a side without a finite maximum has sum 0, or NaN to pass on
-    z = (m == nm || m == -INFINITY ? z : z * ex2((m - nm) * c)) +
-        (om == nm || om == -INFINITY ? oz : oz * ex2((om - nm) * c));
-    m = nm;
-  }
 };
 
 // ----------------------------------------------------------- CTA and cluster
@@ -190,52 +183,89 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
+__device__ __forceinline__ void cluster_arrive() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float4 peer_load(const float4* p, uint32_t rank) {
+__device__ __forceinline__ void peer_store(const float4* p, uint32_t rank, const float4& v) {
   const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(p));
   uint32_t remote;
-  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(remote)
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z),
+               "f"(v.w)
                : "memory");
-  return v;
 }
 
-// Joins four numbers of every thread of the cluster with `op` (commutative
-// pairs of float4), in one order for all: every thread gets the same result.
-// Alternating buffers: a CTA may be one exchange ahead of another.
+// Joins what the threads of a cluster hold. op(v, lanes) joins groups of
+// `lanes` neighbouring lanes; every thread gets the same result. CTAs leave
+// their parts in each other's shared memory, so nobody has to stay behind for a
+// reader. Two sets of buffers: a CTA may be one exchange ahead of another, not
+// two.
 struct Exchange {
   float4 warp[2][kThreads / 32];
-  float4 cta[2];
+  float4 cta[2][kMaxCluster];
 };
 template <class Op>
-__device__ __forceinline__ float4 exchange(float4 v, Exchange& x, int& turn, uint32_t size, Op op) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const float4 o = make_float4(__shfl_xor_sync(0xffffffffu, v.x, off), __shfl_xor_sync(0xffffffffu, v.y, off),
-                                 __shfl_xor_sync(0xffffffffu, v.z, off), __shfl_xor_sync(0xffffffffu, v.w, off));
-    v = op(v, o);
-  }
-  const int t = turn & 1;
+__device__ __forceinline__ float4 exchange(float4 v, const float4& none, Exchange& x, int& turn, uint32_t size,
+                                           uint32_t rank, Op op) {
+  static_assert(kThreads == 512, "16 warps join in half a warp's lanes");
+  const int t = turn & 1, lane = threadIdx.x & 31;
   ++turn;
-  if ((threadIdx.x & 31) == 0) x.warp[t][threadIdx.x >> 5] = v;
+  v = op(v, 32);
+  if (lane == 0) x.warp[t][threadIdx.x >> 5] = v;
   __syncthreads();
-  v = x.warp[t][0];
-#pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) v = op(v, x.warp[t][w]);
+  v = op(x.warp[t][lane & 15], 16);
   if (size == 1) return v;
-  if (threadIdx.x == 0) x.cta[t] = v;
-  cluster_sync();
-  v = peer_load(&x.cta[t], 0);
-  for (uint32_t r = 1; r < size; ++r) v = op(v, peer_load(&x.cta[t], r));
+  if (turn == 1) cluster_wait();  // the others have started (the arrival is at the kernel's start)
+  if (threadIdx.x < size) peer_store(&x.cta[t][rank], threadIdx.x, v);
+  cluster_arrive();
+  cluster_wait();
+  return op((lane & 7) < int(size) ? x.cta[t][lane & 7] : none, 8);
+}
+
+__device__ __forceinline__ float lanes_max(float v, int lanes) {
+  for (int off = lanes / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
   return v;
 }
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  for (int off = lanes / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+struct SumOp {  // two sums
+  __device__ __forceinline__ float4 operator()(const float4& v, int lanes) const {
+    return make_float4(lanes_sum(v.x, lanes), lanes_sum(v.y, lanes), 0.f, 0.f);
+  }
+};
+struct BestOp {  // (score, index bits)
+  __device__ __forceinline__ float4 operator()(const float4& v, int lanes) const {
+    float score = v.x;
+    int index = __float_as_int(v.y);
+    for (int off = lanes / 2; off > 0; off >>= 1) {
+      const float s = __shfl_xor_sync(0xffffffffu, score, off);
+      const int i = __shfl_xor_sync(0xffffffffu, index, off);
+      if (better(s, i, score, index)) {
+        score = s;
+        index = i;
+      }
+    }
+    return make_float4(score, __int_as_float(index), 0.f, 0.f);
+  }
+};
+struct OnlineOp {  // (m_p, z_p, m_q, z_q)
+  float c;
+  // a part without a finite maximum has sum 0, or NaN to pass on
+  __device__ __forceinline__ float scaled(float z, float m, float top) const {
+    return m == top || m == -INFINITY ? z : z * ex2((m - top) * c);
+  }
+  __device__ __forceinline__ float4 operator()(const float4& v, int lanes) const {
+    const float mp = lanes_max(v.x, lanes), mq = lanes_max(v.z, lanes);
+    return make_float4(mp, lanes_sum(scaled(v.y, v.x, mp), lanes), mq, lanes_sum(scaled(v.w, v.z, mq), lanes));
+  }
+};
 
 // A node's children that were rejected, in order: what P has become. `regular`:
 // every rejection left something, and where there are draft probabilities
@@ -248,35 +278,24 @@ struct Levels {
   bool has_q, regular;
 };
 
-// P of eight tokens from `at` on after the first `n` rejections, in place: x
-// holds P's weights over their sum, wq Q's weights.
+// P of eight tokens from `at` on after the first `n` rejections, in place, for
+// regular levels: x holds P's weights over their sum, wq Q's weights.
 __device__ __forceinline__ void remaining8(float (&x)[8], const float (&wq)[8], int at, const Levels& lv, int n) {
   for (int i = 0; i < n; ++i) {
     const float over_p = lv.over_p[i];
-    if (over_p == 0.0f) continue;
-    uint32_t gone = 0;
-    if (!lv.has_q) {
-      const unsigned e = unsigned(lv.token[i] - at);
-      if (e < 8u) gone = 1u << e;
-    } else if (!lv.regular) {
-      for (int j = 0; j < i; ++j) {
-        const unsigned e = unsigned(lv.token[j] - at);
-        if (e < 8u) gone |= 1u << e;
-      }
-    }
-    const float over_q = lv.has_q ? lv.over_q[i] : 0.0f;
+    if (lv.has_q) {
+      const float over_q = lv.over_q[i];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float q = wq[e] * over_q;
-      if (lv.has_q)
-        x[e] = fmaxf(x[e] - (gone >> e & 1u ? 0.0f : q), 0.0f) * over_p;
-      else
-        x[e] = gone >> e & 1u ? 0.0f : x[e] * over_p;
+      for (int e = 0; e < 8; ++e) x[e] = fmaxf(fmaf(-over_q, wq[e], x[e]), 0.0f) * over_p;
+    } else {
+      const int gone = lv.token[i] - at;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = e == gone ? 0.0f : x[e] * over_p;
     }
   }
 }
 
-// The same of one token.
+// The same of one token, for any levels.
 __device__ __forceinline__ float remaining(float x, float wq, int v, const Levels& lv, int n) {
   for (int i = 0; i < n; ++i) {
     if (lv.over_p[i] == 0.0f) continue;
@@ -292,36 +311,12 @@ __device__ __forceinline__ float remaining(float x, float wq, int v, const Level
   return x;
 }
 
-// Weights of eight logits: NaN and infinities only where `safe`.
-__device__ __forceinline__ void weights8(const uint4& v, float m, float c, float scale, bool safe, float (&w)[8]) {
+// Weights of eight logits without NaN and with a finite maximum.
+__device__ __forceinline__ void weights8(const uint4& v, float m, float c, float scale, float (&w)[8]) {
   unpack8(v, w);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = (safe ? weight(w[e], m, c) : ex2((w[e] - m) * c)) * scale;
+  for (int e = 0; e < 8; ++e) w[e] = ex2((w[e] - m) * c) * scale;
 }
-
-struct SumOp {
-  __device__ float4 operator()(const float4& a, const float4& b) const {
-    return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
-  }
-};
-struct BestOp {  // (score, index bits)
-  __device__ float4 operator()(const float4& a, const float4& b) const {
-    return better(b.x, __float_as_int(b.y), a.x, __float_as_int(a.y)) ? b : a;
-  }
-};
-struct OnlineOp {  // (m_p, z_p, m_q, z_q)
-  float c;
-  __device__ float4 operator()(const float4& a, const float4& b) const {
-    Online p, q;
-    p.m = a.x;
-    p.z = a.y;
-    q.m = a.z;
-    q.z = a.w;
-    p.join(b.x, b.y, c);
-    q.join(b.z, b.w, c);
-    return make_float4(p.m, p.z, q.m, q.z);
-  }
-};
 
 // A cluster per node: its statistics, and its children's tests.
 __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyParams p) {
@@ -329,41 +324,41 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
   __shared__ int s_child[kMaxNodes], s_token[kMaxNodes];
   __shared__ float s_lp[kMaxNodes], s_lq[kMaxNodes], s_u[kMaxNodes];  // children's logits and uniforms
   __shared__ float s_over_q[kMaxNodes], s_over_p[kMaxNodes];
-  __shared__ int s_kids;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t size = cluster_size(), rank = cluster_rank();
+  if (size > 1) cluster_arrive();
   const int b = blockIdx.y, node = blockIdx.x / size;
   const int begin = p.cu_q[b], next = p.cu_q[b + 1];
   const float temperature = p.temps[b];
   const int n = min(min(next, p.rows) - begin, p.max_q);
   if (node == 0 && rank == 0 && threadIdx.x == 0) p.best[b] = VerifyBest{0ull, 0u, 0u};
-  if (begin < 0 || node >= n) return;  // all of a cluster
+  if (begin < 0 || node >= n) {  // all of a cluster
+    if (size > 1) cluster_wait();
+    return;
+  }
   VerifyRow* ws = p.ws + begin;
   const int row = begin + node;
   const Row lp(p.logits + (long long)row * p.vocab, p.vocab);
   const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
-  if (threadIdx.x < 32) {
-    int kids = 0;
-    for (int base = node + 1; base < n; base += 32) {
-      const int i = base + threadIdx.x;
-      const bool mine = i < n && p.parents[begin + i] == node;
-      const unsigned hits = __ballot_sync(0xffffffffu, mine);
-      if (mine) {
-        const int at = kids + __popc(hits & ((1u << threadIdx.x) - 1u)), t = p.tokens[begin + i];
-        const bool inside = t >= 0 && t < p.vocab;
-        s_child[at] = i;
-        s_token[at] = t;
-        s_u[at] = p.uniforms[begin + i];
-        s_lp[at] = inside ? __bfloat162float(lp.p[t]) : -INFINITY;
-        s_lq[at] = inside && lq ? __bfloat162float(lq[t]) : -INFINITY;
-      }
-      kids += __popc(hits);
+  // Every warp counts the children; the first one collects them, beside the others' pass over the logits.
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int kids = 0;
+  for (int base = node + 1; base < n; base += 32) {
+    const int i = base + lane;
+    const bool mine = i < n && p.parents[begin + i] == node;
+    const unsigned hits = __ballot_sync(0xffffffffu, mine);
+    if (mine && warp == 0) {
+      const int at = kids + __popc(hits & ((1u << lane) - 1u)), t = p.tokens[begin + i];
+      const bool inside = t >= 0 && t < p.vocab;
+      s_child[at] = i;
+      s_token[at] = t;
+      s_u[at] = p.uniforms[begin + i];
+      s_lp[at] = inside ? __bfloat162float(lp.p[t]) : -INFINITY;
+      s_lq[at] = inside && lq ? __bfloat162float(lq[t]) : -INFINITY;
     }
-    if (threadIdx.x == 0) s_kids = kids;
+    kids += __popc(hits);
   }
-  __syncthreads();
-  const int kids = s_kids;
   const bool writes = rank == 0 && threadIdx.x == 0;
   if (writes) {  // a node that is no node's child is tested by nobody
     const int parent = p.parents[row];
@@ -374,6 +369,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
       ws[node].winner = -1;
       ws[node].rejected = 0;
     }
+    if (size > 1) cluster_wait();
     return;
   }
   // this CTA's groups
@@ -398,8 +394,9 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
         }
       }
     }
-    __syncwarp();
-    const float4 top = exchange(make_float4(best, __int_as_float(best_index), 0.f, 0.f), s_x, turn, size, BestOp());
+    const float4 top = exchange(make_float4(best, __int_as_float(best_index), 0.f, 0.f),
+                                make_float4(-INFINITY, __int_as_float(kNone), 0.f, 0.f), s_x, turn, size, rank,
+                                BestOp());
     best_index = __float_as_int(top.y);
     if (best_index == kNone) best_index = 0;
     if (writes) {
@@ -412,7 +409,6 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
       ws[node].winner = winner;
       ws[node].rejected = 0;
     }
-    if (size > 1) cluster_sync();  // nobody leaves while its shared memory is read
     return;
   }
   const float c = inv_temperature(temperature);
@@ -431,8 +427,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
 #pragma unroll 4
       for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) op.add(load8(lp.p, 8 * g - lp.shift, p.vocab), c);
     }
-    __syncwarp();
-    const float4 all = exchange(make_float4(op.m, op.z, oq.m, oq.z), s_x, turn, size, OnlineOp{c});
+    const float4 all = exchange(make_float4(op.m, op.z, oq.m, oq.z), make_float4(-INFINITY, 0.f, -INFINITY, 0.f), s_x,
+                                turn, size, rank, OnlineOp{c});
     m_p = all.x;
     z_p = all.y;
     m_q = all.z;
@@ -443,19 +439,13 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
                     (lq && m_q == -INFINITY);
   if (safe) {
     float2 z = make_float2(0.f, 0.f);
-    float f[8];
-    for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
-      const int at = 8 * g - lp.shift;
-      weights8(load8(lp.p, at, p.vocab), m_p, c, 1.0f, true, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) z.x += f[i];
-      if (!lq) continue;
-      weights8(load8(lq, at, p.vocab), m_q, c, 1.0f, true, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) z.y += f[i];
+    for (int v = 8 * g0 - lp.shift + int(threadIdx.x); v < min(8 * g1 - lp.shift, p.vocab); v += kThreads) {
+      if (v < 0) continue;
+      z.x += weight(__bfloat162float(lp.p[v]), m_p, c);
+      if (lq) z.y += weight(__bfloat162float(lq[v]), m_q, c);
     }
-    __syncwarp();
-    const float4 all = exchange(make_float4(z.x, z.y, 0.f, 0.f), s_x, turn, size, SumOp());
+    const float4 all = exchange(make_float4(z.x, z.y, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f), s_x, turn, size, rank,
+                                SumOp());
     z_p = all.x;
     z_q = all.y;
   }
@@ -501,27 +491,38 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
     // what is left of P, and Q's sum without the rejected tokens (added up anew: a difference would cancel where the
     // tokens had most)
     float left = 0.0f, rest = 0.0f;
+    if (lv.regular && !safe) {
 #pragma unroll 2
-    for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
-      const int at = 8 * g - lp.shift;
-      float x[8], w[8];
-      weights8(load8(lp.p, at, p.vocab), m_p, c, over_z, safe, x);
-      if (lq) {
-        weights8(load8(lq, at, p.vocab), m_q, c, 1.0f, safe, w);
-        uint32_t gone = 0;
-        for (int j = 0; j <= i; ++j) {
-          const unsigned e = unsigned(s_token[j] - at);
-          if (e < 8u) gone |= 1u << e;
+      for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
+        const int at = 8 * g - lp.shift;
+        float x[8], w[8];
+        weights8(load8(lp.p, at, p.vocab), m_p, c, over_z, x);
+        if (lq) {
+          weights8(load8(lq, at, p.vocab), m_q, c, 1.0f, w);
+          uint32_t gone = 0;
+          for (int j = 0; j <= i; ++j) {
+            const unsigned e = unsigned(s_token[j] - at);
+            if (e < 8u) gone |= 1u << e;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) rest += gone >> e & 1u ? 0.0f : w[e];
         }
+        remaining8(x, w, at, lv, i + 1);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) rest += gone >> e & 1u ? 0.0f : w[e];
+        for (int e = 0; e < 8; ++e) left += x[e];
       }
-      remaining8(x, w, at, lv, i + 1);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) left += x[e];
+    } else {
+      for (int v = 8 * g0 - lp.shift + int(threadIdx.x); v < min(8 * g1 - lp.shift, p.vocab); v += kThreads) {
+        if (v < 0) continue;
+        const float wv = lq ? weight(__bfloat162float(lq[v]), m_q, c) : 0.0f;
+        bool gone = false;
+        for (int j = 0; j <= i; ++j) gone |= s_token[j] == v;
+        rest += gone ? 0.0f : wv;
+        left += remaining(weight(__bfloat162float(lp.p[v]), m_p, c) * over_z, wv, v, lv, i + 1);
+      }
     }
-    __syncwarp();
-    const float4 all = exchange(make_float4(left, rest, 0.f, 0.f), s_x, turn, size, SumOp());
+    const float4 all = exchange(make_float4(left, rest, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f), s_x, turn, size,
+                                rank, SumOp());
     const float over_p = all.x > 0.0f ? 1.0f / all.x : 0.0f;
     if (threadIdx.x == 0) {
       s_over_p[i] = over_p;
@@ -543,7 +544,6 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
     r.winner = winner;
     r.rejected = lv.regular && !safe ? rejected : ~rejected;
   }
-  if (size > 1) cluster_sync();  // nobody leaves while its shared memory is read
 }
 
 // ---------------------------------------------------------------- next token
@@ -638,8 +638,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
   const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
   const uint64_t seed = p.seeds[row];
   const int stored = ws[last].rejected;
-  const bool safe = stored < 0;  // see VerifyRow
-  const int rejected = safe ? ~stored : stored;
+  const int rejected = stored < 0 ? ~stored : stored;  // see VerifyRow
   const float m_p = ws[last].m_p, z_p = ws[last].z_p, m_q = ws[last].m_q;  // of nodes with children
   // this CTA's chunks of kSampleThreads groups
   const int chunks = (lp.groups + kSampleThreads - 1) / kSampleThreads;
@@ -679,7 +678,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
     }
     __syncthreads();
   }
-  const Levels lv{s_token, s_over_q, s_over_p, lq != nullptr, !safe};
+  const Levels lv{s_token, s_over_q, s_over_p, lq != nullptr, stored >= 0};
   const float c = inv_temperature(temperature), over_z = z_p > 0.0f ? 1.0f / z_p : 0.0f;
   // the exact score: the sampler's where nothing was rejected
   auto score = [&](float l, float prob, int v, int levels) {
@@ -702,43 +701,48 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
   } else {
     // P where something was rejected; else weights relative to the first chunk's maximum
     float top = 0.0f, w[8], x[8];
-    auto probabilities = [&](const uint4& a, const uint4& q, int at, bool careful) {
+    auto probabilities = [&](const uint4& a, const uint4& q, int at) {
       if (rejected == 0) {
-        weights8(a, top, c, 1.0f, careful, x);
+        weights8(a, top, c, 1.0f, x);
       } else {
-        weights8(a, m_p, c, over_z, careful, x);
-        if (lq) weights8(q, m_q, c, 1.0f, careful, w);
+        weights8(a, m_p, c, over_z, x);
+        if (lq) weights8(q, m_q, c, 1.0f, w);
         remaining8(x, w, at, lv, rejected);
+      }
+    };
+    // Every token of a chunk, for what the bounds do not cover (NaN and infinite logits, irregular levels).
+    auto score_all = [&](int k) {
+      const int from = 8 * k * kSampleThreads - lp.shift, to = min(from + 8 * kSampleThreads, p.vocab);
+      for (int v = from + int(threadIdx.x); v < to; v += kSampleThreads) {
+        if (v < 0) continue;
+        const float l = __bfloat162float(lp.p[v]);
+        float pr = 0.0f;
+        if (rejected)
+          pr = remaining(weight(l, m_p, c) * over_z, lq ? weight(__bfloat162float(lq[v]), m_q, c) : 0.0f, v, lv,
+                         rejected);
+        best = max_key(best, sort_key(score(l, pr, v, rejected), v));
       }
     };
     int at = 8 * (chunk * kSampleThreads + int(threadIdx.x)) - lp.shift;
     if (rejected == 0) top = sample_max(max8(vp), s_red);
-    probabilities(vp, vq, at, safe);
+    probabilities(vp, vq, at);
     float z = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) z += x[e];
     z = sample_sum(z, s_red);
-    bool careful = safe;
-    if (!(z < INFINITY)) {  // NaN or infinite logits
-      careful = true;
-      probabilities(vp, vq, at, true);
-      z = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z += x[e];
-      z = sample_sum(z, s_red);
-    }
     const float base = rejected == 0 ? __fdividef(top, temperature) : 0.0f;  // log of the weights' unit
-    const bool bounded = z > 0.0f && top > -INFINITY && top < INFINITY;
+    // false with NaN too
+    const bool bounded = lv.regular && z > 0.0f && z < INFINITY && top > -INFINITY && top < INFINITY;
     float least = base + logf(z) - 2.5f;  // a score; with 1/1000 for the roundings of the scores
     least += 1e-3f * (1.0f + fabsf(least));
-    // e^2.5 and a little; (1 - u) is the inverted hash's 23 bits and a half step
-    const float first = __fdividef(12.2f, z);
-    // 1 - u < x scale: the 23 bits as the mantissa of a number in [1, 2)
+    // 1 - u < x scale, 1 - u being the inverted hash's 23 bits and a half step: the bits as the mantissa of a number
+    // in [1, 2). NaN may.
     auto may = [&](uint64_t hash, float prob, float scale) {
       const uint32_t k = uint32_t(hash >> 41) ^ 0x7fffffu;
-      return __uint_as_float(0x3f800000u | k) <= fmaf(prob, scale, 1.0f);
+      return !(__uint_as_float(0x3f800000u | k) > fmaf(prob, scale, 1.0f));
     };
     if (bounded) {
+      const float first = __fdividef(12.2f, z);  // e^2.5 and a little
       uint64_t t = uint64_t(int64_t(at)) * 0xd2b74407b1ce6e93ULL;
 #pragma unroll
       for (int e = 0; e < 8; ++e, t += 0xd2b74407b1ce6e93ULL)
@@ -756,31 +760,39 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
     }
     best = sample_key(best, s_key);
     if (!bounded || s_listed > kMaxList || !(key_score(best) >= least)) {
-      best = 0ull;
-      float f[8];
-      unpack8(vp, f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (at + e >= 0 && at + e < p.vocab)
-          best = max_key(best, sort_key(score(f[e], x[e], at + e, rejected), at + e));
+      score_all(chunk);
       best = sample_key(best, s_key);
     }
     // The other chunks: a token is scored where it may beat the best so far.
+    if (chunk + int(gridDim.x) < chunks) load(chunk + gridDim.x, vp, vq);
     while ((chunk += gridDim.x) < chunks) {
-      at = 8 * (chunk * kSampleThreads + int(threadIdx.x)) - lp.shift;
-      load(chunk, vp, vq);
-      probabilities(vp, vq, at, careful);
-      float f[8];
-      unpack8(vp, f);
-      // e^-(best - base) and a little; everything is scored where there is no finite best yet
       const float l = key_score(best);
-      const float scale = l > -INFINITY && l < INFINITY ? __expf(base - l + 2e-3f * (1.0f + fabsf(l))) : INFINITY;
+      if (!lv.regular || !(l > -INFINITY && l < INFINITY)) {
+        score_all(chunk);
+        continue;
+      }
+      at = 8 * (chunk * kSampleThreads + int(threadIdx.x)) - lp.shift;
+      const uint4 v = vp;
+      probabilities(vp, vq, at);
+      if (chunk + int(gridDim.x) < chunks) load(chunk + gridDim.x, vp, vq);
+      const float scale = __expf(base - l + 2e-3f * (1.0f + fabsf(l)));  // e^-(best - base) and a little
       uint64_t t = uint64_t(int64_t(at)) * 0xd2b74407b1ce6e93ULL;
+      uint32_t hits = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e, t += 0xd2b74407b1ce6e93ULL)
-        if (!(scale < INFINITY) || !(x[e] == x[e]) || may(splitmix64(seed ^ t), x[e], scale))
-          if (at + e >= 0 && at + e < p.vocab)
-            best = max_key(best, sort_key(score(f[e], x[e], at + e, rejected), at + e));
+        hits |= may(splitmix64(seed ^ t), x[e], scale) ? 1u << e : 0u;
+      while (hits) {
+        const int e = __ffs(hits) - 1;
+        hits &= hits - 1;
+        if (at + e < 0 || at + e >= p.vocab) continue;
+        const uint32_t word = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
+        float pr = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) pr = e == i ? x[i] : pr;
+        best = max_key(best, sort_key(score(__uint_as_float(e & 1 ? word & 0xffff0000u : word << 16), pr, at + e,
+                                            rejected),
+                                      at + e));
+      }
     }
     best = sample_key(best, s_key);
   }
@@ -824,9 +836,9 @@ cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft,
   VerifyParams p{static_cast<const __nv_bfloat16*>(logits), static_cast<const __nv_bfloat16*>(draft), tokens, parents,
                  uniforms, seeds, temps, cu_q, out_tokens, path, counts, accept, static_cast<VerifyRow*>(ws),
                  reinterpret_cast<VerifyBest*>(static_cast<VerifyRow*>(ws) + rows), rows, max_q, vocab};
-  // CTAs a node: 16 thousand logits each where the nodes fill the GPU, 4 thousand where they do not.
+  // CTAs a node: 32 thousand logits each where the nodes fill the GPU, 4 thousand where they do not.
   int cluster = 1;
-  while (cluster < kMaxCluster && vocab >= 2 * cluster * ((long long)rows * cluster < 2LL * sms ? 4096 : 16384))
+  while (cluster < kMaxCluster && vocab >= 2 * cluster * ((long long)rows * cluster < 2LL * sms ? 4096 : 32768))
     cluster *= 2;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
