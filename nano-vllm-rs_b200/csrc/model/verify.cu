@@ -48,7 +48,7 @@ namespace {
 
 using namespace sample_math;
 
-constexpr int kThreads = 512;        // of a nodes CTA
+constexpr int kThreads = 256;        // of a nodes CTA
 constexpr int kSampleThreads = 512;  // of a sample CTA, 8 tokens a thread and chunk
 constexpr int kMaxList = 256;        // tokens of the first chunk that may reach its bound
 constexpr int kMaxCluster = 8;
@@ -96,6 +96,32 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Pairs of FP32 in one instruction (the ALU's f32x2 forms).
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mov.b64 rc, {%6, %7};\n\tfma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
 // exp((l - m) / T) with c = log2(e) / T. The difference of two BF16 is exact
 // in FP32 (or as good), so the argument's error is relative. NaN logits have
 // no probability; an infinite one takes all of it.
@@ -131,6 +157,40 @@ __device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int at, int voc
   return make_uint4(uint32_t(lo), uint32_t(lo >> 32), uint32_t(hi), uint32_t(hi >> 32));
 }
 
+// Calls f(at, p's group, q's group) for a thread's groups in [g0, g1) (elements
+// from `at` on). kBatch groups' loads are issued before any is worked on; groups
+// that cross an end of the row, and all where q is aligned otherwise than p,
+// are read element by element.
+template <int kBatch, class F>
+__device__ __forceinline__ void each_group(const Row& p, const __nv_bfloat16* q, int g0, int g1, F&& f) {
+  const bool even = q == nullptr || ((reinterpret_cast<uintptr_t>(q) ^ reinterpret_cast<uintptr_t>(p.p)) & 15) == 0;
+  const int lo = even ? max(g0, p.shift ? 1 : 0) : g1, hi = even ? min(g1, (p.vocab + p.shift) >> 3) : g1;
+  const uint4* vp = reinterpret_cast<const uint4*>(p.p - p.shift);
+  const uint4* vq = reinterpret_cast<const uint4*>(q ? q - p.shift : p.p - p.shift);
+  for (int g = lo + int(threadIdx.x); g < hi; g += kBatch * kThreads) {
+    uint4 a[kBatch], b[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (g + u * kThreads < hi) {
+        a[u] = __ldg(vp + g + u * kThreads);
+        if (q) b[u] = __ldg(vq + g + u * kThreads);
+      }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (g + u * kThreads < hi) f(8 * (g + u * kThreads) - p.shift, a[u], b[u]);
+  }
+  for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
+    if (g >= lo && g < hi) {
+      g += max(0, (hi - 1 - g) / kThreads) * kThreads;  // past the groups above
+      continue;
+    }
+    const int at = 8 * g - p.shift;
+    uint4 b = make_uint4(0u, 0u, 0u, 0u);
+    if (q) b = load8(q, at, p.vocab);
+    f(at, load8(p.p, at, p.vocab), b);
+  }
+}
+
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -147,6 +207,16 @@ __device__ __forceinline__ float max8(const uint4& v) {
   return fmaxf(__low2float(m), __high2float(m));
 }
 
+// (l - m) c of eight logits.
+__device__ __forceinline__ void exponents8(const uint4& v, float m, float c, float2 (&x)[4]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x[i] = mul2(add2(make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)),
+                     make_float2(-m, -m)),
+                make_float2(c, c));
+}
+
 // Running maximum and sum of exp((l - m) / T). NaN and infinite logits make
 // the sum NaN (the caller then adds it up anew with weight()).
 struct Online {
@@ -161,14 +231,12 @@ struct Online {
       if (!(gm == gm)) z = NAN;
       return;
     }
-    float f[8], s0 = 0.0f, s1 = 0.0f;
-    unpack8(v, f);
+    float2 w[4];
+    exponents8(v, m, c, w);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      s0 += ex2((f[i] - m) * c);
-      s1 += ex2((f[i + 1] - m) * c);
-    }
-    z += s0 + s1;
+    for (int i = 0; i < 4; ++i) w[i] = make_float2(ex2(w[i].x), ex2(w[i].y));
+    const float2 t = add2(add2(w[0], w[1]), add2(w[2], w[3]));
+    z += t.x + t.y;
   }
 };
 
@@ -212,13 +280,14 @@ struct Exchange {
 template <class Op>
 __device__ __forceinline__ float4 exchange(float4 v, const float4& none, Exchange& x, int& turn, uint32_t size,
                                            uint32_t rank, Op op) {
-  static_assert(kThreads == 512, "16 warps join in half a warp's lanes");
+  constexpr int kWarps = kThreads / 32;
+  static_assert((kWarps & (kWarps - 1)) == 0 && kWarps <= 32, "the warps' parts join in one warp's lanes");
   const int t = turn & 1, lane = threadIdx.x & 31;
   ++turn;
   v = op(v, 32);
   if (lane == 0) x.warp[t][threadIdx.x >> 5] = v;
   __syncthreads();
-  v = op(x.warp[t][lane & 15], 16);
+  v = op(x.warp[t][lane & (kWarps - 1)], kWarps);
   if (size == 1) return v;
   if (turn == 1) cluster_wait();  // the others have started (the arrival is at the kernel's start)
   if (threadIdx.x < size) peer_store(&x.cta[t][rank], threadIdx.x, v);
@@ -280,17 +349,21 @@ struct Levels {
 
 // P of eight tokens from `at` on after the first `n` rejections, in place, for
 // regular levels: x holds P's weights over their sum, wq Q's weights.
-__device__ __forceinline__ void remaining8(float (&x)[8], const float (&wq)[8], int at, const Levels& lv, int n) {
+__device__ __forceinline__ void remaining8(float2 (&x)[4], const float2 (&wq)[4], int at, const Levels& lv, int n) {
   for (int i = 0; i < n; ++i) {
     const float over_p = lv.over_p[i];
     if (lv.has_q) {
-      const float over_q = lv.over_q[i];
+      const float less = -lv.over_q[i];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = fmaxf(fmaf(-over_q, wq[e], x[e]), 0.0f) * over_p;
+      for (int e = 0; e < 4; ++e) {
+        const float2 d = fma2(make_float2(less, less), wq[e], x[e]);
+        x[e] = mul2(make_float2(fmaxf(d.x, 0.0f), fmaxf(d.y, 0.0f)), make_float2(over_p, over_p));
+      }
     } else {
       const int gone = lv.token[i] - at;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = e == gone ? 0.0f : x[e] * over_p;
+      for (int e = 0; e < 4; ++e)
+        x[e] = make_float2(2 * e == gone ? 0.0f : x[e].x * over_p, 2 * e + 1 == gone ? 0.0f : x[e].y * over_p);
     }
   }
 }
@@ -312,18 +385,19 @@ __device__ __forceinline__ float remaining(float x, float wq, int v, const Level
 }
 
 // Weights of eight logits without NaN and with a finite maximum.
-__device__ __forceinline__ void weights8(const uint4& v, float m, float c, float scale, float (&w)[8]) {
-  unpack8(v, w);
+__device__ __forceinline__ void weights8(const uint4& v, float m, float c, float2 (&w)[4]) {
+  exponents8(v, m, c, w);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = ex2((w[e] - m) * c) * scale;
+  for (int e = 0; e < 4; ++e) w[e] = make_float2(ex2(w[e].x), ex2(w[e].y));
 }
 
 // A cluster per node: its statistics, and its children's tests.
-__global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kThreads, 4) verify_nodes_kernel(const VerifyParams p) {
   __shared__ Exchange s_x;
   __shared__ int s_child[kMaxNodes], s_token[kMaxNodes];
   __shared__ float s_lp[kMaxNodes], s_lq[kMaxNodes], s_u[kMaxNodes];  // children's logits and uniforms
   __shared__ float s_over_q[kMaxNodes], s_over_p[kMaxNodes];
+  __shared__ int s_tested[2];  // of two children in a row: 1 accepted, 0 rejected, -1 rejected irregularly
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t size = cluster_size(), rank = cluster_rank();
@@ -378,22 +452,20 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
   if (!(temperature > 0.0f)) {
     float best = -INFINITY;
     int best_index = kNone;
-#pragma unroll 4
-    for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
-      const uint4 v = load8(lp.p, 8 * g - lp.shift, p.vocab);
-      if (max8(v) > best || best_index == kNone) {
+    each_group<4>(lp, nullptr, g0, g1, [&](int at, const uint4& v, const uint4&) {
+      if (max8(v) >= best || best_index == kNone) {  // a row's first tokens may come last
         float f[8];
         unpack8(v, f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int t = 8 * g - lp.shift + i;
+          const int t = at + i;
           if (t >= 0 && t < p.vocab && better(f[i], t, best, best_index)) {
             best = f[i];
             best_index = t;
           }
         }
       }
-    }
+    });
     const float4 top = exchange(make_float4(best, __int_as_float(best_index), 0.f, 0.f),
                                 make_float4(-INFINITY, __int_as_float(kNone), 0.f, 0.f), s_x, turn, size, rank,
                                 BestOp());
@@ -415,18 +487,13 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
   float m_p, z_p, m_q, z_q;
   {
     Online op, oq;
-    if (lq) {
-#pragma unroll 4
-      for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
-        const int at = 8 * g - lp.shift;
-        const uint4 vp = load8(lp.p, at, p.vocab), vq = load8(lq, at, p.vocab);
+    if (lq)
+      each_group<2>(lp, lq, g0, g1, [&](int, const uint4& vp, const uint4& vq) {
         op.add(vp, c);
         oq.add(vq, c);
-      }
-    } else {
-#pragma unroll 4
-      for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) op.add(load8(lp.p, 8 * g - lp.shift, p.vocab), c);
-    }
+      });
+    else
+      each_group<4>(lp, nullptr, g0, g1, [&](int, const uint4& vp, const uint4&) { op.add(vp, c); });
     const float4 all = exchange(make_float4(op.m, op.z, oq.m, oq.z), make_float4(-INFINITY, 0.f, -INFINITY, 0.f), s_x,
                                 turn, size, rank, OnlineOp{c});
     m_p = all.x;
@@ -454,63 +521,80 @@ __global__ void __launch_bounds__(kThreads, 2) verify_nodes_kernel(const VerifyP
   int winner = -1, rejected = 0;
   float mass = z_q;
   for (int i = 0; i < kids; ++i) {
-    // every thread works out the child's probability
-    const int t = s_token[i];
-    const float wq = lq ? weight(s_lq[i], m_q, c) : 0.0f;
-    const float pt = remaining(weight(s_lp[i], m_p, c) * over_z, wq, t, lv, i);
-    const float over_q = mass > 0.0f ? 1.0f / mass : 0.0f;
-    float qt = 1.0f;
-    if (lq) {
-      bool gone = false;
-      for (int j = 0; j < i; ++j) gone |= s_token[j] == t;
-      qt = gone ? 0.0f : wq * over_q;
+    // A warp works out the child's probability. With no sibling behind it only the first CTA's has to.
+    const bool end = i + 1 == kids;
+    if (warp == 0 && (!end || rank == 0)) {
+      const int t = s_token[i];
+      const float wq = lq ? weight(s_lq[i], m_q, c) : 0.0f;
+      const float pt = remaining(weight(s_lp[i], m_p, c) * over_z, wq, t, lv, i);
+      const float over_q = mass > 0.0f ? 1.0f / mass : 0.0f;
+      float qt = 1.0f;
+      if (lq) {
+        bool gone = false;
+        for (int j = 0; j < i; ++j) gone |= s_token[j] == t;
+        qt = gone ? 0.0f : wq * over_q;
+      }
+      const float a = !(pt > 0.0f) ? 0.0f : (qt > 0.0f ? fminf(pt / qt, 1.0f) : 1.0f);
+      const bool taken = s_u[i] < a;
+      if (lane == 0) {
+        s_over_q[i] = over_q;
+        s_over_p[i] = 1.0f;  // what the pass below adds up is its inverse
+        s_tested[i & 1] = taken ? 1 : (a < 1.0f || !lq ? 0 : -1);  // a uniform of 1 or more rejects anything
+        if (rank == 0) {
+          p.accept[begin + s_child[i]] = a;
+          if (!taken && end) {  // no sibling needs the sums; the draw does without
+            ws[s_child[i]].over_q = over_q;
+            ws[s_child[i]].over_p = 1.0f;
+          }
+        }
+      }
+      __syncwarp();
     }
-    const float a = !(pt > 0.0f) ? 0.0f : (qt > 0.0f ? fminf(pt / qt, 1.0f) : 1.0f);
-    const bool taken = s_u[i] < a;
-    if (writes) p.accept[begin + s_child[i]] = a;
-    if (taken) {
+    if (end) {
+      if (warp != 0 || rank != 0) return;
+    } else {
+      __syncthreads();
+    }
+    const int tested = s_tested[i & 1];
+    if (tested > 0) {
       winner = s_child[i];
-      if (rank == 0)
-        for (int j = i + 1 + int(threadIdx.x); j < kids; j += kThreads) p.accept[begin + s_child[j]] = 0.0f;
+      if (warp != 0 || rank != 0) return;
+      for (int j = i + 1 + lane; j < kids; j += 32) p.accept[begin + s_child[j]] = 0.0f;
       break;
     }
     rejected = i + 1;
-    lv.regular = lv.regular && (a < 1.0f || !lq);  // a uniform of 1 or more rejects anything
-    if (threadIdx.x == 0) {
-      s_over_q[i] = over_q;
-      s_over_p[i] = 1.0f;  // what the pass below adds up is its inverse
-    }
-    if (i + 1 == kids) {  // no sibling needs the sums; the draw does without
-      if (writes) {
-        ws[s_child[i]].over_q = over_q;
-        ws[s_child[i]].over_p = 1.0f;
-      }
-      break;
-    }
-    __syncthreads();
+    lv.regular = lv.regular && tested == 0;
+    if (end) break;
+    const float over_q = s_over_q[i];
     // what is left of P, and Q's sum without the rejected tokens (added up anew: a difference would cancel where the
     // tokens had most)
     float left = 0.0f, rest = 0.0f;
     if (lv.regular && !safe) {
-#pragma unroll 2
-      for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
-        const int at = 8 * g - lp.shift;
-        float x[8], w[8];
-        weights8(load8(lp.p, at, p.vocab), m_p, c, over_z, x);
+      each_group<2>(lp, lq, g0, g1, [&](int at, const uint4& vp, const uint4& vq) {
+        float2 x[4], w[4];
+        weights8(vp, m_p, c, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], make_float2(over_z, over_z));
         if (lq) {
-          weights8(load8(lq, at, p.vocab), m_q, c, 1.0f, w);
+          weights8(vq, m_q, c, w);
           uint32_t gone = 0;
           for (int j = 0; j <= i; ++j) {
             const unsigned e = unsigned(s_token[j] - at);
             if (e < 8u) gone |= 1u << e;
           }
+          if (gone) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) rest += gone >> e & 1u ? 0.0f : w[e];
+            for (int e = 0; e < 4; ++e)
+              rest += (gone >> (2 * e) & 1u ? 0.0f : w[e].x) + (gone >> (2 * e + 1) & 1u ? 0.0f : w[e].y);
+          } else {
+            const float2 t = add2(add2(w[0], w[1]), add2(w[2], w[3]));
+            rest += t.x + t.y;
+          }
         }
         remaining8(x, w, at, lv, i + 1);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) left += x[e];
-      }
+        const float2 t = add2(add2(x[0], x[1]), add2(x[2], x[3]));
+        left += t.x + t.y;
+      });
     } else {
       for (int v = 8 * g0 - lp.shift + int(threadIdx.x); v < min(8 * g1 - lp.shift, p.vocab); v += kThreads) {
         if (v < 0) continue;
@@ -596,6 +680,13 @@ __device__ __forceinline__ unsigned long long sample_key(unsigned long long v, u
 }
 static_assert(kSampleThreads == 512, "the reductions above are over 16 warps");
 
+// The exact score: the sampler's of a logit where nothing was rejected, else
+// of a probability. Few tokens come here, so it is not inlined.
+__device__ __noinline__ float exact_score(float x, float temperature, uint64_t seed, int v, bool logit) {
+  if (logit) return gumbel_score(x, temperature, seed, v);
+  return x > 0.0f ? logf(x) - gumbel_log(seed, v) : NAN;
+}
+
 // CTA (part, sequence): the accepted path, and the best of the part's tokens.
 __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const VerifyParams p) {
   __shared__ float s_red[16];
@@ -680,10 +771,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
   }
   const Levels lv{s_token, s_over_q, s_over_p, lq != nullptr, stored >= 0};
   const float c = inv_temperature(temperature), over_z = z_p > 0.0f ? 1.0f / z_p : 0.0f;
-  // the exact score: the sampler's where nothing was rejected
   auto score = [&](float l, float prob, int v, int levels) {
-    if (levels == 0) return gumbel_score(l, temperature, seed, v);
-    return prob > 0.0f ? logf(prob) - gumbel_log(seed, v) : NAN;
+    return exact_score(levels == 0 ? l : prob, temperature, seed, v, levels == 0);
   };
   unsigned long long best = 0ull;
   if (!(temperature > 0.0f)) {
@@ -700,16 +789,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
     best = sample_key(best, s_key);
   } else {
     // P where something was rejected; else weights relative to the first chunk's maximum
-    float top = 0.0f, w[8], x[8];
+    float top = 0.0f;
+    float2 x[4];
     auto probabilities = [&](const uint4& a, const uint4& q, int at) {
-      if (rejected == 0) {
-        weights8(a, top, c, 1.0f, x);
-      } else {
-        weights8(a, m_p, c, over_z, x);
-        if (lq) weights8(q, m_q, c, 1.0f, w);
+      weights8(a, rejected ? m_p : top, c, x);
+      if (rejected) {
+        float2 w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], make_float2(over_z, over_z));
+        if (lq) weights8(q, m_q, c, w);
         remaining8(x, w, at, lv, rejected);
       }
     };
+    auto pick = [&](int e) { return e & 1 ? x[e >> 1].y : x[e >> 1].x; };  // of a constant e
     // Every token of a chunk, for what the bounds do not cover (NaN and infinite logits, irregular levels).
     auto score_all = [&](int k) {
       const int from = 8 * k * kSampleThreads - lp.shift, to = min(from + 8 * kSampleThreads, p.vocab);
@@ -726,10 +818,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
     int at = 8 * (chunk * kSampleThreads + int(threadIdx.x)) - lp.shift;
     if (rejected == 0) top = sample_max(max8(vp), s_red);
     probabilities(vp, vq, at);
-    float z = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) z += x[e];
-    z = sample_sum(z, s_red);
+    const float2 t = add2(add2(x[0], x[1]), add2(x[2], x[3]));
+    const float z = sample_sum(t.x + t.y, s_red);
     const float base = rejected == 0 ? __fdividef(top, temperature) : 0.0f;  // log of the weights' unit
     // false with NaN too
     const bool bounded = lv.regular && z > 0.0f && z < INFINITY && top > -INFINITY && top < INFINITY;
@@ -746,12 +836,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
       uint64_t t = uint64_t(int64_t(at)) * 0xd2b74407b1ce6e93ULL;
 #pragma unroll
       for (int e = 0; e < 8; ++e, t += 0xd2b74407b1ce6e93ULL)
-        if (may(splitmix64(seed ^ t), x[e], first) && at + e >= 0 && at + e < p.vocab) {
+        if (may(splitmix64(seed ^ t), pick(e), first) && at + e >= 0 && at + e < p.vocab) {
           const int i = atomicAdd(&s_listed, 1);
           if (i < kMaxList) {
             const uint32_t word = e < 2 ? vp.x : e < 4 ? vp.y : e < 6 ? vp.z : vp.w;
             s_list[i] = at + e;
-            s_list_x[i] = make_float2(__uint_as_float(e & 1 ? word & 0xffff0000u : word << 16), x[e]);
+            s_list_x[i] = make_float2(__uint_as_float(e & 1 ? word & 0xffff0000u : word << 16), pick(e));
           }
         }
       __syncthreads();
@@ -780,15 +870,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
       uint32_t hits = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e, t += 0xd2b74407b1ce6e93ULL)
-        hits |= may(splitmix64(seed ^ t), x[e], scale) ? 1u << e : 0u;
+        hits |= may(splitmix64(seed ^ t), pick(e), scale) ? 1u << e : 0u;
       while (hits) {
         const int e = __ffs(hits) - 1;
         hits &= hits - 1;
         if (at + e < 0 || at + e >= p.vocab) continue;
         const uint32_t word = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
-        float pr = x[0];
+        float pr = pick(0);
 #pragma unroll
-        for (int i = 1; i < 8; ++i) pr = e == i ? x[i] : pr;
+        for (int i = 1; i < 8; ++i) pr = e == i ? pick(i) : pr;
         best = max_key(best, sort_key(score(__uint_as_float(e & 1 ? word & 0xffff0000u : word << 16), pr, at + e,
                                             rejected),
                                       at + e));
@@ -855,10 +945,10 @@ cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft,
   cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_nodes_kernel, p);
   if (e != cudaSuccess) return e;
-  // Parts of a sequence: about as many as fit the GPU at once (two CTAs an SM), at most one for each chunk. A CTA's
+  // Parts of a sequence: as many as fit the GPU at once (two CTAs an SM), at most one for each chunk. A CTA's
   // start (the path, the levels, the first bound) costs about as much as two chunks.
   const int chunks = ((vocab + 14) / 8 + kSampleThreads - 1) / kSampleThreads;
-  int parts = int((2LL * sms + batch - 1) / batch);
+  int parts = int(2LL * sms / batch);
   parts = parts < 1 ? 1 : (parts > chunks ? chunks : parts);
   cfg.gridDim = dim3(unsigned(parts), unsigned(batch));
   cfg.blockDim = dim3(kSampleThreads);
