@@ -15,12 +15,17 @@
 // rejected, is distributed as the target's P. Without draft probabilities Q
 // is 1 at the child's token. T = 0 accepts the argmax's child.
 //
-// Two kernels. verify_nodes_kernel tests every node's children as if the node
-// had been reached, so all nodes run at once: a cluster of up to 8 CTAs reads
-// a node's two rows once (running maximum and sum, joined through distributed
-// shared memory), and once more, from L2, for each rejected child that has a
-// sibling behind it. Nodes without children are not read. What bounds it is
-// HBM; one exponential per logit takes 3/4 of the MUFU rate that goes with it.
+// Four kernels. verify_stats_kernel reads the rows of nodes that have children
+// once, cut over CTAs, for their maxima and sums. What bounds it is HBM; one
+// exponential per logit takes 3/4 of the MUFU rate that goes with it.
+// verify_tests_kernel, a warp a node, joins a node's parts and tests its first
+// child, as if the node had been reached, so that all nodes run at once. Nodes
+// whose first child is rejected with a sibling behind it go on a list, and
+// verify_residuals_kernel works through that: a cluster of up to 8 CTAs a node,
+// one more pass over its rows (from L2 where they fit) for each further
+// sibling. As many clusters as fit the GPU take the list in turn: with a cluster
+// launched for every node, 64 trees of 8 nodes took 88 us, as clusters of 4 and 8
+// were dispatched at ~150 ns each.
 //
 // verify_sample_kernel follows the accepted children from the root and draws
 // the next token from the last node's row, cut over CTAs. A token's score is
@@ -48,24 +53,27 @@ namespace {
 
 using namespace sample_math;
 
-constexpr int kThreads = 256;        // of a nodes CTA
+constexpr int kThreads = 256;        // of a stats and a tests CTA
+constexpr int kListThreads = 512;    // of a residuals CTA
 constexpr int kSampleThreads = 512;  // of a sample CTA, 8 tokens a thread and chunk
 constexpr int kMaxList = 256;        // tokens of the first chunk that may reach its bound
-constexpr int kMaxCluster = 8;
+constexpr int kMaxParts = 32;        // CTAs that read a node's rows
+constexpr int kMaxCluster = 8;       // CTAs of a node on the list
 constexpr int kMaxNodes = 1024;      // of one tree (verify_max_nodes)
 constexpr float kLog2e = 1.4426950408889634f;
 
-// What the first kernel leaves per row. For a node with children: its
+// What the first two kernels leave per row. For a node with children: its
 // statistics, accepted child and count of rejected children; for a child that
 // was rejected: the level that its rejection adds.
 struct VerifyRow {
-  float m_p, z_p, m_q, z_q;  // max logit and sum of exp((l - max) / T)
-  float over_q, over_p;      // child: its level (Levels)
-  int winner;                // node: accepted child's place in its sequence, or -1
-  int rejected;              // node: children rejected; its complement where they are not regular (Levels)
+  float m_p, z_p, m_q;   // max logit and sum of exp((l - max) / T)
+  float over_q, over_p;  // child: its level (Levels)
+  int winner;            // node: accepted child's place in its sequence, or -1
+  int rejected;          // node: children rejected; its complement where they are not regular (Levels)
+  int unused;
 };
 
-// The slices' best of a sequence; zeroed by the first kernel.
+// The best of a sequence's parts; zeroed by the first kernel.
 struct VerifyBest {
   unsigned long long key;  // ordered score, then inverted token; 0: none
   unsigned done;           // slices that have added theirs
@@ -87,7 +95,9 @@ struct VerifyParams {
   float* accept;    // [rows]
   VerifyRow* ws;    // [rows]
   VerifyBest* best;  // [batch]
-  int rows, max_q, vocab;
+  float4* part;      // [rows, kMaxParts]: (m_p, z_p, m_q, z_q), or the best logit and its token at T = 0
+  int2* list;        // [1 + rows]: (count, -), then (sequence, node) of the nodes with residuals
+  int rows, max_q, vocab, parts;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -162,26 +172,26 @@ __device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int at, int voc
 // that cross an end of the row, and all where q is aligned otherwise than p,
 // are read element by element.
 template <int kBatch, class F>
-__device__ __forceinline__ void each_group(const Row& p, const __nv_bfloat16* q, int g0, int g1, F&& f) {
+__device__ __forceinline__ void each_group(const Row& p, const __nv_bfloat16* q, int g0, int g1, int threads, F&& f) {
   const bool even = q == nullptr || ((reinterpret_cast<uintptr_t>(q) ^ reinterpret_cast<uintptr_t>(p.p)) & 15) == 0;
   const int lo = even ? max(g0, p.shift ? 1 : 0) : g1, hi = even ? min(g1, (p.vocab + p.shift) >> 3) : g1;
   const uint4* vp = reinterpret_cast<const uint4*>(p.p - p.shift);
   const uint4* vq = reinterpret_cast<const uint4*>(q ? q - p.shift : p.p - p.shift);
-  for (int g = lo + int(threadIdx.x); g < hi; g += kBatch * kThreads) {
+  for (int g = lo + int(threadIdx.x); g < hi; g += kBatch * threads) {
     uint4 a[kBatch], b[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
-      if (g + u * kThreads < hi) {
-        a[u] = __ldg(vp + g + u * kThreads);
-        if (q) b[u] = __ldg(vq + g + u * kThreads);
+      if (g + u * threads < hi) {
+        a[u] = __ldg(vp + g + u * threads);
+        if (q) b[u] = __ldg(vq + g + u * threads);
       }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
-      if (g + u * kThreads < hi) f(8 * (g + u * kThreads) - p.shift, a[u], b[u]);
+      if (g + u * threads < hi) f(8 * (g + u * threads) - p.shift, a[u], b[u]);
   }
-  for (int g = g0 + int(threadIdx.x); g < g1; g += kThreads) {
+  for (int g = g0 + int(threadIdx.x); g < g1; g += threads) {
     if (g >= lo && g < hi) {
-      g += max(0, (hi - 1 - g) / kThreads) * kThreads;  // past the groups above
+      g += max(0, (hi - 1 - g) / threads) * threads;  // past the groups above
       continue;
     }
     const int at = 8 * g - p.shift;
@@ -240,62 +250,8 @@ struct Online {
   }
 };
 
-// ----------------------------------------------------------- CTA and cluster
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_arrive() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
-  __syncwarp();
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void peer_store(const float4* p, uint32_t rank, const float4& v) {
-  const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(p));
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z),
-               "f"(v.w)
-               : "memory");
-}
-
-// Joins what the threads of a cluster hold. op(v, lanes) joins groups of
-// `lanes` neighbouring lanes; every thread gets the same result. CTAs leave
-// their parts in each other's shared memory, so nobody has to stay behind for a
-// reader. Two sets of buffers: a CTA may be one exchange ahead of another, not
-// two.
-struct Exchange {
-  float4 warp[2][kThreads / 32];
-  float4 cta[2][kMaxCluster];
-};
-template <class Op>
-__device__ __forceinline__ float4 exchange(float4 v, const float4& none, Exchange& x, int& turn, uint32_t size,
-                                           uint32_t rank, Op op) {
-  constexpr int kWarps = kThreads / 32;
-  static_assert((kWarps & (kWarps - 1)) == 0 && kWarps <= 32, "the warps' parts join in one warp's lanes");
-  const int t = turn & 1, lane = threadIdx.x & 31;
-  ++turn;
-  v = op(v, 32);
-  if (lane == 0) x.warp[t][threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = op(x.warp[t][lane & (kWarps - 1)], kWarps);
-  if (size == 1) return v;
-  if (turn == 1) cluster_wait();  // the others have started (the arrival is at the kernel's start)
-  if (threadIdx.x < size) peer_store(&x.cta[t][rank], threadIdx.x, v);
-  cluster_arrive();
-  cluster_wait();
-  return op((lane & 7) < int(size) ? x.cta[t][lane & 7] : none, 8);
-}
-
+// ----------------------------------------------------------------- joins
+// op(v, lanes) joins groups of `lanes` neighbouring lanes.
 __device__ __forceinline__ float lanes_max(float v, int lanes) {
   for (int off = lanes / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
   return v;
@@ -335,6 +291,55 @@ struct OnlineOp {  // (m_p, z_p, m_q, z_q)
     return make_float4(mp, lanes_sum(scaled(v.y, v.x, mp), lanes), mq, lanes_sum(scaled(v.w, v.z, mq), lanes));
   }
 };
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void peer_store(const float4* p, uint32_t rank, const float4& v) {
+  const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(p));
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z),
+               "f"(v.w)
+               : "memory");
+}
+
+// Joins what the threads of a cluster (or of a CTA, size 1) hold; all get the
+// same result. CTAs leave their parts in each other's shared memory, so nobody
+// has to stay behind for a reader. Two sets of buffers: a CTA may be one
+// exchange ahead of another, not two.
+template <int kT>
+struct Exchange {
+  float4 warp[2][kT / 32];
+  float4 cta[2][kMaxCluster];
+};
+template <int kT, class Op>
+__device__ __forceinline__ float4 exchange(float4 v, const float4& none, Exchange<kT>& x, int& turn, uint32_t size,
+                                           uint32_t rank, Op op) {
+  constexpr int kWarps = kT / 32;
+  static_assert((kWarps & (kWarps - 1)) == 0 && kWarps <= 32, "the warps' parts join in one warp's lanes");
+  const int t = turn++ & 1, lane = threadIdx.x & 31;
+  v = op(v, 32);
+  if (lane == 0) x.warp[t][threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = op(x.warp[t][lane & (kWarps - 1)], kWarps);
+  if (size == 1) return v;
+  if (threadIdx.x < size) peer_store(&x.cta[t][rank], threadIdx.x, v);
+  cluster_sync();
+  return op((lane & 7) < int(size) ? x.cta[t][lane & 7] : none, 8);
+}
 
 // A node's children that were rejected, in order: what P has become. `regular`:
 // every rejection left something, and where there are draft probabilities
@@ -391,68 +396,36 @@ __device__ __forceinline__ void weights8(const uint4& v, float m, float c, float
   for (int e = 0; e < 4; ++e) w[e] = make_float2(ex2(w[e].x), ex2(w[e].y));
 }
 
-// A cluster per node: its statistics, and its children's tests.
-__global__ void __launch_bounds__(kThreads, 4) verify_nodes_kernel(const VerifyParams p) {
-  __shared__ Exchange s_x;
-  __shared__ int s_child[kMaxNodes], s_token[kMaxNodes];
-  __shared__ float s_lp[kMaxNodes], s_lq[kMaxNodes], s_u[kMaxNodes];  // children's logits and uniforms
-  __shared__ float s_over_q[kMaxNodes], s_over_p[kMaxNodes];
-  __shared__ int s_tested[2];  // of two children in a row: 1 accepted, 0 rejected, -1 rejected irregularly
+// CTA (part, node, sequence): the part's maximum and sum of the node's rows.
+__global__ void __launch_bounds__(kThreads, 4) verify_stats_kernel(const VerifyParams p) {
+  __shared__ Exchange<kThreads> s_x;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const uint32_t size = cluster_size(), rank = cluster_rank();
-  if (size > 1) cluster_arrive();
-  const int b = blockIdx.y, node = blockIdx.x / size;
+  const int b = blockIdx.z, node = blockIdx.y, part = blockIdx.x;
   const int begin = p.cu_q[b], next = p.cu_q[b + 1];
   const float temperature = p.temps[b];
   const int n = min(min(next, p.rows) - begin, p.max_q);
-  if (node == 0 && rank == 0 && threadIdx.x == 0) p.best[b] = VerifyBest{0ull, 0u, 0u};
-  if (begin < 0 || node >= n) {  // all of a cluster
-    if (size > 1) cluster_wait();
-    return;
-  }
-  VerifyRow* ws = p.ws + begin;
+  if (node == 0 && part == 0 && threadIdx.x == 0) p.best[b] = VerifyBest{0ull, 0u, 0u};
+  if (b == 0 && node == 0 && part == 0 && threadIdx.x == 0) p.list[0] = make_int2(0, 0);
+  if (begin < 0 || node >= n) return;
+  bool mine = false;
+  for (int i = node + 1 + int(threadIdx.x); i < n; i += kThreads) mine |= p.parents[begin + i] == node;
+  const bool inner = __syncthreads_or(mine);
   const int row = begin + node;
+  if (!inner && part == 0 && threadIdx.x == 0) {
+    p.ws[row].winner = -1;
+    p.ws[row].rejected = 0;
+  }
+  if (!inner) return;
   const Row lp(p.logits + (long long)row * p.vocab, p.vocab);
   const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
-  // Every warp counts the children; the first one collects them, beside the others' pass over the logits.
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int kids = 0;
-  for (int base = node + 1; base < n; base += 32) {
-    const int i = base + lane;
-    const bool mine = i < n && p.parents[begin + i] == node;
-    const unsigned hits = __ballot_sync(0xffffffffu, mine);
-    if (mine && warp == 0) {
-      const int at = kids + __popc(hits & ((1u << lane) - 1u)), t = p.tokens[begin + i];
-      const bool inside = t >= 0 && t < p.vocab;
-      s_child[at] = i;
-      s_token[at] = t;
-      s_u[at] = p.uniforms[begin + i];
-      s_lp[at] = inside ? __bfloat162float(lp.p[t]) : -INFINITY;
-      s_lq[at] = inside && lq ? __bfloat162float(lq[t]) : -INFINITY;
-    }
-    kids += __popc(hits);
-  }
-  const bool writes = rank == 0 && threadIdx.x == 0;
-  if (writes) {  // a node that is no node's child is tested by nobody
-    const int parent = p.parents[row];
-    if (node == 0 || parent < 0 || parent >= node) p.accept[row] = 0.0f;
-  }
-  if (kids == 0) {
-    if (writes) {
-      ws[node].winner = -1;
-      ws[node].rejected = 0;
-    }
-    if (size > 1) cluster_wait();
-    return;
-  }
-  // this CTA's groups
-  const int per = (lp.groups + int(size) - 1) / int(size), g0 = int(rank) * per, g1 = min(g0 + per, lp.groups);
+  const int per = (lp.groups + p.parts - 1) / p.parts, g0 = part * per, g1 = min(g0 + per, lp.groups);
   int turn = 0;
+  float4 all;
   if (!(temperature > 0.0f)) {
     float best = -INFINITY;
     int best_index = kNone;
-    each_group<4>(lp, nullptr, g0, g1, [&](int at, const uint4& v, const uint4&) {
+    each_group<4>(lp, nullptr, g0, g1, kThreads, [&](int at, const uint4& v, const uint4&) {
       if (max8(v) >= best || best_index == kNone) {  // a row's first tokens may come last
         float f[8];
         unpack8(v, f);
@@ -466,167 +439,269 @@ __global__ void __launch_bounds__(kThreads, 4) verify_nodes_kernel(const VerifyP
         }
       }
     });
-    const float4 top = exchange(make_float4(best, __int_as_float(best_index), 0.f, 0.f),
-                                make_float4(-INFINITY, __int_as_float(kNone), 0.f, 0.f), s_x, turn, size, rank,
-                                BestOp());
-    best_index = __float_as_int(top.y);
-    if (best_index == kNone) best_index = 0;
-    if (writes) {
-      int winner = -1;
-      for (int i = 0; i < kids; ++i) {
-        const bool taken = winner < 0 && s_token[i] == best_index;
-        p.accept[begin + s_child[i]] = taken ? 1.0f : 0.0f;
-        if (taken) winner = s_child[i];
-      }
+    all = exchange(make_float4(best, __int_as_float(best_index), 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f), s_x, turn, 1,
+                   0, BestOp());
+  } else {
+    const float c = inv_temperature(temperature);
+    Online op, oq;
+    if (lq)
+      each_group<2>(lp, lq, g0, g1, kThreads, [&](int, const uint4& vp, const uint4& vq) {
+        op.add(vp, c);
+        oq.add(vq, c);
+      });
+    else
+      each_group<4>(lp, nullptr, g0, g1, kThreads, [&](int, const uint4& vp, const uint4&) { op.add(vp, c); });
+    all = exchange(make_float4(op.m, op.z, oq.m, oq.z), make_float4(0.f, 0.f, 0.f, 0.f), s_x, turn, 1, 0, OnlineOp{c});
+  }
+  if (threadIdx.x == 0) p.part[(long long)row * kMaxParts + part] = all;
+}
+
+// A node's statistics, joined from its parts by the lanes of a warp.
+__device__ __forceinline__ float4 join_parts(const VerifyParams& p, int row, float c) {
+  const int lane = threadIdx.x & 31;
+  return OnlineOp{c}(lane < p.parts ? p.part[(long long)row * kMaxParts + lane]
+                                    : make_float4(-INFINITY, 0.f, -INFINITY, 0.f), 32);
+}
+// Whether a node's sums have to be taken anew: NaN or infinite logits, or none but -inf (the maxima are right).
+__device__ __forceinline__ bool unsafe_sums(const float4& s, bool has_q) {
+  return !(s.y == s.y) || !(s.w == s.w) || s.x == INFINITY || s.z == INFINITY || s.x == -INFINITY ||
+         (has_q && s.z == -INFINITY);
+}
+// a = min(1, P(t) / Q(t))
+__device__ __forceinline__ float acceptance(float pt, float qt) {
+  return !(pt > 0.0f) ? 0.0f : (qt > 0.0f ? fminf(pt / qt, 1.0f) : 1.0f);
+}
+
+// A warp a node: the test of its first child, and at T = 0 of all.
+__global__ void __launch_bounds__(kThreads) verify_tests_kernel(const VerifyParams p, int batch) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long at = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, b = int(at / p.max_q), node = int(at % p.max_q);
+  if (b >= batch) return;
+  const int begin = p.cu_q[b], next = p.cu_q[b + 1];
+  const float temperature = p.temps[b];
+  const int n = min(min(next, p.rows) - begin, p.max_q);
+  if (begin < 0 || node >= n) return;
+  const int row = begin + node;
+  VerifyRow* ws = p.ws + begin;
+  if (lane == 0) {  // a node that is no node's child is tested by nobody
+    const int parent = p.parents[row];
+    if (node == 0 || parent < 0 || parent >= node) p.accept[row] = 0.0f;
+  }
+  int kids = 0, first = -1;
+  for (int base = node + 1; base < n; base += 32) {
+    const int i = base + lane;
+    const unsigned hits = __ballot_sync(0xffffffffu, i < n && p.parents[begin + i] == node);
+    if (first < 0 && hits) first = base + __ffs(hits) - 1;
+    kids += __popc(hits);
+  }
+  if (kids == 0) return;
+  int winner = -1;
+  if (!(temperature > 0.0f)) {
+    const float4 top = BestOp()(lane < p.parts ? p.part[(long long)row * kMaxParts + lane]
+                                               : make_float4(-INFINITY, __int_as_float(kNone), 0.f, 0.f), 32);
+    const int best = __float_as_int(top.y) == kNone ? 0 : __float_as_int(top.y);
+    for (int base = node + 1; base < n; base += 32) {
+      const int i = base + lane;
+      const bool child = i < n && p.parents[begin + i] == node;
+      const unsigned hits = __ballot_sync(0xffffffffu, child && p.tokens[begin + i] == best);
+      const int taken = winner < 0 && hits ? base + __ffs(hits) - 1 : -1;
+      if (taken >= 0) winner = taken;
+      if (child) p.accept[begin + i] = i == taken ? 1.0f : 0.0f;
+    }
+    if (lane == 0) {
       ws[node].winner = winner;
       ws[node].rejected = 0;
     }
     return;
   }
   const float c = inv_temperature(temperature);
-  float m_p, z_p, m_q, z_q;
-  {
-    Online op, oq;
-    if (lq)
-      each_group<2>(lp, lq, g0, g1, [&](int, const uint4& vp, const uint4& vq) {
-        op.add(vp, c);
-        oq.add(vq, c);
-      });
-    else
-      each_group<4>(lp, nullptr, g0, g1, [&](int, const uint4& vp, const uint4&) { op.add(vp, c); });
-    const float4 all = exchange(make_float4(op.m, op.z, oq.m, oq.z), make_float4(-INFINITY, 0.f, -INFINITY, 0.f), s_x,
-                                turn, size, rank, OnlineOp{c});
-    m_p = all.x;
-    z_p = all.y;
-    m_q = all.z;
-    z_q = all.w;
+  const int t = p.tokens[begin + first];
+  const bool inside = t >= 0 && t < p.vocab;
+  const float lp = inside ? __bfloat162float(p.logits[(long long)row * p.vocab + t]) : -INFINITY;
+  const float lq = inside && p.draft ? __bfloat162float(p.draft[(long long)row * p.vocab + t]) : -INFINITY;
+  const float u = p.uniforms[begin + first];
+  const float4 stats = join_parts(p, row, c);
+  const bool safe = unsafe_sums(stats, p.draft != nullptr);
+  const float over_q = stats.w > 0.0f ? 1.0f / stats.w : 0.0f;
+  const float a = acceptance(weight(lp, stats.x, c) * (1.0f / stats.y),
+                             p.draft ? weight(lq, stats.z, c) * over_q : 1.0f);
+  if (safe || (!(u < a) && kids > 1)) {
+    if (lane == 0) p.list[1 + atomicAdd(&p.list[0].x, 1)] = make_int2(b, node);
+    return;
   }
-  // NaN or infinite logits (or none but -inf): the maxima are right, the sums are taken anew
-  const bool safe = !(z_p == z_p) || !(z_q == z_q) || m_p == INFINITY || m_q == INFINITY || m_p == -INFINITY ||
-                    (lq && m_q == -INFINITY);
-  if (safe) {
-    float2 z = make_float2(0.f, 0.f);
-    for (int v = 8 * g0 - lp.shift + int(threadIdx.x); v < min(8 * g1 - lp.shift, p.vocab); v += kThreads) {
-      if (v < 0) continue;
-      z.x += weight(__bfloat162float(lp.p[v]), m_p, c);
-      if (lq) z.y += weight(__bfloat162float(lq[v]), m_q, c);
+  if (u < a) {
+    winner = first;
+    for (int i = first + 1 + lane; i < n; i += 32)
+      if (p.parents[begin + i] == node) p.accept[begin + i] = 0.0f;
+  }
+  if (lane == 0) {
+    p.accept[begin + first] = a;
+    ws[first].over_q = over_q;
+    ws[first].over_p = 1.0f;  // no sibling needs the sum; the draw does without
+    VerifyRow& r = ws[node];
+    r.m_p = stats.x;
+    r.z_p = stats.y;
+    r.m_q = stats.z;
+    r.winner = winner;
+    // a uniform of 1 or more rejects anything: then it is not regular
+    r.rejected = winner >= 0 ? 0 : (a < 1.0f || !p.draft ? 1 : ~1);
+  }
+}
+
+// Clusters take the list's nodes in turn: all their children's tests.
+__global__ void __launch_bounds__(kListThreads, 2) verify_residuals_kernel(const VerifyParams p) {
+  __shared__ Exchange<kListThreads> s_x;
+  __shared__ int s_child[kMaxNodes], s_token[kMaxNodes];
+  __shared__ float s_lp[kMaxNodes], s_lq[kMaxNodes], s_u[kMaxNodes];  // children's logits and uniforms
+  __shared__ float s_over_q[kMaxNodes], s_over_p[kMaxNodes];
+  __shared__ int s_tested[2];  // of two children in a row: 1 accepted, 0 rejected, -1 rejected irregularly
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint32_t size = cluster_size(), rank = cluster_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int count = p.list[0].x, step = int(gridDim.x / size);
+  const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+  int turn = 0;
+  if (size > 1) cluster_sync();  // all have started
+  for (int at = int(blockIdx.x / size); at < count; at += step) {
+    const int b = p.list[1 + at].x, node = p.list[1 + at].y;
+    const int begin = p.cu_q[b], n = min(min(p.cu_q[b + 1], p.rows) - begin, p.max_q), row = begin + node;
+    VerifyRow* ws = p.ws + begin;
+    const Row lp(p.logits + (long long)row * p.vocab, p.vocab);
+    const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
+    // every warp counts the children, the first one collects them
+    int kids = 0;
+    for (int base = node + 1; base < n; base += 32) {
+      const int i = base + lane;
+      const bool child = i < n && p.parents[begin + i] == node;
+      const unsigned hits = __ballot_sync(0xffffffffu, child);
+      if (child && warp == 0) {
+        const int k = kids + __popc(hits & ((1u << lane) - 1u)), t = p.tokens[begin + i];
+        const bool inside = t >= 0 && t < p.vocab;
+        s_child[k] = i;
+        s_token[k] = t;
+        s_u[k] = p.uniforms[begin + i];
+        s_lp[k] = inside ? __bfloat162float(lp.p[t]) : -INFINITY;
+        s_lq[k] = inside && lq ? __bfloat162float(lq[t]) : -INFINITY;
+      }
+      kids += __popc(hits);
     }
-    const float4 all = exchange(make_float4(z.x, z.y, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f), s_x, turn, size, rank,
-                                SumOp());
-    z_p = all.x;
-    z_q = all.y;
-  }
-  const float over_z = z_p > 0.0f ? 1.0f / z_p : 0.0f;
-  Levels lv{s_token, s_over_q, s_over_p, lq != nullptr, true};
-  int winner = -1, rejected = 0;
-  float mass = z_q;
-  for (int i = 0; i < kids; ++i) {
-    // A warp works out the child's probability. With no sibling behind it only the first CTA's has to.
-    const bool end = i + 1 == kids;
-    if (warp == 0 && (!end || rank == 0)) {
-      const int t = s_token[i];
-      const float wq = lq ? weight(s_lq[i], m_q, c) : 0.0f;
-      const float pt = remaining(weight(s_lp[i], m_p, c) * over_z, wq, t, lv, i);
-      const float over_q = mass > 0.0f ? 1.0f / mass : 0.0f;
-      float qt = 1.0f;
-      if (lq) {
+    const float c = inv_temperature(p.temps[b]);
+    const float4 stats = join_parts(p, row, c);
+    const float m_p = stats.x, m_q = stats.z;
+    float z_p = stats.y, z_q = stats.w;
+    const int per = (lp.groups + int(size) - 1) / int(size), g0 = int(rank) * per, g1 = min(g0 + per, lp.groups);
+    const int v0 = max(8 * g0 - lp.shift, 0), v1 = min(8 * g1 - lp.shift, p.vocab);
+    const bool safe = unsafe_sums(stats, lq != nullptr);
+    if (safe) {
+      float2 z = make_float2(0.f, 0.f);
+      for (int v = v0 + int(threadIdx.x); v < v1; v += kListThreads) {
+        z.x += weight(__bfloat162float(lp.p[v]), m_p, c);
+        if (lq) z.y += weight(__bfloat162float(lq[v]), m_q, c);
+      }
+      const float4 all = exchange(make_float4(z.x, z.y, 0.f, 0.f), none, s_x, turn, size, rank, SumOp());
+      z_p = all.x;
+      z_q = all.y;
+    }
+    const float over_z = z_p > 0.0f ? 1.0f / z_p : 0.0f;
+    Levels lv{s_token, s_over_q, s_over_p, lq != nullptr, true};
+    int winner = -1, rejected = 0;
+    float mass = z_q;
+    for (int i = 0; i < kids; ++i) {
+      const bool end = i + 1 == kids;
+      if (warp == 0) {  // the child's probability
+        __syncwarp();
+        const int t = s_token[i];
+        const float wq = lq ? weight(s_lq[i], m_q, c) : 0.0f;
+        const float pt = remaining(weight(s_lp[i], m_p, c) * over_z, wq, t, lv, i);
+        const float over_q = mass > 0.0f ? 1.0f / mass : 0.0f;
         bool gone = false;
         for (int j = 0; j < i; ++j) gone |= s_token[j] == t;
-        qt = gone ? 0.0f : wq * over_q;
-      }
-      const float a = !(pt > 0.0f) ? 0.0f : (qt > 0.0f ? fminf(pt / qt, 1.0f) : 1.0f);
-      const bool taken = s_u[i] < a;
-      if (lane == 0) {
-        s_over_q[i] = over_q;
-        s_over_p[i] = 1.0f;  // what the pass below adds up is its inverse
-        s_tested[i & 1] = taken ? 1 : (a < 1.0f || !lq ? 0 : -1);  // a uniform of 1 or more rejects anything
-        if (rank == 0) {
-          p.accept[begin + s_child[i]] = a;
-          if (!taken && end) {  // no sibling needs the sums; the draw does without
-            ws[s_child[i]].over_q = over_q;
-            ws[s_child[i]].over_p = 1.0f;
-          }
+        const float a = acceptance(pt, lq ? (gone ? 0.0f : wq * over_q) : 1.0f);
+        const bool taken = s_u[i] < a;
+        if (lane == 0) {
+          s_over_q[i] = over_q;
+          s_over_p[i] = 1.0f;  // what the pass below adds up is its inverse
+          s_tested[i & 1] = taken ? 1 : (a < 1.0f || !lq ? 0 : -1);  // a uniform of 1 or more rejects anything
+          if (rank == 0) p.accept[begin + s_child[i]] = a;
         }
       }
-      __syncwarp();
-    }
-    if (end) {
-      if (warp != 0 || rank != 0) return;
-    } else {
+      __syncthreads();
+      const int tested = s_tested[i & 1];
+      if (tested > 0) {
+        winner = s_child[i];
+        if (rank == 0)
+          for (int j = i + 1 + int(threadIdx.x); j < kids; j += kListThreads) p.accept[begin + s_child[j]] = 0.0f;
+        break;
+      }
+      rejected = i + 1;
+      lv.regular = lv.regular && tested == 0;
+      const float over_q = s_over_q[i];
+      float over_p = 1.0f;  // where no sibling needs the sum; the draw does without
+      if (!end) {
+        // what is left of P, and Q's sum without the rejected tokens (added up anew: a difference would cancel where
+        // the tokens had most)
+        float left = 0.0f, rest = 0.0f;
+        if (lv.regular && !safe) {
+          each_group<2>(lp, lq, g0, g1, kListThreads, [&](int from, const uint4& vp, const uint4& vq) {
+            float2 x[4], w[4];
+            weights8(vp, m_p, c, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], make_float2(over_z, over_z));
+            if (lq) {
+              weights8(vq, m_q, c, w);
+              uint32_t gone = 0;
+              for (int j = 0; j <= i; ++j) {
+                const unsigned e = unsigned(s_token[j] - from);
+                if (e < 8u) gone |= 1u << e;
+              }
+              if (gone) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  rest += (gone >> (2 * e) & 1u ? 0.0f : w[e].x) + (gone >> (2 * e + 1) & 1u ? 0.0f : w[e].y);
+              } else {
+                const float2 t = add2(add2(w[0], w[1]), add2(w[2], w[3]));
+                rest += t.x + t.y;
+              }
+            }
+            remaining8(x, w, from, lv, i + 1);
+            const float2 t = add2(add2(x[0], x[1]), add2(x[2], x[3]));
+            left += t.x + t.y;
+          });
+        } else {
+          for (int v = v0 + int(threadIdx.x); v < v1; v += kListThreads) {
+            const float wv = lq ? weight(__bfloat162float(lq[v]), m_q, c) : 0.0f;
+            bool gone = false;
+            for (int j = 0; j <= i; ++j) gone |= s_token[j] == v;
+            rest += gone ? 0.0f : wv;
+            left += remaining(weight(__bfloat162float(lp.p[v]), m_p, c) * over_z, wv, v, lv, i + 1);
+          }
+        }
+        const float4 all = exchange(make_float4(left, rest, 0.f, 0.f), none, s_x, turn, size, rank, SumOp());
+        over_p = all.x > 0.0f ? 1.0f / all.x : 0.0f;
+        lv.regular = lv.regular && over_p > 0.0f;
+        mass = all.y;
+      }
+      if (threadIdx.x == 0) {
+        s_over_p[i] = over_p;
+        if (rank == 0) {
+          ws[s_child[i]].over_q = over_q;
+          ws[s_child[i]].over_p = over_p;
+        }
+      }
       __syncthreads();
     }
-    const int tested = s_tested[i & 1];
-    if (tested > 0) {
-      winner = s_child[i];
-      if (warp != 0 || rank != 0) return;
-      for (int j = i + 1 + lane; j < kids; j += 32) p.accept[begin + s_child[j]] = 0.0f;
-      break;
+    if (rank == 0 && threadIdx.x == 0) {
+      VerifyRow& r = ws[node];
+      r.m_p = m_p;
+      r.z_p = z_p;
+      r.m_q = m_q;
+      r.winner = winner;
+      r.rejected = lv.regular && !safe ? rejected : ~rejected;
     }
-    rejected = i + 1;
-    lv.regular = lv.regular && tested == 0;
-    if (end) break;
-    const float over_q = s_over_q[i];
-    // what is left of P, and Q's sum without the rejected tokens (added up anew: a difference would cancel where the
-    // tokens had most)
-    float left = 0.0f, rest = 0.0f;
-    if (lv.regular && !safe) {
-      each_group<2>(lp, lq, g0, g1, [&](int at, const uint4& vp, const uint4& vq) {
-        float2 x[4], w[4];
-        weights8(vp, m_p, c, x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], make_float2(over_z, over_z));
-        if (lq) {
-          weights8(vq, m_q, c, w);
-          uint32_t gone = 0;
-          for (int j = 0; j <= i; ++j) {
-            const unsigned e = unsigned(s_token[j] - at);
-            if (e < 8u) gone |= 1u << e;
-          }
-          if (gone) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              rest += (gone >> (2 * e) & 1u ? 0.0f : w[e].x) + (gone >> (2 * e + 1) & 1u ? 0.0f : w[e].y);
-          } else {
-            const float2 t = add2(add2(w[0], w[1]), add2(w[2], w[3]));
-            rest += t.x + t.y;
-          }
-        }
-        remaining8(x, w, at, lv, i + 1);
-        const float2 t = add2(add2(x[0], x[1]), add2(x[2], x[3]));
-        left += t.x + t.y;
-      });
-    } else {
-      for (int v = 8 * g0 - lp.shift + int(threadIdx.x); v < min(8 * g1 - lp.shift, p.vocab); v += kThreads) {
-        if (v < 0) continue;
-        const float wv = lq ? weight(__bfloat162float(lq[v]), m_q, c) : 0.0f;
-        bool gone = false;
-        for (int j = 0; j <= i; ++j) gone |= s_token[j] == v;
-        rest += gone ? 0.0f : wv;
-        left += remaining(weight(__bfloat162float(lp.p[v]), m_p, c) * over_z, wv, v, lv, i + 1);
-      }
-    }
-    const float4 all = exchange(make_float4(left, rest, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f), s_x, turn, size,
-                                rank, SumOp());
-    const float over_p = all.x > 0.0f ? 1.0f / all.x : 0.0f;
-    if (threadIdx.x == 0) {
-      s_over_p[i] = over_p;
-      if (rank == 0) {
-        ws[s_child[i]].over_q = over_q;
-        ws[s_child[i]].over_p = over_p;
-      }
-    }
-    lv.regular = lv.regular && over_p > 0.0f;
-    mass = all.y;
-    __syncthreads();
-  }
-  if (writes) {
-    VerifyRow& r = ws[node];
-    r.m_p = m_p;
-    r.z_p = z_p;
-    r.m_q = m_q;
-    r.z_q = z_q;
-    r.winner = winner;
-    r.rejected = lv.regular && !safe ? rejected : ~rejected;
+    __syncthreads();  // the lists above are free for the next node
   }
 }
 
@@ -916,35 +991,55 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
 int verify_max_nodes() { return kMaxNodes; }
 
 size_t verify_workspace(int rows, int batch) {
-  return size_t(rows) * sizeof(VerifyRow) + size_t(batch) * sizeof(VerifyBest);
+  return size_t(rows) * (kMaxParts * sizeof(float4) + sizeof(VerifyRow)) + size_t(batch) * sizeof(VerifyBest) +
+         (size_t(rows) + 1) * sizeof(int2);
 }
 
 cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft, const int* tokens,
                           const int* parents, const float* uniforms, const uint64_t* seeds, const float* temps,
                           const int* cu_q, int* out_tokens, int* path, int* counts, float* accept, int rows, int batch,
                           int max_q, int vocab, void* ws, int sms) {
+  float4* const part = static_cast<float4*>(ws);
+  VerifyRow* const row = reinterpret_cast<VerifyRow*>(part + size_t(rows) * kMaxParts);
+  VerifyBest* const best = reinterpret_cast<VerifyBest*>(row + rows);
   VerifyParams p{static_cast<const __nv_bfloat16*>(logits), static_cast<const __nv_bfloat16*>(draft), tokens, parents,
-                 uniforms, seeds, temps, cu_q, out_tokens, path, counts, accept, static_cast<VerifyRow*>(ws),
-                 reinterpret_cast<VerifyBest*>(static_cast<VerifyRow*>(ws) + rows), rows, max_q, vocab};
-  // CTAs a node: 32 thousand logits each where the nodes fill the GPU, 4 thousand where they do not.
-  int cluster = 1;
-  while (cluster < kMaxCluster && vocab >= 2 * cluster * ((long long)rows * cluster < 2LL * sms ? 4096 : 32768))
-    cluster *= 2;
+                 uniforms, seeds, temps, cu_q, out_tokens, path, counts, accept, row, best, part,
+                 reinterpret_cast<int2*>(best + batch), rows, max_q, vocab, 1};
+  // CTAs that read a node's rows: 16 thousand logits each where that fills the GPU several times over, else 4 thousand.
+  const long long coarse = (vocab + 16383) / 16384;
+  p.parts = int(rows * coarse >= 8LL * sms ? coarse : (vocab + 4095) / 4096);
+  if (p.parts > kMaxParts) p.parts = kMaxParts;
+  // Programmatic dependents: launched while the kernel before them ends; they wait for it before any global access.
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(p.parts), unsigned(max_q), unsigned(batch));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, verify_stats_kernel, p);
+  if (e != cudaSuccess) return e;
+  const long long nodes = (long long)max_q * batch;
+  cfg.gridDim = dim3(unsigned((nodes + kThreads / 32 - 1) / (kThreads / 32)));
+  e = cudaLaunchKernelEx(&cfg, verify_tests_kernel, p, batch);
+  if (e != cudaSuccess) return e;
+  // Clusters for the list: CTAs of 4 thousand logits or more, two an SM, a few left for the clusters' placing.
+  int cluster = 1;
+  while (cluster < kMaxCluster && vocab >= 2 * cluster * 4096) cluster *= 2;
+  long long clusters = 2LL * sms * 7 / 8 / cluster;
+  clusters = clusters < 1 ? 1 : (clusters > rows ? rows : clusters);
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = unsigned(cluster);
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(max_q) * unsigned(cluster), unsigned(batch));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cfg.attrs = attr;
+  cfg.gridDim = dim3(unsigned(clusters * cluster));
+  cfg.blockDim = dim3(kListThreads);
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_nodes_kernel, p);
+  e = cudaLaunchKernelEx(&cfg, verify_residuals_kernel, p);
   if (e != cudaSuccess) return e;
+  cfg.numAttrs = 1;
   // Parts of a sequence: as many as fit the GPU at once (two CTAs an SM), at most one for each chunk. A CTA's
   // start (the path, the levels, the first bound) costs about as much as two chunks.
   const int chunks = ((vocab + 14) / 8 + kSampleThreads - 1) / kSampleThreads;
@@ -952,7 +1047,6 @@ cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft,
   parts = parts < 1 ? 1 : (parts > chunks ? chunks : parts);
   cfg.gridDim = dim3(unsigned(parts), unsigned(batch));
   cfg.blockDim = dim3(kSampleThreads);
-  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, verify_sample_kernel, p);
 }
 
