@@ -21,7 +21,7 @@
 // verify_tests_kernel, a warp a node, joins a node's parts and tests its first
 // child, as if the node had been reached, so that all nodes run at once. Nodes
 // whose first child is rejected with a sibling behind it go on a list, and
-// verify_residuals_kernel works through that: a cluster of up to 8 CTAs a node,
+// verify_residuals_kernel works through that: a cluster of up to 4 CTAs a node,
 // one more pass over its rows (from L2 where they fit) for each further
 // sibling. As many clusters as fit the GPU take the list in turn: with a cluster
 // launched for every node, 64 trees of 8 nodes took 88 us, as clusters of 4 and 8
@@ -33,7 +33,7 @@
 // logarithms, ~100 instructions in all, for 152 thousand tokens a sequence. A
 // token can only beat a score L if 1 - u < P(v) e^-L (as -log u >= 1 - u), so
 // the hash alone sorts out nearly all tokens once L is known. The best score of
-// a CTA's first 4096 tokens, of weight Z, is below log Z - 5/2 five times in
+// a CTA's first 2048 tokens, of weight Z, is below log Z - 5/2 five times in
 // a million (exp(-e^2.5)): with that L the ~12 tokens that are left are scored;
 // if none reached L all of them are. Their best is the L of the CTA's other
 // tokens. What bounds it is the issue rate: ~35 instructions a token. The CTAs'
@@ -55,10 +55,10 @@ using namespace sample_math;
 
 constexpr int kThreads = 256;        // of a stats and a tests CTA
 constexpr int kListThreads = 512;    // of a residuals CTA
-constexpr int kSampleThreads = 512;  // of a sample CTA, 8 tokens a thread and chunk
+constexpr int kSampleThreads = 256;  // of a sample CTA, 8 tokens a thread and chunk
 constexpr int kMaxList = 256;        // tokens of the first chunk that may reach its bound
 constexpr int kMaxParts = 32;        // CTAs that read a node's rows
-constexpr int kMaxCluster = 8;       // CTAs of a node on the list
+constexpr int kMaxCluster = 4;       // CTAs of a node on the list
 constexpr int kMaxNodes = 1024;      // of one tree (verify_max_nodes)
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -66,7 +66,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // statistics, accepted child and count of rejected children; for a child that
 // was rejected: the level that its rejection adds.
 struct VerifyRow {
-  float m_p, z_p, m_q;   // max logit and sum of exp((l - max) / T)
+  float m_p, z_p, m_q;   // a logit near the highest, and the sum of exp((l - m) / T)
   float over_q, over_p;  // child: its level (Levels)
   int winner;            // node: accepted child's place in its sequence, or -1
   int rejected;          // node: children rejected; its complement where they are not regular (Levels)
@@ -227,6 +227,13 @@ __device__ __forceinline__ void exponents8(const uint4& v, float m, float c, flo
                 make_float2(c, c));
 }
 
+// Weights of eight logits without NaN and with a finite maximum.
+__device__ __forceinline__ void weights8(const uint4& v, float m, float c, float2 (&w)[4]) {
+  exponents8(v, m, c, w);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = make_float2(ex2(w[e].x), ex2(w[e].y));
+}
+
 // Running maximum and sum of exp((l - m) / T). NaN and infinite logits make
 // the sum NaN (the caller then adds it up anew with weight()).
 struct Online {
@@ -263,6 +270,11 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
 struct SumOp {  // two sums
   __device__ __forceinline__ float4 operator()(const float4& v, int lanes) const {
     return make_float4(lanes_sum(v.x, lanes), lanes_sum(v.y, lanes), 0.f, 0.f);
+  }
+};
+struct MaxOp {  // two maxima, x and z
+  __device__ __forceinline__ float4 operator()(const float4& v, int lanes) const {
+    return make_float4(lanes_max(v.x, lanes), 0.f, lanes_max(v.z, lanes), 0.f);
   }
 };
 struct BestOp {  // (score, index bits)
@@ -338,7 +350,7 @@ __device__ __forceinline__ float4 exchange(float4 v, const float4& none, Exchang
   if (size == 1) return v;
   if (threadIdx.x < size) peer_store(&x.cta[t][rank], threadIdx.x, v);
   cluster_sync();
-  return op((lane & 7) < int(size) ? x.cta[t][lane & 7] : none, 8);
+  return op((lane & (kMaxCluster - 1)) < int(size) ? x.cta[t][lane & (kMaxCluster - 1)] : none, kMaxCluster);
 }
 
 // A node's children that were rejected, in order: what P has become. `regular`:
@@ -389,13 +401,6 @@ __device__ __forceinline__ float remaining(float x, float wq, int v, const Level
   return x;
 }
 
-// Weights of eight logits without NaN and with a finite maximum.
-__device__ __forceinline__ void weights8(const uint4& v, float m, float c, float2 (&w)[4]) {
-  exponents8(v, m, c, w);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = make_float2(ex2(w[e].x), ex2(w[e].y));
-}
-
 // CTA (part, node, sequence): the part's maximum and sum of the node's rows.
 __global__ void __launch_bounds__(kThreads, 4) verify_stats_kernel(const VerifyParams p) {
   __shared__ Exchange<kThreads> s_x;
@@ -442,16 +447,41 @@ __global__ void __launch_bounds__(kThreads, 4) verify_stats_kernel(const VerifyP
     all = exchange(make_float4(best, __int_as_float(best_index), 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f), s_x, turn, 1,
                    0, BestOp());
   } else {
+    // Any finite logit near the maximum serves as the unit that sums are taken in: the highest of the part's first
+    // groups. Only where a sum does not stay finite with it are the maxima followed.
     const float c = inv_temperature(temperature);
-    Online op, oq;
+    const float4 none = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+    float4 unit = none;
+    if (g0 + int(threadIdx.x) < g1) {
+      const int at = 8 * (g0 + int(threadIdx.x)) - lp.shift;
+      unit.x = max8(load8(lp.p, at, p.vocab));
+      if (lq) unit.z = max8(load8(lq, at, p.vocab));
+    }
+    unit = exchange(unit, none, s_x, turn, 1, 0, MaxOp());
+    float2 z_p = make_float2(0.f, 0.f), z_q = z_p;
+    auto sum = [&](const uint4& v, float m) {
+      float2 w[4];
+      weights8(v, m, c, w);
+      return add2(add2(w[0], w[1]), add2(w[2], w[3]));
+    };
     if (lq)
       each_group<2>(lp, lq, g0, g1, kThreads, [&](int, const uint4& vp, const uint4& vq) {
-        op.add(vp, c);
-        oq.add(vq, c);
+        z_p = add2(z_p, sum(vp, unit.x));
+        z_q = add2(z_q, sum(vq, unit.z));
       });
     else
-      each_group<4>(lp, nullptr, g0, g1, kThreads, [&](int, const uint4& vp, const uint4&) { op.add(vp, c); });
-    all = exchange(make_float4(op.m, op.z, oq.m, oq.z), make_float4(0.f, 0.f, 0.f, 0.f), s_x, turn, 1, 0, OnlineOp{c});
+      each_group<4>(lp, nullptr, g0, g1, kThreads,
+                    [&](int, const uint4& vp, const uint4&) { z_p = add2(z_p, sum(vp, unit.x)); });
+    all = exchange(make_float4(z_p.x + z_p.y, z_q.x + z_q.y, 0.f, 0.f), none, s_x, turn, 1, 0, SumOp());
+    all = make_float4(unit.x, all.x, unit.z, all.y);
+    if (!(all.y < INFINITY) || !(all.w < INFINITY)) {
+      Online op, oq;
+      each_group<1>(lp, lq, g0, g1, kThreads, [&](int, const uint4& vp, const uint4& vq) {
+        op.add(vp, c);
+        if (lq) oq.add(vq, c);
+      });
+      all = exchange(make_float4(op.m, op.z, oq.m, oq.z), none, s_x, turn, 1, 0, OnlineOp{c});
+    }
   }
   if (threadIdx.x == 0) p.part[(long long)row * kMaxParts + part] = all;
 }
@@ -720,40 +750,35 @@ __device__ __forceinline__ unsigned long long max_key(unsigned long long a, unsi
   return a > b ? a : b;
 }
 
+// Joins over a sample CTA's warps; every thread gets the result.
+constexpr int kSampleWarps = kSampleThreads / 32;
+static_assert((kSampleWarps & (kSampleWarps - 1)) == 0, "the warps' parts join in one warp's lanes");
+
 __device__ __forceinline__ float sample_sum(float v, float* s) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  v = lanes_sum(v, 32);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = s[threadIdx.x & 15];
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  return v;
+  return lanes_sum(s[threadIdx.x & (kSampleWarps - 1)], kSampleWarps);
 }
 __device__ __forceinline__ float sample_max(float v, float* s) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+  v = lanes_max(v, 32);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = s[threadIdx.x & 15];
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return lanes_max(s[threadIdx.x & (kSampleWarps - 1)], kSampleWarps);
+}
+__device__ __forceinline__ unsigned long long lanes_key(unsigned long long v, int lanes) {
+  for (int off = lanes / 2; off > 0; off >>= 1) v = max_key(v, __shfl_xor_sync(0xffffffffu, v, off));
   return v;
 }
 __device__ __forceinline__ unsigned long long sample_key(unsigned long long v, unsigned long long* s) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v = max_key(v, __shfl_xor_sync(0xffffffffu, v, off));
+  v = lanes_key(v, 32);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = s[threadIdx.x & 15];
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) v = max_key(v, __shfl_xor_sync(0xffffffffu, v, off));
-  return v;
+  return lanes_key(s[threadIdx.x & (kSampleWarps - 1)], kSampleWarps);
 }
-static_assert(kSampleThreads == 512, "the reductions above are over 16 warps");
 
 // The exact score: the sampler's of a logit where nothing was rejected, else
 // of a probability. Few tokens come here, so it is not inlined.
@@ -763,9 +788,9 @@ __device__ __noinline__ float exact_score(float x, float temperature, uint64_t s
 }
 
 // CTA (part, sequence): the accepted path, and the best of the part's tokens.
-__global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const VerifyParams p) {
-  __shared__ float s_red[16];
-  __shared__ unsigned long long s_key[16];
+__global__ void __launch_bounds__(kSampleThreads, 4) verify_sample_kernel(const VerifyParams p) {
+  __shared__ float s_red[kSampleWarps];
+  __shared__ unsigned long long s_key[kSampleWarps];
   __shared__ int s_winner[kMaxNodes], s_path[kMaxNodes], s_token[kMaxNodes];
   __shared__ float s_over_q[kMaxNodes], s_over_p[kMaxNodes];
   __shared__ int s_list[kMaxList];        // tokens that may reach the bound
@@ -1040,10 +1065,10 @@ cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft,
   e = cudaLaunchKernelEx(&cfg, verify_residuals_kernel, p);
   if (e != cudaSuccess) return e;
   cfg.numAttrs = 1;
-  // Parts of a sequence: as many as fit the GPU at once (two CTAs an SM), at most one for each chunk. A CTA's
+  // Parts of a sequence: as many as fit the GPU at once (four CTAs an SM), at most one for each chunk. A CTA's
   // start (the path, the levels, the first bound) costs about as much as two chunks.
   const int chunks = ((vocab + 14) / 8 + kSampleThreads - 1) / kSampleThreads;
-  int parts = int(2LL * sms / batch);
+  int parts = int(4LL * sms / batch);
   parts = parts < 1 ? 1 : (parts > chunks ? chunks : parts);
   cfg.gridDim = dim3(unsigned(parts), unsigned(batch));
   cfg.blockDim = dim3(kSampleThreads);
