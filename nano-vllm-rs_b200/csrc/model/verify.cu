@@ -96,7 +96,7 @@ struct VerifyParams {
   VerifyRow* ws;    // [rows]
   VerifyBest* best;  // [batch]
   float4* part;      // [rows, kMaxParts]: (m_p, z_p, m_q, z_q), or the best logit and its token at T = 0
-  int2* list;        // [1 + rows]: (count, -), then (sequence, node) of the nodes with residuals
+  int4* list;        // [1 + rows]: (count, -), then (sequence, node, first row, nodes) of those with residuals
   int rows, max_q, vocab, parts;
 };
 
@@ -402,7 +402,7 @@ __device__ __forceinline__ float remaining(float x, float wq, int v, const Level
 }
 
 // CTA (part, node, sequence): the part's maximum and sum of the node's rows.
-__global__ void __launch_bounds__(kThreads, 4) verify_stats_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kThreads, 6) verify_stats_kernel(const VerifyParams p) {
   __shared__ Exchange<kThreads> s_x;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_stats_kernel(const VerifyP
   const float temperature = p.temps[b];
   const int n = min(min(next, p.rows) - begin, p.max_q);
   if (node == 0 && part == 0 && threadIdx.x == 0) p.best[b] = VerifyBest{0ull, 0u, 0u};
-  if (b == 0 && node == 0 && part == 0 && threadIdx.x == 0) p.list[0] = make_int2(0, 0);
+  if (b == 0 && node == 0 && part == 0 && threadIdx.x == 0) p.list[0] = make_int4(0, 0, 0, 0);
   if (begin < 0 || node >= n) return;
   bool mine = false;
   for (int i = node + 1 + int(threadIdx.x); i < n; i += kThreads) mine |= p.parents[begin + i] == node;
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(kThreads) verify_tests_kernel(const VerifyPara
   const float a = acceptance(weight(lp, stats.x, c) * (1.0f / stats.y),
                              p.draft ? weight(lq, stats.z, c) * over_q : 1.0f);
   if (safe || (!(u < a) && kids > 1)) {
-    if (lane == 0) p.list[1 + atomicAdd(&p.list[0].x, 1)] = make_int2(b, node);
+    if (lane == 0) p.list[1 + atomicAdd(&p.list[0].x, 1)] = make_int4(b, node, begin, n);
     return;
   }
   if (u < a) {
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kThreads) verify_tests_kernel(const VerifyPara
 }
 
 // Clusters take the list's nodes in turn: all their children's tests.
-__global__ void __launch_bounds__(kListThreads, 2) verify_residuals_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kListThreads, 1) verify_residuals_kernel(const VerifyParams p) {
   __shared__ Exchange<kListThreads> s_x;
   __shared__ int s_child[kMaxNodes], s_token[kMaxNodes];
   __shared__ float s_lp[kMaxNodes], s_lq[kMaxNodes], s_u[kMaxNodes];  // children's logits and uniforms
@@ -596,8 +596,8 @@ __global__ void __launch_bounds__(kListThreads, 2) verify_residuals_kernel(const
   int turn = 0;
   if (size > 1) cluster_sync();  // all have started
   for (int at = int(blockIdx.x / size); at < count; at += step) {
-    const int b = p.list[1 + at].x, node = p.list[1 + at].y;
-    const int begin = p.cu_q[b], n = min(min(p.cu_q[b + 1], p.rows) - begin, p.max_q), row = begin + node;
+    const int4 entry = p.list[1 + at];
+    const int b = entry.x, node = entry.y, begin = entry.z, n = entry.w, row = begin + node;
     VerifyRow* ws = p.ws + begin;
     const Row lp(p.logits + (long long)row * p.vocab, p.vocab);
     const __nv_bfloat16* lq = p.draft ? p.draft + (long long)row * p.vocab : nullptr;
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(kListThreads, 2) verify_residuals_kernel(const
         // the tokens had most)
         float left = 0.0f, rest = 0.0f;
         if (lv.regular && !safe) {
-          each_group<2>(lp, lq, g0, g1, kListThreads, [&](int from, const uint4& vp, const uint4& vq) {
+          each_group<4>(lp, lq, g0, g1, kListThreads, [&](int from, const uint4& vp, const uint4& vq) {
             float2 x[4], w[4];
             weights8(vp, m_p, c, x);
 #pragma unroll
@@ -1017,7 +1017,7 @@ int verify_max_nodes() { return kMaxNodes; }
 
 size_t verify_workspace(int rows, int batch) {
   return size_t(rows) * (kMaxParts * sizeof(float4) + sizeof(VerifyRow)) + size_t(batch) * sizeof(VerifyBest) +
-         (size_t(rows) + 1) * sizeof(int2);
+         (size_t(rows) + 1) * sizeof(int4);
 }
 
 cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft, const int* tokens,
@@ -1029,9 +1029,10 @@ cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft,
   VerifyBest* const best = reinterpret_cast<VerifyBest*>(row + rows);
   VerifyParams p{static_cast<const __nv_bfloat16*>(logits), static_cast<const __nv_bfloat16*>(draft), tokens, parents,
                  uniforms, seeds, temps, cu_q, out_tokens, path, counts, accept, row, best, part,
-                 reinterpret_cast<int2*>(best + batch), rows, max_q, vocab, 1};
-  // CTAs that read a node's rows: 16 thousand logits each where that fills the GPU several times over, else 4 thousand.
-  const long long coarse = (vocab + 16383) / 16384;
+                 reinterpret_cast<int4*>(best + batch), rows, max_q, vocab, 1};
+  // CTAs that read a node's rows: 32 thousand logits each where that fills the GPU several times over (39 us for 360
+  // inner nodes of 151,936 tokens, 41 us with 16 thousand), else 4 thousand.
+  const long long coarse = (vocab + 32767) / 32768;
   p.parts = int(rows * coarse >= 8LL * sms ? coarse : (vocab + 4095) / 4096);
   if (p.parts > kMaxParts) p.parts = kMaxParts;
   // Programmatic dependents: launched while the kernel before them ends; they wait for it before any global access.
@@ -1050,10 +1051,11 @@ cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft,
   cfg.gridDim = dim3(unsigned((nodes + kThreads / 32 - 1) / (kThreads / 32)));
   e = cudaLaunchKernelEx(&cfg, verify_tests_kernel, p, batch);
   if (e != cudaSuccess) return e;
-  // Clusters for the list: CTAs of 4 thousand logits or more, two an SM, a few left for the clusters' placing.
+  // Clusters for the list: CTAs of 4 thousand logits or more, one an SM (with eight loads in flight a thread 27 us for
+  // 90 nodes of 64 trees; two an SM with half of them 32 us), a few SMs left for the clusters' placing.
   int cluster = 1;
   while (cluster < kMaxCluster && vocab >= 2 * cluster * 4096) cluster *= 2;
-  long long clusters = 2LL * sms * 7 / 8 / cluster;
+  long long clusters = 1LL * sms * 7 / 8 / cluster;
   clusters = clusters < 1 ? 1 : (clusters > rows ? rows : clusters);
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = unsigned(cluster);
