@@ -178,10 +178,11 @@ int nvb_peer_buffer_free(void* ptr);
  *  - lse (may be null) is [total_q, q_heads]. A node that sees no key has
  *    output 0 and lse -inf; so has a sequence with kv_lens < n or longer than
  *    its table.
- *  - num_splits > 1 cuts every sequence's keys into that many ranges with
- *    partials in lse_accum [num_splits, total_q, q_heads] and out_accum
- *    [num_splits, total_q, q_heads, 128] (FP32); calls that may overlap need
- *    their own. nvb_tree_num_splits gives the count for a GPU of num_sms SMs.
+ *  - num_splits cuts every sequence's keys into that many ranges. Where
+ *    nvb_tree_parts(num_splits) > 1 they need lse_accum [num_splits, total_q,
+ *    q_heads] and out_accum [num_splits, total_q, q_heads, 128] (FP32); calls
+ *    that may overlap need their own. nvb_tree_num_splits gives the count for
+ *    a GPU of num_sms SMs.
  *  - a key that a node does not see has no part in its result, whatever
  *    values the cache holds there (infinities and NaN too).
  *  - page ids outside [0, num_blocks) mask their tokens.
@@ -192,6 +193,10 @@ int nvb_paged_tree_fwd(void* stream, const void* q, const void* k, const void* v
                        int max_k, int q_heads, int kv_heads, int block_size, int table_stride,
                        int num_splits, float* lse, float* lse_accum, float* out_accum,
                        int num_blocks);
+/* Parts of a sequence that num_splits ranges leave in lse_accum / out_accum:
+ * 1 where they are joined on chip and the two are not used (they may be null
+ * then), else more; 0 for a count outside [1, 128]. */
+int nvb_tree_parts(int num_splits);
 int nvb_tree_num_splits(int batch, int max_q, int q_heads, int kv_heads, int max_k, int num_sms);
 
 /* Copies within the cache over all layers at once (no counterpart in the

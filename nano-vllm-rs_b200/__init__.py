@@ -13,7 +13,9 @@ registers it as ``nano_vllm_rs_b200``.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
+import math
 import os
 from pathlib import Path
 
@@ -51,6 +53,7 @@ def _declare(lib):
         "nvb_paged_decode_gather_capturable": [_P] * 8 + [c_int] * 8 + [_P] * 5 + [c_int, c_int],
         "nvb_paged_tree_fwd": [_P] * 9 + [c_int] * 10 + [_P] * 3 + [c_int],
         "nvb_tree_num_splits": [c_int] * 6,
+        "nvb_tree_parts": [c_int],
         "nvb_cache_copy_pages": [_P] * 3 + [c_int] + [_P] * 3 + [c_int] * 5,
         "nvb_cache_compact_paths": [_P] * 3 + [c_int] + [_P] * 6 + [c_int] * 7,
         "nvb_peer_buffer_create": [ctypes.c_size_t, ctypes.POINTER(c_void_p), _P],
@@ -133,22 +136,45 @@ def _distinct(output, inputs, name):
             raise NvbError(f"{name} aliases an input or another output")
 
 
-def _exact(t, shape, dtype, name):
-    """_tensor with the shape itself, on the current device (the kernels run there)."""
+def _refuse(t, shape, dtype, name, device):
+    if t.get_device() != device:
+        raise NvbError(f"{name} is on {t.device}, the current device is cuda:{device}")
+    if t.dtype is not dtype:
+        raise NvbError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise NvbError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise NvbError(f"{name} must be contiguous")
+
+
+def _pointers(arguments, written, device):
+    """Addresses of the arguments (name, tensor or None, shape, type): each of
+    that shape and type, contiguous and on the device, and none that is in
+    `written` overlapping another."""
+    pointers, spans, prod = [], [], math.prod
+    for name, t, shape, dtype in arguments:
+        if t is None:
+            pointers.append(None)
+            continue
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != device:
+            _refuse(t, shape, dtype, name, device)
+        p = t.data_ptr()
+        pointers.append(p)
+        spans.append((p, p + prod(shape) * dtype.itemsize, name))
+    spans.sort()
+    end, held = 0, False
+    for a, z, name in spans:
+        if a < end and a < z and (held or name in written):
+            raise NvbError(f"{name} overlaps another argument")
+        if z > end:
+            end, held = z, name in written
+    return pointers
+
+
+def _raw_stream(stream, device):
+    """The stream's handle; that of the device's current stream without one."""
     import torch
 
-    if t is None:
-        raise NvbError(f"{name} is required")
-    if not t.is_cuda:
-        raise NvbError(f"{name} must be a CUDA tensor")
-    if t.dtype != dtype:
-        raise NvbError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
-        raise NvbError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise NvbError(f"{name} must be contiguous")
-    if t.device.index != torch.cuda.current_device():
-        raise NvbError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device)
 
 
 def num_splits(batch, q_heads, kv_heads, max_k, num_sms):
@@ -288,18 +314,26 @@ def paged_fwd(q, k, v, out, cu_q, kv_lens, block_table, *, batch, max_q, max_k, 
                                 _ptr(out_accum), num_blocks))
 
 
+_sm_counts = {}
+
+
 def tree_num_splits(batch, max_q, q_heads, kv_heads, max_k, num_sms=None):
     """Split count of paged_tree_fwd for a GPU of num_sms SMs (default: the current device's)."""
     if num_sms is None:
         import torch
 
-        num_sms = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
+        device = torch.cuda.current_device()
+        num_sms = _sm_counts.get(device)
+        if num_sms is None:
+            num_sms = _sm_counts[device] = torch.cuda.get_device_properties(device).multi_processor_count
     return library().nvb_tree_num_splits(batch, max_q, q_heads, kv_heads, max_k, num_sms)
 
 
 def tree_scratch(num_splits_, total_q, q_heads, device):
-    """Caller-owned FP32 scratch (lse_accum, out_accum) of paged_tree_fwd; (None, None) for one split."""
-    return splitkv_scratch(num_splits_, total_q, q_heads, device) if num_splits_ > 1 else (None, None)
+    """Caller-owned FP32 scratch (lse_accum, out_accum) of paged_tree_fwd; (None, None) where it needs none."""
+    if library().nvb_tree_parts(num_splits_) == 1:
+        return None, None
+    return splitkv_scratch(num_splits_, total_q, q_heads, device)
 
 
 def paged_tree_fwd(q, k, v, out, cu_q, kv_lens, block_table, tree_mask, *, batch, max_q, max_k, q_heads, kv_heads,
@@ -311,37 +345,28 @@ def paged_tree_fwd(q, k, v, out, cu_q, kv_lens, block_table, tree_mask, *, batch
     last of its kv_lens[b] keys in the same order; tree_mask [total_q, words]
     int64 has bit t % 64 of word t // 64 set where a node attends to node t
     (host.tree_mask). The keys before the tree are visible to all. lse, where
-    given, is [total_q, q_heads].
+    given, is [total_q, q_heads]. lse_accum and out_accum: tree_scratch of
+    num_splits.
     """
     import torch
 
-    total_q, words = q.shape[0], tree_mask.shape[-1]
+    total_q, words, device = q.shape[0], tree_mask.shape[-1], torch.cuda.current_device()
     if check:
         bf16, i32, f32 = torch.bfloat16, torch.int32, torch.float32
-        for t, nm in ((q, "q"), (out, "out")):
-            _exact(t, (total_q, q_heads, 128), bf16, nm)
-        for t, nm in ((k, "k"), (v, "v")):
-            _exact(t, (num_blocks, block_size, kv_heads, 128), bf16, nm)
-        _exact(cu_q, (batch + 1,), i32, "cu_q")
-        _exact(kv_lens, (batch,), i32, "kv_lens")
-        _exact(block_table, (batch, table_stride), i32, "block_table")
-        _exact(tree_mask, (total_q, words), torch.int64, "tree_mask")
-        outputs = [out]
-        if lse is not None:
-            _exact(lse, (total_q, q_heads), f32, "lse")
-            outputs.append(lse)
-        if num_splits > 1:
-            _exact(lse_accum, (num_splits, total_q, q_heads), f32, "lse_accum")
-            _exact(out_accum, (num_splits, total_q, q_heads, 128), f32, "out_accum")
-            outputs += [lse_accum, out_accum]
-        taken = [q, k, v, cu_q, kv_lens, block_table, tree_mask]
-        for o in outputs:
-            _distinct(o, taken, "output")
-            taken.append(o)
-    _check(library().nvb_paged_tree_fwd(_stream(stream), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(cu_q),
-                                        _ptr(kv_lens), _ptr(block_table), _ptr(tree_mask), words, batch, total_q,
-                                        max_q, max_k, q_heads, kv_heads, block_size, table_stride, num_splits,
-                                        _ptr(lse), _ptr(lse_accum), _ptr(out_accum), num_blocks))
+        rows, cache = (total_q, q_heads, 128), (num_blocks, block_size, kv_heads, 128)
+        pointers = _pointers(
+            (("q", q, rows, bf16), ("k", k, cache, bf16), ("v", v, cache, bf16), ("out", out, rows, bf16),
+             ("cu_q", cu_q, (batch + 1,), i32), ("kv_lens", kv_lens, (batch,), i32),
+             ("block_table", block_table, (batch, table_stride), i32),
+             ("tree_mask", tree_mask, (total_q, words), torch.int64), ("lse", lse, (total_q, q_heads), f32),
+             ("lse_accum", lse_accum, (num_splits, total_q, q_heads), f32),
+             ("out_accum", out_accum, (num_splits, total_q, q_heads, 128), f32)),
+            ("out", "lse", "lse_accum", "out_accum"), device)
+    else:
+        pointers = [t.data_ptr() if t is not None else None
+                    for t in (q, k, v, out, cu_q, kv_lens, block_table, tree_mask, lse, lse_accum, out_accum)]
+    _check(library().nvb_paged_tree_fwd(_raw_stream(stream, device), *pointers[:8], words, batch, total_q, max_q, max_k, q_heads,
+                                        kv_heads, block_size, table_stride, num_splits, *pointers[8:], num_blocks))
 
 
 class CacheLayers:
@@ -357,30 +382,31 @@ class CacheLayers:
             raise NvbError(f"{len(k_caches)} K caches and {len(v_caches)} V caches")
         if k_caches[0].dim() != 4:
             raise NvbError("a cache must be [num_blocks, block_size, kv_heads, head_dim]")
-        self.shape = tuple(k_caches[0].shape)
-        for i, (k, v) in enumerate(zip(k_caches, v_caches)):
-            _exact(k, self.shape, torch.bfloat16, f"k_caches[{i}]")
-            _exact(v, self.shape, torch.bfloat16, f"v_caches[{i}]")
-        spans = sorted(_span(t) for t in k_caches + v_caches)
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise NvbError("two caches overlap")
-        self.layers = len(k_caches)
-        self.extent = (spans[0][0], spans[-1][1])
-        self.device = k_caches[0].device
+        self.shape, self.layers = tuple(k_caches[0].shape), len(k_caches)
+        self.device = torch.cuda.current_device()
+        names = [(f"{n}[{i}]", t) for n, ts in (("k_caches", k_caches), ("v_caches", v_caches)) for i, t in enumerate(ts)]
+        pointers = _pointers([(n, t, self.shape, torch.bfloat16) for n, t in names], [n for n, _ in names], self.device)
         self._tensors = k_caches + v_caches
-        self._k = (c_void_p * self.layers)(*[t.data_ptr() for t in k_caches])
-        self._v = (c_void_p * self.layers)(*[t.data_ptr() for t in v_caches])
+        self._starts = sorted(pointers)
+        self._bytes = k_caches[0].numel() * 2
+        self._k = (c_void_p * self.layers)(*pointers[:self.layers])
+        self._v = (c_void_p * self.layers)(*pointers[self.layers:])
 
-    def _apart(self, tensors):
+    def _pointers(self, arguments, written=()):
+        """Addresses of the arguments, checked; none may lie in a cache."""
         import torch
 
-        if self.device.index != torch.cuda.current_device():
-            raise NvbError(f"the caches are on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
-        for t in tensors:
-            a0, a1 = _span(t)
-            if a0 < self.extent[1] and self.extent[0] < a1 and any(
-                    a0 < s[1] and s[0] < a1 for s in map(_span, self._tensors)):
-                raise NvbError("an argument lies in a cache")
+        if self.device != torch.cuda.current_device():
+            raise NvbError(f"the caches are on cuda:{self.device}, the current device is "
+                           f"cuda:{torch.cuda.current_device()}")
+        pointers = _pointers(arguments, written, self.device)
+        for (name, t, shape, dtype), p in zip(arguments, pointers):
+            if p is None:
+                continue
+            i = bisect.bisect_right(self._starts, p + math.prod(shape) * dtype.itemsize - 1) - 1
+            if i >= 0 and p < self._starts[i] + self._bytes:
+                raise NvbError(f"{name} lies in a cache")
+        return pointers
 
 
 def cache_copy_pages(layers, src, dst, rows=None, *, stream=None):
@@ -391,13 +417,10 @@ def cache_copy_pages(layers, src, dst, rows=None, *, stream=None):
     import torch
 
     num_blocks, block_size, kv_heads, head_dim = layers.shape
-    pairs = src.numel()
-    arguments = [src, dst] + ([rows] if rows is not None else [])
-    for t, nm in zip(arguments, ("src", "dst", "rows")):
-        _exact(t, (pairs,), torch.int32, nm)
-    layers._apart(arguments)
-    _check(library().nvb_cache_copy_pages(_stream(stream), layers._k, layers._v, layers.layers, _ptr(src), _ptr(dst),
-                                          _ptr(rows), pairs, kv_heads, head_dim, block_size, num_blocks))
+    pairs, i32 = src.numel(), torch.int32
+    pointers = layers._pointers((("src", src, (pairs,), i32), ("dst", dst, (pairs,), i32), ("rows", rows, (pairs,), i32)))
+    _check(library().nvb_cache_copy_pages(_raw_stream(stream, layers.device), layers._k, layers._v, layers.layers, *pointers, pairs,
+                                          kv_heads, head_dim, block_size, num_blocks))
 
 
 def cache_compact_paths(layers, cu_q, kv_lens, block_table, path, counts, new_kv_lens, *, stream=None):
@@ -408,23 +431,16 @@ def cache_compact_paths(layers, cu_q, kv_lens, block_table, path, counts, new_kv
     import torch
 
     num_blocks, block_size, kv_heads, head_dim = layers.shape
-    batch = kv_lens.numel()
+    batch, i32 = kv_lens.numel(), torch.int32
     if path.dim() != 2 or block_table.dim() != 2:
         raise NvbError("path and block_table must have a row for each sequence")
-    i32 = torch.int32
-    _exact(cu_q, (batch + 1,), i32, "cu_q")
-    _exact(kv_lens, (batch,), i32, "kv_lens")
-    _exact(block_table, (batch, block_table.shape[1]), i32, "block_table")
-    _exact(path, (batch, path.shape[1]), i32, "path")
-    _exact(counts, (batch,), i32, "counts")
-    _exact(new_kv_lens, (batch,), i32, "new_kv_lens")
-    inputs = [cu_q, kv_lens, block_table, path, counts]
-    _distinct(new_kv_lens, inputs, "new_kv_lens")
-    layers._apart(inputs + [new_kv_lens])
-    _check(library().nvb_cache_compact_paths(_stream(stream), layers._k, layers._v, layers.layers, _ptr(cu_q),
-                                             _ptr(kv_lens), _ptr(block_table), _ptr(path), _ptr(counts),
-                                             _ptr(new_kv_lens), batch, path.shape[1], kv_heads, head_dim, block_size,
-                                             block_table.shape[1], num_blocks))
+    table_stride, path_stride = block_table.shape[1], path.shape[1]
+    pointers = layers._pointers(
+        (("cu_q", cu_q, (batch + 1,), i32), ("kv_lens", kv_lens, (batch,), i32),
+         ("block_table", block_table, (batch, table_stride), i32), ("path", path, (batch, path_stride), i32),
+         ("counts", counts, (batch,), i32), ("new_kv_lens", new_kv_lens, (batch,), i32)), ("new_kv_lens",))
+    _check(library().nvb_cache_compact_paths(_raw_stream(stream, layers.device), layers._k, layers._v, layers.layers, *pointers, batch,
+                                             path_stride, kv_heads, head_dim, block_size, table_stride, num_blocks))
 
 
 def attention(q, kcache, vcache, positions, seq_indices, tables, out, *, rows, q_heads, kv_heads, head_dim,

@@ -634,6 +634,16 @@ __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const 
 
 }  // namespace tree_detail
 
+namespace tree_detail {
+// CTAs that join their ranges on chip: the largest cluster whose size divides the splits.
+int tree_cluster(int num_splits) {
+  int cluster = 1;
+  for (int c = 2; c <= kMaxCluster; ++c)
+    if (num_splits % c == 0) cluster = c;
+  return cluster;
+}
+}  // namespace tree_detail
+
 cudaError_t launch_tree(const TreeParams& p, const void* k, const void* v, cudaStream_t stream) {
   using namespace tree_detail;
   CUtensorMap kmap, vmap;
@@ -656,10 +666,7 @@ cudaError_t launch_tree(const TreeParams& p, const void* k, const void* v, cudaS
   const int row_tiles = (p.max_q * group + kRows - 1) / kRows;
   const long long grid = (long long)p.batch * p.kvh * p.num_splits * row_tiles;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-  // The largest cluster whose size divides the splits.
-  int cluster = 1;
-  for (int c = 2; c <= kMaxCluster; ++c)
-    if (p.num_splits % c == 0) cluster = c;
+  const int cluster = tree_cluster(p.num_splits);
   // Programmatic dependents: launched while the kernel before them ends; they wait for it before any global access.
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -690,17 +697,21 @@ cudaError_t launch_tree(const TreeParams& p, const void* k, const void* v, cudaS
 
 extern "C" {
 
+int nvb_tree_parts(int num_splits) {
+  return num_splits < 1 || num_splits > 128 ? 0 : num_splits / nvb::tree_detail::tree_cluster(num_splits);
+}
+
 int nvb_tree_num_splits(int batch, int max_q, int q_heads, int kv_heads, int max_k, int num_sms) {
   if (batch <= 0 || max_q <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || max_k <= 0 ||
       num_sms <= 0 || num_sms > 1024)
     return 0;
   const long long tiles = ((long long)max_q * (q_heads / kv_heads) + 127) / 128;  // row tiles of a kv head
   const long long work = (long long)batch * kv_heads * tiles;
-  long long splits = 2LL * num_sms / work;             // two resident CTAs an SM
-  const long long by_len = (max_k + 255) / 256;        // at least 256 keys a split
-  if (splits > by_len) splits = by_len;
-  if (splits > 128) splits = 128;
-  return splits < 1 ? 1 : int(splits);
+  const long long fit = 2LL * num_sms / work;  // CTAs that fit at once, two an SM, for each unit of work
+  // Powers of two join on chip in clusters of 8 at most. A range of less than two tiles costs more to join than to read.
+  int splits = 1;
+  while (2 * splits <= fit && splits < 128 && 2LL * splits * 128 <= max_k) splits *= 2;
+  return splits;
 }
 
 int nvb_paged_tree_fwd(void* stream, const void* q, const void* k, const void* v, void* out, const int* cu_q,
@@ -714,7 +725,7 @@ int nvb_paged_tree_fwd(void* stream, const void* q, const void* k, const void* v
       q_heads % kv_heads || block_size <= 0 || block_size % 256 || table_stride <= 0 ||
       (long long)max_k > (long long)block_size * table_stride || (long long)block_size * table_stride > INT_MAX ||
       (long long)total_q * q_heads > INT_MAX || num_splits < 1 || num_splits > 128 ||
-      (num_splits > 1 && (!lse_accum || !out_accum)))
+      (nvb_tree_parts(num_splits) > 1 && (!lse_accum || !out_accum)))
     return fail("invalid paged tree attention BF16 hdim128 arguments");
   if (mask_words < 1 || mask_words > 16 || max_q > 64 * mask_words)
     return fail("tree_mask needs a bit for each of max_q nodes in 1 to 16 words (max_q %d, %d words)", max_q,

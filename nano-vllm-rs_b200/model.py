@@ -361,38 +361,25 @@ def layer_verify(logits, draft_logits, tokens, parents, uniforms, seeds, tempera
     when not given."""
     import torch
 
-    if logits.dim() != 2 or out_tokens.dim() != 2 or temperatures.dim() != 1:
-        raise ValueError("logits must be [rows, vocab], out_tokens [batch, max_q] and temperatures [batch]")
-    (rows, vocab), (batch, max_q) = logits.shape, out_tokens.shape
-    i32, f32 = torch.int32, torch.float32
-    seed_type = seeds.dtype if seeds.dtype == torch.uint64 else torch.int64
-    device = torch.cuda.current_device()
-    wanted = [("logits", logits, (rows, vocab), torch.bfloat16), ("tokens", tokens, (rows,), i32),
-              ("parents", parents, (rows,), i32), ("uniforms", uniforms, (rows,), f32),
-              ("seeds", seeds, (rows,), seed_type), ("temperatures", temperatures, (batch,), f32),
-              ("cu_q", cu_q, (batch + 1,), i32), ("out_tokens", out_tokens, (batch, max_q), i32),
-              ("path", path, (batch, max_q), i32), ("counts", counts, (batch,), i32),
-              ("accept_prob", accept_prob, (rows,), f32)]
-    if draft_logits is not None:
-        wanted.append(("draft_logits", draft_logits, (rows, vocab), torch.bfloat16))
-    if workspace is not None:
-        wanted.append(("workspace", workspace, (workspace.numel(),), torch.uint8))
-    for name, t, shape, dtype in wanted:
-        if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device.index != device \
-                or not t.is_cuda:
-            raise ValueError(f"{name} must be a contiguous {dtype} tensor {shape} on cuda:{device}")
-    written = ("out_tokens", "path", "counts", "accept_prob", "workspace")
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name) for name, t, _, _ in wanted)
-    end, held = 0, False
-    for a, z, name in spans:  # what is written overlaps nothing
-        if a < end and (held or name in written):
-            raise ValueError(f"{name} overlaps another argument")
-        if z > end:
-            end, held = z, name in written
+    from . import NvbError, _pointers, _raw_stream
+
+    if logits.dim() != 2 or out_tokens.dim() != 2:
+        raise ValueError("logits must be [rows, vocab] and out_tokens [batch, max_q]")
+    (rows, vocab), (batch, max_q), device = logits.shape, out_tokens.shape, torch.cuda.current_device()
+    i32, f32, bf16 = torch.int32, torch.float32, torch.bfloat16
     ws = workspace
     if ws is None:
         ws = torch.empty(max(16, verify_workspace_bytes(rows, batch)), dtype=torch.uint8, device=logits.device)
-    _check(library().nvbe_layer_verify(_s(stream), _p(logits), _p(draft_logits) if draft_logits is not None else None,
-                                       _p(tokens), _p(parents), _p(uniforms), _p(seeds), _p(temperatures), _p(cu_q),
-                                       _p(out_tokens), _p(path), _p(counts), _p(accept_prob), rows, batch, max_q,
-                                       vocab, _p(ws), ws.numel()))
+    try:
+        pointers = _pointers(
+            (("logits", logits, (rows, vocab), bf16), ("draft_logits", draft_logits, (rows, vocab), bf16),
+             ("tokens", tokens, (rows,), i32), ("parents", parents, (rows,), i32), ("uniforms", uniforms, (rows,), f32),
+             ("seeds", seeds, (rows,), torch.uint64 if seeds.dtype is torch.uint64 else torch.int64),
+             ("temperatures", temperatures, (batch,), f32), ("cu_q", cu_q, (batch + 1,), i32),
+             ("out_tokens", out_tokens, (batch, max_q), i32), ("path", path, (batch, max_q), i32),
+             ("counts", counts, (batch,), i32), ("accept_prob", accept_prob, (rows,), f32),
+             ("workspace", ws, (ws.numel(),), torch.uint8)),
+            ("out_tokens", "path", "counts", "accept_prob", "workspace"), device)
+    except NvbError as e:
+        raise ValueError(str(e)) from None
+    _check(library().nvbe_layer_verify(_raw_stream(stream, device), *pointers[:12], rows, batch, max_q, vocab, pointers[12], ws.numel()))

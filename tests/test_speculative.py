@@ -124,7 +124,7 @@ def _tree(lib, **kw):
                                  dict(max_q=65), dict(batch=0), dict(batch=65536), dict(total_q=0), dict(max_q=0),
                                  dict(max_k=0), dict(max_k=513), dict(qh=5), dict(qh=258, kvh=2), dict(kvh=0),
                                  dict(bs=128), dict(stride=0), dict(stride=1 << 24), dict(splits=0),
-                                 dict(splits=129), dict(splits=2, lse_accum=P(0)), dict(splits=2, out_accum=P(0)),
+                                 dict(splits=129), dict(splits=16, lse_accum=P(0)), dict(splits=11, out_accum=P(0)),
                                  dict(blocks=0), dict(blocks=1 << 24), dict(q=P(264)),
                                  dict(total_q=1 << 30)])
 def test_tree_refuses_on_the_host(nvb, bad):
@@ -135,6 +135,7 @@ def test_tree_refuses_on_the_host(nvb, bad):
 
 def test_tree_num_splits(nvb):
     lib = nvb.library()
+    assert [lib.nvb_tree_parts(s) for s in (0, 1, 2, 7, 8, 9, 11, 16, 128, 129)] == [0, 1, 1, 1, 1, 3, 11, 2, 16, 0]
     for bad in ((0, 4, 16, 8, 100, 148), (1, 0, 16, 8, 100, 148), (1, 4, 16, 5, 100, 148), (1, 4, 16, 8, 0, 148),
                 (1, 4, 16, 8, 100, 0)):
         assert lib.nvb_tree_num_splits(*bad) == 0

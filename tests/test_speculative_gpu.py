@@ -226,7 +226,7 @@ def test_tree_attention_equals_the_causal_and_decode_entry_points(nvb):
     case = Case([9, 20, 3], [300, 40, 129], 8, 2, "chain", seed=10, spare_rows=0)
     a = case.args()
     out, lse = case.run(nvb, 2, args=a)
-    other, _ = torch.empty_like(out), None
+    other = torch.empty_like(out)
     nvb.paged_fwd(a["q"], a["k"], a["v"], other, a["cu_q"], a["kv_lens"], a["block_table"], **case.shape())
     ref = case.reference()
     close(case, out, lse, ref)
