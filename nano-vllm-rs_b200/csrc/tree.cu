@@ -225,21 +225,27 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (lane == 0) {
       tma_prefetch_desc(&kmap);
       tma_prefetch_desc(&vmap);
+      const int final = fd_bs.div((t0 + ntiles - 1) * kKeys);
       int issued = 0, page = page0, last = fd_bs.div(t0 * kKeys);
+      int ahead = last < final ? table[last + 1] : -1;  // the next page, loaded a page ahead
+      int behind = page;                                // the one before: K runs a tile ahead of V
       for (int i = 0; i < 2 * ntiles; ++i) {
         const bool is_v = i > 0 && ((i & 1) == 0 || i == 2 * ntiles - 1);
         const int j = i == 0 ? 0 : (i == 2 * ntiles - 1 ? ntiles - 1 : (is_v ? i / 2 - 1 : (i + 1) / 2));
         const int key0 = (t0 + j) * kKeys, logical = fd_bs.div(key0), slot = i % kSlots;
-        if (logical != last) {
-          page = table[logical];
+        if (logical > last) {
+          behind = page;
+          page = ahead;
           last = logical;
+          ahead = logical < final ? table[logical + 1] : -1;
         }
+        const int mine = logical == last ? page : behind;
         // released by the MMA that read the slot's last load: S of a K tile, PV of a V tile
         if (i >= kSlots && !wait(&bars[kEmpty + slot], ((i / kSlots) + 1) & 1)) break;
-        if (page_ok(page, p.num_blocks)) {
+        if (page_ok(mine, p.num_blocks)) {
           const CUtensorMap* map = is_v ? &vmap : &kmap;
           unsigned char* dst = smem_raw + kRingOff + slot * kTileBytes;
-          const int trow = page * p.block_size + (key0 - logical * p.block_size);
+          const int trow = mine * p.block_size + (key0 - logical * p.block_size);
           mbar_arrive_expect_tx(&bars[kFull + slot], kTileBytes);
           tma_load_3d(dst, map, &bars[kFull + slot], 0, kvhead, trow);
           tma_load_3d(dst + kHalf, map, &bars[kFull + slot], 64, kvhead, trow);
@@ -303,9 +309,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     const float sl2 = p.scale_log2;
     float m_used = -INFINITY, l = 0.0f;
     bool alive = true;
+    // The next tile's page is loaded a tile ahead: with the shared memory taken by the tiles little is left for L1,
+    // so the load goes to L2 (several hundred cycles, as long as the exponentials).
+    int page = table[fd_bs.div(t0 * kKeys)];
     for (int j = 0; j < ntiles; ++j) {
       const int key0 = (t0 + j) * kKeys;
-      const bool ok = page_ok(table[fd_bs.div(key0)], p.num_blocks);
+      const bool ok = page_ok(page, p.num_blocks);
+      if (j + 1 < ntiles) page = table[fd_bs.div(key0 + kKeys)];
       const bool plain = ok && key0 + kKeys <= ctx;  // every row sees every key
       const int real = ok ? min(kKeys, len - key0) : 0;  // keys of the sequence
       unsigned long long seen = ~0ull;
@@ -437,10 +447,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (mend && row_ok) {  // what the tree keys' V rows held beside numbers
         for (int t = max(0, t0 * kKeys - ctx); t < min(n, (t0 + ntiles) * kKeys - ctx); ++t) {
           if (!(mask_window(mask, p.mask_words, t) & 1)) continue;
-          const int page = table[fd_bs.div(ctx + t)];
-          if (!page_ok(page, p.num_blocks)) continue;
+          const int vpage = table[fd_bs.div(ctx + t)];
+          if (!page_ok(vpage, p.num_blocks)) continue;
           const __nv_bfloat16* row =
-              vcache + (((long long)page * p.block_size + (ctx + t - fd_bs.div(ctx + t) * p.block_size)) * p.kvh +
+              vcache + (((long long)vpage * p.block_size + (ctx + t - fd_bs.div(ctx + t) * p.block_size)) * p.kvh +
                         kvhead) * 128 + 32 * h;
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
