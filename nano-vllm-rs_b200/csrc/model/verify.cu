@@ -23,9 +23,10 @@
 // whose first child is rejected with a sibling behind it go on a list, and
 // verify_residuals_kernel works through that: a cluster of up to 4 CTAs a node,
 // one more pass over its rows (from L2 where they fit) for each further
-// sibling. As many clusters as fit the GPU take the list in turn: with a cluster
-// launched for every node, 64 trees of 8 nodes took 88 us, as clusters of 4 and 8
-// were dispatched at ~150 ns each.
+// sibling. As many clusters as fit the GPU take the list in turn. (One kernel with a
+// cluster for every node, doing all of this, took 88 us for 64 trees of 8 nodes,
+// the three take 38 + 4 + 27 us: most of a node's cluster's time went on its
+// start, its joins and its tests, with nothing to read.)
 //
 // verify_sample_kernel follows the accepted children from the root and draws
 // the next token from the last node's row, cut over CTAs. A token's score is
