@@ -142,7 +142,8 @@ __device__ __forceinline__ float weight(float l, float m, float c) {
   return m == -INFINITY ? 0.0f : ex2((l - m) * c);
 }
 
-__device__ __forceinline__ float inv_temperature(float t) { return fminf(kLog2e / t, 1e38f); }
+// log2(e) / T, never 0: logits of -inf have no probability at any temperature (0 times them is NaN)
+__device__ __forceinline__ float inv_temperature(float t) { return fminf(fmaxf(kLog2e / t, 1.2e-38f), 1e38f); }
 
 // ------------------------------------------------------------- rows of logits
 // A row starts at any element (odd vocabularies), so it is read in the aligned
@@ -559,7 +560,15 @@ __global__ void __launch_bounds__(kThreads) verify_tests_kernel(const VerifyPara
   const float a = acceptance(weight(lp, stats.x, c) * (1.0f / stats.y),
                              p.draft ? weight(lq, stats.z, c) * over_q : 1.0f);
   if (safe || (!(u < a) && kids > 1)) {
-    if (lane == 0) p.list[1 + atomicAdd(&p.list[0].x, 1)] = make_int4(b, node, begin, n);
+    if (lane == 0) {
+      const int place = atomicAdd(&p.list[0].x, 1);
+      if (place < p.rows) {
+        p.list[1 + place] = make_int4(b, node, begin, n);
+      } else {  // sequences that overlap: more nodes than rows
+        ws[node].winner = -1;
+        ws[node].rejected = 0;
+      }
+    }
     return;
   }
   if (u < a) {
@@ -592,7 +601,7 @@ __global__ void __launch_bounds__(kListThreads, 1) verify_residuals_kernel(const
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t size = cluster_size(), rank = cluster_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int count = p.list[0].x, step = int(gridDim.x / size);
+  const int count = min(p.list[0].x, p.rows), step = int(gridDim.x / size);
   const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
   int turn = 0;
   if (size > 1) cluster_sync();  // all have started
@@ -818,7 +827,7 @@ __global__ void __launch_bounds__(kSampleThreads, 4) verify_sample_kernel(const 
   if (threadIdx.x == 0) {
     int at = 0, count = 1;
     s_path[0] = 0;
-    while (s_winner[at] > at) {
+    while (s_winner[at] > at && s_winner[at] < n) {  // n: sequences that overlap write each other's
       at = s_winner[at];
       s_path[count++] = at;
     }

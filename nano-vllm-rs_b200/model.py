@@ -369,7 +369,8 @@ def layer_verify(logits, draft_logits, tokens, parents, uniforms, seeds, tempera
     i32, f32, bf16 = torch.int32, torch.float32, torch.bfloat16
     ws = workspace
     if ws is None:
-        ws = torch.empty(max(16, verify_workspace_bytes(rows, batch)), dtype=torch.uint8, device=logits.device)
+        with torch.cuda.stream(stream):  # of that stream's memory: it is given on after this call returns
+            ws = torch.empty(max(16, verify_workspace_bytes(rows, batch)), dtype=torch.uint8, device=logits.device)
     try:
         pointers = _pointers(
             (("logits", logits, (rows, vocab), bf16), ("draft_logits", draft_logits, (rows, vocab), bf16),

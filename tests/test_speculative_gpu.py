@@ -301,6 +301,94 @@ def test_tree_attention_captured_with_changing_lengths(nvb):
             close(case, out, lse, case.reference())
 
 
+@pytest.mark.parametrize("splits", [11, 12, 24, 97])
+def test_tree_attention_splits_that_leave_parts(nvb, splits):
+    # clusters of 1, 6, 8 and 1, with 11, 2, 3 and 97 parts joined by the second kernel
+    check(nvb, Case([9, 3, 40, 1], [1500, 0, 1000, 127], 8, 2, seed=splits), splits)
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+def test_tree_attention_the_largest_tree(nvb, splits):
+    # 1,024 nodes of 16 words: 16 row tiles of 128 rows a head group
+    check(nvb, Case([1024, 3], [70, 300], 4, 2, "tree", seed=40), splits)
+
+
+def test_tree_attention_lengths_below_zero(nvb):
+    # a length that wraps around with the nodes subtracted is no length
+    case = Case([4, 4, 4], [100, 100, 100], 4, 2, seed=41)
+    a = case.args()
+    a["kv_lens"] = torch.tensor([-2 ** 31, -1, case.lens[2]], dtype=torch.int32, device="cuda")
+    for splits in (1, 3):
+        out, lse = case.run(nvb, splits, args=a)
+        assert (out[:8] == 0).all() and (lse[:8] == -math.inf).all() and torch.isfinite(lse[8:12]).all()
+
+
+def test_tree_attention_between_the_other_kernels(nvb):
+    # tree, causal and decode calls queued on one stream without a wait: kernels that are launched while the one before
+    # them runs, and take tensor memory. Each leaves the bits that it leaves alone.
+    case = Case([16] * 24, [700] * 24, 8, 2, "chain", seed=42, spare_rows=0)
+    one = Case([1] * 24, [700] * 24, 8, 2, "chain", seed=43, spare_rows=0)
+    a, d = case.args(), one.args()
+    rows = lambda c: torch.zeros(c.rows, 8, 128, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    scratch = {s: nvb.tree_scratch(s, case.rows, 8, "cuda") for s in (1, 2, 11)}
+
+    def tree(out, splits):
+        la, oa = scratch[splits]
+        nvb.paged_tree_fwd(**a, out=out, num_splits=splits, lse_accum=la, out_accum=oa, **case.shape())
+
+    def causal(out, x, c):
+        nvb.paged_fwd(x["q"], x["k"], x["v"], out, x["cu_q"], x["kv_lens"], x["block_table"], **c.shape())
+
+    calls = [lambda o: tree(o, 1), lambda o: causal(o, a, case), lambda o: tree(o, 11), lambda o: causal(o, d, one),
+             lambda o: tree(o, 2)]
+    want = []
+    for i, call in enumerate(calls):
+        out = rows(one if i == 3 else case)
+        call(out)
+        torch.cuda.synchronize()
+        want.append(out)
+    outs = [[torch.zeros_like(w) for w in want] for _ in range(8)]
+    torch.cuda.synchronize()
+    for turn in outs:
+        for call, out in zip(calls, turn):
+            call(out)
+    torch.cuda.synchronize()
+    assert nvb.device_error() == 0
+    for turn in outs:
+        for w, out in zip(want, turn):
+            assert torch.equal(w, out)
+
+
+def test_tree_attention_parts_captured_and_at_the_same_time(nvb):
+    # two graphs whose splits leave parts, with scratch of their own, replayed side by side over one cache
+    case = Case([9, 3, 30], [1500, 0, 1000], 8, 2, seed=44)
+    want, _ = case.run(nvb, 11)
+    a, graphs = case.args(), []
+    for _ in range(2):
+        (la, oa), stream = nvb.tree_scratch(11, case.rows, 8, "cuda"), torch.cuda.Stream()
+        out = torch.full_like(want, 7.0)
+        torch.cuda.synchronize()
+
+        def step(out=out, la=la, oa=oa, stream=stream):
+            nvb.paged_tree_fwd(**a, out=out, num_splits=11, lse_accum=la, out_accum=oa, stream=stream, **case.shape())
+
+        step()
+        stream.synchronize()
+        graphs.append((nvb.capture(step, keep=[a, out, la, oa], stream=stream), out, la, oa, stream))
+    for _ in range(3):
+        for _, out, la, oa, _ in graphs:
+            out.fill_(7.0)
+            la.fill_(math.nan)
+            oa.fill_(math.nan)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for graph, _, _, _, stream in graphs:
+                graph.replay(stream)
+        torch.cuda.synchronize()
+        for _, out, _, _, _ in graphs:
+            assert torch.equal(out, want)
+
+
 def test_tree_attention_in_a_cache_past_32_bit_offsets(nvb):
     # 8,704 pages of 256 x 8 x 128 elements: the last ones start past 2^31
     blocks = 8704
@@ -548,6 +636,62 @@ def test_verify_captured_and_on_two_streams(nvb):
         torch.cuda.synchronize()
         for case, (_, _, o, _, _) in zip(cases, runs):
             same(case, o)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("temperature", [3e38, math.inf])
+def test_verify_at_endless_temperatures(nvb, draft, temperature):
+    # as at 1e30, where every finite logit has the same weight too, and logits of -inf none
+    runs = []
+    for t in (1e30, temperature):
+        case = Drafts([7, 1, 4], 900, 3, draft, [t] * 3, seed=54)
+        for x in (case.logits, case.draft) if draft else (case.logits,):
+            x[:, ::3] = -math.inf
+        runs.append(case.run(nvb))
+    for name in runs[0]:
+        assert torch.equal(runs[0][name], runs[1][name]), name
+    assert (runs[1]["accept_prob"][1:7] > 0).any()
+    last = runs[1]["out_tokens"].gather(1, (runs[1]["counts"] - 1).long()[:, None])
+    assert (last % 3 != 0).all()
+
+
+def test_verify_workspace_of_a_call_on_another_stream(nvb):
+    # The workspace of a call without one is not given on to work of the current stream that may run before the call.
+    case, stream = Drafts([8] * 4, 20000, 3, True, seed=55), torch.cuda.Stream()
+    a, ref = case.args(), case.reference()
+    size = nvb.model.verify_workspace_bytes(len(case.tokens), 4)
+    for _ in range(4):
+        o = case.outputs()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(20_000_000)
+        nvb.model.layer_verify(**a, **o, stream=stream)
+        for _ in range(50):
+            torch.full((size,), 0xff, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        same(case, o, ref)
+
+
+def test_verify_sequences_that_overlap_stay_in_bounds(nvb):
+    # cu_q that falls: five sequences share eight rows, so that more nodes than rows have rejected children, and a row
+    # is written by several. What comes out is not defined, but it names nodes, and nothing behind the workspace changes.
+    case = Drafts([8], 500, 3, True, [1.0], seed=53)
+    for parents in ([-1, 0, 0, 0, 1, 1, 4, 4], [-1, 0, 0, 2, 2, 0, 0, 6]):
+        for cu in ([0, 8] * 5, [0, 8, 4, 8, 2, 8, 4, 8, 0, 8]):
+            case.parents[:8] = parents
+            case.uniforms[:] = 1.0
+            a, batch = case.args(), 9
+            a["cu_q"] = torch.tensor(cu, dtype=torch.int32, device="cuda")
+            a["temperatures"] = torch.ones(batch, device="cuda")
+            i32 = dict(dtype=torch.int32, device="cuda")
+            o = dict(out_tokens=torch.zeros(batch, 8, **i32), path=torch.zeros(batch, 8, **i32),
+                     counts=torch.zeros(batch, **i32), accept_prob=torch.zeros(len(case.tokens), device="cuda"))
+            size = nvb.model.verify_workspace_bytes(len(case.tokens), batch)
+            ws = torch.full((size + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+            nvb.model.layer_verify(**a, **o, workspace=ws[:size])
+            assert (ws[size:] == 0x5a).all()
+            assert (o["counts"] >= 0).all() and (o["counts"] <= 8).all() and (o["counts"][1::2] == 0).all()
+            assert (o["path"] >= -1).all() and (o["path"] < 8).all()
 
 
 def test_verify_refuses(nvb):
