@@ -36,6 +36,13 @@
 // second kernel. More splits (few sequences, long contexts) are several
 // clusters a sequence, whose joined rows go through lse_accum / out_accum.
 //
+// Measured (32 query and 8 KV heads, B200, copy rate 6.57 TB/s): 37 sequences
+// of 8192 keys with 32 nodes each 190 us (6.56 TB/s); 64 of ~4050 keys with 32
+// nodes 168 us (6.34 TB/s, launch included); 4 of ~32700 keys in 8 splits
+// 91 us (5.86 TB/s: a launch has 256 CTAs, 40 of the 296 places stay empty); 1
+// of 400 keys 8.6 us, where the launch, two round trips to memory and the join
+// are the time.
+//
 // Keys that a node does not see get probability 0; their V rows must not hold
 // infinities or NaN, as 0 times those is not 0. V rows of keys that nobody
 // sees (behind the sequence, bad pages) are zeroed in shared memory. A tree
@@ -138,7 +145,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     tree_kernel(const TreeParams p, const FastDiv fd_group, const FastDiv fd_bs, const int row_tiles,
                 const __nv_bfloat16* __restrict__ vcache, const __grid_constant__ CUtensorMap kmap,
                 const __grid_constant__ CUtensorMap vmap) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + kTmemSlotOff);
@@ -178,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int begin = p.cu_q[b], next = p.cu_q[b + 1], len = p.kv_lens[b];
   const int n = min(next, p.total_q) - begin, ctx = len - n;
   const int row0 = tile * kRows, rows = begin < 0 ? 0 : min(n, p.max_q) * group - row0;  // none for all of a cluster
-  const bool valid = ctx >= 0 && (long long)len <= (long long)p.table_stride * p.block_size;
+  const bool valid = len >= n && len >= 0 && (long long)len <= (long long)p.table_stride * p.block_size;
   const int tiles_total = valid ? (len + kKeys - 1) / kKeys : 0;
   const int per_split = (tiles_total + p.num_splits - 1) / p.num_splits;
   const int t0 = split * per_split, ntiles = rows > 0 ? max(0, min(t0 + per_split, tiles_total) - t0) : 0;
@@ -216,6 +222,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // The next kernel may be scheduled now: a CTA of it that takes TMEM and waits for this grid finds that all of this
+  // grid's CTAs have theirs.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   float2* stats = reinterpret_cast<float2*>(smem_raw + kStatsOff);
   if (!work) {
@@ -642,9 +651,6 @@ __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const 
   if (lane == 0 && p.lse) p.lse[item] = total == 0.0f ? -INFINITY : mx + __logf(total);
 }
 
-}  // namespace tree_detail
-
-namespace tree_detail {
 // CTAs that join their ranges on chip: the largest cluster whose size divides the splits.
 int tree_cluster(int num_splits) {
   int cluster = 1;
