@@ -133,8 +133,9 @@ struct TreeParams {
   float* out_accum;          // [splits, total_q, qh, 128] (splits > 1)
   int batch, total_q, max_q, qh, kvh, block_size, table_stride, num_blocks, num_splits, mask_words;
   float scale_log2;
+  bool by_length;            // set by launch_tree: sequences in falling order of kv_lens
 };
-cudaError_t launch_tree(const TreeParams& p, const void* k, const void* v, cudaStream_t stream);
+cudaError_t launch_tree(TreeParams p, const void* k, const void* v, int max_k, cudaStream_t stream);
 
 // Native-form attention for head dimensions other than 128 (generic.cu).
 cudaError_t launch_generic_attention(const void* q, const void* k, const void* v, void* out, const int* positions,

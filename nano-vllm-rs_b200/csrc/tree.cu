@@ -63,6 +63,8 @@ constexpr int kTileBytes = 2 * kHalf;   // K or V tile 64 x 128 BF16
 constexpr int kQHalf = kRows * 128;     // Q: 128 rows x 64 BF16, twice
 constexpr int kSlots = 5;               // ring slots shared by K and V tiles
 constexpr int kThreads = 192;
+constexpr int kMaxOrdered = 64;         // sequences that a launch puts in order
+constexpr int kOrderedKeys = 2048;      // keys of a range from which on it does
 constexpr int kMaxCluster = 8;          // CTAs that join through shared memory
 constexpr int kTmemCols = 256;
 constexpr int kOCol = 128;              // S/P buffers at 0 and 64
@@ -75,13 +77,14 @@ enum Bar { kFull = 0, kEmpty = kFull + kSlots, kSFull = kEmpty + kSlots, kPFull 
            kPVDone = kPFull + 2, kODone, kDrain, kNumBars };
 constexpr int kTmemSlotOff = kNumBars * 8;
 constexpr int kFlagOff = kTmemSlotOff + 4;
+constexpr int kLensOff = (kFlagOff + 4 + 15) & ~15;  // int [kMaxOrdered]: lengths, while the sequences are put in order
 constexpr int kOutRow = 272;      // bytes of a row of the output in the ring
 constexpr int kSumRow = 132 * 4;  // bytes of a row of O in the ring at the join: 4 banks apart from the next
 constexpr int kHeadBytes = 1024;  // tiles start at the next 1 KB boundary
 constexpr int kStatsOff = kHeadBytes;  // float2 [128] where Q was: a row's maximum in use and sum, for the join
 constexpr int kFactorOff = kStatsOff + kRows * 8;  // float [rows of a CTA][cluster]
 static_assert(kFactorOff + kRows * kMaxCluster * 4 <= kHeadBytes + 2 * kQHalf, "the join's tables fit where Q was");
-static_assert(kFlagOff + 4 <= kHeadBytes, "barrier block must fit below the first 1 KB boundary");
+static_assert(kLensOff + kMaxOrdered * 4 <= kHeadBytes, "barrier block must fit below the first 1 KB boundary");
 static_assert(kRows * kSumRow <= kSlots * kTileBytes && kOutRow <= kSumRow, "the ring holds the rows of O at the join");
 constexpr int kRingOff = kHeadBytes + 2 * kQHalf;
 constexpr int kSmemBytes = kRingOff + kSlots * kTileBytes;  // two CTAs an SM: at most 113 KB each
@@ -158,7 +161,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   cta /= p.num_splits;
   const int tile = cta % row_tiles;
   cta /= row_tiles;
-  const int kvhead = cta % p.kvh, b = cta / p.kvh;
+  const int kvhead = cta % p.kvh;
+  int b = cta / p.kvh;
   const int group = p.qh / p.kvh;
 
   // Set-up that needs no input runs beside the end of the kernel before this one.
@@ -181,6 +185,25 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   // That kernel has completed, its writes are visible.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.by_length) {  // the b-th longest sequence (see launch_tree); equal lengths in their order
+    const int t = threadIdx.x, len = t < p.batch ? p.kv_lens[t] : INT_MIN;  // after the last: behind all
+    int* lens = reinterpret_cast<int*>(smem_raw + kLensOff);
+    if (t < kMaxOrdered) lens[t] = len;
+    __syncthreads();
+    if (t < p.batch) {
+      int place = 0;
+      for (int u = 0; u < p.batch; u += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(lens + u);
+        place += (o.x > len || (o.x == len && u < t)) + (o.y > len || (o.y == len && u + 1 < t)) +
+                 (o.z > len || (o.z == len && u + 2 < t)) + (o.w > len || (o.w == len && u + 3 < t));
+      }
+      if (place == b) *bad_v = t;
+    }
+    __syncthreads();
+    b = *bad_v;
+    __syncthreads();
+    if (t == 0) *bad_v = 0;
+  }
   const int begin = p.cu_q[b], next = p.cu_q[b + 1], len = p.kv_lens[b];
   const int n = min(next, p.total_q) - begin, ctx = len - n;
   const int row0 = tile * kRows, rows = begin < 0 ? 0 : min(n, p.max_q) * group - row0;  // none for all of a cluster
@@ -660,7 +683,16 @@ int tree_cluster(int num_splits) {
 }
 }  // namespace tree_detail
 
-cudaError_t launch_tree(const TreeParams& p, const void* k, const void* v, cudaStream_t stream) {
+static int sm_count() {
+  static int counts[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int& n = counts[dev & 63];
+  if (!n && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n = 0;
+  return n;
+}
+
+cudaError_t launch_tree(TreeParams p, const void* k, const void* v, int max_k, cudaStream_t stream) {
   using namespace tree_detail;
   CUtensorMap kmap, vmap;
   {
@@ -683,6 +715,11 @@ cudaError_t launch_tree(const TreeParams& p, const void* k, const void* v, cudaS
   const long long grid = (long long)p.batch * p.kvh * p.num_splits * row_tiles;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
   const int cluster = tree_cluster(p.num_splits);
+  // Ragged batches: the longest sequences' CTAs start first and the short ones fill in behind and beside them (64
+  // sequences of 16 to 8192 keys 237 -> 194 us; 16 of 500 to 8192 with 192 rows and two splits 127 -> 106). Only where
+  // CTAs share an SM or wait for one, for ranges that outlast the ordering (~1 us a CTA: 190 sequences of 512 keys
+  // 86 -> 99 us with it), and for at most 64 sequences (150 of 16 to 4096 keys, four CTAs one behind the other: 208 -> 216).
+  p.by_length = grid > sm_count() && p.batch > 1 && p.batch <= kMaxOrdered && max_k >= p.num_splits * kOrderedKeys;
   // Programmatic dependents: launched while the kernel before them ends; they wait for it before any global access.
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -727,6 +764,14 @@ int nvb_tree_num_splits(int batch, int max_q, int q_heads, int kv_heads, int max
   // Powers of two join on chip in clusters of 8 at most. A range of less than two tiles costs more to join than to read.
   int splits = 1;
   while (2 * splits <= fit && splits < 128 && 2LL * splits * 128 <= max_k) splits *= 2;
+  // The lengths of a batch are not known here. Long ranges are cut further, to 2560 keys and eight CTAs an SM at most,
+  // so that a batch of different lengths does not wait for its longest (32 query and 8 KV heads: 10, 20, 32, 48 and 64
+  // sequences of 500 to 32768, 32768, 8192, 8192 and 16384 keys 164 -> 66, 280 -> 89, 71 -> 49, 102 -> 78 and
+  // 188 -> 114 us). Where all are of one length that costs 6 to 14 % (32 of 8192: 168 -> 177 us, 20: 135 -> 154), and
+  // more the shorter the ranges (24 of 2048, two ranges: 44 -> 58).
+  while (2 * splits * work <= 8LL * num_sms && 2 * splits <= nvb::tree_detail::kMaxCluster &&
+         2LL * splits * 2560 <= max_k)
+    splits *= 2;
   return splits;
 }
 
@@ -772,7 +817,7 @@ int nvb_paged_tree_fwd(void* stream, const void* q, const void* k, const void* v
   p.num_splits = num_splits;
   p.mask_words = mask_words;
   p.scale_log2 = kScaleLog2;
-  return cuda_status(launch_tree(p, k, v, static_cast<cudaStream_t>(stream)), "tree attention launch");
+  return cuda_status(launch_tree(p, k, v, max_k, static_cast<cudaStream_t>(stream)), "tree attention launch");
 }
 
 }  // extern "C"

@@ -313,6 +313,28 @@ def test_tree_attention_the_largest_tree(nvb, splits):
     check(nvb, Case([1024, 3], [70, 300], 4, 2, "tree", seed=40), splits)
 
 
+@pytest.mark.parametrize("batch, kvh, splits", [(64, 4, 1), (64, 4, 2), (23, 8, 1), (65, 4, 1), (2, 80, 1)])
+def test_tree_attention_of_ragged_batches(nvb, batch, kvh, splits):
+    # more CTAs than SMs and long ranges: the sequences are taken in the order of their lengths. Equal lengths, empty
+    # sequences, a length that does not fit and one below zero among them.
+    rng = np.random.RandomState(batch)
+    ctxs = rng.choice([0, 1, 60, 61, 200, 300], batch)
+    nodes = rng.choice([0, 1, 3, 4], batch)
+    ctxs[batch // 2], nodes[batch // 2] = 3900, 4
+    case = Case(nodes.tolist(), ctxs.tolist(), 2 * kvh, kvh, seed=batch)
+    a, want = case.args(), case.reference()
+    close(case, *case.run(nvb, splits, args=a), want)
+    if batch < 8:
+        return
+    nodes[[3, 5]] = 2
+    case = Case(nodes.tolist(), ctxs.tolist(), 2 * kvh, kvh, seed=batch + 1)
+    a, want = case.args(), case.reference()
+    a["kv_lens"][3], a["kv_lens"][5] = -7, case.stride * 256 + 1
+    for b in (3, 5):
+        want[0][case.cu[b]:case.cu[b + 1]], want[1][case.cu[b]:case.cu[b + 1]] = 0, -math.inf
+    close(case, *case.run(nvb, splits, args=a), want)
+
+
 def test_tree_attention_lengths_below_zero(nvb):
     # a length that wraps around with the nodes subtracted is no length
     case = Case([4, 4, 4], [100, 100, 100], 4, 2, seed=41)
