@@ -21,11 +21,11 @@
 // verify_tests_kernel, a warp a node, joins a node's parts and tests its first
 // child, as if the node had been reached, so that all nodes run at once. Nodes
 // whose first child is rejected with a sibling behind it go on a list, and
-// verify_residuals_kernel works through that: a cluster of up to 4 CTAs a node,
+// verify_residuals_kernel works through that: a cluster of up to 8 CTAs a node,
 // one more pass over its rows (from L2 where they fit) for each further
 // sibling. As many clusters as fit the GPU take the list in turn. (One kernel with a
 // cluster for every node, doing all of this, took 88 us for 64 trees of 8 nodes,
-// the three take 38 + 4 + 27 us: most of a node's cluster's time went on its
+// the three take 38 + 4 + 24 us: most of a node's cluster's time went on its
 // start, its joins and its tests, with nothing to read.)
 //
 // verify_sample_kernel follows the accepted children from the root and draws
@@ -40,6 +40,12 @@
 // tokens. What bounds it is the issue rate: ~35 instructions a token. The CTAs'
 // best meet in a 64-bit maximum (score, then the lowest token), which no
 // order of arrival changes.
+//
+// Measured (B200; 64 trees of 8 nodes, vocabulary 151,936, draft logits): 38 +
+// 4 + 24 + 31 us, 95 together, for the 188 MB that have to be read (29 us).
+// The sums take 160 MB of them at 4.2 TB/s, with 1.5 waves of CTAs and 59 % of
+// the issue slots; the draw uses 61 % of those. One tree of 5 nodes takes 16.6
+// us: four kernels, each a chain of reads that wait for one another.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -55,11 +61,11 @@ namespace {
 using namespace sample_math;
 
 constexpr int kThreads = 256;        // of a stats and a tests CTA
-constexpr int kListThreads = 512;    // of a residuals CTA
+constexpr int kListThreads = 256;    // of a residuals CTA
 constexpr int kSampleThreads = 256;  // of a sample CTA, 8 tokens a thread and chunk
 constexpr int kMaxList = 256;        // tokens of the first chunk that may reach its bound
 constexpr int kMaxParts = 32;        // CTAs that read a node's rows
-constexpr int kMaxCluster = 4;       // CTAs of a node on the list
+constexpr int kMaxCluster = 8;       // CTAs of a node on the list
 constexpr int kMaxNodes = 1024;      // of one tree (verify_max_nodes)
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -591,7 +597,7 @@ __global__ void __launch_bounds__(kThreads) verify_tests_kernel(const VerifyPara
 }
 
 // Clusters take the list's nodes in turn: all their children's tests.
-__global__ void __launch_bounds__(kListThreads, 1) verify_residuals_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kListThreads, 2) verify_residuals_kernel(const VerifyParams p) {
   __shared__ Exchange<kListThreads> s_x;
   __shared__ int s_child[kMaxNodes], s_token[kMaxNodes];
   __shared__ float s_lp[kMaxNodes], s_lq[kMaxNodes], s_u[kMaxNodes];  // children's logits and uniforms
@@ -1061,11 +1067,12 @@ cudaError_t launch_verify(cudaStream_t s, const void* logits, const void* draft,
   cfg.gridDim = dim3(unsigned((nodes + kThreads / 32 - 1) / (kThreads / 32)));
   e = cudaLaunchKernelEx(&cfg, verify_tests_kernel, p, batch);
   if (e != cudaSuccess) return e;
-  // Clusters for the list: CTAs of 4 thousand logits or more, one an SM (with eight loads in flight a thread 27 us for
-  // 90 nodes of 64 trees; two an SM with half of them 32 us), a few SMs left for the clusters' placing.
+  // Clusters for the list: CTAs of 4 thousand logits or more, two an SM, so that one's tests and joins run beside the
+  // other's passes (64 trees, the whole call 95 us; 512 threads with one CTA an SM and clusters of 4 98, of 8 101;
+  // two of 256 in clusters of 4 104, of 2 127), a few SMs left for the clusters' placing.
   int cluster = 1;
   while (cluster < kMaxCluster && vocab >= 2 * cluster * 4096) cluster *= 2;
-  long long clusters = 1LL * sms * 7 / 8 / cluster;
+  long long clusters = 2LL * sms * 7 / 8 / cluster;
   clusters = clusters < 1 ? 1 : (clusters > rows ? rows : clusters);
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = unsigned(cluster);

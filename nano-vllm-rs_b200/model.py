@@ -12,6 +12,7 @@ reference's nv_* entry points (kernels/kernels.cu:470-500) with a stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -369,7 +370,8 @@ def layer_verify(logits, draft_logits, tokens, parents, uniforms, seeds, tempera
     i32, f32, bf16 = torch.int32, torch.float32, torch.bfloat16
     ws = workspace
     if ws is None:
-        with torch.cuda.stream(stream):  # of that stream's memory: it is given on after this call returns
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+            # of that stream's memory: it is given on after this call returns
             ws = torch.empty(max(16, verify_workspace_bytes(rows, batch)), dtype=torch.uint8, device=logits.device)
     try:
         pointers = _pointers(
