@@ -15,7 +15,6 @@ from __future__ import annotations
 
 import bisect
 import ctypes
-import math
 import os
 from pathlib import Path
 
@@ -150,7 +149,7 @@ def _pointers(arguments, written, device):
     """Addresses of the arguments (name, tensor or None, shape, type): each of
     that shape and type, contiguous and on the device, and none that is in
     `written` overlapping another."""
-    pointers, spans, prod = [], [], math.prod
+    pointers, spans = [], []
     for name, t, shape, dtype in arguments:
         if t is None:
             pointers.append(None)
@@ -159,7 +158,7 @@ def _pointers(arguments, written, device):
             _refuse(t, shape, dtype, name, device)
         p = t.data_ptr()
         pointers.append(p)
-        spans.append((p, p + prod(shape) * dtype.itemsize, name))
+        spans.append((p, p + t.nbytes, name))
     spans.sort()
     end, held = 0, False
     for a, z, name in spans:
@@ -403,7 +402,7 @@ class CacheLayers:
         for (name, t, shape, dtype), p in zip(arguments, pointers):
             if p is None:
                 continue
-            i = bisect.bisect_right(self._starts, p + math.prod(shape) * dtype.itemsize - 1) - 1
+            i = bisect.bisect_right(self._starts, p + t.nbytes - 1) - 1
             if i >= 0 and p < self._starts[i] + self._bytes:
                 raise NvbError(f"{name} lies in a cache")
         return pointers
