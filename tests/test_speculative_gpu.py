@@ -660,6 +660,53 @@ def test_verify_captured_and_on_two_streams(nvb):
             same(case, o)
 
 
+def test_verify_the_longest_chain(nvb):
+    # 1,024 nodes whose drafts are all accepted: the draft's logits are the target's
+    case = Drafts([1024, 5], 300, 1, True, [1.0, 0.0], seed=56, noise=0.0)
+    o = case.run(nvb)
+    same(case, o)
+    assert o["counts"][0] == 1024 and o["path"][0].tolist() == list(range(1024))
+
+
+def test_verify_the_widest_tree(nvb):
+    # 1,023 children of one node, looked up: 290 tokens are rejected one after the other, and then again with nothing left
+    case = Drafts([1024], 300, 1, False, [1.0], seed=57)
+    case.parents[1:1024] = 0
+    case.tokens[1:1024] = np.arange(1023) % 290
+    case.uniforms[:] = 0.9999
+    o = case.run(nvb)
+    same(case, o)
+    assert o["counts"][0] == 1 and o["out_tokens"][0, 0] >= 290
+
+
+def test_verify_logits_past_32_bit_offsets(nvb):
+    # 14,200 rows of 151,936 logits: the last tree's start past 2^31 elements. It gets what it gets alone.
+    vocab, ones = 151936, 14200
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 10 GB for the logits")
+    case = Drafts([6], vocab, 2, True, [0.8], seed=58)
+    want, a = case.run(nvb), case.args()
+    rows = ones + 6
+    big = {}
+    for name in ("logits", "draft_logits"):
+        big[name] = torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda")
+        big[name][ones:] = a[name][:6]
+    for name in ("tokens", "parents", "uniforms", "seeds"):
+        big[name] = torch.cat([a[name].new_full((ones,), -1) if name == "parents" else a[name].new_zeros(ones), a[name][:6]])
+    big["temperatures"] = torch.cat([torch.zeros(ones, device="cuda"), a["temperatures"]])
+    big["cu_q"] = torch.cat([torch.arange(ones + 1, dtype=torch.int32, device="cuda"),
+                             torch.tensor([rows], dtype=torch.int32, device="cuda")])
+    i32 = dict(dtype=torch.int32, device="cuda")
+    o = dict(out_tokens=torch.zeros(ones + 1, 6, **i32), path=torch.zeros(ones + 1, 6, **i32),
+             counts=torch.zeros(ones + 1, **i32), accept_prob=torch.zeros(rows, device="cuda"))
+    nvb.model.layer_verify(**big, **o)
+    for name in ("out_tokens", "path", "counts"):
+        assert torch.equal(o[name][-1], want[name][0]), name
+    # the sums of a row are cut in other places: FP32 sums of 151,936 terms, in threads of a few hundred
+    assert (o["accept_prob"][-6:] - want["accept_prob"][:6]).abs().max() <= 1e-5
+    assert (o["counts"][:-1] == 1).all() and (o["out_tokens"][:-1, 0] == 0).all()
+
+
 @pytest.mark.parametrize("draft", [True, False])
 @pytest.mark.parametrize("temperature", [3e38, math.inf])
 def test_verify_at_endless_temperatures(nvb, draft, temperature):
