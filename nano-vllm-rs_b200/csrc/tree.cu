@@ -225,8 +225,27 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int s = 0; s < 2; ++s) mbar_init(&bars[kPFull + s], max(active, 1));
     fence_barrier_init();
   }
+  // Load `place` of the ring (K or V of 64 keys from key0 on); a bad page's slot stays as it is, its keys are masked.
+  auto load_tile = [&](int place, const CUtensorMap* map, int page, int logical, int key0) {
+    const int slot = place % kSlots;
+    if (!page_ok(page, p.num_blocks)) {
+      mbar_arrive(&bars[kFull + slot]);
+      return;
+    }
+    unsigned char* dst = smem_raw + kRingOff + slot * kTileBytes;
+    const int trow = page * p.block_size + (key0 - logical * p.block_size);
+    mbar_arrive_expect_tx(&bars[kFull + slot], kTileBytes);
+    tma_load_3d(dst, map, &bars[kFull + slot], 0, kvhead, trow);
+    tma_load_3d(dst + kHalf, map, &bars[kFull + slot], 64, kvhead, trow);
+  };
   int page0 = -1;
-  if (work && threadIdx.x == 0) page0 = table[fd_bs.div(t0 * kKeys)];
+  if (work && threadIdx.x == 0) {
+    // The first K tile is on its way while the rows load Q (0.5 us of a CTA's start: 32 sequences of 128 to 1024 keys
+    // 23.6 -> 22.7 us, 190 of 512 91 -> 87).
+    const int logical = fd_bs.div(t0 * kKeys);
+    page0 = table[logical];
+    load_tile(0, &kmap, page0, logical, t0 * kKeys);
+  }
   if (work && row_ok) {
     // this row of Q, K-major and 128-byte swizzled (rows past the last node stay as they are: their lanes' results
     // are dropped)
@@ -258,12 +277,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       tma_prefetch_desc(&kmap);
       tma_prefetch_desc(&vmap);
       const int final = fd_bs.div((t0 + ntiles - 1) * kKeys);
-      int issued = 0, page = page0, last = fd_bs.div(t0 * kKeys);
+      int issued = 1, page = page0, last = fd_bs.div(t0 * kKeys);
       int ahead = last < final ? table[last + 1] : -1;  // the next page, loaded a page ahead
       int behind = page;                                // the one before: K runs a tile ahead of V
-      for (int i = 0; i < 2 * ntiles; ++i) {
-        const bool is_v = i > 0 && ((i & 1) == 0 || i == 2 * ntiles - 1);
-        const int j = i == 0 ? 0 : (i == 2 * ntiles - 1 ? ntiles - 1 : (is_v ? i / 2 - 1 : (i + 1) / 2));
+      for (int i = 1; i < 2 * ntiles; ++i) {
+        const bool is_v = (i & 1) == 0 || i == 2 * ntiles - 1;
+        const int j = i == 2 * ntiles - 1 ? ntiles - 1 : (is_v ? i / 2 - 1 : (i + 1) / 2);
         const int key0 = (t0 + j) * kKeys, logical = fd_bs.div(key0), slot = i % kSlots;
         if (logical > last) {
           behind = page;
@@ -271,19 +290,9 @@ __global__ void __launch_bounds__(kThreads, 2)
           last = logical;
           ahead = logical < final ? table[logical + 1] : -1;
         }
-        const int mine = logical == last ? page : behind;
         // released by the MMA that read the slot's last load: S of a K tile, PV of a V tile
         if (i >= kSlots && !wait(&bars[kEmpty + slot], ((i / kSlots) + 1) & 1)) break;
-        if (page_ok(mine, p.num_blocks)) {
-          const CUtensorMap* map = is_v ? &vmap : &kmap;
-          unsigned char* dst = smem_raw + kRingOff + slot * kTileBytes;
-          const int trow = mine * p.block_size + (key0 - logical * p.block_size);
-          mbar_arrive_expect_tx(&bars[kFull + slot], kTileBytes);
-          tma_load_3d(dst, map, &bars[kFull + slot], 0, kvhead, trow);
-          tma_load_3d(dst + kHalf, map, &bars[kFull + slot], 64, kvhead, trow);
-        } else {
-          mbar_arrive(&bars[kFull + slot]);
-        }
+        load_tile(i, is_v ? &vmap : &kmap, logical == last ? page : behind, logical, key0);
         issued = i + 1;
       }
       // Every copy has landed before the CTA may exit (on the normal path its readers have waited for it).
