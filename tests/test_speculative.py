@@ -145,6 +145,17 @@ def test_tree_num_splits(nvb):
                 assert 1 <= nvb.tree_num_splits(batch, nodes, 32, 8, max_k, 148) <= 128
 
 
+def test_tree_num_splits_joins_on_chip_and_cuts_long_ranges(nvb):
+    for batch in (1, 2, 5, 16, 37, 64, 300):
+        for max_k in (64, 400, 2048, 8192, 32768, 131072):
+            splits = nvb.tree_num_splits(batch, 8, 32, 8, max_k, 148)
+            assert splits & (splits - 1) == 0 and (splits == 1 or max_k >= 128 * splits)
+            # past the CTAs that fit the GPU only for long ranges, and then only what one cluster joins
+            if splits > 1 and batch * 8 * splits > 296:
+                assert splits <= 8 and max_k >= 2560 * splits and batch * 8 * splits <= 8 * 148
+    assert nvb.tree_num_splits(64, 8, 32, 8, 4200, 148) == 1 and nvb.tree_num_splits(64, 8, 32, 8, 16384, 148) == 2
+
+
 def _layers(*values):
     return (P * len(values))(*values)
 
