@@ -108,15 +108,24 @@ def argmax(l):
 
 
 def verify(logits, draft, tokens, parents, uniforms, seeds, temps, cu, max_q, eps=3e-5):
-    """(out_tokens, path, counts, accept_prob, bound, margin): bound is how far
-    accept_prob may be off where every probability is eps off (relative), and
-    margin how near the nearest decision was to falling the other way (so that
-    the tests know that their inputs are not borderline)."""
+    """(out_tokens, path, counts, accept_prob, bound, margin, drawable): bound is
+    how far accept_prob may be off where every probability is eps off (relative),
+    and margin how near the nearest decision was to falling the other way (so that
+    the tests know that their inputs are not borderline).
+
+    drawable[b]: the next tokens that such probabilities may draw where something
+    was rejected. What is left of P, p = max(P - Q, 0) / sum, is off by e = eps
+    (P + Q) / sum and more with each level, so a token's score lies between
+    log(p - e) and log(p + e) plus its noise, and may be the highest where its
+    upper end reaches the best lower end. That is one token, unless P and Q agree
+    so far that their difference is below the rounding of either: where they put
+    all but 1e-28 on the same few tokens, 32-bit differences of those tokens are
+    rounding (1e-8), and outweigh what the others have left."""
     rows, vocab = logits.shape
     batch = len(temps)
     out, path = np.full((batch, max_q), -1), np.full((batch, max_q), -1)
     counts, prob, bound = np.zeros(batch, int), np.zeros(rows), np.zeros(rows)
-    margin = math.inf
+    margin, drawable = math.inf, [set() for _ in range(batch)]
     for b in range(batch):
         n, first = cu[b + 1] - cu[b], cu[b]
         if n <= 0:
@@ -168,7 +177,7 @@ def verify(logits, draft, tokens, parents, uniforms, seeds, temps, cu, max_q, ep
                 total = rest.sum()
                 if total > 0:
                     p, ep = rest / total, erest / total + rest * erest.sum() / total ** 2
-                left[node] = p
+                left[node] = p, ep
         at, seq = 0, [0]
         while winner[at] >= 0:
             at = winner[at]
@@ -181,10 +190,14 @@ def verify(logits, draft, tokens, parents, uniforms, seeds, temps, cu, max_q, ep
             out[b, len(seq) - 1] = argmax(logits[r])
             continue
         with np.errstate(divide="ignore"):
-            score = (np.log(left[at]) if left[at] is not None else
-                     np.where(np.isnan(logits[r]), -np.inf, logits[r]) / temps[b]) + gumbel(int(seeds[r]), vocab)
+            noise = gumbel(int(seeds[r]), vocab)
+            if left[at] is not None:
+                (p, ep), score = left[at], np.log(left[at][0]) + noise
+                drawable[b] = set(np.nonzero(np.log(p + ep) + noise >= (np.log(np.maximum(p - ep, 0)) + noise).max())[0])
+            else:
+                score = np.where(np.isnan(logits[r]), -np.inf, logits[r]) / temps[b] + noise
         out[b, len(seq) - 1] = int(np.argmax(score))
         top = np.sort(score)[-2:]
         if len(top) == 2 and np.isfinite(top).all():
             margin = min(margin, top[1] - top[0])
-    return out, path, counts, prob, bound, margin
+    return out, path, counts, prob, bound, margin, drawable
