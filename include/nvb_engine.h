@@ -288,14 +288,16 @@ int nvbe_layer_sample(void* stream, const void* logits, const float* temperature
  * becomes the current node. A rejected one leaves P = max(P - Q, 0) / sum
  * (unchanged where that sum is 0) and Q without t, renormalised, to its next
  * sibling (drafts of one node are drawn without replacement). Without
- * draft_logits Q is 1 at t. P, Q and their difference are 32-bit values: where
- * the two agree to the last bits, what is left of P is their rounding (drafts
- * drawn from Q are rejected there as rarely, 1e-7 of all tokens). Once a node's children are all rejected the next
+ * draft_logits Q is 1 at t. Once a node's children are all rejected the next
  * token is drawn from the P that is left, with the sampler's Gumbel stream
  * of the node's seed; where nothing was rejected it is the token that
  * nvbe_layer_sample draws. T = 0: a child is accepted where its token is the
  * argmax of logits (the lowest index of equal ones), which is the next token
  * otherwise. NaN logits have probability 0, tokens outside [0, vocab) too.
+ *
+ * P and Q are 32-bit values, below 2^-126 they are 0. Where the two agree to
+ * the last bits what is left of P is their rounding; drafts drawn from Q are
+ * rejected there as rarely as it is small (1e-7).
  *
  *   path [batch, max_q]: nodes of the accepted path, the root (0) first
  *   counts [batch]: nodes on the path = tokens emitted

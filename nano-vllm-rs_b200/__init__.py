@@ -364,8 +364,9 @@ def paged_tree_fwd(q, k, v, out, cu_q, kv_lens, block_table, tree_mask, *, batch
     else:
         pointers = [t.data_ptr() if t is not None else None
                     for t in (q, k, v, out, cu_q, kv_lens, block_table, tree_mask, lse, lse_accum, out_accum)]
-    _check(library().nvb_paged_tree_fwd(_raw_stream(stream, device), *pointers[:8], words, batch, total_q, max_q, max_k, q_heads,
-                                        kv_heads, block_size, table_stride, num_splits, *pointers[8:], num_blocks))
+    _check(library().nvb_paged_tree_fwd(_raw_stream(stream, device), *pointers[:8], words, batch, total_q, max_q,
+                                        max_k, q_heads, kv_heads, block_size, table_stride, num_splits, *pointers[8:],
+                                        num_blocks))
 
 
 class CacheLayers:
@@ -418,8 +419,8 @@ def cache_copy_pages(layers, src, dst, rows=None, *, stream=None):
     num_blocks, block_size, kv_heads, head_dim = layers.shape
     pairs, i32 = src.numel(), torch.int32
     pointers = layers._pointers((("src", src, (pairs,), i32), ("dst", dst, (pairs,), i32), ("rows", rows, (pairs,), i32)))
-    _check(library().nvb_cache_copy_pages(_raw_stream(stream, layers.device), layers._k, layers._v, layers.layers, *pointers, pairs,
-                                          kv_heads, head_dim, block_size, num_blocks))
+    _check(library().nvb_cache_copy_pages(_raw_stream(stream, layers.device), layers._k, layers._v, layers.layers,
+                                          *pointers, pairs, kv_heads, head_dim, block_size, num_blocks))
 
 
 def cache_compact_paths(layers, cu_q, kv_lens, block_table, path, counts, new_kv_lens, *, stream=None):
@@ -438,8 +439,9 @@ def cache_compact_paths(layers, cu_q, kv_lens, block_table, path, counts, new_kv
         (("cu_q", cu_q, (batch + 1,), i32), ("kv_lens", kv_lens, (batch,), i32),
          ("block_table", block_table, (batch, table_stride), i32), ("path", path, (batch, path_stride), i32),
          ("counts", counts, (batch,), i32), ("new_kv_lens", new_kv_lens, (batch,), i32)), ("new_kv_lens",))
-    _check(library().nvb_cache_compact_paths(_raw_stream(stream, layers.device), layers._k, layers._v, layers.layers, *pointers, batch,
-                                             path_stride, kv_heads, head_dim, block_size, table_stride, num_blocks))
+    _check(library().nvb_cache_compact_paths(_raw_stream(stream, layers.device), layers._k, layers._v, layers.layers,
+                                             *pointers, batch, path_stride, kv_heads, head_dim, block_size,
+                                             table_stride, num_blocks))
 
 
 def attention(q, kcache, vcache, positions, seq_indices, tables, out, *, rows, q_heads, kv_heads, head_dim,

@@ -385,4 +385,5 @@ def layer_verify(logits, draft_logits, tokens, parents, uniforms, seeds, tempera
             ("out_tokens", "path", "counts", "accept_prob", "workspace"), device)
     except NvbError as e:
         raise ValueError(str(e)) from None
-    _check(library().nvbe_layer_verify(_raw_stream(stream, device), *pointers[:12], rows, batch, max_q, vocab, pointers[12], ws.numel()))
+    _check(library().nvbe_layer_verify(_raw_stream(stream, device), *pointers[:12], rows, batch, max_q, vocab,
+                                       pointers[12], ws.numel()))
