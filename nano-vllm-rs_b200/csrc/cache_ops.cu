@@ -5,6 +5,11 @@
 //
 // Both move bytes only: the bound is HBM bandwidth (each row read once and
 // written once), or the latency of one load and one store for small calls.
+//
+// Measured (B200, 56 caches of 8 heads of 128, copy rate 6.57 TB/s): 16 whole
+// pages, 940 MB, 145 us (6.48 TB/s); the paths of 64 trees of 8 to 32 nodes, 117
+// MB, 22 us (5.3 TB/s: a CTA reads counts, path and table before it moves 16 KB);
+// one tree 2.7 us.
 #include "internal.cuh"
 
 namespace nvb {
@@ -51,7 +56,8 @@ constexpr int kMoveThreads = 128;
 // takes the moves in order, kUnroll at a time. That is enough for moves whose
 // source is another one's target: the path grows strictly, so path[d] >= d,
 // and a row that move d overwrites (ctx + d) is no later move's source
-// (path[d'] >= d' > d).
+// (path[d'] >= d' > d). Batches of 4, 12 and 16 rows take 22.8, 22.7 and 24.5 us
+// where 8 take 22.1; several caches a CTA, which share the path's reads, 24 to 55.
 template <class Vec>
 __global__ void __launch_bounds__(kMoveThreads)
     compact_paths_kernel(const __grid_constant__ LayerPtrs ptrs, const int* __restrict__ cu_q,
