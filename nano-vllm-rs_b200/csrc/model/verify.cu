@@ -68,12 +68,16 @@ constexpr int kMaxParts = 32;        // CTAs that read a node's rows
 constexpr int kMaxCluster = 8;       // CTAs of a node on the list
 constexpr int kMaxNodes = 1024;      // of one tree (verify_max_nodes)
 constexpr float kLog2e = 1.4426950408889634f;
+// A part's sum in its unit (verify_stats_kernel) stays below this. The join takes every part to the highest unit: a
+// part whose factor is flushed to 0 there (units more than 126 binary orders apart) then is less than 2^-66 of the
+// total, which is 1 at least and at most kMaxParts times this.
+constexpr float kMaxUnit = 0x1p60f;
 
 // What the first two kernels leave per row. For a node with children: its
 // statistics, accepted child and count of rejected children; for a child that
 // was rejected: the level that its rejection adds.
 struct VerifyRow {
-  float m_p, z_p, m_q;   // a logit near the highest, and the sum of exp((l - m) / T)
+  float m_p, z_p, m_q;   // a logit at most kMaxUnit below the highest, and the sum of exp((l - m) / T)
   float over_q, over_p;  // child: its level (Levels)
   int winner;            // node: accepted child's place in its sequence, or -1
   int rejected;          // node: children rejected; its complement where they are not regular (Levels)
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 6) verify_stats_kernel(const VerifyP
                    0, BestOp());
   } else {
     // Any finite logit near the maximum serves as the unit that sums are taken in: the highest of the part's first
-    // groups. Only where a sum does not stay finite with it are the maxima followed.
+    // groups. Where the sum shows it to be far below the maximum (or is not finite) the maxima are followed.
     const float c = inv_temperature(temperature);
     const float4 none = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
     float4 unit = none;
@@ -482,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 6) verify_stats_kernel(const VerifyP
                     [&](int, const uint4& vp, const uint4&) { z_p = add2(z_p, sum(vp, unit.x)); });
     all = exchange(make_float4(z_p.x + z_p.y, z_q.x + z_q.y, 0.f, 0.f), none, s_x, turn, 1, 0, SumOp());
     all = make_float4(unit.x, all.x, unit.z, all.y);
-    if (!(all.y < INFINITY) || !(all.w < INFINITY)) {
+    if (!(all.y < kMaxUnit) || !(all.w < kMaxUnit)) {
       Online op, oq;
       each_group<1>(lp, lq, g0, g1, kThreads, [&](int, const uint4& vp, const uint4& vq) {
         op.add(vp, c);

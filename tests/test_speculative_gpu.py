@@ -1017,3 +1017,90 @@ def test_the_models_caches_make_a_handle(nvb):
             assert (c[0, :100] == layer + 1).all() and (c[0, 100:] == 0).all() and (c[1] == 0).all()
     del handle
     model.close()
+
+
+# ------------------------------------------- sums of rows with far outliers
+def _padded(case, rows):
+    """Arguments and outputs of `rows` rows, those behind the case's own without a sequence. (From 237 rows on, at
+    148 SMs, a row of 151,936 tokens is read in 5 parts, below that in 32.)"""
+    a, o = case.args(), case.outputs()
+    more = rows - len(case.tokens)
+    if more > 0:
+        for name in ("logits", "draft_logits", "tokens", "parents", "uniforms", "seeds"):
+            if a[name] is not None:
+                a[name] = torch.cat([a[name], a[name].new_zeros(more, *a[name].shape[1:])])
+        o["accept_prob"] = torch.full((rows,), 7.0, device="cuda")
+    return a, o
+
+
+def _same_with_rows(nvb, case, rows):
+    ref = case.reference()
+    # these inputs leave one token that may be drawn, whatever the roundings
+    assert all(len(d) <= 1 for d in ref[-1])
+    a, o = _padded(case, rows)
+    nvb.model.layer_verify(**a, **o)
+    n = len(case.tokens)
+    assert (o["accept_prob"][n:] == 7.0).all()
+    same(case, {**o, "accept_prob": o["accept_prob"][:n]}, ref)
+
+
+@pytest.mark.parametrize("where", ["target", "draft"])
+@pytest.mark.parametrize("temperature", [0.1, 0.25])
+@pytest.mark.parametrize("rows", [0, 240])
+def test_verify_leaders_behind_the_first_tokens_of_a_part(nvb, rows, temperature, where):
+    # Two tokens share a row's probability, far above all others. T = 0.1: one among the first tokens of the row, the
+    # other behind the first 2,048 of a part that begins 87.5 temperatures lower. T = 0.25: both 88.5 temperatures above
+    # the first tokens of their parts, so that either part's sum in the unit of those is finite and the two together
+    # are not. The drafted token is the second of them.
+    vocab = 151936
+    part = 8 * -(-(vocab // 8) // (5 if rows else 32))
+    case = Drafts([2, 2, 2], vocab, 1, where == "draft", [temperature] * 3, seed=70)
+    if temperature == 0.1:
+        row = torch.randn(vocab, generator=torch.Generator().manual_seed(71)).clamp(-2, 2) * 4
+        row[100], row[part + 7], row[part + 3000] = 24.75, 16.0, 24.75
+        token = part + 3000
+    else:
+        row = torch.full((vocab,), -20.0)
+        row[::part] = 0.0
+        row[part + 3000] = row[2 * part + 4000] = 22.125
+        token = 2 * part + 4000
+    flat = torch.full((vocab,), -30.0)
+    flat[token], flat[5] = 0.0, 1.4 * temperature  # 0.2 and 0.8
+    for r in (0, 2, 4):
+        (case.logits if where == "target" else case.draft)[r] = row
+        if where == "draft":
+            case.logits[r] = flat
+        case.tokens[r + 1] = token
+    case.uniforms[[1, 3, 5]] = [0.1, 0.75, 0.55]
+    _, _, _, prob, _, _, _ = case.reference()
+    assert abs(prob[1] - (0.5 if where == "target" else 0.4)) < 0.01
+    _same_with_rows(nvb, case, rows)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("rows", [0, 240])
+@pytest.mark.parametrize("temperature", [0.04, 0.15])
+def test_verify_low_temperatures_of_long_rows(nvb, temperature, rows, draft):
+    case = Drafts([2] * 24, 151936, 1, draft, [temperature] * 24, seed=72)
+    # the drafts: the target's second highest, whose probability lies between 0 and 1/2
+    top = case.logits.float().topk(2, 1).indices.numpy()
+    case.tokens[1:48:2] = top[0:48:2, 1]
+    _same_with_rows(nvb, case, rows)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("rows", [0, 240])
+@pytest.mark.parametrize("low", [-70.0, -78.0, -85.0])
+def test_verify_parts_that_begin_far_below_the_rest(nvb, low, rows, draft):
+    vocab = 151936
+    part = 8 * -(-(vocab // 8) // (5 if rows else 32))
+    case = Drafts([2] * 12, vocab, 1, draft, [1.0] * 12, seed=73)
+    for r in range(0, 24, 2):
+        for x in (case.logits, case.draft) if draft else (case.logits,):
+            for i in range(r % 3, -(-vocab // part), 3):
+                x[r, i * part:i * part + 2048] = low
+    # the drafts: likely tokens of those parts
+    for r in range(0, 24, 2):
+        at = (r % 3) * part + 2048
+        case.tokens[r + 1] = at + int(case.logits[r, at:at + part - 2048].float().argmax())
+    _same_with_rows(nvb, case, rows)
