@@ -509,9 +509,11 @@ __device__ __forceinline__ bool unsafe_sums(const float4& s, bool has_q) {
   return !(s.y == s.y) || !(s.w == s.w) || s.x == INFINITY || s.z == INFINITY || s.x == -INFINITY ||
          (has_q && s.z == -INFINITY);
 }
-// a = min(1, P(t) / Q(t))
+// a = min(1, P(t) / Q(t)). Below 2^-126 a probability is 0: weights are flushed there in a unit that may lie below the
+// highest logit, so what is left of smaller ones goes by the unit.
 __device__ __forceinline__ float acceptance(float pt, float qt) {
-  return !(pt > 0.0f) ? 0.0f : (qt > 0.0f ? fminf(pt / qt, 1.0f) : 1.0f);
+  constexpr float kLeast = 0x1p-126f;
+  return !(pt >= kLeast) ? 0.0f : (qt >= kLeast ? fminf(pt / qt, 1.0f) : 1.0f);
 }
 
 // A warp a node: the test of its first child, and at T = 0 of all.
