@@ -135,7 +135,10 @@ int nvbh_pool_fork(NvbhBlockPool* pool, const int32_t* blocks, size_t num_blocks
 /* Releases the pages that a sequence cut to `tokens` tokens does not need any
  * more (drafts that were rejected), the last first; *num_blocks becomes the
  * number it keeps and the released entries of blocks -1. A kept last page that
- * another sequence references must be copied before tokens are written to it. */
+ * is cut and published under more than `tokens` tokens leaves the prefix cache,
+ * as what is behind the cut will be overwritten; unless another sequence
+ * references it at that time: then it stays, and must be copied before tokens
+ * are written to it. */
 int nvbh_pool_truncate(NvbhBlockPool* pool, int32_t* blocks, size_t* num_blocks, size_t tokens,
                        size_t block_size);
 

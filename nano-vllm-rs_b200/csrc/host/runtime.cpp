@@ -359,6 +359,11 @@ int nvbh_pool_truncate(NvbhBlockPool* p, int32_t* blocks, size_t* num_blocks, si
     nvbh_pool_release(p, blocks[i - 1]);
     blocks[i - 1] = -1;
   }
+  if (tokens % block_size) {
+    // A page cut in its middle will hold other tokens than its prefix says.
+    const auto& last = p->blocks[size_t(blocks[need - 1])];
+    if (last.references == 1 && last.has_prefix && last.tokens.size() > tokens) p->invalidate(blocks[need - 1]);
+  }
   *num_blocks = need;
   return 0;
 }

@@ -110,6 +110,48 @@ def test_truncate_refuses_and_keeps(host):
     assert [pool.references(x) for x in blocks] == [2, 1]  # a shared page loses one user
 
 
+def test_truncate_into_a_published_page_takes_it_out_of_the_cache(host):
+    # the sequence writes over what is behind its 300 tokens: nobody may find the page under its 512 any more
+    pool, tokens = host.BlockPool(4), list(range(600))
+    blocks = [pool.allocate(), pool.allocate()]
+    for i in range(2):
+        pool.publish(blocks[i], tokens[:256 * (i + 1)])
+    assert pool.truncate(blocks, 300, 256) == blocks
+    assert pool.find(tokens[:512]) == -1 and pool.find(tokens[:256]) == blocks[0] and pool.cached_keys() == 1
+    other = tokens[:300] + [7] * 212
+    pool.publish(blocks[1], other)  # filled anew
+    assert pool.find(other) == blocks[1] and pool.find(tokens[:512]) == -1
+
+
+@pytest.mark.parametrize("tokens", [0, 256, 512])
+def test_truncate_at_a_pages_end_keeps_the_cache(host, tokens):
+    pool, text = host.BlockPool(4), list(range(512))
+    blocks = [pool.allocate(), pool.allocate()]
+    for i in range(2):
+        pool.publish(blocks[i], text[:256 * (i + 1)])
+    pool.truncate(blocks, tokens, 256)
+    assert [pool.find(text[:256]), pool.find(text)] == blocks  # whole, and free or in use
+
+
+def test_truncate_into_a_page_that_another_sequence_holds_keeps_it_for_that_one(host):
+    pool, text = host.BlockPool(4), list(range(512))
+    blocks = [pool.allocate(), pool.allocate()]
+    for i in range(2):
+        pool.publish(blocks[i], text[:256 * (i + 1)])
+    child, _ = pool.fork(blocks, 512, 256)
+    assert pool.truncate(child, 300, 256) == blocks and pool.references(blocks[1]) == 2
+    assert pool.find(text) == blocks[1]  # the child copies it before it writes
+    assert pool.truncate(blocks, 256, 256) == blocks[:1] and pool.find(text) == blocks[1]
+
+
+def test_truncate_keeps_a_page_published_for_no_more_than_is_kept(host):
+    pool, text = host.BlockPool(4), list(range(300))
+    blocks = [pool.allocate(), pool.allocate()]
+    pool.publish(blocks[1], text)
+    pool.truncate(blocks, 300, 256)
+    assert pool.find(text) == blocks[1]
+
+
 # -------------------------------------------------- argument checks of the ABI
 def _tree(lib, **kw):
     a = dict(q=NZ, mask=NZ, words=1, batch=1, total_q=2, max_q=2, max_k=300, qh=4, kvh=2, bs=256, stride=2, splits=1,
