@@ -117,10 +117,10 @@ def test_truncate_into_a_published_page_takes_it_out_of_the_cache(host):
     for i in range(2):
         pool.publish(blocks[i], tokens[:256 * (i + 1)])
     assert pool.truncate(blocks, 300, 256) == blocks
-    assert pool.find(tokens[:512]) == -1 and pool.find(tokens[:256]) == blocks[0] and pool.cached_keys() == 1
+    assert pool.find(tokens[:512]) is None and pool.find(tokens[:256]) == blocks[0] and pool.cached_keys() == 1
     other = tokens[:300] + [7] * 212
     pool.publish(blocks[1], other)  # filled anew
-    assert pool.find(other) == blocks[1] and pool.find(tokens[:512]) == -1
+    assert pool.find(other) == blocks[1] and pool.find(tokens[:512]) is None
 
 
 @pytest.mark.parametrize("tokens", [0, 256, 512])
