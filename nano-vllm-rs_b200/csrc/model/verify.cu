@@ -758,10 +758,10 @@ __global__ void __launch_bounds__(kListThreads, 2) verify_residuals_kernel(const
 }
 
 // ---------------------------------------------------------------- next token
-// Scores as an integer that orders like them, then the lowest token first.
+// Scores as an integer that orders like them (-0 as 0), then the lowest token first.
 __device__ __forceinline__ unsigned long long sort_key(float score, int token) {
   if (!(score == score)) return 0ull;  // NaN is never it
-  const uint32_t u = __float_as_uint(score), o = u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(__fadd_rn(score, 0.0f)), o = u & 0x80000000u ? ~u : u | 0x80000000u;
   return (static_cast<unsigned long long>(o) << 32) | (0xffffffffu - uint32_t(token));
 }
 __device__ __forceinline__ float key_score(unsigned long long key) {

@@ -1113,3 +1113,24 @@ def test_verify_parts_that_begin_far_below_the_rest(nvb, low, rows, draft):
         at = (r % 3) * part + 2048
         case.tokens[r + 1] = at + int(case.logits[r, at:at + part - 2048].float().argmax())
     _same_with_rows(nvb, case, rows)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("value", [0.0, -0.0])
+def test_verify_zeros_of_either_sign_are_equal_logits(nvb, draft, value):
+    # T = 0, the highest logits are zeros: the lowest index among them, whatever their signs, as the sampler takes it;
+    # for the test of a draft and for the next token, of nodes with and without children
+    vocab = 20011
+    case = Drafts([1, 2, 2, 3], vocab, 1, draft, [0.0] * 4, seed=75)
+    rows, at = len(case.tokens), [17, 9000, 9001, 20010]
+    case.logits[:] = -1.5
+    for r in range(rows):
+        case.logits[r, at[r % 3:]] = torch.tensor([value, -value, 0.0, -0.0][:len(at) - r % 3]).to(torch.bfloat16)
+    case.parents[:8] = [-1, -1, 0, -1, 0, -1, 0, 1]
+    case.tokens[:8] = [0, 0, at[1], 0, at[1], 0, at[2], at[1]]
+    o = case.run(nvb)
+    same(case, o)
+    assert o["counts"].tolist() == [1, 2, 1, 2]
+    want, seeds = torch.empty(rows, dtype=torch.int32, device="cuda"), torch.from_numpy(case.seeds).cuda()
+    nvb.model.layer_sample(case.logits.cuda(), torch.zeros(rows, device="cuda"), seeds, want)
+    assert [want[i].item() for i in (0, 2, 3, 6)] == [o["out_tokens"][b, c - 1].item() for b, c in enumerate([1, 2, 1, 2])]
