@@ -373,10 +373,13 @@ int nvbh_tree_mask(const int32_t* parents, const int32_t* cu_q, size_t sequences
   g_error[0] = 0;
   if (!cu_q || words == 0 || (sequences && (!parents || !mask))) return fail("invalid tree mask arguments");
   if (cu_q[0] != 0) return fail("cu_q must start at 0");
+  // all offsets first: with one that falls, those before it may lie behind the last, where the arrays end
   for (size_t s = 0; s < sequences; ++s) {
     if (cu_q[s + 1] < cu_q[s]) return fail("cu_q must not decrease");
+    if (size_t(cu_q[s + 1] - cu_q[s]) > 64 * words) return fail("a tree has more nodes than its mask has bits");
+  }
+  for (size_t s = 0; s < sequences; ++s) {
     const size_t begin = size_t(cu_q[s]), n = size_t(cu_q[s + 1]) - begin;
-    if (n > 64 * words) return fail("a tree has more nodes than its mask has bits");
     for (size_t i = 0; i < n; ++i) {
       const int32_t parent = parents[begin + i];
       if (parent < -1 || parent >= (long long)i || (i == 0 && parent != -1))

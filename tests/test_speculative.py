@@ -47,6 +47,18 @@ def test_tree_mask_refuses_more_rows_than_parents(host):
         host.tree_mask([-1], [0, 2])
 
 
+@pytest.mark.parametrize("cu", [[0, 10, 5], [0, 3, 12, 2, 5], [0, 5, 100, 5], [0, 6, -1, 5]])
+def test_tree_mask_refuses_falling_offsets_before_it_writes(host, cu):
+    # the rows that such offsets reach in between lie behind the arrays, which end at the last offset's
+    with pytest.raises(host.HostError):
+        host.tree_mask([-1] * 5, cu)
+    parents, offsets = np.full(128, -1, np.int32), np.array(cu, np.int32)
+    mask, depth = np.full((128, 2), 77, np.uint64), np.full(128, 77, np.int32)
+    ptr = lambda x: x.ctypes.data_as(P)  # noqa: E731
+    assert host.library().nvbh_tree_mask(ptr(parents), ptr(offsets), len(cu) - 1, 2, ptr(mask), ptr(depth)) == -1
+    assert (mask == 77).all() and (depth == 77).all()
+
+
 # ------------------------------------------------------------ forked page lists
 @pytest.mark.parametrize("tokens", [0, 1, 255, 256, 257, 512, 700])
 def test_fork_shares_full_pages_and_copies_the_partial_one(host, tokens):
