@@ -174,7 +174,7 @@ int nvb_peer_buffer_free(void* ptr);
  *
  *  - max_q bounds every sequence's nodes (at most 64 * mask_words, mask_words
  *    in [1, 16]), max_k its kv_lens. Sequences without nodes, and rows of q
- *    and out at and behind cu_q[batch], are left alone.
+ *    and out before cu_q[0] and from cu_q[batch] on, are left alone.
  *  - lse (may be null) is [total_q, q_heads]. A node that sees no key has
  *    output 0 and lse -inf; so has a sequence with kv_lens < n or longer than
  *    its table.

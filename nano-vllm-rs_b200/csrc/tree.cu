@@ -637,8 +637,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const 
   const long long item = (long long)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
   const long long stride = (long long)p.total_q * p.qh;
   if (item >= stride) return;
-  // rows behind the last sequence have no partials and keep what they hold
-  const bool live = item < (long long)p.cu_q[p.batch] * p.qh;
+  // rows before the first sequence and behind the last have no partials and keep what they hold
+  const bool live = item >= (long long)p.cu_q[0] * p.qh && item < (long long)p.cu_q[p.batch] * p.qh;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float total = 0.0f, mx = -INFINITY;
   for (int s0 = 0; s0 < parts; s0 += kCombineBatch) {

@@ -412,6 +412,18 @@ def test_tree_attention_parts_captured_and_at_the_same_time(nvb):
             assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("splits", [1, 2, 11])
+def test_tree_attention_leaves_rows_before_the_first_sequence(nvb, splits):
+    # a call on a slice of a larger batch: its first sequence starts behind others' rows, which are not its own
+    case = Case([4, 9, 2], [300, 700, 40], 8, 2, seed=45, spare_rows=3)
+    want, want_lse = case.run(nvb, splits)
+    a = case.args()
+    part = {**a, "cu_q": a["cu_q"][1:], "kv_lens": a["kv_lens"][1:], "block_table": a["block_table"][1:].contiguous()}
+    out, lse = case.run(nvb, splits, args=part, batch=2)
+    assert (out[:4] == 7.0).all() and (lse[:4] == 7.0).all() and (out[15:] == 7.0).all() and (lse[15:] == 7.0).all()
+    assert torch.equal(out[4:15], want[4:15]) and torch.equal(lse[4:15], want_lse[4:15])
+
+
 def test_tree_attention_in_a_cache_past_32_bit_offsets(nvb):
     # 8,704 pages of 256 x 8 x 128 elements: the last ones start past 2^31
     blocks = 8704
