@@ -179,8 +179,8 @@ int nvb_peer_buffer_free(void* ptr);
  *    output 0 and lse -inf; so has a sequence with kv_lens < n or longer than
  *    its table.
  *  - num_splits cuts every sequence's keys into that many ranges. Where
- *    nvb_tree_parts(num_splits) > 1 they need lse_accum [num_splits, total_q,
- *    q_heads] and out_accum [num_splits, total_q, q_heads, 128] (FP32); calls
+ *    parts = nvb_tree_parts(num_splits) > 1 they need lse_accum [parts, total_q,
+ *    q_heads] and out_accum [parts, total_q, q_heads, 128] (FP32); calls
  *    that may overlap need their own. nvb_tree_num_splits gives the count for
  *    a GPU of num_sms SMs.
  *  - a key that a node does not see has no part in its result, whatever

@@ -329,10 +329,12 @@ def tree_num_splits(batch, max_q, q_heads, kv_heads, max_k, num_sms=None):
 
 
 def tree_scratch(num_splits_, total_q, q_heads, device):
-    """Caller-owned FP32 scratch (lse_accum, out_accum) of paged_tree_fwd; (None, None) where it needs none."""
-    if library().nvb_tree_parts(num_splits_) == 1:
+    """Caller-owned FP32 scratch (lse_accum, out_accum) of paged_tree_fwd: one row of each for each of the
+    nvb_tree_parts(num_splits) parts; (None, None) where it needs none."""
+    parts = library().nvb_tree_parts(num_splits_)
+    if parts == 1:
         return None, None
-    return splitkv_scratch(num_splits_, total_q, q_heads, device)
+    return splitkv_scratch(parts, total_q, q_heads, device)
 
 
 def paged_tree_fwd(q, k, v, out, cu_q, kv_lens, block_table, tree_mask, *, batch, max_q, max_k, q_heads, kv_heads,
@@ -345,7 +347,7 @@ def paged_tree_fwd(q, k, v, out, cu_q, kv_lens, block_table, tree_mask, *, batch
     int64 has bit t % 64 of word t // 64 set where a node attends to node t
     (host.tree_mask). The keys before the tree are visible to all. lse, where
     given, is [total_q, q_heads]. lse_accum and out_accum: tree_scratch of
-    num_splits.
+    num_splits (or more parts).
     """
     import torch
 
@@ -353,13 +355,17 @@ def paged_tree_fwd(q, k, v, out, cu_q, kv_lens, block_table, tree_mask, *, batch
     if check:
         bf16, i32, f32 = torch.bfloat16, torch.int32, torch.float32
         rows, cache = (total_q, q_heads, 128), (num_blocks, block_size, kv_heads, 128)
+        lse_parts = out_parts = 1
+        if lse_accum is not None or out_accum is not None:
+            parts = library().nvb_tree_parts(num_splits)
+            lse_parts, out_parts = (parts if t is None else max((parts, *t.shape[:1])) for t in (lse_accum, out_accum))
         pointers = _pointers(
             (("q", q, rows, bf16), ("k", k, cache, bf16), ("v", v, cache, bf16), ("out", out, rows, bf16),
              ("cu_q", cu_q, (batch + 1,), i32), ("kv_lens", kv_lens, (batch,), i32),
              ("block_table", block_table, (batch, table_stride), i32),
              ("tree_mask", tree_mask, (total_q, words), torch.int64), ("lse", lse, (total_q, q_heads), f32),
-             ("lse_accum", lse_accum, (num_splits, total_q, q_heads), f32),
-             ("out_accum", out_accum, (num_splits, total_q, q_heads, 128), f32)),
+             ("lse_accum", lse_accum, (lse_parts, total_q, q_heads), f32),
+             ("out_accum", out_accum, (out_parts, total_q, q_heads, 128), f32)),
             ("out", "lse", "lse_accum", "out_accum"), device)
     else:
         pointers = [t.data_ptr() if t is not None else None

@@ -129,8 +129,8 @@ struct TreeParams {
   const int* block_table;    // [batch, table_stride]
   const unsigned long long* mask;  // [total_q, mask_words]
   float* lse;                // [total_q, qh] or null
-  float* lse_accum;          // [splits, total_q, qh]      (splits > 1)
-  float* out_accum;          // [splits, total_q, qh, 128] (splits > 1)
+  float* lse_accum;          // [parts, total_q, qh]       (parts > 1, nvb_tree_parts)
+  float* out_accum;          // [parts, total_q, qh, 128]  (parts > 1)
   int batch, total_q, max_q, qh, kvh, block_size, table_stride, num_blocks, num_splits, mask_words;
   float scale_log2;
   bool by_length;            // set by launch_tree: sequences in falling order of kv_lens

@@ -199,6 +199,16 @@ def test_tree_num_splits(nvb):
                 assert 1 <= nvb.tree_num_splits(batch, nodes, 32, 8, max_k, 148) <= 128
 
 
+@pytest.mark.parametrize("splits", [1, 2, 8, 9, 11, 24, 64, 97, 128])
+def test_tree_scratch_has_a_row_for_each_part(nvb, splits):
+    parts = nvb.library().nvb_tree_parts(splits)
+    lse, out = nvb.tree_scratch(splits, 5, 4, "cpu")
+    if parts == 1:
+        assert lse is None and out is None
+    else:
+        assert lse.shape == (parts, 5, 4) and out.shape == (parts, 5, 4, 128)
+
+
 def test_tree_num_splits_joins_on_chip_and_cuts_long_ranges(nvb):
     for batch in (1, 2, 5, 16, 37, 64, 300):
         for max_k in (64, 400, 2048, 8192, 32768, 131072):

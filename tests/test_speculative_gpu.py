@@ -308,6 +308,28 @@ def test_tree_attention_splits_that_leave_parts(nvb, splits):
     check(nvb, Case([9, 3, 40, 1], [1500, 0, 1000, 127], 8, 2, seed=splits), splits)
 
 
+@pytest.mark.parametrize("splits", [1, 2, 11, 24, 128])
+def test_tree_attention_scratch_of_its_parts_or_more(nvb, splits):
+    # what lies behind the parts' rows is not written, fewer rows are refused, and a row for each split is enough
+    case, parts = Case([9, 3], [1500, 40], 8, 2, seed=46), nvb.library().nvb_tree_parts(splits)
+    want, want_lse = case.run(nvb, splits)
+    a, f32 = case.args(), dict(dtype=torch.float32, device="cuda")
+    for rows in {splits, parts + 1}:
+        la, oa = torch.full((rows, case.rows, 8), 3.0, **f32), torch.full((rows, case.rows, 8, 128), 3.0, **f32)
+        out, lse = torch.full_like(want, 7.0), torch.full_like(want_lse, 7.0)
+        nvb.paged_tree_fwd(**a, out=out, lse=lse, num_splits=splits, lse_accum=la, out_accum=oa, **case.shape())
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        used = parts if parts > 1 else 0
+        assert (la[used:] == 3.0).all() and (oa[used:] == 3.0).all()
+    if parts > 1:
+        la, oa = nvb.tree_scratch(splits, case.rows, 8, "cuda")
+        for bad in (dict(lse_accum=la[1:], out_accum=oa), dict(lse_accum=la, out_accum=oa[1:]),
+                    dict(lse_accum=la, out_accum=None), dict(lse_accum=None, out_accum=oa),
+                    dict(lse_accum=la, out_accum=oa[:, 1:]), dict(lse_accum=la[0, 0, 0], out_accum=oa)):
+            with pytest.raises(nvb.NvbError):
+                nvb.paged_tree_fwd(**a, out=out, lse=lse, num_splits=splits, **bad, **case.shape())
+
+
 @pytest.mark.parametrize("splits", [1, 2])
 def test_tree_attention_the_largest_tree(nvb, splits):
     # 1,024 nodes of 16 words: 16 row tiles of 128 rows a head group
