@@ -552,19 +552,33 @@ class Graph:
             pass
 
 
+_captures = []  # what each capture that is under way keeps
+
+
+def _hold(*tensors):
+    """Keeps the memory that a call allocated for itself for the graph that is being captured."""
+    if _captures:
+        _captures[-1].extend(tensors)
+
+
 def capture(fn, keep=(), stream=None):
-    """Captures the device work `fn()` enqueues on `stream` into a Graph."""
+    """Captures the device work `fn()` enqueues on `stream` into a Graph, which
+    keeps `keep` and the workspaces that the calls in `fn` allocate."""
     s = _stream(stream)
     lib = library()
     _check(lib.nvb_capture_begin(s))
+    kept = list(keep)
+    _captures.append(kept)
     try:
         fn()
     except BaseException:
         lib.nvb_capture_abort(s)
         raise
+    finally:
+        _captures[:] = [c for c in _captures if c is not kept]
     handle = ctypes.c_void_p(0)
     _check(lib.nvb_capture_end(s, ctypes.byref(handle)))
-    return Graph(handle, list(keep))
+    return Graph(handle, kept)
 
 
 def version():

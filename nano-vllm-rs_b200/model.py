@@ -303,6 +303,8 @@ def layer_gemm(x, w, y, silu=False, stream=None, workspace=None):
     not given."""
     import torch
 
+    from . import _hold
+
     M, K = x.shape
     N = w.shape[0]
     if w.shape[1] != K or x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16 or y.dtype != torch.bfloat16:
@@ -310,7 +312,10 @@ def layer_gemm(x, w, y, silu=False, stream=None, workspace=None):
     if tuple(y.shape) != (M, N // 2 if silu else N) or not (x.is_contiguous() and w.is_contiguous() and y.is_contiguous()):
         raise ValueError("y must be a contiguous [M, N] (or [M, N / 2] with silu) tensor")
     nbytes = library().nvbe_gemm_workspace_bytes(M, N, K, int(silu))
-    ws = workspace if workspace is not None else torch.empty(max(16, nbytes), dtype=torch.uint8, device=x.device)
+    ws = workspace
+    if ws is None:
+        ws = torch.empty(max(16, nbytes), dtype=torch.uint8, device=x.device)
+        _hold(ws)
     _check(library().nvbe_layer_gemm(_s(stream), _p(x), _p(w), _p(y), M, N, K, int(silu), _p(ws), ws.numel()))
 
 
@@ -320,6 +325,8 @@ def layer_gemm_sample(x, w, logits, temperatures, seeds, out, stream=None):
     plus the per-tile fold."""
     import torch
 
+    from . import _hold
+
     M, K = x.shape
     N = w.shape[0]
     if tuple(logits.shape) != (M, N) or logits.dtype != torch.bfloat16 or out.shape[0] != M:
@@ -327,6 +334,7 @@ def layer_gemm_sample(x, w, logits, temperatures, seeds, out, stream=None):
     tiles = library().nvbe_gemm_sample_tiles(N)
     ps = torch.empty(M * tiles, dtype=torch.float32, device=x.device)
     pi = torch.empty(M * tiles, dtype=torch.int32, device=x.device)
+    _hold(ps, pi)
     _check(library().nvbe_layer_gemm_sample(_s(stream), _p(x), _p(w), _p(logits), M, N, K, _p(temperatures),
                                             _p(seeds), _p(out), _p(ps), _p(pi)))
 
@@ -338,10 +346,13 @@ def gemm_device_error():
 def layer_sample(logits, temperatures, seeds, out, stream=None):
     import torch
 
+    from . import _hold
+
     rows, vocab = logits.shape
     parts = library().nvbe_sample_partitions(vocab)
     ps = torch.empty(rows * parts, dtype=torch.float32, device=logits.device)
     pi = torch.empty(rows * parts, dtype=torch.int32, device=logits.device)
+    _hold(ps, pi)
     _check(library().nvbe_layer_sample(_s(stream), _p(logits), _p(temperatures), _p(seeds), _p(out), _p(ps), _p(pi),
                                        rows, vocab))
 
@@ -359,10 +370,10 @@ def layer_verify(logits, draft_logits, tokens, parents, uniforms, seeds, tempera
     out_tokens and path are [batch, max_q] int32, counts [batch] int32 and
     accept_prob [rows] FP32; seeds are int64 (or uint64) words. `workspace` (a
     CUDA uint8 tensor of verify_workspace_bytes(rows, batch)) is allocated per call
-    when not given."""
+    when not given (a call that is being captured leaves it to the graph)."""
     import torch
 
-    from . import NvbError, _pointers, _raw_stream
+    from . import NvbError, _hold, _pointers, _raw_stream
 
     if logits.dim() != 2 or out_tokens.dim() != 2:
         raise ValueError("logits must be [rows, vocab] and out_tokens [batch, max_q]")
@@ -373,6 +384,7 @@ def layer_verify(logits, draft_logits, tokens, parents, uniforms, seeds, tempera
         with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
             # of that stream's memory: it is given on after this call returns
             ws = torch.empty(max(16, verify_workspace_bytes(rows, batch)), dtype=torch.uint8, device=logits.device)
+        _hold(ws)
     try:
         pointers = _pointers(
             (("logits", logits, (rows, vocab), bf16), ("draft_logits", draft_logits, (rows, vocab), bf16),

@@ -282,3 +282,28 @@ def test_verify_workspace_grows_with_the_rows(nvb):
 def test_engine_header_functions_are_exported(nvb):
     lib = nvb.model.library()
     assert lib.nvbe_layer_verify and lib.nvbe_verify_workspace_bytes
+
+
+# ------------------------------------------------- memory that a graph holds on to
+def test_a_graph_keeps_the_workspaces_of_its_calls(nvb, monkeypatch):
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: 0
+
+    monkeypatch.setattr(nvb, "library", lambda: Library())
+    monkeypatch.setattr(nvb, "_stream", lambda stream=None: P(0))
+    given, first, second, failed = object(), object(), object(), object()
+    nvb._hold(failed)  # no capture is under way: the call's own memory goes back
+
+    def broken():
+        nvb._hold(failed)
+        raise ValueError
+
+    def outer():
+        nvb._hold(first)
+        with pytest.raises(ValueError):
+            nvb.capture(broken)
+        nvb._hold(second)
+
+    graph = nvb.capture(outer, keep=[given])
+    assert graph._keep == [given, first, second] and nvb._captures == []

@@ -715,6 +715,42 @@ def test_verify_captured_and_on_two_streams(nvb):
             same(case, o)
 
 
+@pytest.mark.parametrize("what", ["verify", "sample"])
+def test_a_captured_call_without_a_workspace_keeps_its_own(nvb, what):
+    # what a replay writes is not memory that was given on since
+    case, stream = Drafts([6, 9, 2], 40000, 2, True, seed=74), torch.cuda.Stream()
+    a, o, out = case.args(), case.outputs(), torch.zeros(19, dtype=torch.int32, device="cuda")
+    t = a["temperatures"].repeat_interleave(torch.tensor([6, 9, 4], device="cuda"))
+    torch.cuda.synchronize()
+
+    def call(out=out, o=o):
+        if what == "verify":
+            nvb.model.layer_verify(**a, **o, stream=stream)
+        else:
+            nvb.model.layer_sample(a["logits"], t, a["seeds"], out, stream=stream)
+
+    with torch.cuda.stream(stream):
+        want, want_out = case.outputs(), torch.zeros_like(out)
+        call(want_out, want)  # leaves memory that the capture takes without asking the device for more
+        stream.synchronize()
+        graph = nvb.capture(call, keep=[a, o, out, t], stream=stream)
+        held = [x for x in graph._keep if isinstance(x, torch.Tensor) and x is not out and x is not t]
+        spans = [(x.data_ptr(), x.data_ptr() + x.nbytes) for x in held]
+        assert spans
+        size = max(x.nbytes for x in held)
+        later = [torch.full((size,), 0x5a, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        for x in later:
+            assert all(x.data_ptr() >= z or x.data_ptr() + size <= y for y, z in spans)
+    for _ in range(2):
+        for x in o.values():
+            x.fill_(7)
+        torch.cuda.synchronize()
+        graph.replay(stream)
+        torch.cuda.synchronize()
+        assert all((x == 0x5a).all() for x in later)
+        assert torch.equal(out, want_out) and (what == "sample" or all(torch.equal(o[n], want[n]) for n in o))
+
+
 def test_verify_the_longest_chain(nvb):
     # 1,024 nodes whose drafts are all accepted: the draft's logits are the target's
     case = Drafts([1024, 5], 300, 1, True, [1.0, 0.0], seed=56, noise=0.0)
