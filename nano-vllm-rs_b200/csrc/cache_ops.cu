@@ -185,6 +185,9 @@ int nvb_cache_copy_pages(void* stream, void* const* k_layers, void* const* v_lay
   if (pairs < 0 || pairs > num_blocks) return fail("pairs must be in [0, num_blocks]");
   if (pairs == 0) return 0;
   if (!src_pages || !dst_pages) return fail("src_pages and dst_pages are required");
+  if ((reinterpret_cast<uintptr_t>(src_pages) | reinterpret_cast<uintptr_t>(dst_pages) |
+       reinterpret_cast<uintptr_t>(rows)) & 3)
+    return fail("src_pages, dst_pages and rows must be 4-byte aligned");
   for (int l = 0; l < layers; l += kCacheLayers) {
     const int n = layers - l < kCacheLayers ? layers - l : kCacheLayers;
     if (int rc = cuda_status(launch_copy_pages(static_cast<cudaStream_t>(stream), k_layers + l, v_layers + l, n,
@@ -207,6 +210,10 @@ int nvb_cache_compact_paths(void* stream, void* const* k_layers, void* const* v_
       path_stride < 1 || table_stride < 1)
     return fail("invalid path compaction arguments");
   if (new_kv_lens == kv_lens) return fail("new_kv_lens must not be kv_lens");
+  if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(kv_lens) |
+       reinterpret_cast<uintptr_t>(block_table) | reinterpret_cast<uintptr_t>(path) |
+       reinterpret_cast<uintptr_t>(counts) | reinterpret_cast<uintptr_t>(new_kv_lens)) & 3)
+    return fail("cu_q, kv_lens, block_table, path, counts and new_kv_lens must be 4-byte aligned");
   for (int l = 0; l < layers; l += kCacheLayers) {
     const int n = layers - l < kCacheLayers ? layers - l : kCacheLayers;
     if (int rc = cuda_status(launch_compact_paths(static_cast<cudaStream_t>(stream), k_layers + l, v_layers + l, n,

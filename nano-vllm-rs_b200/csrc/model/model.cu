@@ -628,6 +628,16 @@ int nvbe_layer_verify(void* stream, const void* logits, const void* draft_logits
     return mfail("invalid verify arguments");
   if (max_q > nvbm::verify_max_nodes())
     return mfail("a tree has at most %d nodes (max_q %d)", nvbm::verify_max_nodes(), max_q);
+  const uintptr_t halves = reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(draft_logits);
+  uintptr_t words = 0;
+  for (const void* p : {static_cast<const void*>(tokens), static_cast<const void*>(parents),
+                        static_cast<const void*>(uniforms), static_cast<const void*>(temperatures),
+                        static_cast<const void*>(cu_q), static_cast<const void*>(out_tokens),
+                        static_cast<const void*>(path), static_cast<const void*>(counts),
+                        static_cast<const void*>(accept_prob)})
+    words |= reinterpret_cast<uintptr_t>(p);
+  if ((halves & 1) || (words & 3) || (reinterpret_cast<uintptr_t>(seeds) & 7))
+    return mfail("verify needs logits 2-byte, seeds 8-byte and the other arrays 4-byte aligned");
   const size_t need = nvbm::verify_workspace(rows, batch);
   if (!workspace || !aligned16(workspace) || workspace_bytes < need)
     return mfail("verify needs a 16-byte aligned workspace of %zu bytes (got %zu)", need, workspace_bytes);

@@ -805,6 +805,10 @@ int nvb_paged_tree_fwd(void* stream, const void* q, const void* k, const void* v
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (out_accum && !aligned16(out_accum)) ||
       (reinterpret_cast<uintptr_t>(tree_mask) & 7))
     return fail("q, k, v, out and out_accum must be 16-byte aligned, tree_mask 8-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(kv_lens) |
+       reinterpret_cast<uintptr_t>(block_table) | reinterpret_cast<uintptr_t>(lse) |
+       reinterpret_cast<uintptr_t>(lse_accum)) & 3)
+    return fail("cu_q, kv_lens, block_table, lse and lse_accum must be 4-byte aligned");
   TreeParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.out = static_cast<__nv_bfloat16*>(out);

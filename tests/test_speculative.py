@@ -187,6 +187,16 @@ def test_tree_refuses_on_the_host(nvb, bad):
     assert lib.nvb_last_error().decode()
 
 
+@pytest.mark.parametrize("at, off", [(i, o) for i in (5, 6, 7) for o in (1, 2)] + [(8, 4)] +
+                         [(i, o) for i in (19, 20, 21) for o in (1, 2)] + [(21, 4)])
+def test_tree_refuses_addresses_that_its_types_cannot_have(nvb, at, off):
+    lib = nvb.library()
+    args = [P(0), *[NZ] * 8, 1, 1, 2, 2, 300, 4, 2, 256, 2, 11, NZ, NZ, NZ, 2]
+    args[at] = P(256 + off)
+    assert lib.nvb_paged_tree_fwd(*args) == -1
+    assert "aligned" in lib.nvb_last_error().decode()
+
+
 def test_tree_num_splits(nvb):
     lib = nvb.library()
     assert [lib.nvb_tree_parts(s) for s in (0, 1, 2, 7, 8, 9, 11, 16, 128, 129)] == [0, 1, 1, 1, 1, 3, 11, 2, 16, 0]
@@ -261,6 +271,19 @@ def test_compact_paths_refuses_on_the_host(nvb, bad):
     assert lib.nvb_last_error().decode()
 
 
+@pytest.mark.parametrize("off", [1, 2])
+@pytest.mark.parametrize("at", range(6))
+def test_cache_copies_refuse_addresses_that_their_types_cannot_have(nvb, at, off):
+    lib = nvb.library()
+    caches = [_layers(4096, 8192), _layers(12288, 16384), 2]
+    ints = [P(1024 * (i + 1) + (off if i == at else 0)) for i in range(6)]
+    assert lib.nvb_cache_compact_paths(P(0), *caches, *ints, 1, 4, 2, 128, 256, 2, 4) == -1
+    assert "aligned" in lib.nvb_last_error().decode()
+    if at < 3:
+        assert lib.nvb_cache_copy_pages(P(0), *caches, *ints[:3], 1, 2, 128, 256, 4) == -1
+        assert "aligned" in lib.nvb_last_error().decode()
+
+
 @pytest.mark.parametrize("bad", [dict(logits=P(0)), dict(rows=0), dict(batch=0), dict(batch=65536), dict(max_q=0),
                                  dict(max_q=1025), dict(vocab=0), dict(ws=P(0)), dict(ws=P(264)), dict(size=8)])
 def test_verify_refuses_on_the_host(nvb, bad):
@@ -271,6 +294,20 @@ def test_verify_refuses_on_the_host(nvb, bad):
                                a["max_q"], a["vocab"], a["ws"], a["size"])
     assert rc == -1
     assert lib.nvbe_model_last_error().decode()
+
+
+VERIFY_POINTERS = ["logits", "draft", "tokens", "parents", "uniforms", "seeds", "temperatures", "cu_q", "out_tokens",
+                   "path", "counts", "accept"]
+
+
+@pytest.mark.parametrize("name, off", [(n, 1) for n in VERIFY_POINTERS] + [(n, 2) for n in VERIFY_POINTERS[2:]] +
+                         [("seeds", 4)])
+def test_verify_refuses_addresses_that_its_types_cannot_have(nvb, name, off):
+    # (the kernels would read them, which no library catches)
+    lib = nvb.model.library()
+    pointers = [P(256 + off) if n == name else NZ for n in VERIFY_POINTERS]
+    assert lib.nvbe_layer_verify(P(0), *pointers, 2, 1, 2, 10, NZ, 1 << 20) == -1
+    assert "aligned" in lib.nvbe_model_last_error().decode()
 
 
 def test_verify_workspace_grows_with_the_rows(nvb):
