@@ -308,7 +308,7 @@ int nvbe_layer_sample(void* stream, const void* logits, const float* temperature
  *
  * Entries behind counts are -1; a sequence without rows has counts 0. Rows at
  * and behind cu_q[batch] are neither read nor written. max_q bounds the nodes
- * of a sequence (at most 1024). `workspace`: 16-byte aligned,
+ * of a sequence (at most 1024); vocab is at most 2^30. `workspace`: 16-byte aligned,
  * nvbe_verify_workspace_bytes(rows, batch) bytes, written before it is read; calls
  * that may overlap need one each. Allocates nothing and can be captured. */
 size_t nvbe_verify_workspace_bytes(int rows, int batch);

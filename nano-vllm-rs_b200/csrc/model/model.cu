@@ -626,6 +626,8 @@ int nvbe_layer_verify(void* stream, const void* logits, const void* draft_logits
   if (!logits || !tokens || !parents || !uniforms || !seeds || !temperatures || !cu_q || !out_tokens || !path ||
       !counts || !accept_prob || rows <= 0 || batch <= 0 || batch > 65535 || max_q <= 0 || vocab <= 0)
     return mfail("invalid verify arguments");
+  // places in a row are int32, and some steps go past its end by up to 32767
+  if (vocab > 1 << 30) return mfail("verify takes a vocab of at most 2^30 tokens (got %d)", vocab);
   if (max_q > nvbm::verify_max_nodes())
     return mfail("a tree has at most %d nodes (max_q %d)", nvbm::verify_max_nodes(), max_q);
   const uintptr_t halves = reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(draft_logits);

@@ -296,6 +296,13 @@ def test_verify_refuses_on_the_host(nvb, bad):
     assert lib.nvbe_model_last_error().decode()
 
 
+@pytest.mark.parametrize("vocab", [(1 << 30) + 1, (1 << 31) - 1])
+def test_verify_refuses_vocabularies_past_its_index_arithmetic(nvb, vocab):
+    lib = nvb.model.library()
+    assert lib.nvbe_layer_verify(P(0), *[NZ] * 12, 2, 1, 2, vocab, NZ, 1 << 20) == -1
+    assert "vocab" in lib.nvbe_model_last_error().decode()
+
+
 VERIFY_POINTERS = ["logits", "draft", "tokens", "parents", "uniforms", "seeds", "temperatures", "cu_q", "out_tokens",
                    "path", "counts", "accept"]
 
