@@ -987,7 +987,9 @@ __global__ void __launch_bounds__(kSampleThreads, 4) verify_sample_kernel(const 
       const uint4 v = vp;
       probabilities(vp, vq, at);
       if (chunk + int(gridDim.x) < chunks) load(chunk + gridDim.x, vp, vq);
-      const float scale = __expf(base - l + 2e-3f * (1.0f + fabsf(l)));  // e^-(best - base) and a little
+      // e^-(best - base) and a little; no less than e^-80, as weights go up to the largest float and their product with
+      // a scale that is flushed, or of a few bits, bounds nothing (a larger one only has more tokens scored)
+      const float scale = __expf(fmaxf(base - l + 2e-3f * (1.0f + fabsf(l)), -80.0f));
       uint64_t t = uint64_t(int64_t(at)) * 0xd2b74407b1ce6e93ULL;
       uint32_t hits = 0;
 #pragma unroll

@@ -1204,3 +1204,27 @@ def test_verify_zeros_of_either_sign_are_equal_logits(nvb, draft, value):
     want, seeds = torch.empty(rows, dtype=torch.int32, device="cuda"), torch.from_numpy(case.seeds).cuda()
     nvb.model.layer_sample(case.logits.cuda(), torch.zeros(rows, device="cuda"), seeds, want)
     assert [want[i].item() for i in (0, 2, 3, 6)] == [o["out_tokens"][b, c - 1].item() for b, c in enumerate([1, 2, 1, 2])]
+
+
+def test_verify_draws_what_wins_at_the_end_of_the_floats_range(nvb):
+    # One CTA a sequence, chunks of 2,048 tokens. The first chunk's logits are 104 temperatures below zero. A token of
+    # the second one scores 0.1; one of the third, 88.7 temperatures above the first chunk (e^88.7 is nearly the largest
+    # float) with a noise of 15.5, scores 0.2 and is the one to draw. e^-104.1, by which the second's score outweighs
+    # the first chunk's weights, is below every float.
+    vocab, rows, seed, leader, token = 8192, 600, 1178, 3509, 5554  # both of the 183rd group of their chunks
+    row = torch.full((vocab,), -3.0)
+    row[:2048], row[leader], row[token] = -1.0, 0.00326, -151 / 1024
+    row = row.to(torch.bfloat16)
+    t = np.float32(1.0) / np.float32(104.0)
+    score = spec_ref.as64(row) / np.float64(t) + spec_ref.gumbel(seed, vocab)
+    assert np.argmax(score) == token and 0.05 < score[leader] < score[token] - 0.05 < 0.2
+    i32 = dict(dtype=torch.int32, device="cuda")
+    logits, seeds = row.expand(rows, vocab).contiguous().cuda(), torch.full((rows,), seed, device="cuda")
+    temps = torch.full((rows,), float(t), device="cuda")
+    out, path, counts = torch.zeros(rows, 1, **i32), torch.zeros(rows, 1, **i32), torch.zeros(rows, **i32)
+    nvb.model.layer_verify(logits, None, torch.zeros(rows, **i32), torch.full((rows,), -1, **i32),
+                           torch.zeros(rows, device="cuda"), seeds, temps, torch.arange(rows + 1, **i32), out, path,
+                           counts, torch.empty(rows, device="cuda"))
+    want = torch.empty(rows, **i32)
+    nvb.model.layer_sample(logits, temps, seeds, want)
+    assert (want == token).all() and torch.equal(out[:, 0], want)
