@@ -201,3 +201,44 @@ def verify(logits, draft, tokens, parents, uniforms, seeds, temps, cu, max_q, ep
         if len(top) == 2 and np.isfinite(top).all():
             margin = min(margin, top[1] - top[0])
     return out, path, counts, prob, bound, margin, drawable
+
+
+def drawn_from(logits, draft, tokens, parents, seeds, temps, cu, path, counts, eps=3e-5):
+    """For each sequence the next tokens that may be drawn behind its path where every probability is eps off
+    (relative), or None where nothing was rejected there (then verify's token is the one). As verify's `drawable`, but a
+    factor that all tokens share is no error of a score: the sum that P is divided by counts only where Q is taken from
+    P after it."""
+    out = []
+    for b in range(len(temps)):
+        n, first, last = cu[b + 1] - cu[b], cu[b], path[b][counts[b] - 1]
+        kids = [i for i in range(last + 1, n) if parents[first + i] == last] if counts[b] else []
+        if not kids or not temps[b] > 0:
+            out.append(None)
+            continue
+        p, vocab = softmax(logits[first + last], temps[b]), logits.shape[1]
+        q = softmax(draft[first + last], temps[b]) if draft is not None else None
+        ep, shared = eps * p, 0.0
+        eq = eps * q if q is not None else None
+        for i in kids:
+            t, inside = tokens[first + i], 0 <= tokens[first + i] < vocab
+            if q is None:
+                rest = p.copy()
+                if inside:
+                    rest[t] = 0
+                erest = np.where(rest > 0, ep, 0)
+            else:
+                rest, erest, shared = np.maximum(p - q, 0), ep + shared * p + eq, 0.0
+                q, eq = q.copy(), eq.copy()
+                if inside:
+                    q[t] = eq[t] = 0
+                if q.sum() > 0:
+                    eq, q = eq / q.sum() + q * eq.sum() / q.sum() ** 2, q / q.sum()
+            total = rest.sum()
+            if total > 0:
+                p, ep, shared = rest / total, erest / total, shared + erest.sum() / total
+        with np.errstate(divide="ignore"):
+            noise = gumbel(int(seeds[first + last]), vocab)
+            low, high = np.log(np.maximum(p - ep, 0)) + noise, np.log(p + ep) + noise
+        # a score of log 0 is nobody's
+        out.append({int(t) for t in np.nonzero((high >= low.max()) & (high > -math.inf))[0]})
+    return out

@@ -328,6 +328,27 @@ def test_engine_header_functions_are_exported(nvb):
     assert lib.nvbe_layer_verify and lib.nvbe_verify_workspace_bytes
 
 
+# ------------------------------------------------- the drawn token's tolerance
+def test_tokens_that_may_be_drawn_are_those_that_rounding_reaches():
+    rng, vocab = np.random.RandomState(1), 50
+    logits, draft = rng.randn(3, vocab) * 2, rng.randn(3, vocab) * 2
+    tokens, parents, seeds = np.array([0, 4, 9]), np.array([-1, 0, 0]), np.array([5, 6, 7])
+    args = (tokens, parents, seeds, [1.0], [0, 3], [[0]], [1])
+    for d, eps in ((draft, 0.2), (None, 0.9)):
+        one, = spec_ref.drawn_from(logits, d, *args)
+        more, = spec_ref.drawn_from(logits, d, *args, eps=eps)
+        assert len(one) == 1 and one < more and len(more) < vocab
+    assert spec_ref.drawn_from(logits, draft, tokens, parents, seeds, [0.0], [0, 3], [[0]], [1]) == [None]
+    assert spec_ref.drawn_from(logits, draft, tokens, parents, seeds, [1.0], [0, 3], [[0, 2]], [2]) == [None]
+    # drafts equal to the target but for one token: what is left is that token and the rounding of the likely ones; a
+    # token without probability is never among them
+    near = logits.copy()
+    near[0, 7] += 1e-9
+    logits[0, 20:] = near[0, 20:] = -np.inf
+    few, = spec_ref.drawn_from(near, logits, *args)
+    assert few and max(few) < 20
+
+
 # ------------------------------------------------- memory that a graph holds on to
 def test_a_graph_keeps_the_workspaces_of_its_calls(nvb, monkeypatch):
     class Library:

@@ -1228,3 +1228,40 @@ def test_verify_draws_what_wins_at_the_end_of_the_floats_range(nvb):
     want = torch.empty(rows, **i32)
     nvb.model.layer_sample(logits, temps, seeds, want)
     assert (want == token).all() and torch.equal(out[:, 0], want)
+
+
+# -------------------------------------- the drawn token, where `same` leaves it open
+def _only(case, o, ref):
+    f = spec_ref.as64
+    sets = spec_ref.drawn_from(f(case.logits), f(case.draft) if case.draft is not None else None, case.tokens,
+                               case.parents, case.seeds, case.temps, case.cu, ref[1], ref[2])
+    for b, tokens in enumerate(sets):
+        assert tokens is None or o["out_tokens"][b, ref[2][b] - 1].item() in tokens
+    return [None if tokens is None else sorted(tokens) for tokens in sets]
+
+
+def test_verify_the_widest_tree_draws_the_one_token(nvb):
+    # 290 rejected looked-up drafts: what is left of P is divided 290 times, by the same sums for every token
+    case = Drafts([1024], 300, 1, False, [1.0], seed=57)
+    case.parents[1:1024] = 0
+    case.tokens[1:1024] = np.arange(1023) % 290
+    case.uniforms[:] = 0.9999
+    o, ref = case.run(nvb), case.reference()
+    assert _only(case, o, ref) == [[295]]
+
+
+def test_verify_draws_among_the_tokens_that_rounding_leaves(nvb):
+    # P and Q put all but 1e-28 on the same three tokens: their difference there is rounding, or another token is drawn
+    case = Drafts([6, 5, 4], 40000, 3, True, [1.0, 1.0, 0.0], seed=59)
+    for x in (case.logits, case.draft):
+        x[:, 30000:30003] = 70.0 + torch.tensor([0.0, 2.0, -2.0])
+    o, ref = case.run(nvb), case.reference()
+    assert _only(case, o, ref)[0] == [12457, 30000, 30001, 30002]
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("spec", VERIFY)
+def test_verify_draws_the_one_token(nvb, spec, draft):
+    case = Drafts(**spec, draft=draft, seed=len(spec["sizes"]) + spec["vocab"])
+    o, ref = case.run(nvb), case.reference()
+    assert all(tokens is None or len(tokens) == 1 for tokens in _only(case, o, ref))
