@@ -185,6 +185,9 @@ int nvb_peer_buffer_free(void* ptr);
  *    a GPU of num_sms SMs.
  *  - a key that a node does not see has no part in its result, whatever
  *    values the cache holds there (infinities and NaN too).
+ *  - scores, row maxima and sums are FP32; each probability is rounded to BF16
+ *    for its product with V, as in this library's other tensor-core kernels:
+ *    up to 2^-8 of sum p |v| beside the output's own rounding.
  *  - page ids outside [0, num_blocks) mask their tokens.
  * Other limits as nvb_paged_fwd_ex; batch at most 65535. */
 int nvb_paged_tree_fwd(void* stream, const void* q, const void* k, const void* v, void* out,
@@ -207,7 +210,8 @@ int nvb_tree_num_splits(int batch, int max_q, int q_heads, int kv_heads, int max
  * nvb_cache_copy_pages copies page src_pages[i] to page dst_pages[i] for each
  * of `pairs` pairs (device arrays), the first rows[i] tokens of it where rows
  * is not null: the pages that forked sequences must not share
- * (nvbh_pool_fork). Pairs with a page outside [0, num_blocks) are skipped.
+ * (nvbh_pool_fork). Pairs with a page outside [0, num_blocks) are skipped;
+ * there are at most num_blocks pairs.
  * Pairs run in any order: no page may be the target of two pairs, nor the
  * target of one and the source of another.
  *

@@ -1091,6 +1091,9 @@ def test_the_models_caches_make_a_handle(nvb):
 
 
 # ------------------------------------------- sums of rows with far outliers
+# Weights are taken in a unit up to 90 binary orders below the highest logit. Exponents of up to 90 are off by 90 * 2^-24
+# steps of their product, 4e-6 of a weight and as much of a sum; log2(e) / T is off by 2^-23, 6e-6 over 72 orders; a
+# thread's sum has up to 16 terms in a row and 20 joins behind it, 2e-6. Together less than the 3e-5 of spec_ref.verify.
 def _padded(case, rows):
     """Arguments and outputs of `rows` rows, those behind the case's own without a sequence. (From 237 rows on, at
     148 SMs, a row of 151,936 tokens is read in 5 parts, below that in 32.)"""
