@@ -361,8 +361,8 @@ int nvbh_pool_truncate(NvbhBlockPool* p, int32_t* blocks, size_t* num_blocks, si
   }
   if (tokens % block_size) {
     // A page cut in its middle will hold other tokens than its prefix says.
-    const auto& last = p->blocks[size_t(blocks[need - 1])];
-    if (last.references == 1 && last.has_prefix && last.tokens.size() > tokens) p->invalidate(blocks[need - 1]);
+    const int32_t last = blocks[need - 1];
+    if (nvbh_pool_references(p, last) == 1 && p->blocks[size_t(last)].tokens.size() > tokens) p->invalidate(last);
   }
   *num_blocks = need;
   return 0;

@@ -164,6 +164,13 @@ def test_truncate_keeps_a_page_published_for_no_more_than_is_kept(host):
     assert pool.find(text) == blocks[1]
 
 
+@pytest.mark.parametrize("page", [-1, 3, 2 ** 31 - 1, -2 ** 31])
+def test_truncate_into_a_page_that_the_pool_does_not_have_keeps_it_as_it_is(host, page):
+    pool = host.BlockPool(3)
+    blocks = [page, pool.allocate()]
+    assert pool.truncate(blocks, 100, 256) == [page] and pool.in_use() == 0
+
+
 # -------------------------------------------------- argument checks of the ABI
 def _tree(lib, **kw):
     a = dict(q=NZ, mask=NZ, words=1, batch=1, total_q=2, max_q=2, max_k=300, qh=4, kvh=2, bs=256, stride=2, splits=1,
