@@ -232,6 +232,15 @@ __device__ __forceinline__ float max8(const uint4& v) {
   return fmaxf(__low2float(m), __high2float(m));
 }
 
+// Whether one of eight logits is NaN: magnitudes above infinity's.
+__device__ __forceinline__ bool has_nan(const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) found |= (w[i] & 0x7fffu) > 0x7f80u || (w[i] & 0x7fff0000u) > 0x7f800000u;
+  return found;
+}
+
 // (l - m) c of eight logits.
 __device__ __forceinline__ void exponents8(const uint4& v, float m, float c, float2 (&x)[4]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -259,8 +268,8 @@ struct Online {
       z = m == -INFINITY ? z : z * ex2((m - gm) * c);
       m = gm;
     }
-    if (!(m > -INFINITY)) {  // nothing but -inf so far, or NaN
-      if (!(gm == gm)) z = NAN;
+    if (!(m > -INFINITY)) {  // nothing but -inf so far, or NaN, which max8 leaves out
+      if (has_nan(v)) z = NAN;
       return;
     }
     float2 w[4];

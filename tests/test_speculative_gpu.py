@@ -1268,3 +1268,27 @@ def test_verify_draws_the_one_token(nvb, spec, draft):
     case = Drafts(**spec, draft=draft, seed=len(spec["sizes"]) + spec["vocab"])
     o, ref = case.run(nvb), case.reference()
     assert all(tokens is None or len(tokens) == 1 for tokens in _only(case, o, ref))
+
+
+@pytest.mark.parametrize("where", ["target", "draft", "both", "lookup"])
+@pytest.mark.parametrize("vocab", [3, 1500, 40001])
+def test_verify_missing_logits_among_masked_ones(nvb, vocab, where):
+    # NaN whose neighbours are all -inf (or lie outside the row): they are seen as missing there too, and what is left
+    # after rejections is a number
+    case = Drafts([5, 6, 4], vocab, 3, where != "lookup", [1.0, 4.0, 1.0], seed=77)
+    masked = max(1, vocab - max(2, vocab // 3))
+    for name, x in (("target", case.logits), ("draft", case.draft)):
+        if name == where or where == "both" or (where == "lookup" and name == "target"):
+            x[:, :masked] = -math.inf
+            x[:, :masked:max(1, masked // 3)] = math.nan
+    for b, n in enumerate(case.sizes):  # the drafts: the target's likely tokens, and one that is missing
+        first = case.cu[b]
+        case.parents[first + 1:first + n] = 0
+        likely = masked + case.logits[first, masked:].float().argsort(descending=True).numpy()
+        case.tokens[first + 1:first + n] = np.resize(likely[:n - 2], n - 1)
+        case.tokens[first + 2] = 0
+    case.uniforms[:] = 0.9999
+    ref = case.reference()
+    o = case.run(nvb)
+    same(case, o, ref)
+    _only(case, o, ref)
