@@ -231,6 +231,108 @@ int nvb_cache_compact_paths(void* stream, void* const* k_layers, void* const* v_
                             int path_stride, int kv_heads, int head_dim, int block_size,
                             int table_stride, int num_blocks);
 
+/* Latent attention: a cache with one latent vector a token (no counterpart
+ * in the reference, whose models keep keys and values a head).
+ *
+ *   cache   [num_blocks, block_size, 576] bf16: 512 normalised latent values,
+ *           then 64 rotated key values that all heads share
+ *
+ * nvb_latent_store appends a step's tokens. kv holds `rows` rows of 576 values
+ * kv_stride elements apart (512 latent values, 64 key values); row r goes to
+ * cache slot slots[r] as x * weight / sqrt(mean(x^2) + eps) over the first 512
+ * (weight [512] bf16) and the last 64 rotated by position positions[r]. Slots
+ * outside [0, block_size * num_blocks) are skipped; no two rows may have the
+ * same slot. The rotary parts of the queries are rotated by the same call: q
+ * and q_out are the first of `rows` x q_heads parts of 64 values, at row and
+ * head strides of their own (in elements), so that they may be slices of
+ * longer heads; q_out may be q itself, with the same strides, and must not
+ * overlap it otherwise. kv may be null (queries only: weight, slots and cache
+ * are not used), and so may q (q_heads, q_out and their strides are not used).
+ * Pair i of a part is its elements (i, i + 32), or (2i, 2i + 1) with
+ * `interleaved`, turned by (cos, sin) = rope_table[position, i] and [position,
+ * 32 + i]; rope_table is [max_positions, 64] FP32 (nvbh_rope_table, or
+ * nvb_rope_cache with head_dim 64); positions outside it turn by nothing.
+ * Values are computed in FP32 and rounded to BF16 once.
+ *
+ * nvb_latent_gather makes the first cu_k[b + 1] - cu_k[b] cached rows of every
+ * sequence contiguous, in order: row cu_k[b] + j of latent (512 values) and of
+ * rope (64 values), at strides of their own. The projection that expands
+ * latents into keys and values reads `latent`, nvb_latent_prefill_fwd `rope`.
+ * Rows of pages outside [0, num_blocks), and behind the page table, are zero;
+ * rows before cu_k[0] and from cu_k[batch] on are left alone.
+ *
+ * Strides are multiples of 8 elements, all but the int arrays is 16-byte
+ * aligned. */
+int nvb_latent_store(void* stream, const void* kv, long long kv_stride, const void* weight,
+                     const int* positions, const int* slots, void* cache, const void* q,
+                     long long q_row_stride, long long q_head_stride, void* q_out,
+                     long long out_row_stride, long long out_head_stride, int rows, int q_heads,
+                     int interleaved, int block_size, int num_blocks, float eps,
+                     const float* rope_table, int max_positions);
+int nvb_latent_gather(void* stream, const void* cache, const int* block_table, const int* cu_k,
+                      void* latent, long long latent_stride, void* rope, long long rope_stride,
+                      int batch, int total_k, int block_size, int table_stride, int num_blocks);
+
+/* Absorbed form: attention over the latent cache itself, for decode steps and
+ * for short runs of queries (drafts, short chunks). Keys are the cache's rows
+ * (576), values their first 512, for all heads the same:
+ *
+ *   o_i = sum_j p_ij c_j[:512] / sum_j p_ij,  p_ij = exp(scale q_i . c_j)
+ *
+ * q [total_q, q_heads, 576] has the queries times the expansion of the keys in
+ * its first 512 values and the rotated part in its last 64; out [total_q,
+ * q_heads, 512] awaits the expansion of the values. Sequence b's queries
+ * [cu_q[b], cu_q[b + 1]) are the last of its kv_lens[b] tokens (bottom-right
+ * causal mask): query i of n sees the first kv_lens[b] - n + i + 1 keys.
+ *
+ *  - lse (may be null) is [total_q, q_heads]. A query that sees no key has
+ *    output 0 and lse -inf; so have all of a sequence whose kv_lens is
+ *    negative or longer than its table. Rows before cu_q[0] and from
+ *    cu_q[batch] on are left alone. Page ids outside [0, num_blocks) mask
+ *    their tokens.
+ *  - max_q (the most queries of a sequence) and the lengths only guide how the
+ *    work is shared out; results do not depend on the order in which CTAs run.
+ *  - a key that a query does not see has no part in its result, whatever the
+ *    cache holds there.
+ *  - scores, row maxima and sums are FP32; each probability is rounded to BF16
+ *    for its product with the values: up to 2^-8 of sum p |c| beside the
+ *    output's own rounding.
+ *  - scratch: FP32, nvb_latent_scratch_floats(num_sms) elements for a GPU of
+ *    num_sms SMs, whatever the batch (fewer make the call use fewer SMs; at
+ *    least nvb_latent_scratch_floats(1)). Nothing is kept in it from one call
+ *    for the next; calls that may overlap need their own.
+ * Limits: block_size a multiple of 64, q_heads at most 256, batch at most
+ * 65535, block_size * table_stride and block_size * num_blocks below 2^31. */
+int nvb_paged_latent_fwd(void* stream, const void* q, const void* cache, void* out, const int* cu_q,
+                         const int* kv_lens, const int* block_table, int batch, int total_q,
+                         int max_q, int q_heads, int block_size, int table_stride, int num_blocks,
+                         float scale, float* lse, float* scratch, long long scratch_floats);
+long long nvb_latent_scratch_floats(int num_sms);
+
+/* Expanded form: causal attention of prompts and chunks over keys and values
+ * that were expanded from latents.
+ *
+ *   q       [total_q, q_heads, 192]: 128 values, then the 64 rotated ones
+ *   kv      [total_k, q_heads, 256]: a head's 128 key values, then its 128 values
+ *   k_rope  [total_k] rows of 64 values, rope_stride elements apart: the rotated
+ *           part of the keys, the same for all heads
+ *   out     [total_q, q_heads, 128]
+ *   score   scale * (q[:128] . kv[:128] + q[128:] . k_rope)
+ *
+ * Sequence b has queries [cu_q[b], cu_q[b + 1]) and keys [cu_k[b], cu_k[b + 1]);
+ * its queries are the last of its keys (bottom-right causal mask), so a chunk
+ * behind a cached part has that part's keys expanded before its own
+ * (nvb_latent_gather). lse (may be null) is [total_q, q_heads]. A query that
+ * sees no key has output 0 and lse -inf, so have all of a sequence whose keys
+ * are not within [0, total_k]; rows that belong to no sequence are left alone.
+ * max_q must be at least the most queries of a sequence: rows past it are left
+ * alone too. Keys a query does not see have no part in its result. Rounding as
+ * nvb_paged_latent_fwd. Limits: q_heads at most 256, batch at most 65535. */
+int nvb_latent_prefill_fwd(void* stream, const void* q, const void* kv, const void* k_rope,
+                           long long rope_stride, void* out, const int* cu_q, const int* cu_k,
+                           int batch, int total_q, int total_k, int max_q, int q_heads, float scale,
+                           float* lse);
+
 /* Thread-local message for the last failing call on this thread
  * (kernels/flash_native/flash_native.cu:15, kernels/kernels.cu:28). */
 const char* nvb_last_error(void);

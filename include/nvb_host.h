@@ -151,6 +151,25 @@ int nvbh_pool_truncate(NvbhBlockPool* pool, int32_t* blocks, size_t* num_blocks,
 int nvbh_tree_mask(const int32_t* parents, const int32_t* cu_q, size_t sequences, size_t words,
                    uint64_t* mask, int32_t* depth);
 
+/* Rotary table of nvb_latent_store (and, with dim 128, of nvb_qkv_rope_cached):
+ * table [positions, dim] holds cos of pair i at [position, i] and sin at
+ * [position, dim / 2 + i], of the angle position * f_i, computed in 64 bits
+ * and multiplied by `magnitude`. f_i = theta^(-2 i / dim), changed for contexts
+ * longer than the model was trained on (factor >= 1) by `scaling`:
+ *   0  not at all (factor is not used)
+ *   1  linear: f_i / factor
+ *   2  base: theta times factor^(dim / (dim - 2)), so that the slowest pair
+ *      turns `factor` times slower and the fastest as before
+ *   3  by wavelength: pairs that turn fewer than `slow` times over
+ *      original_positions are divided by factor, those that turn more than
+ *      `fast` times keep f_i, with a linear blend in the number of turns
+ *      between (slow < fast)
+ *   4  by pair: as 3, with the blend linear in the pair's index between the
+ *      (fractional) indices that turn `fast` and `slow` times, rounded outwards
+ *      to whole pairs (YaRN: Peng, Quesnelle, Fan, Shippole 2023) */
+int nvbh_rope_table(float* table, size_t positions, size_t dim, double theta, int scaling, double factor,
+                    double original_positions, double slow, double fast, double magnitude);
+
 /* One sequence's slice of a forward pass (the reference's Segment plus the
  * sequence fields make_batch reads, src/runtime.rs:355-358, 728-777). */
 typedef struct NvbhSegment {

@@ -29,6 +29,7 @@ _host = None
 
 c_int, c_float, c_void_p, c_char_p = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_char_p
 _P = c_void_p
+_LL = ctypes.c_longlong
 
 
 def _declare(lib):
@@ -55,6 +56,11 @@ def _declare(lib):
         "nvb_tree_parts": [c_int],
         "nvb_cache_copy_pages": [_P] * 3 + [c_int] + [_P] * 3 + [c_int] * 5,
         "nvb_cache_compact_paths": [_P] * 3 + [c_int] + [_P] * 6 + [c_int] * 7,
+        "nvb_latent_store": [_P, _P, _LL, _P, _P, _P, _P, _P, _LL, _LL, _P, _LL, _LL] + [c_int] * 5 + [c_float, _P, c_int],
+        "nvb_latent_gather": [_P] * 5 + [_LL, _P, _LL] + [c_int] * 5,
+        "nvb_paged_latent_fwd": [_P] * 7 + [c_int] * 7 + [c_float, _P, _P, _LL],
+        "nvb_latent_scratch_floats": [c_int],
+        "nvb_latent_prefill_fwd": [_P] * 4 + [_LL] + [_P] * 3 + [c_int] * 5 + [c_float, _P],
         "nvb_peer_buffer_create": [ctypes.c_size_t, ctypes.POINTER(c_void_p), _P],
         "nvb_peer_buffer_open": [_P, ctypes.POINTER(c_void_p)],
         "nvb_peer_buffer_close": [_P],
@@ -64,6 +70,7 @@ def _declare(lib):
         fn = getattr(lib, name)
         fn.argtypes = args
         fn.restype = None if name in ("nvb_capture_abort", "nvb_graph_destroy") else c_int
+    lib.nvb_latent_scratch_floats.restype = _LL
     for name in ("nvb_last_error", "nvb_version"):
         getattr(lib, name).restype = c_char_p
         getattr(lib, name).argtypes = []
@@ -316,15 +323,21 @@ def paged_fwd(q, k, v, out, cu_q, kv_lens, block_table, *, batch, max_q, max_k, 
 _sm_counts = {}
 
 
+def _num_sms(device):
+    count = _sm_counts.get(device)
+    if count is None:
+        import torch
+
+        count = _sm_counts[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return count
+
+
 def tree_num_splits(batch, max_q, q_heads, kv_heads, max_k, num_sms=None):
     """Split count of paged_tree_fwd for a GPU of num_sms SMs (default: the current device's)."""
     if num_sms is None:
         import torch
 
-        device = torch.cuda.current_device()
-        num_sms = _sm_counts.get(device)
-        if num_sms is None:
-            num_sms = _sm_counts[device] = torch.cuda.get_device_properties(device).multi_processor_count
+        num_sms = _num_sms(torch.cuda.current_device())
     return library().nvb_tree_num_splits(batch, max_q, q_heads, kv_heads, max_k, num_sms)
 
 
@@ -448,6 +461,198 @@ def cache_compact_paths(layers, cu_q, kv_lens, block_table, path, counts, new_kv
     _check(library().nvb_cache_compact_paths(_raw_stream(stream, layers.device), layers._k, layers._v, layers.layers,
                                              *pointers, batch, path_stride, kv_heads, head_dim, block_size,
                                              table_stride, num_blocks))
+
+
+LATENT_DIM, LATENT_ROPE, LATENT_WIDTH = 512, 64, 576  # of a row of the latent cache
+
+
+def _strided(name, t, shape, device):
+    """(first, behind the last byte, name) of a BF16 CUDA tensor of that shape whose last dimension is contiguous."""
+    import torch
+
+    if t.dtype is not torch.bfloat16 or t.shape != shape or t.get_device() != device or (
+            t.stride(-1) != 1 or any(s < 0 for s in t.stride())):
+        if t.dtype is torch.bfloat16 and t.shape == shape and t.get_device() == device:
+            raise NvbError(f"{name}'s last dimension must be contiguous")
+        _refuse(t, shape, torch.bfloat16, name, device)
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + 2 * (last + 1), name
+
+
+def _apart(written, others):
+    """Refuses a written tensor's span that overlaps another's."""
+    for i, (a, z, name) in enumerate(written):
+        for x, y, other in written[:i] + others:
+            if a < y and x < z:
+                raise NvbError(f"{name} overlaps {other}")
+
+
+def _plain(name, t, shape, dtype, device):
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != device:
+        _refuse(t, shape, dtype, name, device)
+    return t.data_ptr(), t.data_ptr() + t.nbytes, name
+
+
+def _latent_cache(cache):
+    if cache.dim() != 3 or cache.shape[2] != LATENT_WIDTH:
+        raise NvbError(f"cache must be [num_blocks, block_size, {LATENT_WIDTH}], got {tuple(cache.shape)}")
+    return cache.shape[0], cache.shape[1]
+
+
+def latent_store(kv, weight, positions, slots, cache, *, rope_table, eps=1e-6, q=None, q_out=None, interleaved=False,
+                 stream=None):
+    """Appends a step's latents to the latent cache and rotates the queries'
+    rotary parts (nvb_latent_store).
+
+    kv [rows, 576] (its rows may be slices of longer ones): 512 latent values,
+    normalised with `weight` [512] and `eps`, and 64 key values, rotated by
+    positions [rows] int32; row r goes to slot slots[r] of cache [num_blocks,
+    block_size, 576]. q and q_out [rows, heads, 64] are slices of the queries:
+    q_out is q itself (the default) or does not overlap it. kv None rotates
+    queries only (weight, slots and cache None). rope_table [positions, 64]:
+    host.rope_table.
+    """
+    import torch
+
+    device, i32 = torch.cuda.current_device(), torch.int32
+    if kv is None and q is None:
+        raise NvbError("kv or q is required")
+    rows, heads, num_blocks, block_size = (kv if kv is not None else q).shape[0], 0, 0, 0
+    if rope_table.dim() != 2:
+        raise NvbError("rope_table must be [positions, 64]")
+    read = [_plain("positions", positions, (rows,), i32, device),
+            _plain("rope_table", rope_table, (rope_table.shape[0], LATENT_ROPE), torch.float32, device)]
+    written, kv_stride, strides = [], 0, (0, 0, 0, 0)
+    if kv is not None:
+        num_blocks, block_size = _latent_cache(cache)
+        read += [_strided("kv", kv, (rows, LATENT_WIDTH), device), _plain("slots", slots, (rows,), i32, device),
+                 _plain("weight", weight, (LATENT_DIM,), torch.bfloat16, device)]
+        written.append(_plain("cache", cache, cache.shape, torch.bfloat16, device))
+        kv_stride = kv.stride(0) if rows > 1 else max(kv.stride(0), LATENT_WIDTH)
+    elif weight is not None or slots is not None or cache is not None:
+        raise NvbError("weight, slots and cache go with kv")
+    if q is not None:
+        q_out = q if q_out is None else q_out
+        if q.dim() != 3:
+            raise NvbError("q must be [rows, heads, 64]")
+        heads = q.shape[1]
+        span = _strided("q", q, (rows, heads, LATENT_ROPE), device)
+        written.append(_strided("q_out", q_out, (rows, heads, LATENT_ROPE), device))
+        strides = (q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1))
+        if q_out.data_ptr() != q.data_ptr() or strides[:2] != strides[2:]:
+            read.append(span)
+    elif q_out is not None:
+        raise NvbError("q_out goes with q")
+    _apart(written, read)
+    _check(library().nvb_latent_store(
+        _raw_stream(stream, device), _address(kv), kv_stride, _address(weight), positions.data_ptr(), _address(slots),
+        _address(cache), _address(q), strides[0], strides[1], _address(q_out), strides[2], strides[3], rows, heads,
+        int(interleaved), block_size, num_blocks, eps, rope_table.data_ptr(), rope_table.shape[0]))
+
+
+def _address(t):
+    return t.data_ptr() if t is not None else None
+
+
+def latent_gather(cache, block_table, cu_k, latent, rope, *, stream=None):
+    """Copies the first cu_k[b + 1] - cu_k[b] cached rows of every sequence to
+    latent [total_k, 512] and rope [total_k, 64] (nvb_latent_gather); both may
+    be slices of longer rows."""
+    import torch
+
+    device, i32 = torch.cuda.current_device(), torch.int32
+    num_blocks, block_size = _latent_cache(cache)
+    if block_table.dim() != 2 or latent.dim() != 2:
+        raise NvbError("block_table and latent must have rows")
+    (batch, table_stride), total_k = block_table.shape, latent.shape[0]
+    read = [_plain("cache", cache, cache.shape, torch.bfloat16, device),
+            _plain("block_table", block_table, block_table.shape, i32, device),
+            _plain("cu_k", cu_k, (batch + 1,), i32, device)]
+    written = [_strided("latent", latent, (total_k, LATENT_DIM), device),
+               _strided("rope", rope, (total_k, LATENT_ROPE), device)]
+    strides = [t.stride(0) if total_k > 1 else max(t.stride(0), t.shape[1]) for t in (latent, rope)]
+    _apart(written[:1], read)
+    if not _interleaved_rows(latent, rope):
+        _apart(written[1:], read + written[:1])
+    else:
+        _apart(written[1:], read)
+    _check(library().nvb_latent_gather(_raw_stream(stream, device), cache.data_ptr(), block_table.data_ptr(),
+                                       cu_k.data_ptr(), latent.data_ptr(), strides[0], rope.data_ptr(), strides[1],
+                                       batch, total_k, block_size, table_stride, num_blocks))
+
+
+def _interleaved_rows(a, b):
+    """Whether two slices of the same rows lie beside one another in each row."""
+    if a.stride(0) != b.stride(0):
+        return False
+    first, second = (a, b) if a.data_ptr() < b.data_ptr() else (b, a)
+    gap = (second.data_ptr() - first.data_ptr()) // 2
+    return first.shape[1] <= gap and gap + second.shape[1] <= first.stride(0)
+
+
+def latent_scratch(device):
+    """FP32 scratch of paged_latent_fwd on `device`, whatever the batch; calls that may overlap need their own."""
+    import torch
+
+    device = torch.device(device)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch.empty(library().nvb_latent_scratch_floats(_num_sms(index)), dtype=torch.float32, device=device)
+
+
+def paged_latent_fwd(q, cache, out, cu_q, kv_lens, block_table, *, max_q, scale, scratch, lse=None, stream=None):
+    """Absorbed attention over the paged latent cache (nvb_paged_latent_fwd).
+
+    q [total_q, heads, 576] attends to cache [num_blocks, block_size, 576], out
+    [total_q, heads, 512] takes the weighted sums of its first 512 values, lse,
+    where given, [total_q, heads]. Sequence b's queries cu_q[b]..cu_q[b + 1] are
+    the last of its kv_lens[b] tokens. max_q: the most queries of a sequence.
+    scratch: latent_scratch.
+    """
+    import torch
+
+    device, bf16, i32, f32 = torch.cuda.current_device(), torch.bfloat16, torch.int32, torch.float32
+    num_blocks, block_size = _latent_cache(cache)
+    if q.dim() != 3 or block_table.dim() != 2:
+        raise NvbError("q must be [total_q, heads, 576], block_table a row for each sequence")
+    (total_q, heads, _), (batch, table_stride) = q.shape, block_table.shape
+    pointers = _pointers(
+        (("q", q, (total_q, heads, LATENT_WIDTH), bf16), ("cache", cache, cache.shape, bf16),
+         ("out", out, (total_q, heads, LATENT_DIM), bf16), ("cu_q", cu_q, (batch + 1,), i32),
+         ("kv_lens", kv_lens, (batch,), i32), ("block_table", block_table, block_table.shape, i32),
+         ("lse", lse, (total_q, heads), f32), ("scratch", scratch, (scratch.numel(),), f32)),
+        ("out", "lse", "scratch"), device)
+    _check(library().nvb_paged_latent_fwd(_raw_stream(stream, device), *pointers[:6], batch, total_q, max_q, heads,
+                                          block_size, table_stride, num_blocks, scale, *pointers[6:],
+                                          scratch.numel()))
+
+
+def latent_prefill_fwd(q, kv, k_rope, out, cu_q, cu_k, *, max_q, scale, lse=None, stream=None):
+    """Causal attention over expanded latent keys and values (nvb_latent_prefill_fwd).
+
+    q [total_q, heads, 192] (128 values and the 64 rotated ones), kv [total_k,
+    heads, 256] (128 key values and 128 values a head), k_rope [total_k, 64]
+    (rows may be slices of longer ones), out [total_q, heads, 128], lse, where
+    given, [total_q, heads]. Sequence b's queries are the last of its keys
+    cu_k[b]..cu_k[b + 1]. max_q: the most queries of a sequence.
+    """
+    import torch
+
+    device, bf16, i32 = torch.cuda.current_device(), torch.bfloat16, torch.int32
+    if q.dim() != 3 or kv.dim() != 3:
+        raise NvbError("q must be [total_q, heads, 192], kv [total_k, heads, 256]")
+    (total_q, heads, _), total_k, batch = q.shape, kv.shape[0], cu_q.numel() - 1
+    pointers = _pointers(
+        (("q", q, (total_q, heads, 192), bf16), ("kv", kv, (total_k, heads, 256), bf16),
+         ("out", out, (total_q, heads, 128), bf16), ("cu_q", cu_q, (batch + 1,), i32),
+         ("cu_k", cu_k, (batch + 1,), i32), ("lse", lse, (total_q, heads), torch.float32)), ("out", "lse"), device)
+    rope = _strided("k_rope", k_rope, (total_k, LATENT_ROPE), device)
+    stride = k_rope.stride(0) if total_k > 1 else max(k_rope.stride(0), LATENT_ROPE)
+    for t, name in ((out, "out"), (lse, "lse")):
+        if t is not None:
+            _apart([(t.data_ptr(), t.data_ptr() + t.nbytes, name)], [rope])
+    _check(library().nvb_latent_prefill_fwd(_raw_stream(stream, device), pointers[0], pointers[1], k_rope.data_ptr(),
+                                            stride, pointers[2], pointers[3], pointers[4], batch, total_q, total_k,
+                                            max_q, heads, scale, pointers[5]))
 
 
 def attention(q, kcache, vcache, positions, seq_indices, tables, out, *, rows, q_heads, kv_heads, head_dim,

@@ -393,6 +393,50 @@ int nvbh_tree_mask(const int32_t* parents, const int32_t* cu_q, size_t sequences
   return 0;
 }
 
+int nvbh_rope_table(float* table, size_t positions, size_t dim, double theta, int scaling, double factor,
+                    double original_positions, double slow, double fast, double magnitude) {
+  g_error[0] = 0;
+  if (!table || positions == 0 || positions > size_t(kI32Max) || dim < 2 || dim % 2 || dim > 65536)
+    return fail("invalid rope table arguments");
+  if (!(theta > 1.0) || !std::isfinite(theta) || !std::isfinite(magnitude))
+    return fail("theta must be finite and above 1, magnitude finite");
+  if (scaling < 0 || scaling > 4) return fail("scaling must be in [0, 4]");
+  if (scaling && (!(factor >= 1.0) || !std::isfinite(factor))) return fail("factor must be finite and at least 1");
+  if (scaling == 2 && dim < 4) return fail("scaling of the base needs two pairs at least");
+  if (scaling >= 3 && (!(original_positions >= 1.0) || !std::isfinite(original_positions) || !(slow > 0.0) ||
+                       !(fast > slow) || !std::isfinite(fast)))
+    return fail("scaling by turns needs original_positions >= 1 and 0 < slow < fast");
+  const size_t pairs = dim / 2;
+  const double pi = 3.14159265358979323846;
+  const double base = scaling == 2 ? theta * std::pow(factor, double(dim) / double(dim - 2)) : theta;
+  // the (fractional) pair that turns `turns` times over original_positions
+  const auto pair_of = [&](double turns) {
+    return double(dim) * std::log(original_positions / (turns * 2.0 * pi)) / (2.0 * std::log(theta));
+  };
+  std::vector<double> f(pairs);
+  for (size_t i = 0; i < pairs; ++i) {
+    f[i] = std::pow(base, -2.0 * double(i) / double(dim));
+    double slowed = scaling == 1 ? 1.0 : 0.0;  // share of the pair's frequency that is divided by factor
+    if (scaling == 3) {
+      const double turns = original_positions * f[i] / (2.0 * pi);
+      slowed = 1.0 - std::fmin(1.0, std::fmax(0.0, (turns - slow) / (fast - slow)));
+    } else if (scaling == 4) {
+      const double first = std::fmax(0.0, std::floor(pair_of(fast)));
+      const double last = std::fmin(double(dim - 1), std::ceil(pair_of(slow)));
+      // where both border pairs are one, the pairs up to it keep their frequency
+      slowed = std::fmin(1.0, std::fmax(0.0, (double(i) - first) / std::fmax(last - first, 1e-3)));
+    }
+    f[i] *= 1.0 - slowed + slowed / (scaling ? factor : 1.0);
+  }
+  for (size_t t = 0; t < positions; ++t)
+    for (size_t i = 0; i < pairs; ++i) {
+      const double angle = double(t) * f[i];
+      table[t * dim + i] = float(std::cos(angle) * magnitude);
+      table[t * dim + pairs + i] = float(std::sin(angle) * magnitude);
+    }
+  return 0;
+}
+
 void nvbh_pool_force_hash_entry(NvbhBlockPool* p, const uint32_t* prefix, size_t n, int block) {
   p->by_hash[prefix_hash(prefix, n)].push_back(block);
 }

@@ -137,6 +137,36 @@ struct TreeParams {
 };
 cudaError_t launch_tree(TreeParams p, const void* k, const void* v, int max_k, cudaStream_t stream);
 
+// Absorbed attention over the paged latent cache (latent.cu).
+struct LatentParams {
+  const __nv_bfloat16* q;      // [total_q, heads, 576]
+  const __nv_bfloat16* cache;  // [num_blocks, block_size, 576]
+  __nv_bfloat16* out;          // [total_q, heads, 512]
+  const int* cu_q;             // [batch + 1]
+  const int* kv_lens;          // [batch], this step's tokens included
+  const int* block_table;      // [batch, table_stride]
+  float* lse;                  // [total_q, heads] or null
+  float* scratch;
+  int batch, total_q, max_q, heads, block_size, table_stride, num_blocks;
+  float scale;
+};
+cudaError_t launch_latent(const LatentParams& p, cudaStream_t stream);
+
+// Causal attention over expanded latent keys and values (latent_prefill.cu).
+struct LatentPrefillParams {
+  const __nv_bfloat16* q;       // [total_q, heads, 192]
+  const __nv_bfloat16* kv;      // [total_k, heads, 256]: 128 key values, 128 values
+  const __nv_bfloat16* k_rope;  // [total_k] x rope_stride, 64 values
+  __nv_bfloat16* out;           // [total_q, heads, 128]
+  const int* cu_q;              // [batch + 1]
+  const int* cu_k;              // [batch + 1]
+  float* lse;                   // [total_q, heads] or null
+  long long rope_stride;
+  int batch, total_q, total_k, max_q, heads;
+  float scale;
+};
+cudaError_t launch_latent_prefill(const LatentPrefillParams& p, cudaStream_t stream);
+
 // Native-form attention for head dimensions other than 128 (generic.cu).
 cudaError_t launch_generic_attention(const void* q, const void* k, const void* v, void* out, const int* positions,
                                      const int* seq_indices, const int* tables, int rows, int qh, int kvh, int dim,

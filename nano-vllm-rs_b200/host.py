@@ -86,6 +86,7 @@ def library():
                                      ctypes.POINTER(c_size)]
         L.nvbh_pool_truncate.argtypes = [P, P, ctypes.POINTER(c_size), c_size, c_size]
         L.nvbh_tree_mask.argtypes = [P, P, c_size, c_size, P, P]
+        L.nvbh_rope_table.argtypes = [P, c_size, c_size, ctypes.c_double, ctypes.c_int] + [ctypes.c_double] * 5
         L.nvbh_make_batch.argtypes = [ctypes.POINTER(NvbhSegment), c_size, c_size, ctypes.c_uint64,
                                       ctypes.POINTER(NvbhBatchOut)]
         L.nvbh_sampling_seed.argtypes = [ctypes.c_uint64] * 3
@@ -309,6 +310,25 @@ def tree_mask(parents, cu_q, words=None):
     mask, depth = np.zeros((p.size, max(words, 0)), np.int64), np.zeros(p.size, np.int32)
     _check(library().nvbh_tree_mask(_p(p), _p(cu), cu.size - 1, words, _p(mask), _p(depth)))
     return mask, depth
+
+
+ROPE_SCALINGS = {None: 0, "linear": 1, "base": 2, "wavelength": 3, "yarn": 4}
+
+
+def rope_table(positions, dim, theta, scaling=None, factor=1.0, original_positions=0, slow=1.0, fast=32.0,
+               magnitude=1.0):
+    """[positions, dim] float32 cos | sin of rotary positions, computed in 64
+    bits (nvbh_rope_table): scaling is None, "linear", "base", "wavelength" or
+    "yarn"; the last two slow the pairs that turn fewer than `slow` to `fast`
+    times over original_positions."""
+    if scaling not in ROPE_SCALINGS:
+        raise HostError(f"scaling must be one of {list(ROPE_SCALINGS)}")
+    if positions < 1 or dim < 2:
+        raise HostError("positions must be at least 1, dim at least 2")
+    table = np.empty((positions, dim), np.float32)
+    _check(library().nvbh_rope_table(_p(table), positions, dim, theta, ROPE_SCALINGS[scaling], factor,
+                                     original_positions, slow, fast, magnitude))
+    return table
 
 
 def sampling_seed(base, request_id, generated):
