@@ -31,6 +31,7 @@ enum DeviceError : int {
   kErrPrefillAlign = 6,       // prefill: dynamic shared memory base not usable for the tile layout
   kErrGatherWait = 7,         // multi-GPU gather: a peer's completion flag did not arrive in time
   kErrTreeWait = 8,           // a wait of the tree attention gave up
+  kErrLatentWait = 9,         // a wait of the latent attention gave up
 };
 
 constexpr long long kWaitCycles = 4000000000LL;

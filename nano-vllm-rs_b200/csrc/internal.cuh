@@ -146,11 +146,12 @@ struct LatentParams {
   const int* kv_lens;          // [batch], this step's tokens included
   const int* block_table;      // [batch, table_stride]
   float* lse;                  // [total_q, heads] or null
-  float* scratch;
+  float* scratch;              // nvb_latent_scratch_floats
   int batch, total_q, max_q, heads, block_size, table_stride, num_blocks;
+  int min_units, l2_tiles;     // set by launch_latent
   float scale;
 };
-cudaError_t launch_latent(const LatentParams& p, cudaStream_t stream);
+cudaError_t launch_latent(LatentParams p, int ctas, cudaStream_t stream);
 
 // Causal attention over expanded latent keys and values (latent_prefill.cu).
 struct LatentPrefillParams {

@@ -1,74 +1,772 @@
-// Absorbed attention over the paged latent cache (nvb_paged_latent_fwd): the
-// simple form, a warp for each (query, head).
-#include "internal.cuh"
+// Absorbed attention over the paged latent cache (nvb_paged_latent_fwd). No
+// counterpart in the reference, whose models keep keys and values a head.
+//
+//   o_i = sum_j p_ij c_j[:512] / sum_j p_ij,  p_ij = exp(scale q_i . c_j)
+//
+// over the cache rows c_j (576 values) that query i sees. All heads share the
+// rows, so (query, head) pairs are plain rows of one matrix: a CTA takes 64 of
+// them and one range of a sequence's keys, 64 keys a tile:
+//
+//   S = Q C^T      tcgen05.mma M=64 N=64 K=576, both from shared memory
+//   P = exp2(S * scale * log2 e - m), BF16, to shared memory
+//   O^T += C^T P^T tcgen05.mma M=128 (dims) N=rows K=64 (keys), four times
+//
+// The second product is transposed because O with rows as TMEM lanes takes 512
+// columns, all there are, whatever the rows; with dims as lanes it takes 4 x 64,
+// and the scores have room beside it. A tile is loaded once and serves as K
+// (K-major) and as V (MN-major) where it lies.
+//
+// What bounds it: HBM up to 64 rows a sequence. A tile is 73,728 bytes, 1.66 us
+// of an SM's share of the copy rate (~3,150 cycles at 1.9 GHz); its products
+// read 245 KB of operands from shared memory, ~1,920 cycles at 128 bytes a
+// cycle. Q stays (72 KB), two tiles are in flight or in use (144 KB), so one
+// CTA fills an SM.
+//
+// Work: all CTAs run at once and share out the tiles of the whole batch evenly,
+// a CTA taking a run of them in the order of the sequences. Where a run's end
+// cuts a sequence, both CTAs write their part (O^T, maxima, sums) to the
+// scratch, at most two parts a CTA, and a second kernel joins them in the order
+// of the parts. The plan is worked out by each CTA from the lengths on the
+// device, so a captured call follows them.
+#include "prefill_common.cuh"
 
 namespace nvb {
 
 namespace latent_detail {
 
-constexpr int kLatent = 512, kWidth = 576;
+using namespace prefill_common;
 
-__global__ void __launch_bounds__(256) latent_kernel(const LatentParams p) {
-  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (item >= (long long)p.total_q * p.heads) return;
-  const int row = int(item / p.heads);
-  int lo = 0, hi = p.batch;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.cu_q[mid] <= row) lo = mid;
-    else hi = mid - 1;
-  }
-  if (lo >= p.batch || p.cu_q[lo] > row) return;
-  const int n = p.cu_q[lo + 1] - p.cu_q[lo], len = p.kv_lens[lo];
-  const bool valid = len >= 0 && (long long)len <= (long long)p.table_stride * p.block_size;
-  const int seen = valid ? len - n + (row - p.cu_q[lo]) + 1 : 0;
-  float q[18], acc[16], m = -INFINITY, l = 0.0f;
-  for (int i = 0; i < 18; ++i) q[i] = __bfloat162float(p.q[item * kWidth + lane + 32 * i]) * p.scale;
-  for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-  for (int t = 0; t < seen; ++t) {
-    const int page = p.block_table[(long long)lo * p.table_stride + t / p.block_size];
-    if (page < 0 || page >= p.num_blocks) continue;
-    const __nv_bfloat16* k = p.cache + ((long long)page * p.block_size + t % p.block_size) * kWidth;
-    float x[18], s = 0.0f;
-    for (int i = 0; i < 18; ++i) {
-      x[i] = __bfloat162float(k[lane + 32 * i]);
-      s = fmaf(q[i], x[i], s);
+constexpr int kLatent = 512, kWidth = 576;
+constexpr int kRows = 64;                       // rows of a CTA
+constexpr int kKeys = 64;                       // keys of a tile
+constexpr int kChunk = kKeys * 128;             // 64 keys (or rows) x 64 BF16, one swizzled piece
+constexpr int kChunks = kWidth / 64;            // pieces of a tile: the rotated part first, then the latents
+constexpr int kTileBytes = kChunks * kChunk;
+constexpr int kUnits = 5;                       // a tile's barriers: the rotated piece, four pairs of latent ones
+constexpr int kThreads = 256;
+constexpr int kTmemCols = 512;
+constexpr int kOCol = 128;                      // S at 0 and 64, O^T at 128 + 64 p
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kRescaleLog2 = 8.0f;            // the maximum in use moves when it grew by 2^8 (P <= 2^8)
+
+enum Bar { kFull = 0, kEmpty = kFull + 2 * kUnits, kSFull = kEmpty + 2 * kUnits, kPFull = kSFull + 2, kPVDone, kQFree,
+           kOFree, kDrain, kNumBars };
+constexpr int kTmemSlotOff = kNumBars * 8;
+constexpr int kPlanOff = (kTmemSlotOff + 4 + 15) & ~15;   // Plan
+constexpr int kScanOff = kPlanOff + 64;                   // long long [8] and int [8] of the warps' sums
+constexpr int kAlphaOff = kScanOff + 128;                 // float [64]: factors of O's columns
+constexpr int kHeadBytes = 1024;
+static_assert(kAlphaOff + kRows * 4 <= kHeadBytes, "head layout");
+constexpr int kQOff = kHeadBytes;
+constexpr int kRingOff = kQOff + kChunks * kChunk;
+constexpr int kPOff = kRingOff + 2 * kTileBytes;
+constexpr int kSmemBytes = kPOff + kRows * kKeys * 2;
+static_assert(kSmemBytes <= 232448, "per-CTA shared memory limit");
+
+// Scratch of a CTA: two parts (O^T as [p][row / 4][dim][row % 4], then {maximum, sum} of each row) and what the
+// second kernel is to join for it.
+constexpr int kPartFloats = kRows * kLatent + 2 * kRows;
+constexpr int kCtaFloats = 2 * kPartFloats + 16;
+struct Join {
+  int first_row, rows, parts, stride;  // of the output; parts are in this CTA's scratch (1) and every stride-th CTA's behind it (0)
+};
+
+// kind::f16, FP32 accumulate, BF16 A and B.
+constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10);
+constexpr uint32_t kIdescS = kIdesc | ((uint32_t(kRows) >> 4) << 24) | ((uint32_t(kKeys) >> 3) << 17);
+constexpr uint32_t kIdescPV = kIdesc | ((128u >> 4) << 24) | (1u << 15);  // A MN-major (dims contiguous), N by the rows
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, kErrLatentWait); }
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait(bar, parity));
+}
+
+// 16 lanes x 64 columns: thread t has rows t / 4 (r[4 i], r[4 i + 1]) and t / 4 + 8 (r[4 i + 2], r[4 i + 3]) at
+// columns 8 i + 2 (t % 4) and the next.
+__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : NVB_R8(0), NVB_R8(8), NVB_R8(16), NVB_R8(24)
+      : "r"(taddr));
+}
+
+// Whether any of the 128 threads of the softmax warps says yes; all of them meet here.
+__device__ __forceinline__ bool any_of_four_warps(bool yes) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(uint32_t(yes))
+      : "memory");
+  return r != 0;
+}
+
+// Whether a pair of BF16 holds an infinity or NaN: an exponent of all ones carries into the sign's place.
+__device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
+  return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) {  // such halves as 0
+  return w & ~(((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u));
+}
+
+// ---------------------------------------------------------------- plan
+// Units of work: every (sequence, round) has one for its start and one for
+// each tile. A round is `share` row tiles, each a member's of the group of
+// `share` CTAs that reads the round's keys together. Group i takes units
+// [i * per, (i + 1) * per).
+struct Sequence {
+  int begin, n, len, tiles, row_tiles;
+};
+__device__ __forceinline__ Sequence sequence(const LatentParams& p, int b) {
+  Sequence q;
+  q.begin = min(max(p.cu_q[b], 0), p.total_q);
+  q.n = min(max(p.cu_q[b + 1], q.begin), p.total_q) - q.begin;
+  q.len = p.kv_lens[b];
+  const bool valid = q.len > 0 && (long long)q.len <= (long long)p.table_stride * p.block_size;
+  q.tiles = valid ? (q.len + kKeys - 1) / kKeys : 0;
+  q.row_tiles = (q.n * p.heads + kRows - 1) / kRows;
+  return q;
+}
+struct Plan {
+  long long first;  // the unit that sequence b starts at
+  long long u0, u1;
+  int b, share;
+};
+static_assert(sizeof(Plan) <= 64, "plan's place");
+
+struct Segment {
+  int b, begin, n, len, tiles;
+  int row0;     // of the sequence's rows
+  int rows;     // at most 64
+  int t0, t1;   // tiles; t0 = t1: write zeros
+  bool whole;
+};
+// The segments of a CTA, in order; every role walks them by itself.
+struct Walk {
+  long long at;  // first unit of round `round` of sequence b
+  int b, round;
+  __device__ __forceinline__ explicit Walk(const Plan& plan) : at(plan.first), b(plan.b), round(0) {}
+  __device__ __forceinline__ bool next(const LatentParams& p, const Plan& plan, int member, Segment& s) {
+    while (b < p.batch && at < plan.u1) {
+      const Sequence q = sequence(p, b);
+      const int rounds = (q.row_tiles + plan.share - 1) / plan.share;
+      while (round < rounds && at < plan.u1) {
+        const long long start = at;
+        const int tile = round * plan.share + member;
+        at += q.tiles + 1;
+        ++round;
+        if (at <= plan.u0 || tile >= q.row_tiles) continue;
+        const long long t0 = max(plan.u0 - start - 1, 0ll), t1 = min(plan.u1 - start - 1, (long long)q.tiles);
+        if (q.tiles ? t1 <= t0 : start < plan.u0) continue;
+        s.b = b;
+        s.begin = q.begin;
+        s.n = q.n;
+        s.len = q.len;
+        s.tiles = q.tiles;
+        s.row0 = tile * kRows;
+        s.rows = min(kRows, q.n * p.heads - s.row0);
+        s.t0 = q.tiles ? int(t0) : 0;
+        s.t1 = q.tiles ? int(t1) : 0;
+        s.whole = s.t0 == 0 && s.t1 == q.tiles;
+        return true;
+      }
+      if (round < rounds) break;
+      ++b;
+      round = 0;
     }
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    const float mx = fmaxf(m, s), nm = mx == -INFINITY ? 0.0f : mx;
-    const float a = m == mx ? 1.0f : expf(m - nm), w = expf(s - nm);
-    m = mx;
-    l = l * a + w;
-    for (int i = 0; i < 16; ++i) acc[i] = acc[i] * a + w * x[i];
+    return false;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  for (int i = 0; i < 16; ++i) p.out[item * kLatent + lane + 32 * i] = __float2bfloat16_rn(acc[i] * inv);
-  if (lane == 0 && p.lse) p.lse[item] = l == 0.0f ? -INFINITY : m + logf(l);
+};
+
+template <class T>
+__device__ __forceinline__ T warp_sum(T v) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+
+// All threads; the plan is in shared memory when it returns.
+__device__ __forceinline__ void make_plan(const LatentParams& p, unsigned char* smem, int ctas) {
+  Plan* plan = reinterpret_cast<Plan*>(smem + kPlanOff);
+  long long* sums = reinterpret_cast<long long*>(smem + kScanOff);
+  int* most = reinterpret_cast<int*>(smem + kScanOff + 64);
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int each = (p.batch + kThreads - 1) / kThreads;
+  const int b0 = min(t * each, p.batch), b1 = min(b0 + each, p.batch);
+  // Row tiles of one sequence that read its keys at the same time share them in L2 whatever the batch. That costs CTAs
+  // where sequences have fewer row tiles than others, so it is for caches that L2 does not hold as a whole.
+  long long tiles = 0;
+  int rt = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Sequence q = sequence(p, b);
+    if (!q.row_tiles) continue;
+    tiles += q.tiles;
+    rt = max(rt, q.row_tiles);
+  }
+  tiles = warp_sum(tiles);
+  rt = __reduce_max_sync(0xffffffffu, rt);
+  if (lane == 0) {
+    sums[warp] = tiles;
+    most[warp] = rt;
+  }
+  __syncthreads();
+  tiles = 0;
+  rt = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    tiles += sums[w];
+    rt = max(rt, most[w]);
+  }
+  int share = 1;
+  if (tiles > p.l2_tiles && rt > 1) {
+    const int most_share = min(4, ctas);
+    const int rounds = (rt + most_share - 1) / most_share;
+    share = (rt + rounds - 1) / rounds;
+  }
+  long long units = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Sequence q = sequence(p, b);
+    units += (long long)((q.row_tiles + share - 1) / share) * (q.tiles + 1);
+  }
+  long long upto = units;  // with this thread's
+#pragma unroll
+  for (int off = 1; off < 32; off *= 2) {
+    const long long o = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += o;
+  }
+  __syncthreads();
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  long long total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) upto += sums[w];
+    total += sums[w];
+  }
+  const int groups = ctas / share, group = blockIdx.x / share;
+  const long long per = max((total + groups - 1) / groups, (long long)p.min_units);
+  const long long u0 = group < groups ? min(group * per, total) : total, u1 = min(u0 + per, total);
+  if (t == 0) {
+    plan->u0 = u0;
+    plan->u1 = group < groups ? u1 : u0;
+    plan->share = share;
+    plan->b = p.batch;  // unless a sequence has unit u0
+    plan->first = total;
+  }
+  __syncthreads();
+  if (units && upto - units <= u0 && u0 < upto) {
+    long long at = upto - units;
+    for (int b = b0; b < b1; ++b) {
+      const Sequence q = sequence(p, b);
+      const long long mine = (long long)((q.row_tiles + share - 1) / share) * (q.tiles + 1);
+      if (u0 < at + mine) {
+        plan->b = b;
+        plan->first = at;
+        break;
+      }
+      at += mine;
+    }
+  }
+  __syncthreads();
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    latent_kernel(const LatentParams p, const FastDiv fd_heads, const FastDiv fd_bs,
+                  const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap cmap) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kTmemSlotOff);
+  const uint32_t sbase = smem_addr(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // Set-up that needs no input runs beside the end of the kernel before this one.
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2 * kUnits; ++s) {
+      mbar_init(&bars[kFull + s], 1);
+      mbar_init(&bars[kEmpty + s], 1);
+    }
+    mbar_init(&bars[kSFull], 1);
+    mbar_init(&bars[kSFull + 1], 1);
+    mbar_init(&bars[kPFull], 4);
+    mbar_init(&bars[kPVDone], 1);
+    mbar_init(&bars[kQFree], 1);
+    mbar_init(&bars[kOFree], 4);
+    mbar_init(&bars[kDrain], 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // that kernel has completed, its writes are visible
+  make_plan(p, smem, gridDim.x);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Plan plan = *reinterpret_cast<const Plan*>(smem + kPlanOff);
+  const int member = int(blockIdx.x % unsigned(plan.share));
+  float* const part = p.scratch + (long long)blockIdx.x * kCtaFloats;
+  const bool aligned = (sbase & 1023u) == 0;
+  if (!aligned && threadIdx.x == 0) record_error(kErrPrefillAlign);
+
+  Walk walk(plan);
+  Segment s;
+  if (!aligned) {
+  } else if (warp == 0) {
+    // ---------------------------------------------------------- producer
+    if (lane == 0) {
+      tma_prefetch_desc(&qmap);
+      tma_prefetch_desc(&cmap);
+      int g = 0, seg = 0;
+      bool alive = true;
+      while (alive && walk.next(p, plan, member, s)) {
+        if (s.t0 == s.t1) continue;
+        const int* table = p.block_table + (long long)s.b * p.table_stride;
+        const int q_row = s.begin * p.heads + s.row0;
+        // the last S of the segment before this one has read Q
+        if (seg > 0) alive = wait(&bars[kQFree], (seg - 1) & 1);
+        int page = alive ? table[fd_bs.div(s.t0 * kKeys)] : -1;
+        for (int t = s.t0; t < s.t1 && alive; ++t, ++g) {
+          const int key0 = t * kKeys, logical = fd_bs.div(key0), stage = g & 1;
+          const bool ok = page_ok(page, p.num_blocks), with_q = t == s.t0;
+          const int row = ok ? page * p.block_size + (key0 - logical * p.block_size) : 0;
+          unsigned char* tile = smem + kRingOff + stage * kTileBytes;
+          for (int u = 0; u < kUnits; ++u) {
+            uint64_t* full = &bars[kFull + stage * kUnits + u];
+            if (g >= 2 && !wait(&bars[kEmpty + stage * kUnits + u], ((g >> 1) + 1) & 1)) {
+              alive = false;
+              break;
+            }
+            const int c0 = u == 0 ? 0 : 2 * u - 1, c1 = 2 * u;  // pieces of the unit
+            const uint32_t bytes = uint32_t(c1 - c0 + 1) * kChunk * ((ok ? 1 : 0) + (with_q ? 1 : 0));
+            if (bytes) mbar_arrive_expect_tx(full, bytes);
+            else mbar_arrive(full);  // a bad page's keys are masked, whatever the tile holds
+            for (int c = c0; c <= c1; ++c) {
+              const int x = c == 0 ? kLatent : (c - 1) * 64;
+              if (with_q) tma_load_3d(smem + kQOff + c * kChunk, &qmap, full, x, 0, q_row);
+              if (ok) tma_load_3d(tile + c * kChunk, &cmap, full, x, 0, row);
+            }
+          }
+          if (t + 1 < s.t1) {
+            const int next = fd_bs.div(key0 + kKeys);
+            if (next != logical) page = table[next];
+          }
+        }
+        ++seg;
+      }
+      // Every copy has landed before the CTA may exit (on the normal path its readers have waited for it).
+      for (int i = max(0, g - 2); i < g; ++i)
+        for (int u = 0; u < kUnits; ++u)
+          if (!wait(&bars[kFull + (i & 1) * kUnits + u], (i >> 1) & 1)) break;
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      const uint64_t qd = sw128_desc(sbase + kQOff, 16, 1024), kd = sw128_desc(sbase + kRingOff, 16, 1024),
+                     vd = sw128_desc(sbase + kRingOff + kChunk, kChunk, 1024),
+                     pd = sw128_desc(sbase + kPOff, 16, 1024);
+      const uint32_t q_lo = uint32_t(qd), q_hi = uint32_t(qd >> 32), k_lo = uint32_t(kd), k_hi = uint32_t(kd >> 32),
+                     v_lo = uint32_t(vd), v_hi = uint32_t(vd >> 32), p_lo = uint32_t(pd), p_hi = uint32_t(pd >> 32);
+      // S of tile g, as its pieces land
+      auto issue_s = [&](int g, bool last) {
+        const int stage = g & 1;
+        const uint32_t kb = k_lo + uint32_t(stage * (kTileBytes >> 4));
+        for (int u = 0; u < kUnits; ++u) {
+          if (!wait(&bars[kFull + stage * kUnits + u], (g >> 1) & 1)) return false;
+          tc_fence_after();
+          for (int c = u == 0 ? 0 : 2 * u - 1; c <= 2 * u; ++c)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              const uint32_t off = uint32_t(c * kChunk + kk * 32) >> 4;
+              umma_ss(tmem + stage * kKeys, q_lo + off, q_hi, kb + off, k_hi, kIdescS, (c | kk) ? 1u : 0u);
+            }
+        }
+        umma_commit(&bars[kSFull + stage]);
+        umma_commit(&bars[kEmpty + stage * kUnits]);
+        if (last) umma_commit(&bars[kQFree]);
+        return true;
+      };
+      int g = 0, seg = 0;
+      bool alive = true;
+      while (alive && walk.next(p, plan, member, s)) {
+        if (s.t0 == s.t1) continue;
+        const uint32_t idesc = kIdescPV | (uint32_t((s.rows + 15) / 16 * 2) << 17);
+        for (int t = s.t0; t < s.t1 && alive; ++t, ++g) {
+          if (t == s.t0) alive = issue_s(g, t + 1 == s.t1);
+          // S of the next tile beside the rows' work on this one. Its buffer's scores have been read: the P that was
+          // made of them has been waited for.
+          if (alive && t + 1 < s.t1) alive = issue_s(g + 1, t + 2 == s.t1);
+          if (alive && t == s.t0 && seg > 0) alive = wait(&bars[kOFree], (seg - 1) & 1);
+          if (alive) alive = wait(&bars[kPFull], g & 1);
+          if (!alive) break;
+          tc_fence_after();
+          const int stage = g & 1;
+          const uint32_t vb = v_lo + uint32_t(stage * (kTileBytes >> 4));
+          for (int d = 0; d < 4; ++d) {  // 128 dims: two pieces
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)  // 16 keys: 2048 bytes of a piece's rows, 32 bytes of P's
+              umma_ss(tmem + kOCol + 64 * d, vb + uint32_t((2 * d * kChunk + kk * 2048) >> 4), v_hi,
+                      p_lo + uint32_t(kk * 2), p_hi, idesc, (t > s.t0 || kk) ? 1u : 0u);
+            umma_commit(&bars[kEmpty + stage * kUnits + 1 + d]);
+          }
+          umma_commit(&bars[kPVDone]);
+        }
+        ++seg;
+      }
+      // every MMA completes before TMEM is freed
+      umma_commit(&bars[kDrain]);
+      wait(&bars[kDrain], 0);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------- softmax, then the output
+    const int quad = warp & 3;
+    const uint32_t lane_base = tmem + (uint32_t(quad * 32) << 16);
+    const int ra = quad * 16 + (lane >> 2), rb = ra + 8;  // this thread's rows, shared by four lanes
+    float* alphas = reinterpret_cast<float*>(smem + kAlphaOff);
+    const float sl2 = p.scale * 1.4426950408889634f;
+    int g = 0;
+    // A warp whose wait gave up goes on without waiting, so that the four warps still meet at their named barriers.
+    bool alive = true;
+    Join join{0, 0, 0, 0};
+    while (walk.next(p, plan, member, s)) {
+      const long long first = (long long)s.begin * p.heads + s.row0;  // of the output's rows
+      if (s.t0 == s.t1) {  // no keys
+        for (int i = threadIdx.x - 128; i < s.rows * (kLatent / 8); i += 128)
+          *reinterpret_cast<uint4*>(p.out + first * kLatent + i * 8) = make_uint4(0, 0, 0, 0);
+        if (p.lse && threadIdx.x - 128 < s.rows) p.lse[first + threadIdx.x - 128] = -INFINITY;
+        continue;
+      }
+      const int* table = p.block_table + (long long)s.b * p.table_stride;
+      const int ctx = s.len - s.n;  // query i sees keys up to ctx + i
+      const int seen = ctx + fd_heads.div(s.row0) + 1;  // keys that every row sees
+      // rows behind the last one see what that sees; their results are dropped
+      const int lim_a = ctx + fd_heads.div(s.row0 + min(ra, s.rows - 1)),
+                lim_b = ctx + fd_heads.div(s.row0 + min(rb, s.rows - 1));
+      float ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
+      int page = table[fd_bs.div(s.t0 * kKeys)];
+      for (int t = s.t0; t < s.t1; ++t, ++g) {
+        const int key0 = t * kKeys;
+        const bool ok = page_ok(page, p.num_blocks);
+        if (t + 1 < s.t1) page = table[fd_bs.div(key0 + kKeys)];  // a tile ahead: the load goes to L2
+        const int real = ok ? min(kKeys, s.len - key0) : 0;  // keys of the sequence
+        const bool plain = real == kKeys && key0 + kKeys <= seen;
+        alive = alive && wait_warp(&bars[kSFull + (g & 1)], (g >> 1) & 1);
+        tc_fence_after();
+        uint32_t raw[32];
+        tmem_ld_rows(lane_base + (g & 1) * kKeys, raw);
+        tmem_ld_wait();
+        reg_fence(raw);
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(raw[i]);
+        if (!plain) {
+          const int a = min(lim_a - key0, real - 1) - 2 * (lane & 3), b = min(lim_b - key0, real - 1) - 2 * (lane & 3);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (8 * i > a) x[4 * i] = -INFINITY;
+            if (8 * i + 1 > a) x[4 * i + 1] = -INFINITY;
+            if (8 * i > b) x[4 * i + 2] = -INFINITY;
+            if (8 * i + 1 > b) x[4 * i + 3] = -INFINITY;
+          }
+        }
+        float ta = fmaxf(x[0], x[1]), tb = fmaxf(x[2], x[3]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+          ta = max3(ta, x[4 * i], x[4 * i + 1]);
+          tb = max3(tb, x[4 * i + 2], x[4 * i + 3]);
+        }
+#pragma unroll
+        for (int off = 1; off < 4; off *= 2) {
+          ta = fmaxf(ta, __shfl_xor_sync(0xffffffffu, ta, off));
+          tb = fmaxf(tb, __shfl_xor_sync(0xffffffffu, tb, off));
+        }
+        ta *= sl2;
+        tb *= sl2;
+        // The maximum in use moves only when the row's grew by more than 2^8 (or with its first key): O is seldom
+        // rescaled, and P <= 2^8 divides out at the end.
+        const bool grew_a = ta > ma + kRescaleLog2, grew_b = tb > mb + kRescaleLog2;
+        const float fa = grew_a ? fast_exp2(ma - ta) : 1.0f, fb = grew_b ? fast_exp2(mb - tb) : 1.0f;
+        ma = grew_a ? ta : ma;
+        mb = grew_b ? tb : mb;
+        const bool rescale = any_of_four_warps(t > s.t0 && (grew_a || grew_b));
+        const float na = ma == -INFINITY ? 0.0f : -ma, nb = mb == -INFINITY ? 0.0f : -mb;
+        float sa0 = 0.0f, sa1 = 0.0f, sb0 = 0.0f, sb1 = 0.0f;
+        uint32_t pa[8], pb[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          fma2(x[4 * i], x[4 * i + 1], x[4 * i], x[4 * i + 1], sl2, sl2, na, na);
+          fma2(x[4 * i + 2], x[4 * i + 3], x[4 * i + 2], x[4 * i + 3], sl2, sl2, nb, nb);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[4 * i + e] = fast_exp2(x[4 * i + e]);
+          add2(sa0, sa1, sa0, sa1, x[4 * i], x[4 * i + 1]);
+          add2(sb0, sb1, sb0, sb1, x[4 * i + 2], x[4 * i + 3]);
+          // BF16 for the tensor core (the values' type): half a step of each probability. The sum keeps FP32.
+          pa[i] = pack_bf16x2(x[4 * i], x[4 * i + 1]);
+          pb[i] = pack_bf16x2(x[4 * i + 2], x[4 * i + 3]);
+        }
+        la = la * fa + (sa0 + sa1);
+        lb = lb * fb + (sb0 + sb1);
+        if (rescale && (lane & 3) == 0) {
+          alphas[ra] = fa;
+          alphas[rb] = fb;
+        }
+        // the product before this one has read P and is done with O
+        if (g > 0) alive = alive && wait_warp(&bars[kPVDone], (g - 1) & 1);
+        unsigned char* prow = smem + kPOff + ra * 128 + (lane & 3) * 4;  // swizzled: 16-byte piece i of row r at i ^ (r % 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          *reinterpret_cast<uint32_t*>(prow + ((i ^ (ra & 7)) << 4)) = pa[i];
+          *reinterpret_cast<uint32_t*>(prow + 1024 + ((i ^ (ra & 7)) << 4)) = pb[i];
+        }
+        if (rescale) {
+          named_barrier(2, 128);  // the factors are there
+          tc_fence_after();
+          for (int d = 0; d < 4; ++d)
+            for (int c = 0; c < s.rows; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(lane_base + kOCol + 64 * d + c, o);
+              tmem_ld_wait();
+              reg_fence(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alphas[c + i]);
+              tmem_st16(lane_base + kOCol + 64 * d + c, o);
+            }
+          tmem_st_wait();
+        }
+        if (!plain) {
+          // Rows of the tile that may not meet a probability of 0: S has read them as keys, now they are values.
+          unsigned char* v = smem + kRingOff + (g & 1) * kTileBytes + kChunk;
+          const int me = threadIdx.x - 128;
+          // 16-byte piece i of the tile's rows, 64 a row
+          auto piece = [&](int i) {
+            return reinterpret_cast<uint4*>(v + ((i >> 3) & 7) * kChunk + (i >> 6) * 128 + (i & 7) * 16);
+          };
+          for (int i = 64 * real + me; i < 64 * kKeys; i += 128) *piece(i) = make_uint4(0, 0, 0, 0);
+          // What is not finite in a key that only some rows see makes the sums of those rows NaN by its score.
+          for (int i = 64 * min(real, max(0, seen - key0)) + me; i < 64 * real; i += 128) {
+            const uint4 w = *piece(i);
+            if (nonfinite(w.x) | nonfinite(w.y) | nonfinite(w.z) | nonfinite(w.w))
+              *piece(i) = make_uint4(finite_part(w.x), finite_part(w.y), finite_part(w.z), finite_part(w.w));
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[kPFull]);
+      }
+#pragma unroll
+      for (int off = 1; off < 4; off *= 2) {
+        la += __shfl_xor_sync(0xffffffffu, la, off);
+        lb += __shfl_xor_sync(0xffffffffu, lb, off);
+      }
+      float* const mine = part + (s.t0 > 0 ? 0 : 1) * kPartFloats;
+      named_barrier(2, 128);  // nobody rescales any more
+      if ((lane & 3) == 0) {
+        if (s.whole) {
+          alphas[ra] = la == 0.0f ? 0.0f : 1.0f / la;  // NaN stays NaN
+          alphas[rb] = lb == 0.0f ? 0.0f : 1.0f / lb;
+          if (p.lse && ra < s.rows) p.lse[first + ra] = la == 0.0f ? -INFINITY : (ma + fast_log2(la)) * kLn2;
+          if (p.lse && rb < s.rows) p.lse[first + rb] = lb == 0.0f ? -INFINITY : (mb + fast_log2(lb)) * kLn2;
+        } else {
+          float2* stats = reinterpret_cast<float2*>(mine + kRows * kLatent);
+          stats[ra] = make_float2(ma, la);
+          stats[rb] = make_float2(mb, lb);
+        }
+      }
+      named_barrier(2, 128);
+      alive = alive && wait_warp(&bars[kPVDone], (g - 1) & 1);
+      tc_fence_after();
+      const int dim = quad * 32 + lane;
+      for (int d = 0; d < 4; ++d)
+        for (int c = 0; c < s.rows; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(lane_base + kOCol + 64 * d + c, o);
+          tmem_ld_wait();
+          reg_fence(o);
+          if (s.whole) {
+            // Rows c + i and c + i + 1 of this dim; of the neighbour's the other one, so that a store has two dims of a row.
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float u = __uint_as_float(o[i]) * alphas[c + i], v = __uint_as_float(o[i + 1]) * alphas[c + i + 1];
+              const bool odd = lane & 1;
+              const float other = __shfl_xor_sync(0xffffffffu, odd ? u : v, 1);
+              const int row = c + i + (odd ? 1 : 0);
+              if (row < s.rows)
+                *reinterpret_cast<uint32_t*>(p.out + (first + row) * kLatent + d * 128 + (dim & ~1)) =
+                    odd ? pack_bf16x2(other, v) : pack_bf16x2(u, other);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<uint4*>(mine + ((d * 16 + (c + i) / 4) * 128 + dim) * 4) =
+                  make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kOFree]);
+      if (!s.whole && s.t0 == 0) {
+        // the first part of rows that are joined: how many follow
+        const long long per = plan.u1 - plan.u0;  // a cut run is a full one
+        const long long rest = s.tiles - s.t1;
+        join = Join{int(first), s.rows, 1 + int((rest + per - 1) / per), plan.share};
+      }
+    }
+    if (threadIdx.x == 128) *reinterpret_cast<Join*>(part + 2 * kPartFloats) = alive ? join : Join{0, 0, 0, 0};
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// Joins the parts of cut rows: CTA x looks at what CTA x of the first kernel
+// left to join, y takes 128 dims and eight rows. Sum over the parts s of
+// 2^(m_s - max) O_s over the same sum of their row sums, in the order of the
+// parts within each half of them, then of the halves.
+constexpr int kJoinThreads = 512, kJoinRows = 8;
+constexpr int kSlices = kJoinThreads / 256;  // 128 dims x 2 groups of four rows
+constexpr int kMaxParts = 512;               // CTAs
+
+__global__ void __launch_bounds__(kJoinThreads) latent_join_kernel(const LatentParams p) {
+  __shared__ float factor[kMaxParts][kJoinRows];
+  __shared__ float4 sums[kSlices][256];
+  __shared__ float inverse[kJoinRows];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const float* const scratch = p.scratch + (long long)blockIdx.x * kCtaFloats;
+  const Join j = *reinterpret_cast<const Join*>(scratch + 2 * kPartFloats);
+  const int d = blockIdx.y & 3, t = threadIdx.x;
+  const long long step = (long long)j.stride * kCtaFloats;
+  auto at = [&](int s) { return scratch + s * step + (s == 0 ? kPartFloats : 0); };
+  for (int r0 = (blockIdx.y >> 2) * kJoinRows; r0 < j.rows; r0 += (gridDim.y >> 2) * kJoinRows) {
+    const int warp = t >> 5, lane = t & 31;
+    if (warp < kJoinRows) {  // a warp a row: maximum, factors, sum
+      const int row = r0 + warp;
+      float mx = -INFINITY;
+      for (int s = lane; s < j.parts; s += 32) {
+        const float2 v = reinterpret_cast<const float2*>(at(s) + kRows * kLatent)[row];
+        if (v.y != 0.0f) mx = fmaxf(mx, v.x);  // a part without a seen key has no maximum
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+      float total = 0.0f;
+      for (int s = lane; s < j.parts; s += 32) {
+        const float2 v = reinterpret_cast<const float2*>(at(s) + kRows * kLatent)[row];
+        // one whose scores are all NaN has no maximum either, its sum is NaN
+        const float f = v.y == 0.0f ? 0.0f : (v.x == -INFINITY ? NAN : fast_exp2(v.x - mx));
+        factor[s][warp] = f;
+        total += f * v.y;
+      }
+      total = warp_sum(total);
+      if (lane == 0) {
+        inverse[warp] = total == 0.0f ? 0.0f : 1.0f / total;
+        if (d == 0 && p.lse && row < j.rows)
+          p.lse[j.first_row + row] = total == 0.0f ? -INFINITY : (mx + fast_log2(total)) * kLn2;
+      }
+    }
+    __syncthreads();
+    const int slice = t >> 8, group = (t >> 7) & 1, dim = t & 127;
+    const int each = (j.parts + kSlices - 1) / kSlices, s1 = min(j.parts, (slice + 1) * each);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int row = r0 + 4 * group;
+    if (row < j.rows) {
+      const int place = ((d * 16 + row / 4) * 128 + dim) * 4;
+#pragma unroll 8
+      for (int s = slice * each; s < s1; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(at(s) + place);
+        const float4 f = *reinterpret_cast<const float4*>(&factor[s][4 * group]);
+        acc.x = f.x == 0.0f ? acc.x : fmaf(f.x, v.x, acc.x);
+        acc.y = f.y == 0.0f ? acc.y : fmaf(f.y, v.y, acc.y);
+        acc.z = f.z == 0.0f ? acc.z : fmaf(f.z, v.z, acc.z);
+        acc.w = f.w == 0.0f ? acc.w : fmaf(f.w, v.w, acc.w);
+      }
+    }
+    sums[slice][t & 255] = acc;
+    __syncthreads();
+    if (t < 256 && row < j.rows) {
+      for (int k = 1; k < kSlices; ++k) {
+        const float4 v = sums[k][t];
+        acc.x += v.x;
+        acc.y += v.y;
+        acc.z += v.z;
+        acc.w += v.w;
+      }
+      __nv_bfloat16* dst = p.out + ((long long)j.first_row + row) * kLatent + d * 128 + dim;
+      const float* inv = inverse + 4 * group;
+      dst[0] = __float2bfloat16_rn(acc.x * inv[0]);
+      if (row + 1 < j.rows) dst[kLatent] = __float2bfloat16_rn(acc.y * inv[1]);
+      if (row + 2 < j.rows) dst[2 * kLatent] = __float2bfloat16_rn(acc.z * inv[2]);
+      if (row + 3 < j.rows) dst[3 * kLatent] = __float2bfloat16_rn(acc.w * inv[3]);
+    }
+    __syncthreads();
+  }
 }
 
 }  // namespace latent_detail
 
-cudaError_t launch_latent(const LatentParams& p, cudaStream_t stream) {
-  const long long items = (long long)p.total_q * p.heads;
-  latent_detail::latent_kernel<<<unsigned((items + 7) / 8), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+cudaError_t launch_latent(LatentParams p, int ctas, cudaStream_t stream) {
+  using namespace latent_detail;
+  CUtensorMap qmap, cmap;
+  {
+    const uint64_t strides[2] = {kWidth * 2, kWidth * 2};
+    const uint32_t box[3] = {64, 1, uint32_t(kKeys)};
+    const uint64_t q_dims[3] = {kWidth, 1, uint64_t(p.total_q) * uint64_t(p.heads)};
+    const uint64_t c_dims[3] = {kWidth, 1, uint64_t(p.num_blocks) * uint64_t(p.block_size)};
+    if (make_map_3d(p.q, q_dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, &qmap)) return cudaErrorInvalidValue;
+    if (make_map_3d(p.cache, c_dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, &cmap)) return cudaErrorInvalidValue;
+  }
+  static unsigned configured[kContextSlots] = {};
+  cudaError_t e = once_per_context(configured, [] {
+    return cudaFuncSetAttribute(latent_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  });
+  if (e != cudaSuccess) return e;
+  p.min_units = 4;
+  p.l2_tiles = (64 << 20) / kTileBytes;
+  // Programmatic dependents: launched while the kernel before them ends; they wait for it before any global access.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, latent_kernel, p, FastDiv::make(p.heads), FastDiv::make(p.block_size), qmap, cmap);
+  if (e != cudaSuccess || ctas == 1) return e;
+  const long long rows = (long long)p.max_q * p.heads;
+  cfg.gridDim = dim3(unsigned(ctas), unsigned(4 * (((rows < kRows ? rows : kRows) + kJoinRows - 1) / kJoinRows)));
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, latent_join_kernel, p);
 }
 
 }  // namespace nvb
 
 extern "C" {
 
-long long nvb_latent_scratch_floats(int num_sms) { return num_sms < 1 || num_sms > 1024 ? 0 : 1024LL * num_sms; }
+long long nvb_latent_scratch_floats(int num_sms) {
+  return num_sms < 1 || num_sms > nvb::latent_detail::kMaxParts ? 0 : (long long)num_sms * nvb::latent_detail::kCtaFloats;
+}
 
 int nvb_paged_latent_fwd(void* stream, const void* q, const void* cache, void* out, const int* cu_q,
                          const int* kv_lens, const int* block_table, int batch, int total_q, int max_q, int q_heads,
                          int block_size, int table_stride, int num_blocks, float scale, float* lse, float* scratch,
                          long long scratch_floats) {
   g_last_error[0] = 0;
-  if (!q || !cache || !out || !cu_q || !kv_lens || !block_table || !scratch || scratch_floats < nvb_latent_scratch_floats(1) || batch < 1 || batch > 65535 ||
-      total_q < 1 || max_q < 1 || q_heads < 1 || q_heads > 256 || block_size < 1 || table_stride < 1)
+  if (!q || !cache || !out || !cu_q || !kv_lens || !block_table || batch < 1 || batch > 65535 || total_q < 1 ||
+      max_q < 1 || q_heads < 1 || q_heads > 256 || block_size < 1 || table_stride < 1)
     return fail("invalid latent attention arguments");
+  if (!scratch || scratch_floats < nvb_latent_scratch_floats(1))
+    return fail("scratch must hold nvb_latent_scratch_floats(1) elements at least");
   if (block_size % 64) return fail("block_size must be a multiple of 64 (got %d)", block_size);
   if ((long long)block_size * table_stride > INT_MAX || (long long)total_q * q_heads > INT_MAX)
     return fail("block_size * table_stride and total_q * q_heads must fit in int32");
@@ -80,6 +778,9 @@ int nvb_paged_latent_fwd(void* stream, const void* q, const void* cache, void* o
   if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(kv_lens) |
        reinterpret_cast<uintptr_t>(block_table) | reinterpret_cast<uintptr_t>(lse)) & 3)
     return fail("cu_q, kv_lens, block_table and lse must be 4-byte aligned");
+  const int sms = nvb::sm_count();
+  if (sms < 1) return fail("the current device has no SM count");
+  const long long fit = scratch_floats / nvb_latent_scratch_floats(1);
   nvb::LatentParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.cache = static_cast<const __nv_bfloat16*>(cache);
@@ -97,7 +798,8 @@ int nvb_paged_latent_fwd(void* stream, const void* q, const void* cache, void* o
   p.table_stride = table_stride;
   p.num_blocks = num_blocks;
   p.scale = scale;
-  return cuda_status(nvb::launch_latent(p, static_cast<cudaStream_t>(stream)), "latent attention launch");
+  return cuda_status(nvb::launch_latent(p, int(fit < sms ? fit : sms), static_cast<cudaStream_t>(stream)),
+                     "latent attention launch");
 }
 
 }  // extern "C"
