@@ -49,8 +49,10 @@ constexpr int kOCol = 128;                      // S at 0 and 64, O^T at 128 + 6
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kRescaleLog2 = 8.0f;            // the maximum in use moves when it grew by 2^8 (P <= 2^8)
 
-enum Bar { kFull = 0, kEmpty = kFull + 2 * kUnits, kSFull = kEmpty + 2 * kUnits, kPFull = kSFull + 2, kPVDone, kQFree,
-           kOFree, kDrain, kNumBars };
+// kSFull, kSFree: one per S buffer. The rows may be a tile ahead of the S issuer's look at kSFree, so the arrivals of two
+// tiles in a row must not meet in one barrier.
+enum Bar { kFull = 0, kEmpty = kFull + 2 * kUnits, kSFull = kEmpty + 2 * kUnits, kSFree = kSFull + 2, kPFull = kSFree + 2, kPVDone,
+           kQFree, kOFree, kSDrain, kPVDrain, kNumBars };
 constexpr int kTmemSlotOff = kNumBars * 8;
 constexpr int kPlanOff = (kTmemSlotOff + 4 + 15) & ~15;   // Plan
 constexpr int kScanOff = kPlanOff + 64;                   // long long [8] and int [8] of the warps' sums
@@ -79,6 +81,15 @@ constexpr uint32_t kIdescPV = kIdesc | ((128u >> 4) << 24) | (1u << 15);  // A M
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, kErrLatentWait); }
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, wait(bar, parity));
+}
+
+// One thread of the warp, which the compiler knows to be one: the operands of its TMA and MMA instructions then stay in
+// uniform registers. Under `lane == 0` every instruction moves them there again: an MMA takes 45 to 130 cycles to issue,
+// 32 (M = N = 64) to 48 (M = 128, N = 64) this way, which is what it takes to read its operands.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 // 16 lanes x 64 columns: thread t has rows t / 4 (r[4 i], r[4 i + 1]) and t / 4 + 8 (r[4 i + 2], r[4 i + 3]) at
@@ -287,11 +298,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&bars[kSFull], 1);
     mbar_init(&bars[kSFull + 1], 1);
+    mbar_init(&bars[kSFree], 4);
+    mbar_init(&bars[kSFree + 1], 4);
     mbar_init(&bars[kPFull], 4);
     mbar_init(&bars[kPVDone], 1);
     mbar_init(&bars[kQFree], 1);
     mbar_init(&bars[kOFree], 4);
-    mbar_init(&bars[kDrain], 1);
+    mbar_init(&bars[kSDrain], 1);
+    mbar_init(&bars[kPVDrain], 1);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -318,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!aligned) {
   } else if (warp == 0) {
     // ---------------------------------------------------------- producer
-    if (lane == 0) {
+    if (elect_one()) {
       tma_prefetch_desc(&qmap);
       tma_prefetch_desc(&cmap);
       int g = 0, seg = 0;
@@ -364,48 +378,62 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!wait(&bars[kFull + (i & 1) * kUnits + u], (i >> 1) & 1)) break;
     }
   } else if (warp == 1) {
-    // -------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      const uint64_t qd = sw128_desc(sbase + kQOff, 16, 1024), kd = sw128_desc(sbase + kRingOff, 16, 1024),
-                     vd = sw128_desc(sbase + kRingOff + kChunk, kChunk, 1024),
-                     pd = sw128_desc(sbase + kPOff, 16, 1024);
-      const uint32_t q_lo = uint32_t(qd), q_hi = uint32_t(qd >> 32), k_lo = uint32_t(kd), k_hi = uint32_t(kd >> 32),
-                     v_lo = uint32_t(vd), v_hi = uint32_t(vd >> 32), p_lo = uint32_t(pd), p_hi = uint32_t(pd >> 32);
-      // S of tile g, as its pieces land
-      auto issue_s = [&](int g, bool last) {
-        const int stage = g & 1;
-        const uint32_t kb = k_lo + uint32_t(stage * (kTileBytes >> 4));
-        for (int u = 0; u < kUnits; ++u) {
-          if (!wait(&bars[kFull + stage * kUnits + u], (g >> 1) & 1)) return false;
-          tc_fence_after();
-          for (int c = u == 0 ? 0 : 2 * u - 1; c <= 2 * u; ++c)
+    // ------------------------------------------------------ S MMA issuer
+    if (elect_one()) {
+      const uint64_t qd = sw128_desc(sbase + kQOff, 16, 1024), kd = sw128_desc(sbase + kRingOff, 16, 1024);
+      const uint32_t q_lo = uint32_t(qd), q_hi = uint32_t(qd >> 32), k_lo = uint32_t(kd), k_hi = uint32_t(kd >> 32);
+      int g = 0;
+      bool alive = true;
+      while (alive && walk.next(p, plan, member, s)) {
+        for (int t = s.t0; t < s.t1 && alive; ++t, ++g) {
+          const int stage = g & 1;
+          const uint32_t kb = k_lo + uint32_t(stage * (kTileBytes >> 4)), sd = tmem + stage * kKeys;
+          // the scores of the tile before the last have been read
+          if (g >= 2) alive = wait(&bars[kSFree + stage], ((g >> 1) + 1) & 1);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              const uint32_t off = uint32_t(c * kChunk + kk * 32) >> 4;
-              umma_ss(tmem + stage * kKeys, q_lo + off, q_hi, kb + off, k_hi, kIdescS, (c | kk) ? 1u : 0u);
-            }
+          for (int u = 0; u < kUnits; ++u) {  // as the pieces land
+            alive = alive && wait(&bars[kFull + stage * kUnits + u], (g >> 1) & 1);
+            if (!alive) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = u == 0 ? 0 : 2 * u - 1; c <= 2 * u; ++c)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) {
+                const uint32_t off = uint32_t(c * kChunk + kk * 32) >> 4;
+                umma_ss(sd, q_lo + off, q_hi, kb + off, k_hi, kIdescS, (c | kk) ? 1u : 0u);
+              }
+          }
+          if (!alive) break;
+          umma_commit(&bars[kSFull + stage]);
+          umma_commit(&bars[kEmpty + stage * kUnits]);
+          if (t + 1 == s.t1) umma_commit(&bars[kQFree]);
         }
-        umma_commit(&bars[kSFull + stage]);
-        umma_commit(&bars[kEmpty + stage * kUnits]);
-        if (last) umma_commit(&bars[kQFree]);
-        return true;
-      };
+      }
+      // every MMA of this thread completes before TMEM is freed
+      umma_commit(&bars[kSDrain]);
+      wait(&bars[kSDrain], 0);
+    }
+  } else if (warp == 2) {
+    // ----------------------------------------------------- PV MMA issuer
+    // A thread of its own: S of the next tile runs beside the rows' work on this one, but a tile that has not landed yet
+    // does not hold up the product that frees the place for the one after it.
+    if (elect_one()) {
+      const uint64_t vd = sw128_desc(sbase + kRingOff + kChunk, kChunk, 1024), pd = sw128_desc(sbase + kPOff, 16, 1024);
+      const uint32_t v_lo = uint32_t(vd), v_hi = uint32_t(vd >> 32), p_lo = uint32_t(pd), p_hi = uint32_t(pd >> 32);
       int g = 0, seg = 0;
       bool alive = true;
       while (alive && walk.next(p, plan, member, s)) {
         if (s.t0 == s.t1) continue;
         const uint32_t idesc = kIdescPV | (uint32_t((s.rows + 15) / 16 * 2) << 17);
+        // the output of the segment before this one has been read
+        if (seg > 0) alive = wait(&bars[kOFree], (seg - 1) & 1);
         for (int t = s.t0; t < s.t1 && alive; ++t, ++g) {
-          if (t == s.t0) alive = issue_s(g, t + 1 == s.t1);
-          // S of the next tile beside the rows' work on this one. Its buffer's scores have been read: the P that was
-          // made of them has been waited for.
-          if (alive && t + 1 < s.t1) alive = issue_s(g + 1, t + 2 == s.t1);
-          if (alive && t == s.t0 && seg > 0) alive = wait(&bars[kOFree], (seg - 1) & 1);
-          if (alive) alive = wait(&bars[kPFull], g & 1);
+          alive = wait(&bars[kPFull], g & 1);
           if (!alive) break;
           tc_fence_after();
           const int stage = g & 1;
           const uint32_t vb = v_lo + uint32_t(stage * (kTileBytes >> 4));
+#pragma unroll
           for (int d = 0; d < 4; ++d) {  // 128 dims: two pieces
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)  // 16 keys: 2048 bytes of a piece's rows, 32 bytes of P's
@@ -417,9 +445,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++seg;
       }
-      // every MMA completes before TMEM is freed
-      umma_commit(&bars[kDrain]);
-      wait(&bars[kDrain], 0);
+      umma_commit(&bars[kPVDrain]);
+      wait(&bars[kPVDrain], 0);
     }
   } else if (warp >= 4) {
     // ------------------------------------------- softmax, then the output
@@ -460,6 +487,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld_rows(lane_base + (g & 1) * kKeys, raw);
         tmem_ld_wait();
         reg_fence(raw);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[kSFree + (g & 1)]);
         float x[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(raw[i]);
@@ -627,83 +657,133 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of cut rows: CTA x looks at what CTA x of the first kernel
-// left to join, y takes 128 dims and eight rows. Sum over the parts s of
-// 2^(m_s - max) O_s over the same sum of their row sums, in the order of the
-// parts within each half of them, then of the halves.
-constexpr int kJoinThreads = 512, kJoinRows = 8;
-constexpr int kSlices = kJoinThreads / 256;  // 128 dims x 2 groups of four rows
-constexpr int kMaxParts = 512;               // CTAs
+// Joins the parts of cut rows: sum over the parts s of 2^(m_s - max) O_s over
+// the same sum of their row sums, in an order that goes by the parts alone.
+// Every CTA reads what the first kernel's CTAs left to join and takes its share
+// of the pieces: four rows of 512 dims of few parts, 128 threads for each 128
+// dims; or, of many parts, four rows of 128 dims, whose parts the four groups
+// of 128 threads share out. A warp a row works out the parts' factors while the
+// first values are on their way. What bounds it is round trips to L2.
+constexpr int kJoinThreads = 512, kJoinGroups = kJoinThreads / 128;
+constexpr int kJoinBatch = 4;  // values in flight a thread
+constexpr int kFewParts = 8;
+constexpr int kMaxCtas = 512;
 
-__global__ void __launch_bounds__(kJoinThreads) latent_join_kernel(const LatentParams p) {
-  __shared__ float factor[kMaxParts][kJoinRows];
-  __shared__ float4 sums[kSlices][256];
-  __shared__ float inverse[kJoinRows];
+__global__ void __launch_bounds__(kJoinThreads, 3) latent_join_kernel(const LatentParams p, const int ctas) {
+  __shared__ Join items[kMaxCtas];
+  __shared__ int ends[kMaxCtas];  // pieces up to and with an item's
+  __shared__ int warp_ends[kJoinThreads / 32];
+  __shared__ float4 factor[kMaxCtas];
+  __shared__ float4 sums[kJoinGroups - 1][128];
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, group = t >> 7, dim = t & 127;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const float* const scratch = p.scratch + (long long)blockIdx.x * kCtaFloats;
-  const Join j = *reinterpret_cast<const Join*>(scratch + 2 * kPartFloats);
-  const int d = blockIdx.y & 3, t = threadIdx.x;
-  const long long step = (long long)j.stride * kCtaFloats;
-  auto at = [&](int s) { return scratch + s * step + (s == 0 ? kPartFloats : 0); };
-  for (int r0 = (blockIdx.y >> 2) * kJoinRows; r0 < j.rows; r0 += (gridDim.y >> 2) * kJoinRows) {
-    const int warp = t >> 5, lane = t & 31;
-    if (warp < kJoinRows) {  // a warp a row: maximum, factors, sum
-      const int row = r0 + warp;
-      float mx = -INFINITY;
+  {
+    static_assert(kMaxCtas <= kJoinThreads, "a thread an item");
+    Join j{0, 0, 0, 0};
+    if (t < ctas) j = *reinterpret_cast<const Join*>(p.scratch + (long long)t * kCtaFloats + 2 * kPartFloats);
+    if (t < ctas) items[t] = j;
+    int upto = (j.rows + 3) / 4 * (j.parts > kFewParts ? 4 : 1);
+#pragma unroll
+    for (int off = 1; off < 32; off *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += o;
+    }
+    if (lane == 31) warp_ends[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) upto += warp_ends[w];
+    if (t < ctas) ends[t] = upto;
+    __syncthreads();
+  }
+  for (int piece = blockIdx.x; piece < ends[ctas - 1]; piece += gridDim.x) {
+    int lo = 0, hi = ctas - 1;  // the first item that ends behind the piece
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (ends[mid] > piece) hi = mid;
+      else lo = mid + 1;
+    }
+    const Join j = items[lo];
+    const int within = piece - (lo ? ends[lo - 1] : 0);
+    const bool few = j.parts <= kFewParts;
+    const int row = (few ? within : within >> 2) * 4, d = few ? group : within & 3;
+    const float* const scratch = p.scratch + (long long)lo * kCtaFloats;
+    const long long step = (long long)j.stride * kCtaFloats;
+    auto part = [&](int s) { return scratch + s * step + (s == 0 ? kPartFloats : 0); };
+    const int place = ((d * 16 + row / 4) * 128 + dim) * 4;
+    const int every = few ? 1 : kJoinGroups;
+    float4 v[kJoinBatch];
+    auto load = [&](int s0) {
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        const int s = s0 + k * every;
+        v[k] = s < j.parts ? *reinterpret_cast<const float4*>(part(s) + place) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    };
+    int s0 = few ? 0 : group;
+    load(s0);
+    if (warp < 4) {
+      float mx = -INFINITY, total = 0.0f;
       for (int s = lane; s < j.parts; s += 32) {
-        const float2 v = reinterpret_cast<const float2*>(at(s) + kRows * kLatent)[row];
-        if (v.y != 0.0f) mx = fmaxf(mx, v.x);  // a part without a seen key has no maximum
+        const float2 ml = reinterpret_cast<const float2*>(part(s) + kRows * kLatent)[row + warp];
+        if (ml.y != 0.0f) mx = fmaxf(mx, ml.x);  // a part that saw no key has no maximum
       }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      float total = 0.0f;
       for (int s = lane; s < j.parts; s += 32) {
-        const float2 v = reinterpret_cast<const float2*>(at(s) + kRows * kLatent)[row];
-        // one whose scores are all NaN has no maximum either, its sum is NaN
-        const float f = v.y == 0.0f ? 0.0f : (v.x == -INFINITY ? NAN : fast_exp2(v.x - mx));
-        factor[s][warp] = f;
-        total += f * v.y;
+        const float2 ml = reinterpret_cast<const float2*>(part(s) + kRows * kLatent)[row + warp];
+        // one whose scores are all NaN has none either, its sum is NaN
+        const float f = ml.y == 0.0f ? 0.0f : (ml.x == -INFINITY ? NAN : fast_exp2(ml.x - mx));
+        reinterpret_cast<float*>(factor + s)[warp] = f;
+        total += f == 0.0f ? 0.0f : f * ml.y;
       }
       total = warp_sum(total);
-      if (lane == 0) {
-        inverse[warp] = total == 0.0f ? 0.0f : 1.0f / total;
-        if (d == 0 && p.lse && row < j.rows)
-          p.lse[j.first_row + row] = total == 0.0f ? -INFINITY : (mx + fast_log2(total)) * kLn2;
+      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+      for (int s = lane; s < j.parts; s += 32) {
+        float& f = reinterpret_cast<float*>(factor + s)[warp];
+        f = f == 0.0f ? 0.0f : f * inv;
       }
+      if (lane == 0 && p.lse && row + warp < j.rows && (few || d == 0))
+        p.lse[j.first_row + row + warp] = total == 0.0f ? -INFINITY : (mx + fast_log2(total)) * kLn2;
     }
     __syncthreads();
-    const int slice = t >> 8, group = (t >> 7) & 1, dim = t & 127;
-    const int each = (j.parts + kSlices - 1) / kSlices, s1 = min(j.parts, (slice + 1) * each);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int row = r0 + 4 * group;
-    if (row < j.rows) {
-      const int place = ((d * 16 + row / 4) * 128 + dim) * 4;
-#pragma unroll 8
-      for (int s = slice * each; s < s1; ++s) {
-        const float4 v = *reinterpret_cast<const float4*>(at(s) + place);
-        const float4 f = *reinterpret_cast<const float4*>(&factor[s][4 * group]);
-        acc.x = f.x == 0.0f ? acc.x : fmaf(f.x, v.x, acc.x);
-        acc.y = f.y == 0.0f ? acc.y : fmaf(f.y, v.y, acc.y);
-        acc.z = f.z == 0.0f ? acc.z : fmaf(f.z, v.z, acc.z);
-        acc.w = f.w == 0.0f ? acc.w : fmaf(f.w, v.w, acc.w);
+    for (;;) {
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        const int s = s0 + k * every;
+        if (s >= j.parts) break;
+        const float4 f = factor[s];
+        // a part without a seen key may hold anything
+        acc.x = f.x == 0.0f ? acc.x : fmaf(f.x, v[k].x, acc.x);
+        acc.y = f.y == 0.0f ? acc.y : fmaf(f.y, v[k].y, acc.y);
+        acc.z = f.z == 0.0f ? acc.z : fmaf(f.z, v[k].z, acc.z);
+        acc.w = f.w == 0.0f ? acc.w : fmaf(f.w, v[k].w, acc.w);
       }
+      s0 += kJoinBatch * every;
+      if (s0 >= j.parts) break;
+      load(s0);
     }
-    sums[slice][t & 255] = acc;
-    __syncthreads();
-    if (t < 256 && row < j.rows) {
-      for (int k = 1; k < kSlices; ++k) {
-        const float4 v = sums[k][t];
-        acc.x += v.x;
-        acc.y += v.y;
-        acc.z += v.z;
-        acc.w += v.w;
+    if (!few) {
+      if (group > 0) sums[group - 1][dim] = acc;
+      __syncthreads();
+      if (group == 0)
+#pragma unroll
+        for (int k = 0; k < kJoinGroups - 1; ++k) {
+          const float4 o = sums[k][dim];
+          acc.x += o.x;
+          acc.y += o.y;
+          acc.z += o.z;
+          acc.w += o.w;
+        }
+    }
+    if (few || group == 0) {
+      const float a[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float other = __shfl_xor_sync(0xffffffffu, a[i], 1);  // two dims of a row a store
+        if (!(dim & 1) && row + i < j.rows)
+          *reinterpret_cast<uint32_t*>(p.out + ((long long)j.first_row + row + i) * kLatent + d * 128 + dim) =
+              pack_bf16x2(a[i], other);
       }
-      __nv_bfloat16* dst = p.out + ((long long)j.first_row + row) * kLatent + d * 128 + dim;
-      const float* inv = inverse + 4 * group;
-      dst[0] = __float2bfloat16_rn(acc.x * inv[0]);
-      if (row + 1 < j.rows) dst[kLatent] = __float2bfloat16_rn(acc.y * inv[1]);
-      if (row + 2 < j.rows) dst[2 * kLatent] = __float2bfloat16_rn(acc.z * inv[2]);
-      if (row + 3 < j.rows) dst[3 * kLatent] = __float2bfloat16_rn(acc.w * inv[3]);
     }
     __syncthreads();
   }
@@ -742,11 +822,10 @@ cudaError_t launch_latent(LatentParams p, int ctas, cudaStream_t stream) {
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, latent_kernel, p, FastDiv::make(p.heads), FastDiv::make(p.block_size), qmap, cmap);
   if (e != cudaSuccess || ctas == 1) return e;
-  const long long rows = (long long)p.max_q * p.heads;
-  cfg.gridDim = dim3(unsigned(ctas), unsigned(4 * (((rows < kRows ? rows : kRows) + kJoinRows - 1) / kJoinRows)));
+  cfg.gridDim = dim3(unsigned(3 * ctas));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, latent_join_kernel, p);
+  return cudaLaunchKernelEx(&cfg, latent_join_kernel, p, ctas);
 }
 
 }  // namespace nvb
@@ -754,7 +833,7 @@ cudaError_t launch_latent(LatentParams p, int ctas, cudaStream_t stream) {
 extern "C" {
 
 long long nvb_latent_scratch_floats(int num_sms) {
-  return num_sms < 1 || num_sms > nvb::latent_detail::kMaxParts ? 0 : (long long)num_sms * nvb::latent_detail::kCtaFloats;
+  return num_sms < 1 || num_sms > nvb::latent_detail::kMaxCtas ? 0 : (long long)num_sms * nvb::latent_detail::kCtaFloats;
 }
 
 int nvb_paged_latent_fwd(void* stream, const void* q, const void* cache, void* out, const int* cu_q,
