@@ -92,6 +92,18 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+// One arrival, and `bytes` to land; shared-memory addresses.
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void load_piece(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int row) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(0), "r"(row)
+      : "memory");
+}
+
 // 16 lanes x 64 columns: thread t has rows t / 4 (r[4 i], r[4 i + 1]) and t / 4 + 8 (r[4 i + 2], r[4 i + 3]) at
 // columns 8 i + 2 (t % 4) and the next.
 __device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[32]) {
@@ -348,23 +360,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int key0 = t * kKeys, logical = fd_bs.div(key0), stage = g & 1;
           const bool ok = page_ok(page, p.num_blocks), with_q = t == s.t0;
           const int row = ok ? page * p.block_size + (key0 - logical * p.block_size) : 0;
-          unsigned char* tile = smem + kRingOff + stage * kTileBytes;
+          const uint32_t tile = sbase + kRingOff + stage * kTileBytes, full0 = sbase + (kFull + stage * kUnits) * 8;
+#pragma unroll
           for (int u = 0; u < kUnits; ++u) {
-            uint64_t* full = &bars[kFull + stage * kUnits + u];
-            if (g >= 2 && !wait(&bars[kEmpty + stage * kUnits + u], ((g >> 1) + 1) & 1)) {
-              alive = false;
-              break;
+            if (g >= 2) alive = alive && wait(&bars[kEmpty + stage * kUnits + u], ((g >> 1) + 1) & 1);
+            if (!alive) break;
+            constexpr int kPieces[kUnits] = {1, 2, 2, 2, 2};
+            const int c0 = u == 0 ? 0 : 2 * u - 1;
+            const uint32_t full = full0 + u * 8;
+            expect(full, uint32_t(kPieces[u]) * kChunk * ((ok ? 1 : 0) + (with_q ? 1 : 0)));
+            if (with_q) {
+#pragma unroll
+              for (int c = c0; c < c0 + kPieces[u]; ++c)
+                load_piece(sbase + kQOff + c * kChunk, &qmap, full, c == 0 ? kLatent : (c - 1) * 64, q_row);
             }
-            const int c0 = u == 0 ? 0 : 2 * u - 1, c1 = 2 * u;  // pieces of the unit
-            const uint32_t bytes = uint32_t(c1 - c0 + 1) * kChunk * ((ok ? 1 : 0) + (with_q ? 1 : 0));
-            if (bytes) mbar_arrive_expect_tx(full, bytes);
-            else mbar_arrive(full);  // a bad page's keys are masked, whatever the tile holds
-            for (int c = c0; c <= c1; ++c) {
-              const int x = c == 0 ? kLatent : (c - 1) * 64;
-              if (with_q) tma_load_3d(smem + kQOff + c * kChunk, &qmap, full, x, 0, q_row);
-              if (ok) tma_load_3d(tile + c * kChunk, &cmap, full, x, 0, row);
+            if (ok) {  // a bad page's keys are masked, whatever the tile holds
+#pragma unroll
+              for (int c = c0; c < c0 + kPieces[u]; ++c)
+                load_piece(tile + c * kChunk, &cmap, full, c == 0 ? kLatent : (c - 1) * 64, row);
             }
           }
+          if (!alive) break;
           if (t + 1 < s.t1) {
             const int next = fd_bs.div(key0 + kKeys);
             if (next != logical) page = table[next];
