@@ -571,7 +571,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (rescale) {
           named_barrier(2, 128);  // the factors are there
           tc_fence_after();
+#pragma unroll 1
           for (int d = 0; d < 4; ++d)
+#pragma unroll 1
             for (int c = 0; c < s.rows; c += 16) {
               uint32_t o[16];
               tmem_ld16(lane_base + kOCol + 64 * d + c, o);
@@ -627,7 +629,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       alive = alive && wait_warp(&bars[kPVDone], (g - 1) & 1);
       tc_fence_after();
       const int dim = quad * 32 + lane;
+      // Loops kept as loops: a segment runs them once, and straight code would be fetched for it.
+#pragma unroll 1
       for (int d = 0; d < 4; ++d)
+#pragma unroll 1
         for (int c = 0; c < s.rows; c += 16) {
           uint32_t o[16];
           tmem_ld16(lane_base + kOCol + 64 * d + c, o);
@@ -676,29 +681,31 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the parts of cut rows: sum over the parts s of 2^(m_s - max) O_s over
 // the same sum of their row sums, in an order that goes by the parts alone.
 // Every CTA reads what the first kernel's CTAs left to join and takes its share
-// of the pieces: four rows of 512 dims of few parts, 128 threads for each 128
-// dims; or, of many parts, four rows of 128 dims, whose parts the four groups
-// of 128 threads share out. A warp a row works out the parts' factors while the
-// first values are on their way. What bounds it is round trips to L2.
-constexpr int kJoinThreads = 512, kJoinGroups = kJoinThreads / 128;
-constexpr int kJoinBatch = 4;  // values in flight a thread
-constexpr int kFewParts = 8;
+// of the pieces. Of few parts a piece is 16 rows: a thread has one dim of them
+// all. Of many it is four rows of 32 dims, and sixteen groups of 32 threads
+// share the parts out. A warp a row works out the parts' factors while the first
+// values are on their way. What bounds it is round trips to L2, so a piece has
+// as many values in flight as the registers hold.
+constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32;
+constexpr int kFewParts = 16, kFewRows = 16, kManyDims = 32;
 constexpr int kMaxCtas = 512;
+static_assert(kFewRows == kJoinWarps && kFewParts * kFewRows <= 4 * kMaxCtas, "factors: a warp a row");
 
-__global__ void __launch_bounds__(kJoinThreads, 3) latent_join_kernel(const LatentParams p, const int ctas) {
+__global__ void __launch_bounds__(kJoinThreads, 2) latent_join_kernel(const LatentParams p, const int ctas) {
   __shared__ Join items[kMaxCtas];
   __shared__ int ends[kMaxCtas];  // pieces up to and with an item's
-  __shared__ int warp_ends[kJoinThreads / 32];
-  __shared__ float4 factor[kMaxCtas];
-  __shared__ float4 sums[kJoinGroups - 1][128];
-  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, group = t >> 7, dim = t & 127;
+  __shared__ int warp_ends[kJoinWarps];
+  __shared__ float4 factor4[kMaxCtas];  // [part][row of the piece], 16 or 4 rows
+  __shared__ float4 sums[kJoinWarps][kManyDims];
+  float* const factor = reinterpret_cast<float*>(factor4);
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   {
     static_assert(kMaxCtas <= kJoinThreads, "a thread an item");
     Join j{0, 0, 0, 0};
     if (t < ctas) j = *reinterpret_cast<const Join*>(p.scratch + (long long)t * kCtaFloats + 2 * kPartFloats);
     if (t < ctas) items[t] = j;
-    int upto = (j.rows + 3) / 4 * (j.parts > kFewParts ? 4 : 1);
+    int upto = j.parts > kFewParts ? (j.rows + 3) / 4 * (kLatent / kManyDims) : (j.rows + kFewRows - 1) / kFewRows;
 #pragma unroll
     for (int off = 1; off < 32; off *= 2) {
       const int o = __shfl_up_sync(0xffffffffu, upto, off);
@@ -720,85 +727,117 @@ __global__ void __launch_bounds__(kJoinThreads, 3) latent_join_kernel(const Late
     const Join j = items[lo];
     const int within = piece - (lo ? ends[lo - 1] : 0);
     const bool few = j.parts <= kFewParts;
-    const int row = (few ? within : within >> 2) * 4, d = few ? group : within & 3;
+    const int row0 = few ? within * kFewRows : within / (kLatent / kManyDims) * 4;
     const float* const scratch = p.scratch + (long long)lo * kCtaFloats;
     const long long step = (long long)j.stride * kCtaFloats;
     auto part = [&](int s) { return scratch + s * step + (s == 0 ? kPartFloats : 0); };
-    const int place = ((d * 16 + row / 4) * 128 + dim) * 4;
-    const int every = few ? 1 : kJoinGroups;
-    float4 v[kJoinBatch];
-    auto load = [&](int s0) {
-#pragma unroll
-      for (int k = 0; k < kJoinBatch; ++k) {
-        const int s = s0 + k * every;
-        v[k] = s < j.parts ? *reinterpret_cast<const float4*>(part(s) + place) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-    };
-    int s0 = few ? 0 : group;
-    load(s0);
-    if (warp < 4) {
-      float mx = -INFINITY, total = 0.0f;
-      for (int s = lane; s < j.parts; s += 32) {
-        const float2 ml = reinterpret_cast<const float2*>(part(s) + kRows * kLatent)[row + warp];
-        if (ml.y != 0.0f) mx = fmaxf(mx, ml.x);  // a part that saw no key has no maximum
+    auto factors = [&](int rows) {  // of `rows` rows, a warp each
+      if (warp >= rows) return;
+      auto stats = [&](int s) { return reinterpret_cast<const float2*>(part(s) + kRows * kLatent)[row0 + warp]; };
+      const float2 own = lane < j.parts ? stats(lane) : make_float2(0.f, 0.f);
+      float mx = own.y != 0.0f ? own.x : -INFINITY, total = 0.0f;  // a part that saw no key has no maximum
+      for (int s = lane + 32; s < j.parts; s += 32) {
+        const float2 ml = stats(s);
+        if (ml.y != 0.0f) mx = fmaxf(mx, ml.x);
       }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
       for (int s = lane; s < j.parts; s += 32) {
-        const float2 ml = reinterpret_cast<const float2*>(part(s) + kRows * kLatent)[row + warp];
+        const float2 ml = s == lane ? own : stats(s);
         // one whose scores are all NaN has none either, its sum is NaN
         const float f = ml.y == 0.0f ? 0.0f : (ml.x == -INFINITY ? NAN : fast_exp2(ml.x - mx));
-        reinterpret_cast<float*>(factor + s)[warp] = f;
+        factor[s * rows + warp] = f;
         total += f == 0.0f ? 0.0f : f * ml.y;
       }
       total = warp_sum(total);
       const float inv = total == 0.0f ? 0.0f : 1.0f / total;
       for (int s = lane; s < j.parts; s += 32) {
-        float& f = reinterpret_cast<float*>(factor + s)[warp];
+        float& f = factor[s * rows + warp];
         f = f == 0.0f ? 0.0f : f * inv;
       }
-      if (lane == 0 && p.lse && row + warp < j.rows && (few || d == 0))
-        p.lse[j.first_row + row + warp] = total == 0.0f ? -INFINITY : (mx + fast_log2(total)) * kLn2;
-    }
-    __syncthreads();
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (;;) {
+      if (lane == 0 && p.lse && row0 + warp < j.rows && (few || within % (kLatent / kManyDims) == 0))
+        p.lse[j.first_row + row0 + warp] = total == 0.0f ? -INFINITY : (mx + fast_log2(total)) * kLn2;
+    };
+    // a part without a seen key may hold anything
+    auto add = [](float4& a, const float4& f, const float4& v) {
+      a.x = f.x == 0.0f ? a.x : fmaf(f.x, v.x, a.x);
+      a.y = f.y == 0.0f ? a.y : fmaf(f.y, v.y, a.y);
+      a.z = f.z == 0.0f ? a.z : fmaf(f.z, v.z, a.z);
+      a.w = f.w == 0.0f ? a.w : fmaf(f.w, v.w, a.w);
+    };
+    if (few) {
+      const int d = t >> 7, dim = t & 127;
+      constexpr int kQuads = kFewRows / 4, kBatch = 2;
+      const int place = ((d * 16 + row0 / 4) * 128 + dim) * 4;
+      float4 acc[kQuads], v[kBatch][kQuads];
+      auto load = [&](int s0) {
 #pragma unroll
-      for (int k = 0; k < kJoinBatch; ++k) {
-        const int s = s0 + k * every;
-        if (s >= j.parts) break;
-        const float4 f = factor[s];
-        // a part without a seen key may hold anything
-        acc.x = f.x == 0.0f ? acc.x : fmaf(f.x, v[k].x, acc.x);
-        acc.y = f.y == 0.0f ? acc.y : fmaf(f.y, v[k].y, acc.y);
-        acc.z = f.z == 0.0f ? acc.z : fmaf(f.z, v[k].z, acc.z);
-        acc.w = f.w == 0.0f ? acc.w : fmaf(f.w, v[k].w, acc.w);
-      }
-      s0 += kJoinBatch * every;
-      if (s0 >= j.parts) break;
-      load(s0);
-    }
-    if (!few) {
-      if (group > 0) sums[group - 1][dim] = acc;
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+          for (int r = 0; r < kQuads; ++r)
+            v[k][r] = s0 + k < j.parts && row0 + 4 * r < j.rows
+                          ? *reinterpret_cast<const float4*>(part(s0 + k) + place + r * 512)
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      load(0);
+      factors(kFewRows);
       __syncthreads();
-      if (group == 0)
 #pragma unroll
-        for (int k = 0; k < kJoinGroups - 1; ++k) {
-          const float4 o = sums[k][dim];
-          acc.x += o.x;
-          acc.y += o.y;
-          acc.z += o.z;
-          acc.w += o.w;
+      for (int r = 0; r < kQuads; ++r) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s0 = 0; s0 < j.parts; s0 += kBatch) {
+        if (s0) load(s0);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (s0 + k < j.parts)
+#pragma unroll
+            for (int r = 0; r < kQuads; ++r) add(acc[r], factor4[(s0 + k) * kQuads + r], v[k][r]);
+      }
+#pragma unroll
+      for (int r = 0; r < kQuads; ++r) {
+        const float a[4] = {acc[r].x, acc[r].y, acc[r].z, acc[r].w};
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          // two rows of this dim; of the neighbour's the other one, so that a store has two dims of a row
+          const bool odd = dim & 1;
+          const float other = __shfl_xor_sync(0xffffffffu, odd ? a[i] : a[i + 1], 1);
+          const int row = row0 + 4 * r + i + (odd ? 1 : 0);
+          if (row < j.rows)
+            *reinterpret_cast<uint32_t*>(p.out + ((long long)j.first_row + row) * kLatent + d * 128 + (dim & ~1)) =
+                odd ? pack_bf16x2(other, a[i + 1]) : pack_bf16x2(a[i], other);
         }
-    }
-    if (few || group == 0) {
-      const float a[4] = {acc.x, acc.y, acc.z, acc.w};
+      }
+    } else {
+      const int dim0 = within % (kLatent / kManyDims) * kManyDims;  // of the 512
+      const int place = (((dim0 >> 7) * 16 + row0 / 4) * 128 + (dim0 & 127) + lane) * 4;
+      constexpr int kBatch = 8;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f), v[kBatch];
+      auto load = [&](int s0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float other = __shfl_xor_sync(0xffffffffu, a[i], 1);  // two dims of a row a store
-        if (!(dim & 1) && row + i < j.rows)
-          *reinterpret_cast<uint32_t*>(p.out + ((long long)j.first_row + row + i) * kLatent + d * 128 + dim) =
-              pack_bf16x2(a[i], other);
+        for (int k = 0; k < kBatch; ++k) {
+          const int s = s0 + k * kJoinWarps;
+          v[k] = s < j.parts ? *reinterpret_cast<const float4*>(part(s) + place) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      };
+      load(warp);
+      factors(4);
+      __syncthreads();
+      for (int s0 = warp; s0 < j.parts; s0 += kBatch * kJoinWarps) {
+        if (s0 != warp) load(s0);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (s0 + k * kJoinWarps < j.parts) add(acc, factor4[s0 + k * kJoinWarps], v[k]);
+      }
+      sums[warp][lane] = acc;
+      __syncthreads();
+      if (t < 4 * kManyDims) {  // a row of a dim each
+        const int row = t >> 5;
+        float a = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) a += reinterpret_cast<const float*>(&sums[w][lane])[row];
+        const float other = __shfl_xor_sync(0xffffffffu, a, 1);
+        if (!(lane & 1) && row0 + row < j.rows)
+          *reinterpret_cast<uint32_t*>(p.out + ((long long)j.first_row + row0 + row) * kLatent + dim0 + lane) =
+              pack_bf16x2(a, other);
       }
     }
     __syncthreads();
@@ -838,7 +877,7 @@ cudaError_t launch_latent(LatentParams p, int ctas, cudaStream_t stream) {
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, latent_kernel, p, FastDiv::make(p.heads), FastDiv::make(p.block_size), qmap, cmap);
   if (e != cudaSuccess || ctas == 1) return e;
-  cfg.gridDim = dim3(unsigned(3 * ctas));
+  cfg.gridDim = dim3(unsigned(2 * ctas));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, latent_join_kernel, p, ctas);
