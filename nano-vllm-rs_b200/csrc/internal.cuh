@@ -164,9 +164,10 @@ struct LatentPrefillParams {
   float* lse;                   // [total_q, heads] or null
   long long rope_stride;
   int batch, total_q, total_k, max_q, heads;
+  int item_rows;                // set by launch_latent_prefill: queries of a work item
   float scale;
 };
-cudaError_t launch_latent_prefill(const LatentPrefillParams& p, cudaStream_t stream);
+cudaError_t launch_latent_prefill(LatentPrefillParams p, cudaStream_t stream);
 
 // Native-form attention for head dimensions other than 128 (generic.cu).
 cudaError_t launch_generic_attention(const void* q, const void* k, const void* v, void* out, const int* positions,

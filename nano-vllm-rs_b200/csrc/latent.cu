@@ -28,13 +28,13 @@
 // scratch, at most two parts a CTA, and a second kernel joins them in the order
 // of the parts. The plan is worked out by each CTA from the lengths on the
 // device, so a captured call follows them.
-#include "prefill_common.cuh"
+#include "latent_common.cuh"
 
 namespace nvb {
 
 namespace latent_detail {
 
-using namespace prefill_common;
+using namespace latent_common;
 
 constexpr int kLatent = 512, kWidth = 576;
 constexpr int kRows = 64;                       // rows of a CTA
@@ -46,8 +46,6 @@ constexpr int kUnits = 5;                       // a tile's barriers: the rotate
 constexpr int kThreads = 256;
 constexpr int kTmemCols = 512;
 constexpr int kOCol = 128;                      // S at 0 and 64, O^T at 128 + 64 p
-constexpr float kLn2 = 0.693147180559945309f;
-constexpr float kRescaleLog2 = 8.0f;            // the maximum in use moves when it grew by 2^8 (P <= 2^8)
 
 // kSFull, kSFree: one per S buffer. The rows may be a tile ahead of the S issuer's look at kSFree, so the arrivals of two
 // tiles in a row must not meet in one barrier.
@@ -78,32 +76,6 @@ constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10);
 constexpr uint32_t kIdescS = kIdesc | ((uint32_t(kRows) >> 4) << 24) | ((uint32_t(kKeys) >> 3) << 17);
 constexpr uint32_t kIdescPV = kIdesc | ((128u >> 4) << 24) | (1u << 15);  // A MN-major (dims contiguous), N by the rows
 
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, kErrLatentWait); }
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, wait(bar, parity));
-}
-
-// One thread of the warp, which the compiler knows to be one: the operands of its TMA and MMA instructions then stay in
-// uniform registers. Under `lane == 0` every instruction moves them there again: an MMA takes 45 to 130 cycles to issue,
-// 32 (M = N = 64) to 48 (M = 128, N = 64) this way, which is what it takes to read its operands.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r != 0;
-}
-
-// One arrival, and `bytes` to land; shared-memory addresses.
-__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void load_piece(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int row) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(0), "r"(row)
-      : "memory");
-}
-
 // 16 lanes x 64 columns: thread t has rows t / 4 (r[4 i], r[4 i + 1]) and t / 4 + 8 (r[4 i + 2], r[4 i + 3]) at
 // columns 8 i + 2 (t % 4) and the next.
 __device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[32]) {
@@ -124,14 +96,6 @@ __device__ __forceinline__ bool any_of_four_warps(bool yes) {
       : "r"(uint32_t(yes))
       : "memory");
   return r != 0;
-}
-
-// Whether a pair of BF16 holds an infinity or NaN: an exponent of all ones carries into the sign's place.
-__device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
-  return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-}
-__device__ __forceinline__ uint32_t finite_part(uint32_t w) {  // such halves as 0
-  return w & ~(((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u));
 }
 
 // ---------------------------------------------------------------- plan
@@ -368,16 +332,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr int kPieces[kUnits] = {1, 2, 2, 2, 2};
             const int c0 = u == 0 ? 0 : 2 * u - 1;
             const uint32_t full = full0 + u * 8;
-            expect(full, uint32_t(kPieces[u]) * kChunk * ((ok ? 1 : 0) + (with_q ? 1 : 0)));
+            expect_bytes(full, uint32_t(kPieces[u]) * kChunk * ((ok ? 1 : 0) + (with_q ? 1 : 0)));
             if (with_q) {
 #pragma unroll
               for (int c = c0; c < c0 + kPieces[u]; ++c)
-                load_piece(sbase + kQOff + c * kChunk, &qmap, full, c == 0 ? kLatent : (c - 1) * 64, q_row);
+                tma_load_3d_at(sbase + kQOff + c * kChunk, &qmap, full, c == 0 ? kLatent : (c - 1) * 64, 0, q_row);
             }
             if (ok) {  // a bad page's keys are masked, whatever the tile holds
 #pragma unroll
               for (int c = c0; c < c0 + kPieces[u]; ++c)
-                load_piece(tile + c * kChunk, &cmap, full, c == 0 ? kLatent : (c - 1) * 64, row);
+                tma_load_3d_at(tile + c * kChunk, &cmap, full, c == 0 ? kLatent : (c - 1) * 64, 0, row);
             }
           }
           if (!alive) break;
@@ -470,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = tmem + (uint32_t(quad * 32) << 16);
     const int ra = quad * 16 + (lane >> 2), rb = ra + 8;  // this thread's rows, shared by four lanes
     float* alphas = reinterpret_cast<float*>(smem + kAlphaOff);
-    const float sl2 = p.scale * 1.4426950408889634f;
+    const float sl2 = p.scale * kLog2e;
     int g = 0;
     // A warp whose wait gave up goes on without waiting, so that the four warps still meet at their named barriers.
     bool alive = true;

@@ -343,6 +343,30 @@ def test_expanded_ragged_batches(nvb, seed):
     Expanded(queries, keys, [2, 3, 2, 5, 1][seed], seed=seed).go(nvb)
 
 
+@pytest.mark.parametrize("queries, keys, heads", [
+    ([600], [600], 64), ([130, 300, 257, 1, 255], [130, 420, 257, 600, 256], 40), ([129] * 12, [129] * 12, 13),
+    ([300, 5, 200, 140], [260, 5, 10, 1], 50), ([400, 270], [1100, 399], 52)])
+def test_expanded_pairs_of_query_tiles(nvb, queries, keys, heads):
+    # enough items for all SMs: two tiles each, the second one whole, in part or empty, with fewer keys than queries
+    Expanded(queries, keys, heads, seed=heads).go(nvb)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_expanded_pairs_keys_that_a_query_does_not_see(nvb, value):
+    case = Expanded([500, 330], [500, 400], 50, seed=12)
+    clean, clean_lse = case.go(nvb)
+    for key in (3, 130, 300, 499):
+        case.kv[key, :, 128 + key % 128] = value
+    out, lse = case.run(nvb)
+    assert torch.equal(lse, clean_lse) and torch.equal(out[500:], clean[500:])
+    want = torch.zeros(500, 128, dtype=torch.bool, device="cuda")
+    for key in (3, 130, 300, 499):
+        want[key:, key % 128] = True
+    bad = torch.isnan(out[:500]) if math.isnan(value) else out[:500] == value
+    assert torch.equal(bad, want[:, None].expand(500, 50, 128))
+    assert torch.equal(torch.where(bad, 0, out[:500]), torch.where(bad, 0, clean[:500]))
+
+
 def test_expanded_leaves_rows_past_max_q(nvb):
     case = Expanded([300, 40], [300, 50], 2, seed=3)
     want = case.go(nvb)
