@@ -11,7 +11,7 @@ def as64(t):
 
 
 def _attend(q, k, v, seen, scale):
-    """One query: q [h, d] over the keys k [m, h or 1, d] and values v [m, h or 1, e] in `seen` [m].
+    """One query of h heads: q [h, d] over the keys k [m, d] and values v [m, e] in `seen` [m].
 
     Returns the output, the LSE, sum p |v| / sum p per element and the largest
     sum |q k| scale of a head's keys (what the scores' rounding goes by).
@@ -20,20 +20,13 @@ def _attend(q, k, v, seen, scale):
     k, v = k[seen], v[seen]
     if not len(k):
         return np.zeros((h, e)), np.full(h, -np.inf), np.zeros((h, e)), np.zeros(h)
-    # [h, m, d]: products a head; keys that all heads share are one matrix
-    k, v = (np.moveaxis(x, 1, 0) if x.shape[1] > 1 else x[None, :, 0] for x in (k, v))
     with np.errstate(invalid="ignore", over="ignore"):
-        x = (k @ q[:, :, None])[..., 0] * scale if len(k) > 1 else q @ k[0].T * scale
+        x = q @ k.T * scale
         top = x.max(1, keepdims=True)
         p = np.exp(x - top)
         total = p.sum(1)
-        if len(k) > 1:
-            sums = lambda w: (p[:, None, :] @ w)[:, 0]  # noqa: E731
-            size = (np.abs(k) @ np.abs(q)[:, :, None])[..., 0].max(1) * scale
-        else:
-            sums = lambda w: p @ w[0]  # noqa: E731
-            size = (np.abs(q) @ np.abs(k[0]).T).max(1) * scale
-        out, weight = sums(v) / total[:, None], sums(np.abs(v)) / total[:, None]
+        out, weight = p @ v / total[:, None], p @ np.abs(v) / total[:, None]
+        size = (np.abs(q) @ np.abs(k).T).max(1) * scale
         lse = top[:, 0] + np.log(total)
     return out, lse, weight, size
 
@@ -51,13 +44,13 @@ def absorbed(q, cache, cu_q, kv_lens, table, scale):
     for b, length in enumerate(kv_lens):
         n = int(cu_q[b + 1] - cu_q[b])
         if length < 0 or length > table.shape[1] * page:
-            length, keys, ok = 0, np.zeros((0, 1, WIDTH)), np.zeros(0, bool)
+            length, keys, ok = 0, np.zeros((0, WIDTH)), np.zeros(0, bool)
             n_base = -10 ** 9
         else:
             j = np.arange(length)
             pages = table[b, j // page] if length else np.zeros(0, int)
             ok = (pages >= 0) & (pages < blocks)
-            keys = flat[np.where(ok, pages, 0) * page + j % page][:, None]
+            keys = flat[np.where(ok, pages, 0) * page + j % page]
             n_base = length - n
         for i in range(n):
             seen = ok & (np.arange(len(ok)) <= n_base + i)
@@ -67,16 +60,31 @@ def absorbed(q, cache, cu_q, kv_lens, table, scale):
 
 
 def expanded(q, kv, rope, cu_q, cu_k, scale):
+    """As absorbed; kv [keys, heads, 256], rope [keys, 64]. A key that is not finite counts where it is seen only."""
     res = _results(int(cu_q[-1]), q.shape[1], 128)
-    heads = q.shape[1]
     for b in range(len(cu_q) - 1):
         n, m = int(cu_q[b + 1] - cu_q[b]), int(cu_k[b + 1] - cu_k[b])
-        one, r = kv[cu_k[b]:cu_k[b + 1]], rope[cu_k[b]:cu_k[b + 1]]
-        k = np.concatenate([one[..., :128], np.broadcast_to(r[:, None], (m, heads, ROPE))], -1)
-        for i in range(n):
-            seen = np.arange(m) <= m - n + i
-            for x, y in zip(res, _attend(q[cu_q[b] + i], k, one[..., 128:], seen, scale)):
-                x[cu_q[b] + i] = y
+        seen = np.arange(m)[None, :] <= m - n + np.arange(n)[:, None]
+        some = seen.any(1)
+        for h in range(q.shape[1]):
+            one = kv[cu_k[b]:cu_k[b + 1], h]
+            k, v = np.concatenate([one[:, :128], rope[cu_k[b]:cu_k[b + 1]]], 1), one[:, 128:]
+            x = q[cu_q[b]:cu_q[b + 1], h]
+            fine = np.isfinite(v)
+            with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+                s = np.where(seen, x @ k.T * scale, -np.inf)
+                top = np.where(some, s.max(1, initial=-np.inf), 0.0)[:, None]
+                p = np.where(seen, np.exp(s - top), 0.0)
+                total = p.sum(1)
+                inv = np.where(some, 1.0 / total, 0.0)[:, None]
+                out, weight = p @ np.where(fine, v, 0.0) * inv, p @ np.where(fine, np.abs(v), 0.0) * inv
+                for key in np.nonzero(~fine.all(1))[0]:
+                    rows = seen[:, key]
+                    out[rows] += np.where(fine[key], 0.0, p[rows, key, None] * v[key])
+                size = np.where(seen, np.abs(x) @ np.abs(k).T * scale, 0.0).max(1, initial=0.0)
+                lse = np.where(some, top[:, 0] + np.log(total), -np.inf)
+            for r, y in zip(res, (out, lse, weight, size)):
+                r[cu_q[b]:cu_q[b + 1], h] = y
     return res
 
 
