@@ -466,37 +466,41 @@ def cache_compact_paths(layers, cu_q, kv_lens, block_table, path, counts, new_kv
 LATENT_DIM, LATENT_ROPE, LATENT_WIDTH = 512, 64, 576  # of a row of the latent cache
 
 
-def _strided(name, t, shape, device):
-    """(first, behind the last byte, name) of a BF16 CUDA tensor of that shape whose last dimension is contiguous."""
-    import torch
-
-    if t.dtype is not torch.bfloat16 or t.shape != shape or t.get_device() != device or (
-            t.stride(-1) != 1 or any(s < 0 for s in t.stride())):
-        if t.dtype is torch.bfloat16 and t.shape == shape and t.get_device() == device:
+def _views(arguments, device):
+    """(address, address behind the last byte, name) of each argument (name, tensor, shape, type, bytes a value): of that
+    shape and type and on the device; contiguous, or with bytes 0 BF16 whose last dimension is (for slices of rows)."""
+    spans = []
+    for name, t, shape, dtype, size in arguments:
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != device:
+            _refuse(t, shape, dtype, name, device)
+        start = t.data_ptr()
+        if t.is_contiguous():
+            spans.append((start, start + (size or 2) * t.numel(), name))
+            continue
+        if size:
+            _refuse(t, shape, dtype, name, device)
+        strides = t.stride()
+        if strides[-1] != 1 or min(strides) < 0:
             raise NvbError(f"{name}'s last dimension must be contiguous")
-        _refuse(t, shape, torch.bfloat16, name, device)
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + 2 * (last + 1), name
+        last = 0
+        for n, s in zip(shape, strides):
+            last += (n - 1) * s
+        spans.append((start, start + 2 * (last + 1), name))
+    return spans
 
 
 def _apart(written, others):
-    """Refuses a written tensor's span that overlaps another's."""
-    for i, (a, z, name) in enumerate(written):
-        for x, y, other in written[:i] + others:
-            if a < y and x < z:
+    """Refuses a written span that overlaps another."""
+    for a, z, name in written:
+        for x, y, other in others:
+            if a < y and x < z and name is not other:
                 raise NvbError(f"{name} overlaps {other}")
-
-
-def _plain(name, t, shape, dtype, device):
-    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != device:
-        _refuse(t, shape, dtype, name, device)
-    return t.data_ptr(), t.data_ptr() + t.nbytes, name
 
 
 def _latent_cache(cache):
     if cache.dim() != 3 or cache.shape[2] != LATENT_WIDTH:
         raise NvbError(f"cache must be [num_blocks, block_size, {LATENT_WIDTH}], got {tuple(cache.shape)}")
-    return cache.shape[0], cache.shape[1]
+    return cache.shape
 
 
 def latent_store(kv, weight, positions, slots, cache, *, rope_table, eps=1e-6, q=None, q_out=None, interleaved=False,
@@ -514,44 +518,53 @@ def latent_store(kv, weight, positions, slots, cache, *, rope_table, eps=1e-6, q
     """
     import torch
 
-    device, i32 = torch.cuda.current_device(), torch.int32
+    device, i32, bf16 = torch.cuda.current_device(), torch.int32, torch.bfloat16
     if kv is None and q is None:
         raise NvbError("kv or q is required")
-    rows, heads, num_blocks, block_size = (kv if kv is not None else q).shape[0], 0, 0, 0
-    if rope_table.dim() != 2:
-        raise NvbError("rope_table must be [positions, 64]")
-    read = [_plain("positions", positions, (rows,), i32, device),
-            _plain("rope_table", rope_table, (rope_table.shape[0], LATENT_ROPE), torch.float32, device)]
-    written, kv_stride, strides = [], 0, (0, 0, 0, 0)
+    if positions is None or rope_table is None or rope_table.dim() != 2:
+        raise NvbError("positions [rows] and rope_table [positions, 64] are required")
+    rows, max_positions = (kv if kv is not None else q).shape[0], rope_table.shape[0]
+    arguments = [("positions", positions, (rows,), i32, 4),
+                 ("rope_table", rope_table, (max_positions, LATENT_ROPE), torch.float32, 4)]
+    heads = num_blocks = block_size = kv_stride = 0
+    kv_at = weight_at = slots_at = cache_at = q_at = out_at = None
+    strides = out_strides = (0, 0)
     if kv is not None:
-        num_blocks, block_size = _latent_cache(cache)
-        read += [_strided("kv", kv, (rows, LATENT_WIDTH), device), _plain("slots", slots, (rows,), i32, device),
-                 _plain("weight", weight, (LATENT_DIM,), torch.bfloat16, device)]
-        written.append(_plain("cache", cache, cache.shape, torch.bfloat16, device))
-        kv_stride = kv.stride(0) if rows > 1 else max(kv.stride(0), LATENT_WIDTH)
+        if weight is None or slots is None or cache is None:
+            raise NvbError("weight, slots and cache go with kv")
+        num_blocks, block_size, _ = shape = _latent_cache(cache)
+        arguments += (("kv", kv, (rows, LATENT_WIDTH), bf16, 0), ("slots", slots, (rows,), i32, 4),
+                      ("weight", weight, (LATENT_DIM,), bf16, 2), ("cache", cache, shape, bf16, 2))
     elif weight is not None or slots is not None or cache is not None:
         raise NvbError("weight, slots and cache go with kv")
     if q is not None:
-        q_out = q if q_out is None else q_out
         if q.dim() != 3:
             raise NvbError("q must be [rows, heads, 64]")
         heads = q.shape[1]
-        span = _strided("q", q, (rows, heads, LATENT_ROPE), device)
-        written.append(_strided("q_out", q_out, (rows, heads, LATENT_ROPE), device))
-        strides = (q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1))
-        if q_out.data_ptr() != q.data_ptr() or strides[:2] != strides[2:]:
-            read.append(span)
+        arguments.append(("q", q, (rows, heads, LATENT_ROPE), bf16, 0))
+        if q_out is not None:
+            arguments.append(("q_out", q_out, (rows, heads, LATENT_ROPE), bf16, 0))
     elif q_out is not None:
         raise NvbError("q_out goes with q")
-    _apart(written, read)
+    spans = _views(arguments, device)
+    written = []
+    if kv is not None:
+        kv_at, slots_at, weight_at, cache_at = spans[2][0], spans[3][0], spans[4][0], spans[5][0]
+        kv_stride = kv.stride(0) if rows > 1 else LATENT_WIDTH
+        written.append(spans[5])
+    if q is not None:
+        strides = out_strides = q.stride()
+        q_at = out_at = spans[6 if kv is not None else 2][0]
+        if q_out is not None:
+            out_at, out_strides = spans[-1][0], q_out.stride()
+            if out_at == q_at and out_strides[:2] == strides[:2]:
+                spans.pop()  # in place
+        written.append(spans[-1])
+    _apart(written, spans)
     _check(library().nvb_latent_store(
-        _raw_stream(stream, device), _address(kv), kv_stride, _address(weight), positions.data_ptr(), _address(slots),
-        _address(cache), _address(q), strides[0], strides[1], _address(q_out), strides[2], strides[3], rows, heads,
-        int(interleaved), block_size, num_blocks, eps, rope_table.data_ptr(), rope_table.shape[0]))
-
-
-def _address(t):
-    return t.data_ptr() if t is not None else None
+        _raw_stream(stream, device), kv_at, kv_stride, weight_at, spans[0][0], slots_at, cache_at, q_at, strides[0],
+        strides[1], out_at, out_strides[0], out_strides[1], rows, heads, interleaved, block_size, num_blocks, eps,
+        spans[1][0], max_positions))
 
 
 def latent_gather(cache, block_table, cu_k, latent, rope, *, stream=None):
@@ -560,34 +573,27 @@ def latent_gather(cache, block_table, cu_k, latent, rope, *, stream=None):
     be slices of longer rows."""
     import torch
 
-    device, i32 = torch.cuda.current_device(), torch.int32
-    num_blocks, block_size = _latent_cache(cache)
+    device, i32, bf16 = torch.cuda.current_device(), torch.int32, torch.bfloat16
+    num_blocks, block_size, _ = shape = _latent_cache(cache)
     if block_table.dim() != 2 or latent.dim() != 2:
         raise NvbError("block_table and latent must have rows")
     (batch, table_stride), total_k = block_table.shape, latent.shape[0]
-    read = [_plain("cache", cache, cache.shape, torch.bfloat16, device),
-            _plain("block_table", block_table, block_table.shape, i32, device),
-            _plain("cu_k", cu_k, (batch + 1,), i32, device)]
-    written = [_strided("latent", latent, (total_k, LATENT_DIM), device),
-               _strided("rope", rope, (total_k, LATENT_ROPE), device)]
-    strides = [t.stride(0) if total_k > 1 else max(t.stride(0), t.shape[1]) for t in (latent, rope)]
-    _apart(written[:1], read)
-    if not _interleaved_rows(latent, rope):
-        _apart(written[1:], read + written[:1])
-    else:
-        _apart(written[1:], read)
-    _check(library().nvb_latent_gather(_raw_stream(stream, device), cache.data_ptr(), block_table.data_ptr(),
-                                       cu_k.data_ptr(), latent.data_ptr(), strides[0], rope.data_ptr(), strides[1],
-                                       batch, total_k, block_size, table_stride, num_blocks))
+    spans = _views((("cache", cache, shape, bf16, 2), ("block_table", block_table, (batch, table_stride), i32, 4),
+                    ("cu_k", cu_k, (batch + 1,), i32, 4), ("latent", latent, (total_k, LATENT_DIM), bf16, 0),
+                    ("rope", rope, (total_k, LATENT_ROPE), bf16, 0)), device)
+    strides = (latent.stride(0), rope.stride(0)) if total_k > 1 else (LATENT_DIM, LATENT_ROPE)
+    _apart(spans[3:], spans[:3])
+    if strides[0] != strides[1] or not _side_by_side(spans[3][0], LATENT_DIM, spans[4][0], LATENT_ROPE, strides[0]):
+        _apart(spans[3:4], spans[4:])
+    _check(library().nvb_latent_gather(_raw_stream(stream, device), spans[0][0], spans[1][0], spans[2][0],
+                                       spans[3][0], strides[0], spans[4][0], strides[1], batch, total_k, block_size,
+                                       table_stride, num_blocks))
 
 
-def _interleaved_rows(a, b):
-    """Whether two slices of the same rows lie beside one another in each row."""
-    if a.stride(0) != b.stride(0):
-        return False
-    first, second = (a, b) if a.data_ptr() < b.data_ptr() else (b, a)
-    gap = (second.data_ptr() - first.data_ptr()) // 2
-    return first.shape[1] <= gap and gap + second.shape[1] <= first.stride(0)
+def _side_by_side(a, a_values, b, b_values, stride):
+    """Whether two slices of rows `stride` values apart lie beside one another in each row."""
+    gap = (b - a) // 2
+    return a_values <= gap <= stride - b_values or b_values <= -gap <= stride - a_values
 
 
 def latent_scratch(device):
@@ -611,19 +617,22 @@ def paged_latent_fwd(q, cache, out, cu_q, kv_lens, block_table, *, max_q, scale,
     import torch
 
     device, bf16, i32, f32 = torch.cuda.current_device(), torch.bfloat16, torch.int32, torch.float32
-    num_blocks, block_size = _latent_cache(cache)
-    if q.dim() != 3 or block_table.dim() != 2:
-        raise NvbError("q must be [total_q, heads, 576], block_table a row for each sequence")
-    (total_q, heads, _), (batch, table_stride) = q.shape, block_table.shape
-    pointers = _pointers(
-        (("q", q, (total_q, heads, LATENT_WIDTH), bf16), ("cache", cache, cache.shape, bf16),
-         ("out", out, (total_q, heads, LATENT_DIM), bf16), ("cu_q", cu_q, (batch + 1,), i32),
-         ("kv_lens", kv_lens, (batch,), i32), ("block_table", block_table, block_table.shape, i32),
-         ("lse", lse, (total_q, heads), f32), ("scratch", scratch, (scratch.numel(),), f32)),
-        ("out", "lse", "scratch"), device)
-    _check(library().nvb_paged_latent_fwd(_raw_stream(stream, device), *pointers[:6], batch, total_q, max_q, heads,
-                                          block_size, table_stride, num_blocks, scale, *pointers[6:],
-                                          scratch.numel()))
+    num_blocks, block_size, _ = shape = _latent_cache(cache)
+    if q.dim() != 3 or block_table.dim() != 2 or scratch is None:
+        raise NvbError("q must be [total_q, heads, 576], block_table a row for each sequence, scratch latent_scratch's")
+    (total_q, heads, _), (batch, table_stride), floats = q.shape, block_table.shape, scratch.numel()
+    arguments = [("q", q, (total_q, heads, LATENT_WIDTH), bf16, 2), ("cache", cache, shape, bf16, 2),
+                 ("cu_q", cu_q, (batch + 1,), i32, 4), ("kv_lens", kv_lens, (batch,), i32, 4),
+                 ("block_table", block_table, (batch, table_stride), i32, 4),
+                 ("out", out, (total_q, heads, LATENT_DIM), bf16, 2), ("scratch", scratch, (floats,), f32, 4)]
+    if lse is not None:
+        arguments.append(("lse", lse, (total_q, heads), f32, 4))
+    spans = _views(arguments, device)
+    _apart(spans[5:], spans)
+    _check(library().nvb_paged_latent_fwd(
+        _raw_stream(stream, device), spans[0][0], spans[1][0], spans[5][0], spans[2][0], spans[3][0], spans[4][0],
+        batch, total_q, max_q, heads, block_size, table_stride, num_blocks, scale,
+        spans[7][0] if lse is not None else None, spans[6][0], floats))
 
 
 def latent_prefill_fwd(q, kv, k_rope, out, cu_q, cu_k, *, max_q, scale, lse=None, stream=None):
@@ -641,18 +650,17 @@ def latent_prefill_fwd(q, kv, k_rope, out, cu_q, cu_k, *, max_q, scale, lse=None
     if q.dim() != 3 or kv.dim() != 3:
         raise NvbError("q must be [total_q, heads, 192], kv [total_k, heads, 256]")
     (total_q, heads, _), total_k, batch = q.shape, kv.shape[0], cu_q.numel() - 1
-    pointers = _pointers(
-        (("q", q, (total_q, heads, 192), bf16), ("kv", kv, (total_k, heads, 256), bf16),
-         ("out", out, (total_q, heads, 128), bf16), ("cu_q", cu_q, (batch + 1,), i32),
-         ("cu_k", cu_k, (batch + 1,), i32), ("lse", lse, (total_q, heads), torch.float32)), ("out", "lse"), device)
-    rope = _strided("k_rope", k_rope, (total_k, LATENT_ROPE), device)
-    stride = k_rope.stride(0) if total_k > 1 else max(k_rope.stride(0), LATENT_ROPE)
-    for t, name in ((out, "out"), (lse, "lse")):
-        if t is not None:
-            _apart([(t.data_ptr(), t.data_ptr() + t.nbytes, name)], [rope])
-    _check(library().nvb_latent_prefill_fwd(_raw_stream(stream, device), pointers[0], pointers[1], k_rope.data_ptr(),
-                                            stride, pointers[2], pointers[3], pointers[4], batch, total_q, total_k,
-                                            max_q, heads, scale, pointers[5]))
+    arguments = [("q", q, (total_q, heads, 192), bf16, 2), ("kv", kv, (total_k, heads, 256), bf16, 2),
+                 ("k_rope", k_rope, (total_k, LATENT_ROPE), bf16, 0), ("cu_q", cu_q, (batch + 1,), i32, 4),
+                 ("cu_k", cu_k, (batch + 1,), i32, 4), ("out", out, (total_q, heads, 128), bf16, 2)]
+    if lse is not None:
+        arguments.append(("lse", lse, (total_q, heads), torch.float32, 4))
+    spans = _views(arguments, device)
+    _apart(spans[5:], spans)
+    _check(library().nvb_latent_prefill_fwd(
+        _raw_stream(stream, device), spans[0][0], spans[1][0], spans[2][0],
+        k_rope.stride(0) if total_k > 1 else LATENT_ROPE, spans[5][0], spans[3][0], spans[4][0], batch, total_q,
+        total_k, max_q, heads, scale, spans[6][0] if lse is not None else None))
 
 
 def attention(q, kcache, vcache, positions, seq_indices, tables, out, *, rows, q_heads, kv_heads, head_dim,
