@@ -99,10 +99,14 @@ __device__ __forceinline__ bool any_of_four_warps(bool yes) {
 }
 
 // ---------------------------------------------------------------- plan
-// Units of work: every (sequence, round) has one for its start and one for
-// each tile. A round is `share` row tiles, each a member's of the group of
-// `share` CTAs that reads the round's keys together. Group i takes units
-// [i * per, (i + 1) * per).
+// A round is `share` row tiles of a sequence, each a member's of the group of
+// `share` CTAs that reads the round's keys together.
+//
+// The batch is cut as a whole: every round has a unit for its start and one for
+// each tile, and group i takes units [i * per, (i + 1) * per). (Equal ranges of
+// each sequence, a CTA having one, were no faster where they fit: 64 sequences of
+// ~4050 keys and 64 heads on 128 of the SMs 73.5 us, by runs 74.6; 16 heads 67.5
+// and 64.)
 struct Sequence {
   int begin, n, len, tiles, row_tiles;
 };
@@ -118,17 +122,18 @@ __device__ __forceinline__ Sequence sequence(const LatentParams& p, int b) {
 }
 struct Plan {
   long long first;  // the unit that sequence b starts at
-  long long u0, u1;
+  long long u0, u1, per;
   int b, share;
 };
 static_assert(sizeof(Plan) <= 64, "plan's place");
 
 struct Segment {
-  int b, begin, n, len, tiles;
+  int b, begin, n, len;
   int row0;     // of the sequence's rows
   int rows;     // at most 64
   int t0, t1;   // tiles; t0 = t1: write zeros
   bool whole;
+  int parts;    // of the rows, where this is the first of several
 };
 // The segments of a CTA, in order; every role walks them by itself.
 struct Walk {
@@ -147,11 +152,11 @@ struct Walk {
         if (at <= plan.u0 || tile >= q.row_tiles) continue;
         const long long t0 = max(plan.u0 - start - 1, 0ll), t1 = min(plan.u1 - start - 1, (long long)q.tiles);
         if (q.tiles ? t1 <= t0 : start < plan.u0) continue;
+        if (t0 == 0 && t1 < q.tiles) s.parts = 1 + int((q.tiles - t1 + plan.per - 1) / plan.per);
         s.b = b;
         s.begin = q.begin;
         s.n = q.n;
         s.len = q.len;
-        s.tiles = q.tiles;
         s.row0 = tile * kRows;
         s.rows = min(kRows, q.n * p.heads - s.row0);
         s.t0 = q.tiles ? int(t0) : 0;
@@ -174,16 +179,96 @@ __device__ __forceinline__ T warp_sum(T v) {
   return v;
 }
 
-// All threads; the plan is in shared memory when it returns.
+// CTAs that read a round's keys together. Row tiles of one sequence then share them in L2 whatever the batch; that costs
+// CTAs where sequences have fewer row tiles than others, so it is for caches that L2 does not hold as a whole.
+__device__ __forceinline__ int plan_share(const LatentParams& p, long long tiles, int row_tiles, int ctas) {
+  if (tiles <= p.l2_tiles || row_tiles <= 1) return 1;
+  const int most = min(4, ctas), rounds = (row_tiles + most - 1) / most;
+  return (row_tiles + rounds - 1) / rounds;
+}
+__device__ __forceinline__ long long units_of(const Sequence& q, int share) {
+  return (long long)((q.row_tiles + share - 1) / share) * (q.tiles + 1);
+}
+__device__ __forceinline__ void plan_runs(const LatentParams& p, Plan& plan, long long total, int share, int ctas) {
+  const int groups = ctas / share, group = blockIdx.x / share;
+  const long long each = total <= 0x7fffffff ? (unsigned(total) + groups - 1) / unsigned(groups)
+                                             : (total + groups - 1) / groups;
+  plan.per = max(each, (long long)p.min_units);
+  plan.u0 = group < groups ? min(group * plan.per, total) : total;
+  plan.u1 = min(plan.u0 + plan.per, total);
+  plan.share = share;
+  plan.b = p.batch;  // unless a sequence has unit u0
+  plan.first = total;
+}
+template <class T>
+__device__ __forceinline__ T warp_scan(T v, int lane) {
+#pragma unroll
+  for (int off = 1; off < 32; off *= 2) {
+    const T o = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += o;
+  }
+  return v;
+}
+
+// Up to 32 x kPlanEach sequences of usual sizes: every warp works the plan out for itself, in 32 bits. This stands before
+// a CTA's first load, so it has few steps that wait for one another. False where the sizes are too large for it.
+constexpr int kPlanEach = 4;
+__device__ __forceinline__ bool make_plan_warp(const LatentParams& p, int ctas, Plan& plan) {
+  const int lane = threadIdx.x & 31, b0 = lane * kPlanEach;
+  int tiles[kPlanEach], rounds[kPlanEach];
+  bool large = false;  // sizes that 32 bits might not sum
+  int all = 0, most = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanEach; ++i) {
+    tiles[i] = rounds[i] = 0;
+    if (b0 + i < p.batch) {
+      const Sequence q = sequence(p, b0 + i);
+      rounds[i] = q.row_tiles;
+      tiles[i] = q.row_tiles ? q.tiles : 0;
+      large |= q.row_tiles > 128 || q.tiles > 65535;
+      all += min(tiles[i], 65535);
+      most = max(most, q.row_tiles);
+    }
+  }
+  if (__any_sync(0xffffffffu, large)) return false;
+  all = __reduce_add_sync(0xffffffffu, all);
+  most = __reduce_max_sync(0xffffffffu, most);
+  const int share = plan_share(p, all, most, ctas);
+  if (share > 1) {
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i) rounds[i] = (rounds[i] + share - 1) / share;
+  }
+  int units = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanEach; ++i) units += rounds[i] * (tiles[i] + 1);
+  const int upto = warp_scan(units, lane);
+  plan_runs(p, plan, __shfl_sync(0xffffffffu, upto, 31), share, ctas);
+  const int u0 = int(plan.u0);
+  const unsigned has = __ballot_sync(0xffffffffu, units && upto - units <= u0 && u0 < upto);
+  if (has) {
+    int at = upto - units, b = b0;
+#pragma unroll
+    for (int i = 0; i + 1 < kPlanEach; ++i)
+      if (b == b0 + i && u0 >= at + rounds[i] * (tiles[i] + 1)) {
+        at += rounds[i] * (tiles[i] + 1);
+        ++b;
+      }
+    plan.b = __shfl_sync(0xffffffffu, b, __ffs(has) - 1);
+    plan.first = __shfl_sync(0xffffffffu, at, __ffs(has) - 1);
+  }
+  return true;
+}
+
+// Any number of sequences: all threads together; the plan is in shared memory when it returns.
 __device__ __forceinline__ void make_plan(const LatentParams& p, unsigned char* smem, int ctas) {
+  constexpr int kWarps = kThreads / 32;
   Plan* plan = reinterpret_cast<Plan*>(smem + kPlanOff);
   long long* sums = reinterpret_cast<long long*>(smem + kScanOff);
-  int* most = reinterpret_cast<int*>(smem + kScanOff + 64);
+  int* most = reinterpret_cast<int*>(smem + kScanOff + kWarps * 8);
+  static_assert(kWarps * 12 <= 128, "the warps' sums");
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int each = (p.batch + kThreads - 1) / kThreads;
   const int b0 = min(t * each, p.batch), b1 = min(b0 + each, p.batch);
-  // Row tiles of one sequence that read its keys at the same time share them in L2 whatever the batch. That costs CTAs
-  // where sequences have fewer row tiles than others, so it is for caches that L2 does not hold as a whole.
   long long tiles = 0;
   int rt = 0;
   for (int b = b0; b < b1; ++b) {
@@ -201,57 +286,36 @@ __device__ __forceinline__ void make_plan(const LatentParams& p, unsigned char* 
   __syncthreads();
   tiles = 0;
   rt = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     tiles += sums[w];
     rt = max(rt, most[w]);
   }
-  int share = 1;
-  if (tiles > p.l2_tiles && rt > 1) {
-    const int most_share = min(4, ctas);
-    const int rounds = (rt + most_share - 1) / most_share;
-    share = (rt + rounds - 1) / rounds;
-  }
+  const int share = plan_share(p, tiles, rt, ctas);
   long long units = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Sequence q = sequence(p, b);
-    units += (long long)((q.row_tiles + share - 1) / share) * (q.tiles + 1);
-  }
-  long long upto = units;  // with this thread's
-#pragma unroll
-  for (int off = 1; off < 32; off *= 2) {
-    const long long o = __shfl_up_sync(0xffffffffu, upto, off);
-    if (lane >= off) upto += o;
-  }
+  for (int b = b0; b < b1; ++b) units += units_of(sequence(p, b), share);
+  long long upto = warp_scan(units, lane);  // with this thread's
   __syncthreads();
   if (lane == 31) sums[warp] = upto;
   __syncthreads();
   long long total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     if (w < warp) upto += sums[w];
     total += sums[w];
   }
-  const int groups = ctas / share, group = blockIdx.x / share;
-  const long long per = max((total + groups - 1) / groups, (long long)p.min_units);
-  const long long u0 = group < groups ? min(group * per, total) : total, u1 = min(u0 + per, total);
-  if (t == 0) {
-    plan->u0 = u0;
-    plan->u1 = group < groups ? u1 : u0;
-    plan->share = share;
-    plan->b = p.batch;  // unless a sequence has unit u0
-    plan->first = total;
-  }
+  Plan mine;
+  plan_runs(p, mine, total, share, ctas);
+  if (t == 0) *plan = mine;
   __syncthreads();
-  if (units && upto - units <= u0 && u0 < upto) {
+  if (units && upto - units <= mine.u0 && mine.u0 < upto) {
     long long at = upto - units;
     for (int b = b0; b < b1; ++b) {
-      const Sequence q = sequence(p, b);
-      const long long mine = (long long)((q.row_tiles + share - 1) / share) * (q.tiles + 1);
-      if (u0 < at + mine) {
+      const long long here = units_of(sequence(p, b), share);
+      if (mine.u0 < at + here) {
         plan->b = b;
         plan->first = at;
         break;
       }
-      at += mine;
+      at += here;
     }
   }
   __syncthreads();
@@ -291,13 +355,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");  // that kernel has completed, its writes are visible
-  make_plan(p, smem, gridDim.x);
+  Plan plan;
+  const bool by_warp = p.batch <= 32 * kPlanEach && make_plan_warp(p, gridDim.x, plan);  // the same in all warps
+  if (!by_warp) make_plan(p, smem, gridDim.x);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const Plan plan = *reinterpret_cast<const Plan*>(smem + kPlanOff);
+  if (!by_warp) plan = *reinterpret_cast<const Plan*>(smem + kPlanOff);
   const int member = int(blockIdx.x % unsigned(plan.share));
   float* const part = p.scratch + (long long)blockIdx.x * kCtaFloats;
   const bool aligned = (sbase & 1023u) == 0;
@@ -625,10 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[kOFree]);
       if (!s.whole && s.t0 == 0) {
-        // the first part of rows that are joined: how many follow
-        const long long per = plan.u1 - plan.u0;  // a cut run is a full one
-        const long long rest = s.tiles - s.t1;
-        join = Join{int(first), s.rows, 1 + int((rest + per - 1) / per), plan.share};
+        join = Join{int(first), s.rows, s.parts, plan.share};
       }
     }
     if (threadIdx.x == 128) *reinterpret_cast<Join*>(part + 2 * kPartFloats) = alive ? join : Join{0, 0, 0, 0};
@@ -644,55 +707,110 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Joins the parts of cut rows: sum over the parts s of 2^(m_s - max) O_s over
 // the same sum of their row sums, in an order that goes by the parts alone.
-// Every CTA reads what the first kernel's CTAs left to join and takes its share
-// of the pieces. Of few parts a piece is 16 rows: a thread has one dim of them
-// all. Of many it is four rows of 32 dims, and sixteen groups of 32 threads
-// share the parts out. A warp a row works out the parts' factors while the first
-// values are on their way. What bounds it is round trips to L2, so a piece has
-// as many values in flight as the registers hold.
+// Every warp reads what the first kernel's CTAs left to join, and the CTAs take
+// the pieces in turn. Of few parts a piece is 16 rows (of more than two: eight):
+// a thread has one dim of them all. Of many it is four rows of 32 dims, and
+// sixteen groups of 32 threads share the parts out. A warp a row works out the
+// parts' factors while the first values are on their way. What bounds it is
+// round trips to L2, so a piece has as many values in flight as the registers
+// hold.
 constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32;
-constexpr int kFewParts = 16, kFewRows = 16, kManyDims = 32;
-constexpr int kMaxCtas = 512;
-static_assert(kFewRows == kJoinWarps && kFewParts * kFewRows <= 4 * kMaxCtas, "factors: a warp a row");
+constexpr int kFewParts = 16, kManyDims = 32;
+constexpr int kItemsEach = 5, kMaxCtas = 32 * kItemsEach;
+__device__ __forceinline__ int piece_rows(int parts) { return parts <= 2 ? 16 : (parts <= kFewParts ? 8 : 4); }
+
+// a part without a seen key may hold anything
+__device__ __forceinline__ void add_part(float4& a, const float4& f, const float4& v) {
+  a.x = f.x == 0.0f ? a.x : fmaf(f.x, v.x, a.x);
+  a.y = f.y == 0.0f ? a.y : fmaf(f.y, v.y, a.y);
+  a.z = f.z == 0.0f ? a.z : fmaf(f.z, v.z, a.z);
+  a.w = f.w == 0.0f ? a.w : fmaf(f.w, v.w, a.w);
+}
+
+// Few parts, kQuads x 4 rows from row0 on, kBatch parts in flight.
+template <int kQuads, int kBatch, class Part, class Factors>
+__device__ __forceinline__ void join_few(const LatentParams& p, const Join& j, int row0, const float4* factor4, Part part,
+                                         Factors factors) {
+  const int t = threadIdx.x, d = t >> 7, dim = t & 127;
+  const int place = ((d * 16 + row0 / 4) * 128 + dim) * 4;
+  float4 acc[kQuads], v[kBatch][kQuads];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+      for (int r = 0; r < kQuads; ++r)
+        v[k][r] = s0 + k < j.parts && row0 + 4 * r < j.rows
+                      ? *reinterpret_cast<const float4*>(part(s0 + k) + place + r * 512)
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  load(0);
+  factors(4 * kQuads);
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kQuads; ++r) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < j.parts; s0 += kBatch) {
+    if (s0) load(s0);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (s0 + k < j.parts)
+#pragma unroll
+        for (int r = 0; r < kQuads; ++r) add_part(acc[r], factor4[(s0 + k) * kQuads + r], v[k][r]);
+  }
+#pragma unroll
+  for (int r = 0; r < kQuads; ++r) {
+    const float a[4] = {acc[r].x, acc[r].y, acc[r].z, acc[r].w};
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      // two rows of this dim; of the neighbour's the other one, so that a store has two dims of a row
+      const bool odd = dim & 1;
+      const float other = __shfl_xor_sync(0xffffffffu, odd ? a[i] : a[i + 1], 1);
+      const int row = row0 + 4 * r + i + (odd ? 1 : 0);
+      if (row < j.rows)
+        *reinterpret_cast<uint32_t*>(p.out + ((long long)j.first_row + row) * kLatent + d * 128 + (dim & ~1)) =
+            odd ? pack_bf16x2(other, a[i + 1]) : pack_bf16x2(a[i], other);
+    }
+  }
+}
 
 __global__ void __launch_bounds__(kJoinThreads, 2) latent_join_kernel(const LatentParams p, const int ctas) {
-  __shared__ Join items[kMaxCtas];
-  __shared__ int ends[kMaxCtas];  // pieces up to and with an item's
-  __shared__ int warp_ends[kJoinWarps];
-  __shared__ float4 factor4[kMaxCtas];  // [part][row of the piece], 16 or 4 rows
+  __shared__ float4 factor4[kMaxCtas];  // [part][row of the piece]
   __shared__ float4 sums[kJoinWarps][kManyDims];
+  __shared__ Join items[kMaxCtas];
+  static_assert(2 * 16 <= 4 * kMaxCtas && kFewParts * 8 <= 4 * kMaxCtas && kJoinWarps >= 16, "factors: a warp a row");
   float* const factor = reinterpret_cast<float*>(factor4);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  {
-    static_assert(kMaxCtas <= kJoinThreads, "a thread an item");
-    Join j{0, 0, 0, 0};
-    if (t < ctas) j = *reinterpret_cast<const Join*>(p.scratch + (long long)t * kCtaFloats + 2 * kPartFloats);
-    if (t < ctas) items[t] = j;
-    int upto = j.parts > kFewParts ? (j.rows + 3) / 4 * (kLatent / kManyDims) : (j.rows + kFewRows - 1) / kFewRows;
+  static_assert(kMaxCtas <= kJoinThreads, "a thread an item");
+  if (t < ctas) items[t] = *reinterpret_cast<const Join*>(p.scratch + (long long)t * kCtaFloats + 2 * kPartFloats);
+  __syncthreads();
+  int ends[kItemsEach], pieces = 0;  // of items lane, lane + 32, ...: pieces up to and with each
 #pragma unroll
-    for (int off = 1; off < 32; off *= 2) {
-      const int o = __shfl_up_sync(0xffffffffu, upto, off);
-      if (lane >= off) upto += o;
+  for (int i = 0; i < kItemsEach; ++i) {
+    int mine = 0;
+    if (i * 32 + lane < ctas) {
+      const Join j = items[i * 32 + lane];
+      const int rows = piece_rows(j.parts);
+      mine = (j.rows + rows - 1) / rows * (j.parts > kFewParts ? kLatent / kManyDims : 1);
     }
-    if (lane == 31) warp_ends[warp] = upto;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) upto += warp_ends[w];
-    if (t < ctas) ends[t] = upto;
-    __syncthreads();
+    ends[i] = pieces + warp_scan(mine, lane);
+    pieces = __shfl_sync(0xffffffffu, ends[i], 31);
   }
-  for (int piece = blockIdx.x; piece < ends[ctas - 1]; piece += gridDim.x) {
-    int lo = 0, hi = ctas - 1;  // the first item that ends behind the piece
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (ends[mid] > piece) hi = mid;
-      else lo = mid + 1;
+  for (int piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
+    int at = 0, before = 0;  // the item that has it: the number of those that end before it; and their pieces
+#pragma unroll
+    for (int i = 0; i < kItemsEach; ++i) {
+      const int n = __popc(__ballot_sync(0xffffffffu, ends[i] <= piece));
+      const int end = __shfl_sync(0xffffffffu, ends[i], n ? n - 1 : 0);
+      if (n) {
+        at = i * 32 + n;
+        before = end;
+      }
     }
-    const Join j = items[lo];
-    const int within = piece - (lo ? ends[lo - 1] : 0);
+    const Join j = items[at];
+    const int within = piece - before;
     const bool few = j.parts <= kFewParts;
-    const int row0 = few ? within * kFewRows : within / (kLatent / kManyDims) * 4;
-    const float* const scratch = p.scratch + (long long)lo * kCtaFloats;
+    const int row0 = few ? within * piece_rows(j.parts) : within / (kLatent / kManyDims) * 4;
+    const float* const scratch = p.scratch + (long long)at * kCtaFloats;
     const long long step = (long long)j.stride * kCtaFloats;
     auto part = [&](int s) { return scratch + s * step + (s == 0 ? kPartFloats : 0); };
     auto factors = [&](int rows) {  // of `rows` rows, a warp each
@@ -722,54 +840,10 @@ __global__ void __launch_bounds__(kJoinThreads, 2) latent_join_kernel(const Late
       if (lane == 0 && p.lse && row0 + warp < j.rows && (few || within % (kLatent / kManyDims) == 0))
         p.lse[j.first_row + row0 + warp] = total == 0.0f ? -INFINITY : (mx + fast_log2(total)) * kLn2;
     };
-    // a part without a seen key may hold anything
-    auto add = [](float4& a, const float4& f, const float4& v) {
-      a.x = f.x == 0.0f ? a.x : fmaf(f.x, v.x, a.x);
-      a.y = f.y == 0.0f ? a.y : fmaf(f.y, v.y, a.y);
-      a.z = f.z == 0.0f ? a.z : fmaf(f.z, v.z, a.z);
-      a.w = f.w == 0.0f ? a.w : fmaf(f.w, v.w, a.w);
-    };
-    if (few) {
-      const int d = t >> 7, dim = t & 127;
-      constexpr int kQuads = kFewRows / 4, kBatch = 2;
-      const int place = ((d * 16 + row0 / 4) * 128 + dim) * 4;
-      float4 acc[kQuads], v[kBatch][kQuads];
-      auto load = [&](int s0) {
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-#pragma unroll
-          for (int r = 0; r < kQuads; ++r)
-            v[k][r] = s0 + k < j.parts && row0 + 4 * r < j.rows
-                          ? *reinterpret_cast<const float4*>(part(s0 + k) + place + r * 512)
-                          : make_float4(0.f, 0.f, 0.f, 0.f);
-      };
-      load(0);
-      factors(kFewRows);
-      __syncthreads();
-#pragma unroll
-      for (int r = 0; r < kQuads; ++r) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int s0 = 0; s0 < j.parts; s0 += kBatch) {
-        if (s0) load(s0);
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-          if (s0 + k < j.parts)
-#pragma unroll
-            for (int r = 0; r < kQuads; ++r) add(acc[r], factor4[(s0 + k) * kQuads + r], v[k][r]);
-      }
-#pragma unroll
-      for (int r = 0; r < kQuads; ++r) {
-        const float a[4] = {acc[r].x, acc[r].y, acc[r].z, acc[r].w};
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          // two rows of this dim; of the neighbour's the other one, so that a store has two dims of a row
-          const bool odd = dim & 1;
-          const float other = __shfl_xor_sync(0xffffffffu, odd ? a[i] : a[i + 1], 1);
-          const int row = row0 + 4 * r + i + (odd ? 1 : 0);
-          if (row < j.rows)
-            *reinterpret_cast<uint32_t*>(p.out + ((long long)j.first_row + row) * kLatent + d * 128 + (dim & ~1)) =
-                odd ? pack_bf16x2(other, a[i + 1]) : pack_bf16x2(a[i], other);
-        }
-      }
+    if (j.parts <= 2) {
+      join_few<4, 2>(p, j, row0, factor4, part, factors);
+    } else if (few) {
+      join_few<2, 4>(p, j, row0, factor4, part, factors);
     } else {
       const int dim0 = within % (kLatent / kManyDims) * kManyDims;  // of the 512
       const int place = (((dim0 >> 7) * 16 + row0 / 4) * 128 + (dim0 & 127) + lane) * 4;
@@ -789,7 +863,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) latent_join_kernel(const Late
         if (s0 != warp) load(s0);
 #pragma unroll
         for (int k = 0; k < kBatch; ++k)
-          if (s0 + k * kJoinWarps < j.parts) add(acc, factor4[s0 + k * kJoinWarps], v[k]);
+          if (s0 + k * kJoinWarps < j.parts) add_part(acc, factor4[s0 + k * kJoinWarps], v[k]);
       }
       sums[warp][lane] = acc;
       __syncthreads();
@@ -826,7 +900,7 @@ cudaError_t launch_latent(LatentParams p, int ctas, cudaStream_t stream) {
     return cudaFuncSetAttribute(latent_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   });
   if (e != cudaSuccess) return e;
-  p.min_units = 4;
+  p.min_units = 2;
   p.l2_tiles = (64 << 20) / kTileBytes;
   // Programmatic dependents: launched while the kernel before them ends; they wait for it before any global access.
   cudaLaunchAttribute attr[1];
@@ -852,7 +926,7 @@ cudaError_t launch_latent(LatentParams p, int ctas, cudaStream_t stream) {
 extern "C" {
 
 long long nvb_latent_scratch_floats(int num_sms) {
-  return num_sms < 1 || num_sms > nvb::latent_detail::kMaxCtas ? 0 : (long long)num_sms * nvb::latent_detail::kCtaFloats;
+  return num_sms < 1 || num_sms > 1024 ? 0 : (long long)num_sms * nvb::latent_detail::kCtaFloats;
 }
 
 int nvb_paged_latent_fwd(void* stream, const void* q, const void* cache, void* out, const int* cu_q,
@@ -896,7 +970,8 @@ int nvb_paged_latent_fwd(void* stream, const void* q, const void* cache, void* o
   p.table_stride = table_stride;
   p.num_blocks = num_blocks;
   p.scale = scale;
-  return cuda_status(nvb::launch_latent(p, int(fit < sms ? fit : sms), static_cast<cudaStream_t>(stream)),
+  const int most = sms < nvb::latent_detail::kMaxCtas ? sms : nvb::latent_detail::kMaxCtas;
+  return cuda_status(nvb::launch_latent(p, int(fit < most ? fit : most), static_cast<cudaStream_t>(stream)),
                      "latent attention launch");
 }
 
