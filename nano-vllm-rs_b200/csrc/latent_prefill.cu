@@ -110,7 +110,8 @@ __device__ __forceinline__ Sizes sizes(const LatentPrefillParams& p, int b) {
 }
 
 // Items in the order of their claims: by sequence (the longest first, up to kMaxOrdered sequences), its last queries
-// first, heads next to one another. A warp looks at 32 sequences at a time.
+// first, heads next to one another. Tiles are paired from the sequence's end, so that one without a partner, whose steps
+// take as long as a pair's, is the one with the fewest keys. A warp looks at 32 sequences at a time.
 struct Cursor {
   int r0 = -32, base = 0;        // first of the 32, items before them
   int b = -1, items = 0, upto = 0;  // this lane's sequence, its items, items up to and with it among the 32
@@ -147,7 +148,7 @@ __device__ __forceinline__ Item find_item(const LatentPrefillParams& p, const ui
   const int l = __ffs(__ballot_sync(0xffffffffu, c.base + c.upto > v)) - 1;
   const int b = __shfl_sync(0xffffffffu, c.b, l), items = __shfl_sync(0xffffffffu, c.items, l);
   const int within = v - c.base - (__shfl_sync(0xffffffffu, c.upto, l) - items);
-  const int row = within / p.heads, place = items / p.heads - 1 - row;
+  const int row = within / p.heads;
   const Sizes s = sizes(p, b);
   it.b = b;
   it.h = within - row * p.heads;
@@ -155,10 +156,11 @@ __device__ __forceinline__ Item find_item(const LatentPrefillParams& p, const ui
   it.k_begin = s.k_begin;
   it.keys = s.keys;
   it.prefix = s.keys - s.n;
+  const int pair = p.item_rows / kRows, first = (s.q_len + kRows - 1) / kRows - pair * (row + 1);  // tile; -1: tile 0 alone
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    it.q0[x] = place * p.item_rows + x * kRows;
-    it.qx[x] = x * kRows < p.item_rows ? max(0, min(kRows, s.q_len - it.q0[x])) : 0;
+    it.q0[x] = (max(first, 0) + x) * kRows;
+    it.qx[x] = x < pair + min(first, 0) ? min(kRows, s.q_len - it.q0[x]) : 0;
     const int end = it.qx[x] ? max(0, min(s.keys, it.prefix + it.q0[x] + it.qx[x])) : 0;
     it.n[x] = (end + kKeys - 1) / kKeys;
     it.full[x] = max(0, min(s.keys, it.prefix + it.q0[x] + 1)) / kKeys;
@@ -618,11 +620,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 16 * real + lane; e < 16 * kKeys; e += 32) *piece(e) = make_uint4(0, 0, 0, 0);
           // the first key that a query which visits the tile does not see
           const int unseen = it.prefix + 1 + (j < it.n[0] ? it.q0[0] : it.q0[1]);
-          for (int e = 16 * max(0, min(unseen - key0, real)) + lane; e < 16 * real; e += 32) {
+          const int from = 16 * max(0, min(unseen - key0, real)) + lane;
+          // Looked for first: x * 0 adds NaN to a sum where x is not finite. The tile's PV waits for this (a test and a
+          // branch a piece took 8,000 cycles for a whole tile, of an item's ~20,000).
+          __nv_bfloat162 sum[4];
+          const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0f, 0.0f);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sum[c] = zero;
+#pragma unroll 4
+          for (int e = from; e < 16 * real; e += 32) {
             const uint4 w = *piece(e);
-            if (nonfinite(w.x) | nonfinite(w.y) | nonfinite(w.z) | nonfinite(w.w)) {
+            sum[0] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.x), zero, sum[0]);
+            sum[1] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.y), zero, sum[1]);
+            sum[2] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.z), zero, sum[2]);
+            sum[3] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.w), zero, sum[3]);
+          }
+          const __nv_bfloat162 any = __hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3]));
+          if (__hisnan(__low2bfloat16(any)) || __hisnan(__high2bfloat16(any))) {
+            bad[i & 3] = 1;
+            for (int e = from; e < 16 * real; e += 32) {
+              const uint4 w = *piece(e);
               *piece(e) = make_uint4(finite_part(w.x), finite_part(w.y), finite_part(w.z), finite_part(w.w));
-              bad[i & 3] = 1;
             }
           }
           fence_proxy_async_smem();
