@@ -20,8 +20,8 @@ namespace nvb {
 namespace latent_cache_detail {
 
 constexpr int kLatent = 512, kRope = 64, kWidth = kLatent + kRope;
-constexpr int kWarps = 8;
-constexpr int kHeadsPerWarp = 8;  // of the queries: four lanes a head, 16 values a lane
+constexpr int kWarps = 4;
+constexpr int kHeadsPerWarp = 16;  // of the queries: four lanes a head, 16 values a lane of two heads
 
 // 16 values of a 64-value rotary part: `lo` and `hi` hold its 8-value pieces c and c + 4 (c: the lane's place among
 // the head's four) or, interleaved, 2 c and 2 c + 1. Both forms take pairs 8 c .. 8 c + 7 of the table.
@@ -65,59 +65,72 @@ struct StoreParams {
   float eps;
 };
 
-// A warp takes one row's kv, or the rotary parts of eight of its query heads.
+// A warp takes one row's kv, or the rotary parts of 16 of its query heads. All that does not wait for the position is
+// loaded before it (8191 rows of 32 heads: 18.4 us, 4.8 TB/s; eight heads a warp, loaded behind the table, and CTAs of eight warps 24.9).
 __global__ void __launch_bounds__(kWarps * 32) store_kernel(const StoreParams p, const FastDiv fd_units) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const long long at = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (at >= (long long)p.rows * p.units) return;
   const int row = fd_units.div(int(at)), unit = int(at) - row * p.units;
-  const int position = p.positions[row];
-  const bool known = position >= 0 && position < p.max_positions;
   const bool is_kv = p.kv && unit == 0;
+  const int c = lane & 3;  // this lane's pairs of the table: 8 c to 8 c + 7
+  const int lo_at = p.interleaved ? 16 * c : 8 * c, hi_at = p.interleaved ? 16 * c + 8 : 32 + 8 * c;
 
-  // this lane's pairs of the table; positions outside it turn by nothing
-  const int c = lane & 3;
   float cs[8], sn[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    cs[i] = 1.0f;
-    sn[i] = 0.0f;
-  }
-  if (known && (!is_kv || lane < 4)) {
-    const float4* t = reinterpret_cast<const float4*>(p.table + (long long)position * kRope + 8 * c);
+  auto load_angles = [&] {  // positions outside the table turn by nothing
+    const int position = p.positions[row];
+    const bool known = position >= 0 && position < p.max_positions;
+    const float4* t = reinterpret_cast<const float4*>(p.table + (long long)(known ? position : 0) * kRope + 8 * c);
     const float4 c0 = t[0], c1 = t[1], s0 = t[8], s1 = t[9];
     cs[0] = c0.x, cs[1] = c0.y, cs[2] = c0.z, cs[3] = c0.w, cs[4] = c1.x, cs[5] = c1.y, cs[6] = c1.z, cs[7] = c1.w;
     sn[0] = s0.x, sn[1] = s0.y, sn[2] = s0.z, sn[3] = s0.w, sn[4] = s1.x, sn[5] = s1.y, sn[6] = s1.z, sn[7] = s1.w;
-  }
-  const int lo_at = p.interleaved ? 16 * c : 8 * c, hi_at = p.interleaved ? 16 * c + 8 : 32 + 8 * c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      cs[i] = known ? cs[i] : 1.0f;
+      sn[i] = known ? sn[i] : 0.0f;
+    }
+  };
 
   if (!is_kv) {
     const int head = (unit - (p.kv ? 1 : 0)) * kHeadsPerWarp + (lane >> 2);
-    if (head >= p.heads) return;
-    const __nv_bfloat16* src = p.q + row * p.q_row + head * p.q_head;
-    uint4 lo = *reinterpret_cast<const uint4*>(src + lo_at), hi = *reinterpret_cast<const uint4*>(src + hi_at);
-    rotate16(lo, hi, cs, sn, p.interleaved);
-    __nv_bfloat16* dst = p.q_out + row * p.o_row + head * p.o_head;
-    *reinterpret_cast<uint4*>(dst + lo_at) = lo;
-    *reinterpret_cast<uint4*>(dst + hi_at) = hi;
+    uint4 lo[2], hi[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      lo[k] = hi[k] = make_uint4(0, 0, 0, 0);
+      if (head + 8 * k < p.heads) {
+        const __nv_bfloat16* src = p.q + row * p.q_row + (head + 8 * k) * p.q_head;
+        lo[k] = *reinterpret_cast<const uint4*>(src + lo_at);
+        hi[k] = *reinterpret_cast<const uint4*>(src + hi_at);
+      }
+    }
+    load_angles();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (head + 8 * k >= p.heads) break;
+      rotate16(lo[k], hi[k], cs, sn, p.interleaved);
+      __nv_bfloat16* dst = p.q_out + row * p.o_row + (head + 8 * k) * p.o_head;
+      *reinterpret_cast<uint4*>(dst + lo_at) = lo[k];
+      *reinterpret_cast<uint4*>(dst + hi_at) = hi[k];
+    }
     return;
   }
 
-  const int slot = p.slots[row];
-  if (slot < 0 || slot >= p.num_slots) return;  // the whole warp's
   const __nv_bfloat16* src = p.kv + row * p.kv_stride;
-  __nv_bfloat16* dst = p.cache + (long long)slot * kWidth;
   uint4 x[2], w[2], lo = make_uint4(0, 0, 0, 0), hi = lo;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     x[i] = *reinterpret_cast<const uint4*>(src + (i * 32 + lane) * 8);
     w[i] = *reinterpret_cast<const uint4*>(p.weight + (i * 32 + lane) * 8);
   }
+  const int slot = p.slots[row];
   if (lane < 4) {
     lo = *reinterpret_cast<const uint4*>(src + kLatent + lo_at);
     hi = *reinterpret_cast<const uint4*>(src + kLatent + hi_at);
+    load_angles();
   }
+  if (slot < 0 || slot >= p.num_slots) return;  // the whole warp's
+  __nv_bfloat16* dst = p.cache + (long long)slot * kWidth;
   float f[2][8], eps = p.eps;
 #pragma unroll
   for (int i = 0; i < 2; ++i) unpack8(x[i], f[i]);
@@ -167,10 +180,11 @@ struct GatherParams {
   int batch, total_k, block_size, table_stride, num_blocks;
 };
 
-// A warp takes eight rows: each of eight lanes finds one row's place in the
-// cache, then all 32 move its 16-byte pieces (72 a row), all loads before the
-// stores.
-constexpr int kGatherRows = 8;
+// A warp takes four rows: each of four lanes finds one row's place in the
+// cache, then all 32 move their 16-byte pieces (72 a row), all loads before the
+// stores (145,000 keys: 56.4 us, 96 % of the copy rate; one prefix of 1000 2.3,
+// with eight rows a warp 3.0).
+constexpr int kGatherRows = 4;
 constexpr int kPieces = kWidth / 8;
 
 __global__ void __launch_bounds__(kWarps * 32) gather_kernel(const GatherParams p, const FastDiv fd_bs) {
@@ -178,7 +192,7 @@ __global__ void __launch_bounds__(kWarps * 32) gather_kernel(const GatherParams 
   const int lane = threadIdx.x & 31;
   const long long first = ((long long)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kGatherRows;
   if (first >= p.total_k) return;
-  // where lane i < 8 finds row first + i: its row of the cache, -1 for one of a bad page (zeros), -2 for none to write
+  // where lane i < 4 finds row first + i: its row of the cache, -1 for one of a bad page (zeros), -2 for none to write
   int place = -2;
   if (lane < kGatherRows && first + lane < p.total_k) {
     const int row = int(first) + lane;
