@@ -259,10 +259,12 @@ int nvb_cache_compact_paths(void* stream, void* const* k_layers, void* const* v_
  * rope (64 values), at strides of their own. The projection that expands
  * latents into keys and values reads `latent`, nvb_latent_prefill_fwd `rope`.
  * Rows of pages outside [0, num_blocks), and behind the page table, are zero;
- * rows before cu_k[0] and from cu_k[batch] on are left alone.
+ * rows before cu_k[0] and from cu_k[batch] on are left alone. latent and rope
+ * may be slices of the same rows, beside one another in each.
  *
  * Strides are multiples of 8 elements, all but the int arrays is 16-byte
- * aligned. */
+ * aligned. What these four entry points write must not overlap anything else
+ * that they are given (-1). */
 int nvb_latent_store(void* stream, const void* kv, long long kv_stride, const void* weight,
                      const int* positions, const int* slots, void* cache, const void* q,
                      long long q_row_stride, long long q_head_stride, void* q_out,

@@ -466,35 +466,15 @@ def cache_compact_paths(layers, cu_q, kv_lens, block_table, path, counts, new_kv
 LATENT_DIM, LATENT_ROPE, LATENT_WIDTH = 512, 64, 576  # of a row of the latent cache
 
 
-def _views(arguments, device):
-    """(address, address behind the last byte, name) of each argument (name, tensor, shape, type, bytes a value): of that
-    shape and type and on the device; contiguous, or with bytes 0 BF16 whose last dimension is (for slices of rows)."""
-    spans = []
-    for name, t, shape, dtype, size in arguments:
-        if t.dtype is not dtype or t.shape != shape or t.get_device() != device:
+def _refuse_misfit(arguments, device):
+    """The error for the first of the arguments (name, tensor, shape, type, whether only its last dimension has to be
+    contiguous) that does not fit; what they overlap the library checks."""
+    for name, t, shape, dtype, rows in arguments:
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not (rows or t.is_contiguous()):
             _refuse(t, shape, dtype, name, device)
-        start = t.data_ptr()
-        if t.is_contiguous():
-            spans.append((start, start + (size or 2) * t.numel(), name))
-            continue
-        if size:
-            _refuse(t, shape, dtype, name, device)
-        strides = t.stride()
-        if strides[-1] != 1 or min(strides) < 0:
+        if rows and t.stride(-1) != 1:
             raise NvbError(f"{name}'s last dimension must be contiguous")
-        last = 0
-        for n, s in zip(shape, strides):
-            last += (n - 1) * s
-        spans.append((start, start + 2 * (last + 1), name))
-    return spans
-
-
-def _apart(written, others):
-    """Refuses a written span that overlaps another."""
-    for a, z, name in written:
-        for x, y, other in others:
-            if a < y and x < z and name is not other:
-                raise NvbError(f"{name} overlaps {other}")
+    raise NvbError("the arguments do not fit")
 
 
 def _latent_cache(cache):
@@ -523,48 +503,55 @@ def latent_store(kv, weight, positions, slots, cache, *, rope_table, eps=1e-6, q
         raise NvbError("kv or q is required")
     if positions is None or rope_table is None or rope_table.dim() != 2:
         raise NvbError("positions [rows] and rope_table [positions, 64] are required")
+    if kv is not None and kv.dim() != 2:
+        raise NvbError("kv must be [rows, 576]")
     rows, max_positions = (kv if kv is not None else q).shape[0], rope_table.shape[0]
-    arguments = [("positions", positions, (rows,), i32, 4),
-                 ("rope_table", rope_table, (max_positions, LATENT_ROPE), torch.float32, 4)]
     heads = num_blocks = block_size = kv_stride = 0
     kv_at = weight_at = slots_at = cache_at = q_at = out_at = None
     strides = out_strides = (0, 0)
+    at = positions.data_ptr(), rope_table.data_ptr()
+    fine = (positions.dtype is i32 and positions.shape == (rows,) and positions.is_contiguous()
+            and positions.get_device() == device and rope_table.dtype is torch.float32
+            and rope_table.shape[1] == LATENT_ROPE and rope_table.is_contiguous() and rope_table.get_device() == device)
     if kv is not None:
         if weight is None or slots is None or cache is None:
             raise NvbError("weight, slots and cache go with kv")
-        num_blocks, block_size, _ = shape = _latent_cache(cache)
-        arguments += (("kv", kv, (rows, LATENT_WIDTH), bf16, 0), ("slots", slots, (rows,), i32, 4),
-                      ("weight", weight, (LATENT_DIM,), bf16, 2), ("cache", cache, shape, bf16, 2))
+        num_blocks, block_size, _ = _latent_cache(cache)
+        kv_at, weight_at, slots_at, cache_at = kv.data_ptr(), weight.data_ptr(), slots.data_ptr(), cache.data_ptr()
+        kv_stride = kv.stride(0) if rows > 1 else LATENT_WIDTH
+        fine = (fine and kv.dtype is bf16 and kv.shape == (rows, LATENT_WIDTH) and kv.stride(1) == 1
+                and kv.get_device() == device and weight.dtype is bf16 and weight.shape == (LATENT_DIM,)
+                and weight.is_contiguous() and weight.get_device() == device and slots.dtype is i32
+                and slots.shape == (rows,) and slots.is_contiguous() and slots.get_device() == device
+                and cache.dtype is bf16 and cache.is_contiguous() and cache.get_device() == device)
     elif weight is not None or slots is not None or cache is not None:
         raise NvbError("weight, slots and cache go with kv")
     if q is not None:
         if q.dim() != 3:
             raise NvbError("q must be [rows, heads, 64]")
-        heads = q.shape[1]
-        arguments.append(("q", q, (rows, heads, LATENT_ROPE), bf16, 0))
-        if q_out is not None:
-            arguments.append(("q_out", q_out, (rows, heads, LATENT_ROPE), bf16, 0))
+        if q_out is None:
+            q_out = q
+        heads, strides, out_strides = q.shape[1], q.stride(), q_out.stride()
+        q_at, out_at = q.data_ptr(), q_out.data_ptr()
+        shape = (rows, heads, LATENT_ROPE)
+        fine = (fine and q.dtype is bf16 and q.shape == shape and strides[-1] == 1 and q.get_device() == device
+                and q_out.dtype is bf16 and q_out.shape == shape and out_strides[-1] == 1
+                and q_out.get_device() == device)
     elif q_out is not None:
         raise NvbError("q_out goes with q")
-    spans = _views(arguments, device)
-    written = []
-    if kv is not None:
-        kv_at, slots_at, weight_at, cache_at = spans[2][0], spans[3][0], spans[4][0], spans[5][0]
-        kv_stride = kv.stride(0) if rows > 1 else LATENT_WIDTH
-        written.append(spans[5])
-    if q is not None:
-        strides = out_strides = q.stride()
-        q_at = out_at = spans[6 if kv is not None else 2][0]
-        if q_out is not None:
-            out_at, out_strides = spans[-1][0], q_out.stride()
-            if out_at == q_at and out_strides[:2] == strides[:2]:
-                spans.pop()  # in place
-        written.append(spans[-1])
-    _apart(written, spans)
+    if not fine:
+        arguments = [("positions", positions, (rows,), i32, False),
+                     ("rope_table", rope_table, (max_positions, LATENT_ROPE), torch.float32, False)]
+        if kv is not None:
+            arguments += [("kv", kv, (rows, LATENT_WIDTH), bf16, True), ("weight", weight, (LATENT_DIM,), bf16, False),
+                          ("slots", slots, (rows,), i32, False), ("cache", cache, cache.shape, bf16, False)]
+        if q is not None:
+            arguments += [("q", q, shape, bf16, True), ("q_out", q_out, shape, bf16, True)]
+        _refuse_misfit(arguments, device)
     _check(library().nvb_latent_store(
-        _raw_stream(stream, device), kv_at, kv_stride, weight_at, spans[0][0], slots_at, cache_at, q_at, strides[0],
+        _raw_stream(stream, device), kv_at, kv_stride, weight_at, at[0], slots_at, cache_at, q_at, strides[0],
         strides[1], out_at, out_strides[0], out_strides[1], rows, heads, interleaved, block_size, num_blocks, eps,
-        spans[1][0], max_positions))
+        at[1], max_positions))
 
 
 def latent_gather(cache, block_table, cu_k, latent, rope, *, stream=None):
@@ -575,25 +562,24 @@ def latent_gather(cache, block_table, cu_k, latent, rope, *, stream=None):
 
     device, i32, bf16 = torch.cuda.current_device(), torch.int32, torch.bfloat16
     num_blocks, block_size, _ = shape = _latent_cache(cache)
-    if block_table.dim() != 2 or latent.dim() != 2:
+    if block_table.dim() != 2 or latent.dim() != 2 or rope.dim() != 2:
         raise NvbError("block_table and latent must have rows")
     (batch, table_stride), total_k = block_table.shape, latent.shape[0]
-    spans = _views((("cache", cache, shape, bf16, 2), ("block_table", block_table, (batch, table_stride), i32, 4),
-                    ("cu_k", cu_k, (batch + 1,), i32, 4), ("latent", latent, (total_k, LATENT_DIM), bf16, 0),
-                    ("rope", rope, (total_k, LATENT_ROPE), bf16, 0)), device)
+    if not (cache.dtype is bf16 and cache.is_contiguous() and cache.get_device() == device
+            and block_table.dtype is i32 and block_table.is_contiguous() and block_table.get_device() == device
+            and cu_k.dtype is i32 and cu_k.shape == (batch + 1,) and cu_k.is_contiguous()
+            and cu_k.get_device() == device
+            and latent.dtype is bf16 and latent.shape[1] == LATENT_DIM and latent.stride(1) == 1
+            and latent.get_device() == device
+            and rope.dtype is bf16 and rope.shape == (total_k, LATENT_ROPE) and rope.stride(1) == 1
+            and rope.get_device() == device):
+        _refuse_misfit((("cache", cache, shape, bf16, False), ("block_table", block_table, block_table.shape, i32, False),
+                        ("cu_k", cu_k, (batch + 1,), i32, False), ("latent", latent, (total_k, LATENT_DIM), bf16, True),
+                        ("rope", rope, (total_k, LATENT_ROPE), bf16, True)), device)
     strides = (latent.stride(0), rope.stride(0)) if total_k > 1 else (LATENT_DIM, LATENT_ROPE)
-    _apart(spans[3:], spans[:3])
-    if strides[0] != strides[1] or not _side_by_side(spans[3][0], LATENT_DIM, spans[4][0], LATENT_ROPE, strides[0]):
-        _apart(spans[3:4], spans[4:])
-    _check(library().nvb_latent_gather(_raw_stream(stream, device), spans[0][0], spans[1][0], spans[2][0],
-                                       spans[3][0], strides[0], spans[4][0], strides[1], batch, total_k, block_size,
-                                       table_stride, num_blocks))
-
-
-def _side_by_side(a, a_values, b, b_values, stride):
-    """Whether two slices of rows `stride` values apart lie beside one another in each row."""
-    gap = (b - a) // 2
-    return a_values <= gap <= stride - b_values or b_values <= -gap <= stride - a_values
+    _check(library().nvb_latent_gather(_raw_stream(stream, device), cache.data_ptr(), block_table.data_ptr(),
+                                       cu_k.data_ptr(), latent.data_ptr(), strides[0], rope.data_ptr(), strides[1],
+                                       batch, total_k, block_size, table_stride, num_blocks))
 
 
 def latent_scratch(device):
@@ -620,19 +606,29 @@ def paged_latent_fwd(q, cache, out, cu_q, kv_lens, block_table, *, max_q, scale,
     num_blocks, block_size, _ = shape = _latent_cache(cache)
     if q.dim() != 3 or block_table.dim() != 2 or scratch is None:
         raise NvbError("q must be [total_q, heads, 576], block_table a row for each sequence, scratch latent_scratch's")
-    (total_q, heads, _), (batch, table_stride), floats = q.shape, block_table.shape, scratch.numel()
-    arguments = [("q", q, (total_q, heads, LATENT_WIDTH), bf16, 2), ("cache", cache, shape, bf16, 2),
-                 ("cu_q", cu_q, (batch + 1,), i32, 4), ("kv_lens", kv_lens, (batch,), i32, 4),
-                 ("block_table", block_table, (batch, table_stride), i32, 4),
-                 ("out", out, (total_q, heads, LATENT_DIM), bf16, 2), ("scratch", scratch, (floats,), f32, 4)]
-    if lse is not None:
-        arguments.append(("lse", lse, (total_q, heads), f32, 4))
-    spans = _views(arguments, device)
-    _apart(spans[5:], spans)
+    (total_q, heads, width), (batch, table_stride) = q.shape, block_table.shape
+    if not (q.dtype is bf16 and width == LATENT_WIDTH and q.is_contiguous() and q.get_device() == device
+            and cache.dtype is bf16 and cache.is_contiguous() and cache.get_device() == device
+            and out.dtype is bf16 and out.shape == (total_q, heads, LATENT_DIM) and out.is_contiguous()
+            and out.get_device() == device
+            and cu_q.dtype is i32 and cu_q.shape == (batch + 1,) and cu_q.is_contiguous()
+            and cu_q.get_device() == device
+            and kv_lens.dtype is i32 and kv_lens.shape == (batch,) and kv_lens.is_contiguous()
+            and kv_lens.get_device() == device
+            and block_table.dtype is i32 and block_table.is_contiguous() and block_table.get_device() == device
+            and scratch.dtype is f32 and scratch.is_contiguous() and scratch.get_device() == device
+            and (lse is None or lse.dtype is f32 and lse.shape == (total_q, heads) and lse.is_contiguous()
+                 and lse.get_device() == device)):
+        arguments = [("q", q, (total_q, heads, LATENT_WIDTH), bf16, False), ("cache", cache, shape, bf16, False),
+                     ("out", out, (total_q, heads, LATENT_DIM), bf16, False), ("cu_q", cu_q, (batch + 1,), i32, False),
+                     ("kv_lens", kv_lens, (batch,), i32, False),
+                     ("block_table", block_table, block_table.shape, i32, False),
+                     ("scratch", scratch, scratch.shape, f32, False)]
+        _refuse_misfit(arguments + ([("lse", lse, (total_q, heads), f32, False)] if lse is not None else []), device)
     _check(library().nvb_paged_latent_fwd(
-        _raw_stream(stream, device), spans[0][0], spans[1][0], spans[5][0], spans[2][0], spans[3][0], spans[4][0],
-        batch, total_q, max_q, heads, block_size, table_stride, num_blocks, scale,
-        spans[7][0] if lse is not None else None, spans[6][0], floats))
+        _raw_stream(stream, device), q.data_ptr(), cache.data_ptr(), out.data_ptr(), cu_q.data_ptr(),
+        kv_lens.data_ptr(), block_table.data_ptr(), batch, total_q, max_q, heads, block_size, table_stride, num_blocks,
+        scale, lse.data_ptr() if lse is not None else None, scratch.data_ptr(), scratch.numel()))
 
 
 def latent_prefill_fwd(q, kv, k_rope, out, cu_q, cu_k, *, max_q, scale, lse=None, stream=None):
@@ -646,21 +642,31 @@ def latent_prefill_fwd(q, kv, k_rope, out, cu_q, cu_k, *, max_q, scale, lse=None
     """
     import torch
 
-    device, bf16, i32 = torch.cuda.current_device(), torch.bfloat16, torch.int32
-    if q.dim() != 3 or kv.dim() != 3:
+    device, bf16, i32, f32 = torch.cuda.current_device(), torch.bfloat16, torch.int32, torch.float32
+    if q.dim() != 3 or kv.dim() != 3 or k_rope.dim() != 2:
         raise NvbError("q must be [total_q, heads, 192], kv [total_k, heads, 256]")
-    (total_q, heads, _), total_k, batch = q.shape, kv.shape[0], cu_q.numel() - 1
-    arguments = [("q", q, (total_q, heads, 192), bf16, 2), ("kv", kv, (total_k, heads, 256), bf16, 2),
-                 ("k_rope", k_rope, (total_k, LATENT_ROPE), bf16, 0), ("cu_q", cu_q, (batch + 1,), i32, 4),
-                 ("cu_k", cu_k, (batch + 1,), i32, 4), ("out", out, (total_q, heads, 128), bf16, 2)]
-    if lse is not None:
-        arguments.append(("lse", lse, (total_q, heads), torch.float32, 4))
-    spans = _views(arguments, device)
-    _apart(spans[5:], spans)
+    (total_q, heads, width), total_k, batch = q.shape, kv.shape[0], cu_q.numel() - 1
+    if not (q.dtype is bf16 and width == 192 and q.is_contiguous() and q.get_device() == device
+            and kv.dtype is bf16 and kv.shape == (total_k, heads, 256) and kv.is_contiguous()
+            and kv.get_device() == device
+            and k_rope.dtype is bf16 and k_rope.shape == (total_k, LATENT_ROPE) and k_rope.stride(1) == 1
+            and k_rope.get_device() == device
+            and out.dtype is bf16 and out.shape == (total_q, heads, 128) and out.is_contiguous()
+            and out.get_device() == device
+            and cu_q.dtype is i32 and cu_q.dim() == 1 and cu_q.is_contiguous() and cu_q.get_device() == device
+            and cu_k.dtype is i32 and cu_k.shape == (batch + 1,) and cu_k.is_contiguous()
+            and cu_k.get_device() == device
+            and (lse is None or lse.dtype is f32 and lse.shape == (total_q, heads) and lse.is_contiguous()
+                 and lse.get_device() == device)):
+        arguments = [("q", q, (total_q, heads, 192), bf16, False), ("kv", kv, (total_k, heads, 256), bf16, False),
+                     ("k_rope", k_rope, (total_k, LATENT_ROPE), bf16, True),
+                     ("out", out, (total_q, heads, 128), bf16, False), ("cu_q", cu_q, (batch + 1,), i32, False),
+                     ("cu_k", cu_k, (batch + 1,), i32, False)]
+        _refuse_misfit(arguments + ([("lse", lse, (total_q, heads), f32, False)] if lse is not None else []), device)
     _check(library().nvb_latent_prefill_fwd(
-        _raw_stream(stream, device), spans[0][0], spans[1][0], spans[2][0],
-        k_rope.stride(0) if total_k > 1 else LATENT_ROPE, spans[5][0], spans[3][0], spans[4][0], batch, total_q,
-        total_k, max_q, heads, scale, spans[6][0] if lse is not None else None))
+        _raw_stream(stream, device), q.data_ptr(), kv.data_ptr(), k_rope.data_ptr(),
+        k_rope.stride(0) if total_k > 1 else LATENT_ROPE, out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), batch,
+        total_q, total_k, max_q, heads, scale, lse.data_ptr() if lse is not None else None))
 
 
 def attention(q, kcache, vcache, positions, seq_indices, tables, out, *, rows, q_heads, kv_heads, head_dim,

@@ -937,8 +937,8 @@ int nvb_paged_latent_fwd(void* stream, const void* q, const void* cache, void* o
   if (!q || !cache || !out || !cu_q || !kv_lens || !block_table || batch < 1 || batch > 65535 || total_q < 1 ||
       max_q < 1 || q_heads < 1 || q_heads > 256 || block_size < 1 || table_stride < 1)
     return fail("invalid latent attention arguments");
-  if (!scratch || scratch_floats < nvb_latent_scratch_floats(1))
-    return fail("scratch must hold nvb_latent_scratch_floats(1) elements at least");
+  if (!scratch || scratch_floats < nvb_latent_scratch_floats(1) || scratch_floats > (1LL << 40))
+    return fail("scratch must hold nvb_latent_scratch_floats(1) elements at least, 2^40 at most");
   if (block_size % 64) return fail("block_size must be a multiple of 64 (got %d)", block_size);
   if ((long long)block_size * table_stride > INT_MAX || (long long)total_q * q_heads > INT_MAX)
     return fail("block_size * table_stride and total_q * q_heads must fit in int32");
@@ -950,6 +950,16 @@ int nvb_paged_latent_fwd(void* stream, const void* q, const void* cache, void* o
   if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(kv_lens) |
        reinterpret_cast<uintptr_t>(block_table) | reinterpret_cast<uintptr_t>(lse)) & 3)
     return fail("cu_q, kv_lens, block_table and lse must be 4-byte aligned");
+  const long long rows = (long long)total_q * q_heads;
+  const nvb::Stretch stretches[] = {{"out", out, rows * 1024},
+                                    {"lse", lse, rows * 4},
+                                    {"scratch", scratch, scratch_floats * 4},
+                                    {"q", q, rows * 1152},
+                                    {"cache", cache, (long long)num_blocks * block_size * 1152},
+                                    {"cu_q", cu_q, (batch + 1) * 4LL},
+                                    {"kv_lens", kv_lens, batch * 4LL},
+                                    {"block_table", block_table, (long long)batch * table_stride * 4}};
+  if (int rc = nvb::check_apart(stretches, 3)) return rc;
   const int sms = nvb::sm_count();
   if (sms < 1) return fail("the current device has no SM count");
   const long long fit = scratch_floats / nvb_latent_scratch_floats(1);

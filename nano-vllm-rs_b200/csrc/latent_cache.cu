@@ -13,7 +13,7 @@
 //
 // Both kernels move each byte once; what bounds them is HBM, and for a decode
 // step's few rows the launch and one round trip to memory.
-#include "internal.cuh"
+#include "latent_common.cuh"
 
 namespace nvb {
 
@@ -284,6 +284,21 @@ int nvb_latent_store(void* stream, const void* kv, long long kv_stride, const vo
     return fail("kv, weight, cache, q, q_out and rope_table must be 16-byte aligned");
   if ((reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slots)) & 3)
     return fail("positions and slots must be 4-byte aligned");
+  // the last value of a part of 64 at these strides, and one
+  const auto parts = [&](long long row_stride, long long head_stride) {
+    return ((rows - 1) * row_stride + (q_heads - 1) * head_stride + kRope) * 2;
+  };
+  const bool in_place = q && q_out == q && q_row_stride == out_row_stride && q_head_stride == out_head_stride;
+  const nvb::Stretch stretches[] = {
+      {"cache", kv ? cache : nullptr, kv ? (long long)block_size * num_blocks * kWidth * 2 : 0},
+      {"q_out", q ? q_out : nullptr, q ? parts(out_row_stride, out_head_stride) : 0},
+      {"q", in_place ? nullptr : q, q ? parts(q_row_stride, q_head_stride) : 0},
+      {"kv", kv, kv ? ((rows - 1) * kv_stride + kWidth) * 2 : 0},
+      {"weight", kv ? weight : nullptr, kLatent * 2},
+      {"positions", positions, rows * 4LL},
+      {"slots", kv ? slots : nullptr, rows * 4LL},
+      {"rope_table", rope_table, (long long)max_positions * kRope * 4}};
+  if (int rc = nvb::check_apart(stretches, 2)) return rc;
   StoreParams p{};
   p.kv = static_cast<const __nv_bfloat16*>(kv);
   p.weight = static_cast<const __nv_bfloat16*>(weight);
@@ -329,6 +344,19 @@ int nvb_latent_gather(void* stream, const void* cache, const int* block_table, c
     return fail("cache, latent and rope must be 16-byte aligned");
   if ((reinterpret_cast<uintptr_t>(block_table) | reinterpret_cast<uintptr_t>(cu_k)) & 3)
     return fail("block_table and cu_k must be 4-byte aligned");
+  // latent and rope may be slices of the same rows, beside one another in each
+  const long long gap = (static_cast<const char*>(rope) - static_cast<const char*>(latent)) / 2;
+  const bool beside = latent_stride == rope_stride && ((gap >= kLatent && gap + kRope <= latent_stride) ||
+                                                       (-gap >= kRope && kLatent - gap <= latent_stride));
+  const nvb::Stretch sources[] = {{"latent", latent, ((total_k - 1) * latent_stride + kLatent) * 2},
+                                  {"rope", rope, ((total_k - 1) * rope_stride + kRope) * 2},
+                                  {"cache", cache, (long long)num_blocks * block_size * kWidth * 2},
+                                  {"block_table", block_table, (long long)batch * table_stride * 4},
+                                  {"cu_k", cu_k, (batch + 1) * 4LL}};
+  for (int i = 0; i < 2; ++i)
+    for (int j = i + 1; j < 5; ++j)
+      if (!(j == 1 && beside) && nvb::overlap(sources[i], sources[j]))
+        return fail("%s overlaps %s", sources[i].name, sources[j].name);
   GatherParams p{};
   p.cache = static_cast<const __nv_bfloat16*>(cache);
   p.block_table = block_table;

@@ -5,6 +5,26 @@
 #include "prefill_common.cuh"
 
 namespace nvb {
+
+// A named stretch of memory, for the entry points' checks that what they write overlaps nothing else.
+struct Stretch {
+  const char* name;
+  const void* at;  // null: not there
+  long long bytes;
+};
+inline bool overlap(const Stretch& a, const Stretch& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.at && b.at && x < y + uintptr_t(b.bytes) && y < x + uintptr_t(a.bytes);
+}
+// The first `written` of the stretches against all: -1 with the message where two overlap.
+template <int N>
+int check_apart(const Stretch (&s)[N], int written) {
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < N; ++j)
+      if (overlap(s[i], s[j])) return api_detail::fail("%s overlaps %s", s[i].name, s[j].name);
+  return 0;
+}
+
 namespace latent_common {
 
 using namespace prefill_common;

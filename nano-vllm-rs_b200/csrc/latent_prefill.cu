@@ -796,6 +796,15 @@ int nvb_latent_prefill_fwd(void* stream, const void* q, const void* kv, const vo
     return fail("q, kv, k_rope and out must be 16-byte aligned");
   if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k) | reinterpret_cast<uintptr_t>(lse)) & 3)
     return fail("cu_q, cu_k and lse must be 4-byte aligned");
+  const long long rows = (long long)total_q * q_heads;
+  const nvb::Stretch stretches[] = {{"out", out, rows * 256},
+                                    {"lse", lse, rows * 4},
+                                    {"q", q, rows * 384},
+                                    {"kv", kv, (long long)total_k * q_heads * 512},
+                                    {"k_rope", k_rope, ((total_k - 1) * rope_stride + 64) * 2},
+                                    {"cu_q", cu_q, (batch + 1) * 4LL},
+                                    {"cu_k", cu_k, (batch + 1) * 4LL}};
+  if (int rc = nvb::check_apart(stretches, 2)) return rc;
   nvb::LatentPrefillParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.kv = static_cast<const __nv_bfloat16*>(kv);

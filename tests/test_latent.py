@@ -7,7 +7,17 @@ import numpy as np
 import pytest
 import torch
 
-P, NZ = ctypes.c_void_p, 256  # any non-null, 16-byte aligned address: what is refused is refused before use
+P = ctypes.c_void_p
+
+
+def at(i):
+    """An aligned address far from those of other i: what is refused is refused before use."""
+    return (i + 1) << 44
+
+
+def refused(nvb, code, overlap=False):
+    message = nvb.library().nvb_last_error().decode()
+    return code == -1 and ("overlaps" in message) == overlap and message != ""
 
 
 # ------------------------------------------------------------ rotary table
@@ -69,8 +79,8 @@ def test_rope_table_refusals(nvb, bad):
 
 # --------------------------------------------------------------- C entries
 def store(nvb, **kw):
-    a = dict(kv=NZ, kv_stride=576, weight=NZ, positions=NZ, slots=NZ, cache=NZ, q=NZ, qr=192, qh=64, out=NZ, outr=1024,
-             outh=64, rows=2, heads=2, inter=0, bs=64, blocks=2, eps=1e-6, table=NZ, maxp=4)
+    a = dict(kv=at(0), kv_stride=576, weight=at(1), positions=at(2), slots=at(3), cache=at(4), q=at(5), qr=192, qh=64, out=at(6), outr=1024,
+             outh=64, rows=2, heads=2, inter=0, bs=64, blocks=2, eps=1e-6, table=at(7), maxp=4)
     a.update(kw)
     return nvb.library().nvb_latent_store(
         None, a["kv"], a["kv_stride"], a["weight"], a["positions"], a["slots"], a["cache"], a["q"], a["qr"], a["qh"],
@@ -83,16 +93,15 @@ def store(nvb, **kw):
     dict(cache=None), dict(out=None), dict(rows=0), dict(heads=0), dict(heads=1025), dict(maxp=0), dict(bs=0),
     dict(blocks=0), dict(bs=65536, blocks=65536), dict(eps=-1.0), dict(eps=0.0), dict(eps=math.nan), dict(kv_stride=568),
     dict(kv_stride=580), dict(qr=100), dict(qh=-64), dict(outr=96), dict(outh=32), dict(outr=64, outh=64),
-    dict(outr=1024, outh=1024), dict(outr=2 ** 40), dict(kv=NZ + 2), dict(q=NZ + 8), dict(out=NZ + 8),
-    dict(cache=NZ + 8), dict(table=NZ + 4), dict(positions=NZ + 2), dict(slots=NZ + 1),
+    dict(outr=1024, outh=1024), dict(outr=2 ** 40), dict(kv=at(60) + 2), dict(q=at(60) + 8), dict(out=at(60) + 8),
+    dict(cache=at(60) + 8), dict(table=at(60) + 4), dict(positions=at(60) + 2), dict(slots=at(60) + 1),
     dict(rows=2 ** 31 - 1, outr=64, outh=2 ** 31 - 8)])
 def test_store_refusals(nvb, bad):
-    assert store(nvb, **bad) == -1
-    assert nvb.library().nvb_last_error().decode()
+    assert refused(nvb, store(nvb, **bad))
 
 
 def gather(nvb, **kw):
-    a = dict(cache=NZ, table=NZ, cu=NZ, latent=NZ, ls=512, rope=NZ, rs=64, batch=1, total=1, bs=64, stride=1, blocks=1)
+    a = dict(cache=at(0), table=at(1), cu=at(2), latent=at(3), ls=512, rope=at(4), rs=64, batch=1, total=1, bs=64, stride=1, blocks=1)
     a.update(kw)
     return nvb.library().nvb_latent_gather(None, a["cache"], a["table"], a["cu"], a["latent"], a["ls"], a["rope"],
                                            a["rs"], a["batch"], a["total"], a["bs"], a["stride"], a["blocks"])
@@ -101,17 +110,16 @@ def gather(nvb, **kw):
 @pytest.mark.parametrize("bad", [
     dict(cache=None), dict(table=None), dict(cu=None), dict(latent=None), dict(rope=None), dict(batch=0),
     dict(batch=65536), dict(total=0), dict(bs=0), dict(stride=0), dict(blocks=0), dict(bs=2 ** 16, blocks=2 ** 16),
-    dict(ls=504), dict(ls=516), dict(rs=32), dict(rs=66), dict(cache=NZ + 8), dict(latent=NZ + 2), dict(rope=NZ + 8),
-    dict(table=NZ + 2), dict(cu=NZ + 1)])
+    dict(ls=504), dict(ls=516), dict(rs=32), dict(rs=66), dict(cache=at(60) + 8), dict(latent=at(60) + 2), dict(rope=at(60) + 8),
+    dict(table=at(60) + 2), dict(cu=at(60) + 1)])
 def test_gather_refusals(nvb, bad):
-    assert gather(nvb, **bad) == -1
-    assert nvb.library().nvb_last_error().decode()
+    assert refused(nvb, gather(nvb, **bad))
 
 
 def absorbed(nvb, **kw):
     L = nvb.library()
-    a = dict(q=NZ, cache=NZ, out=NZ, cu=NZ, lens=NZ, table=NZ, batch=1, total=1, max_q=1, heads=16, bs=64, stride=1,
-             blocks=1, scale=1.0, lse=None, scratch=NZ, floats=L.nvb_latent_scratch_floats(1))
+    a = dict(q=at(0), cache=at(1), out=at(2), cu=at(3), lens=at(4), table=at(5), batch=1, total=1, max_q=1, heads=16, bs=64, stride=1,
+             blocks=1, scale=1.0, lse=None, scratch=at(6), floats=L.nvb_latent_scratch_floats(1))
     a.update(kw)
     return L.nvb_paged_latent_fwd(None, a["q"], a["cache"], a["out"], a["cu"], a["lens"], a["table"], a["batch"],
                                   a["total"], a["max_q"], a["heads"], a["bs"], a["stride"], a["blocks"], a["scale"],
@@ -123,12 +131,11 @@ def absorbed(nvb, **kw):
     dict(scratch=None), dict(batch=0), dict(batch=65536), dict(total=0), dict(max_q=0), dict(heads=0), dict(heads=257),
     dict(bs=0), dict(bs=32), dict(bs=96), dict(stride=0), dict(bs=2 ** 16, stride=2 ** 16),
     dict(total=2 ** 30, heads=16), dict(blocks=0), dict(bs=2 ** 16, blocks=2 ** 16), dict(scale=0.0),
-    dict(scale=math.nan), dict(scale=math.inf), dict(scale=-1.0), dict(q=NZ + 8), dict(cache=NZ + 2), dict(out=NZ + 8),
-    dict(scratch=NZ + 4), dict(cu=NZ + 2), dict(lens=NZ + 1), dict(table=NZ + 2), dict(lse=NZ + 2), dict(floats=0),
+    dict(scale=math.nan), dict(scale=math.inf), dict(scale=-1.0), dict(q=at(60) + 8), dict(cache=at(60) + 2), dict(out=at(60) + 8),
+    dict(scratch=at(60) + 4), dict(cu=at(60) + 2), dict(lens=at(60) + 1), dict(table=at(60) + 2), dict(lse=at(60) + 2), dict(floats=0),
     dict(floats=-5)])
 def test_absorbed_refusals(nvb, bad):
-    assert absorbed(nvb, **bad) == -1
-    assert nvb.library().nvb_last_error().decode()
+    assert refused(nvb, absorbed(nvb, **bad))
 
 
 def test_scratch_goes_by_the_sms(nvb):
@@ -138,7 +145,7 @@ def test_scratch_goes_by_the_sms(nvb):
 
 
 def expanded(nvb, **kw):
-    a = dict(q=NZ, kv=NZ, rope=NZ, rs=64, out=NZ, cu_q=NZ, cu_k=NZ, batch=1, total_q=1, total_k=1, max_q=1, heads=16,
+    a = dict(q=at(0), kv=at(1), rope=at(2), rs=64, out=at(3), cu_q=at(4), cu_k=at(5), batch=1, total_q=1, total_k=1, max_q=1, heads=16,
              scale=1.0, lse=None)
     a.update(kw)
     return nvb.library().nvb_latent_prefill_fwd(None, a["q"], a["kv"], a["rope"], a["rs"], a["out"], a["cu_q"],
@@ -150,11 +157,43 @@ def expanded(nvb, **kw):
     dict(q=None), dict(kv=None), dict(rope=None), dict(out=None), dict(cu_q=None), dict(cu_k=None), dict(batch=0),
     dict(batch=65536), dict(total_q=0), dict(total_k=0), dict(max_q=0), dict(heads=0), dict(heads=257),
     dict(total_q=2 ** 30), dict(rs=56), dict(rs=68), dict(rs=2 ** 40), dict(scale=0.0), dict(scale=math.nan),
-    dict(q=NZ + 8), dict(kv=NZ + 2), dict(rope=NZ + 8), dict(out=NZ + 4), dict(cu_q=NZ + 2), dict(cu_k=NZ + 1),
-    dict(lse=NZ + 3)])
+    dict(q=at(60) + 8), dict(kv=at(60) + 2), dict(rope=at(60) + 8), dict(out=at(60) + 4), dict(cu_q=at(60) + 2), dict(cu_k=at(60) + 1),
+    dict(lse=at(60) + 3)])
 def test_expanded_refusals(nvb, bad):
-    assert expanded(nvb, **bad) == -1
-    assert nvb.library().nvb_last_error().decode()
+    assert refused(nvb, expanded(nvb, **bad))
+
+
+# --------------------------------------------------------------- overlaps
+@pytest.mark.parametrize("bad", [
+    dict(cache=at(0)), dict(cache=at(0) - 64 * 2 * 1152 + 16), dict(out=at(0) + 1024), dict(q=at(6), qr=1152),
+    dict(q=at(6) + 128), dict(q=at(4) + 16), dict(table=at(6) + 2048 + 112), dict(positions=at(4)),
+    dict(slots=at(6) + 4), dict(weight=at(4) + 64 * 2 * 1152 - 16)])
+def test_store_overlaps(nvb, bad):
+    assert refused(nvb, store(nvb, **bad), overlap=True)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(latent=at(0)), dict(rope=at(0) + 64 * 1152 - 16), dict(rope=at(3) + 16), dict(rope=at(3) + 1008),
+    dict(latent=at(4) - 16), dict(total=3, ls=576, rs=576, rope=at(3) + 1008),
+    dict(total=3, ls=576, rs=576, rope=at(3) + 1040), dict(total=3, ls=576, rs=584, rope=at(3) + 1024),
+    dict(cu=at(3)), dict(table=at(4) + 124)])
+def test_gather_overlaps(nvb, bad):
+    assert refused(nvb, gather(nvb, **bad), overlap=True)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(out=at(0)), dict(out=at(0) + 16 * 1152 - 16), dict(out=at(1) - 16), dict(scratch=at(2) + 16 * 1024 - 16),
+    dict(lse=at(6) + 64), dict(lse=at(2)), dict(cu=at(2) + 4), dict(lens=at(6)), dict(table=at(2) + 8),
+    dict(scratch=at(1) + 64 * 1152 - 16)])
+def test_absorbed_overlaps(nvb, bad):
+    assert refused(nvb, absorbed(nvb, **bad), overlap=True)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(out=at(0) + 16), dict(out=at(1) + 16 * 512 - 16), dict(out=at(2) + 112), dict(lse=at(3) + 4),
+    dict(cu_q=at(3)), dict(cu_k=at(3) + 16 * 256 - 4), dict(total_k=5, rs=576, out=at(2) + 4 * 1152 + 112)])
+def test_expanded_overlaps(nvb, bad):
+    assert refused(nvb, expanded(nvb, **bad), overlap=True)
 
 
 # ------------------------------------------------- the binding's own checks
