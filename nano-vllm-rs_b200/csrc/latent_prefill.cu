@@ -56,11 +56,10 @@ constexpr int kSCol = 0, kOCol = 256;        // S/P of tile x at kSCol + 128 x, 
 constexpr int kLaunchRegs = 128, kSoftmaxRegs = 200, kOtherRegs = 56;
 static_assert(2 * 128 * kSoftmaxRegs + 2 * 128 * kOtherRegs == kThreads * kLaunchRegs, "register split");
 
-// Empty places: one a place. Landed tiles: K alternates between two barriers, V goes round three, since the S issuer may
-// be a tile ahead of the PV issuer (across items): tile g + 2's V may land before tile g's has been looked at, tile
-// g + 3's may not. [2] else: per query tile, or alternating.
+// Empty: one a place. Landed and mended tiles alternate between two barriers: K of tile g + 2, and V behind it, takes
+// places that V of tile g leaves, so all that waits for tile g's has passed. [2] else: per query tile, or alternating.
 enum Bar {
-  kEmpty = 0, kKFull = kEmpty + kSlots, kVFull = kKFull + 2, kVReady = kVFull + 3, kQFull = kVReady + 3, kQFree = kQFull + 2, kSFull = kQFree + 2,
+  kEmpty = 0, kKFull = kEmpty + kSlots, kVFull = kKFull + 2, kVReady = kVFull + 2, kQFull = kVReady + 2, kQFree = kQFull + 2, kSFull = kQFree + 2,
   kPFull = kSFull + 2, kPVDone = kPFull + 2, kODone = kPVDone + 2, kOFree = kODone + 2, kStatsFull = kOFree + 2,
   kStatsFree = kStatsFull + 2, kItemFull = kStatsFree + 2, kItemEmpty = kItemFull + 2, kClaim = kItemEmpty + 2,
   kSDrain, kPVDrain, kNumBars
@@ -343,12 +342,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Set-up that needs no input runs beside the end of the kernel before this one.
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) mbar_init(&bars[kEmpty + s], 1);
-    for (int s = 0; s < 3; ++s) {
-      mbar_init(&bars[kVFull + s], 1);
-      mbar_init(&bars[kVReady + s], 1);
-    }
     for (int s = 0; s < 2; ++s) {
-      for (int bar : {kKFull, kQFull, kQFree, kSFull, kPVDone, kODone, kItemFull}) mbar_init(&bars[bar + s], 1);
+      for (int bar : {kKFull, kVFull, kVReady, kQFull, kQFree, kSFull, kPVDone, kODone, kItemFull}) mbar_init(&bars[bar + s], 1);
       for (int bar : {kPFull, kOFree, kStatsFull, kStatsFree}) mbar_init(&bars[bar + s], 4);
       mbar_init(&bars[kItemEmpty + s], kItemReaders);
     }
@@ -467,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           for (int j = 0; j < nt && alive; ++j) {
             const int row = it.k_begin + j * kKeys;
-            const int bar = kVFull + gv % 3;
+            const int bar = kVFull + (gv & 1);
             load(&kvmap, 128, it.h, row, bar, kTilePieces - kKPieces);
             load(&kvmap, 192, it.h, row, bar, 0);
             ++gv;
@@ -497,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // Every copy has landed before the CTA may exit (on the normal path its readers have waited for it).
       for (int g = max(0, gk - 2); g < gk; ++g) wait_warp(&bars[kKFull + (g & 1)], (g >> 1) & 1);
-      for (int g = max(0, gv - 3); g < gv; ++g) wait_warp(&bars[kVFull + g % 3], (g / 3) & 1);
+      for (int g = max(0, gv - 2); g < gv; ++g) wait_warp(&bars[kVFull + (g & 1)], (g >> 1) & 1);
       for (int x = 0; x < 2; ++x)
         if (ixq[x] > 0) wait_warp(&bars[kQFull + x], (ixq[x] - 1) & 1);
     } else if (warp == 1) {
@@ -561,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int k = kTilePieces * g + kKPieces;
             const uint32_t v0 = v_lo + uint32_t(k % kSlots) * (kPiece >> 4),
                            v1 = v_lo + uint32_t((k + 1) % kSlots) * (kPiece >> 4);
-            alive = wait(&bars[kVReady + g % 3], (g / 3) & 1);
+            alive = wait(&bars[kVReady + (g & 1)], (g >> 1) & 1);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               if (j >= it.n[x]) continue;
@@ -609,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int nt = max(it.n[0], it.n[1]);
         for (int j = 0; j < nt; ++j, ++g) {
           const int k = kTilePieces * g + kKPieces, key0 = j * kKeys;
-          alive = alive && wait_warp(&bars[kVFull + g % 3], (g / 3) & 1);
+          alive = alive && wait_warp(&bars[kVFull + (g & 1)], (g >> 1) & 1);
           if (!alive) break;
           const int real = min(kKeys, it.keys - key0);  // keys of the sequence
           // 16-byte piece i of the tile's rows, 16 a row
@@ -645,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[kVReady + g % 3]);
+          if (lane == 0) mbar_arrive(&bars[kVReady + (g & 1)]);
         }
       }
     } else {
