@@ -292,8 +292,8 @@ int nvb_latent_gather(void* stream, const void* cache, const int* block_table, c
  *    negative or longer than its table. Rows before cu_q[0] and from
  *    cu_q[batch] on are left alone. Page ids outside [0, num_blocks) mask
  *    their tokens.
- *  - max_q (the most queries of a sequence) and the lengths only guide how the
- *    work is shared out; results do not depend on the order in which CTAs run.
+ *  - max_q (the most queries of a sequence) only guides how the work is shared
+ *    out; results do not depend on the order in which CTAs run.
  *  - a key that a query does not see has no part in its result, whatever the
  *    cache holds there.
  *  - scores, row maxima and sums are FP32; each probability is rounded to BF16

@@ -161,6 +161,25 @@ def test_absorbed_ragged_batches(nvb, seed):
     Absorbed(queries, lens, [16, 32, 64, 4, 128, 8][seed], [256, 64, 128, 64, 256, 64][seed], seed=seed).go(nvb)
 
 
+@pytest.mark.parametrize("heads, queries", [(128, [1, 2, 1]), (96, [3, 1, 2]), (256, [1, 1, 2])])
+def test_absorbed_row_tiles_that_read_their_keys_together(nvb, heads, queries):
+    # more tiles than L2 is trusted with, sequences of different numbers of row tiles
+    Absorbed(queries, [30000, 12001, 20000], heads, 64, seed=heads).go(nvb)
+
+
+def test_absorbed_context_of_millions(nvb):
+    # the pages of 1024 keys over and over: each key's probability is shared by its copies
+    times = 4200
+    case = Absorbed([1], [1024], 16, 256, seed=16)
+    args = case.args()
+    args["kv_lens"] = up(np.array([1024 * times], np.int32))
+    args["block_table"] = args["block_table"].repeat(1, times)
+    out, lse = case.run(nvb, args=args)
+    want = ref.absorbed(ref.as64(case.q), ref.as64(case.cache), case.cu, case.lens, case.table, SCALE)
+    want[1] += math.log(times)
+    close(out, lse, want, 1, 576, 1024 * times / 148)
+
+
 @pytest.mark.parametrize("sms", [1, 2, 5, 37])
 def test_absorbed_with_less_scratch(nvb, sms):
     Absorbed([1, 2, 1, 1], [700, 1300, 3, 64], 48, seed=sms, scratch_sms=sms).go(nvb)
