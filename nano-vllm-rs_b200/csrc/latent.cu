@@ -897,7 +897,11 @@ cudaError_t launch_latent(LatentParams p, int ctas, cudaStream_t stream) {
   }
   static unsigned configured[kContextSlots] = {};
   cudaError_t e = once_per_context(configured, [] {
-    return cudaFuncSetAttribute(latent_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    cudaError_t r = cudaFuncSetAttribute(latent_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (r != cudaSuccess) return r;
+    // as the first kernel has it, so that an SM need not change between them
+    return cudaFuncSetAttribute(latent_join_kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                cudaSharedmemCarveoutMaxShared);
   });
   if (e != cudaSuccess) return e;
   // Runs of two units at least (one chat of 500 keys 12.5 us, with four 13.6; 2000 keys of 8 heads 12.4 and 15.2), and no
