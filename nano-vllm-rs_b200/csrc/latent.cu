@@ -28,6 +28,21 @@
 // scratch, at most two parts a CTA, and a second kernel joins them in the order
 // of the parts. The plan is worked out by each CTA from the lengths on the
 // device, so a captured call follows them.
+//
+// Roles (8 warps): warp 0 loads Q and the tiles by TMA, warp 1 issues the S
+// products, warp 2 the PV products, warps 4-7 hold 16 rows each (softmax, and 32
+// of each 128 dims at the end). Every wait is bounded; a timeout records an error
+// code, and the CTA waits for its copies and MMAs, frees TMEM and exits.
+//
+// Measured (B200, copy rate 6.55 TB/s, calls back to back in a graph): 64
+// sequences of ~4050 keys, 64 heads 74 us, of which 63 the first kernel (4.9
+// TB/s; a tile takes 2,800 to 3,300 cycles once both stages are in use, the rate
+// of HBM) and 11 the join; 16 heads 64 us; 4 of ~32400 and 32 heads 43; one of 500
+// keys 10.8. With several row tiles a sequence the chain load -> S -> softmax ->
+// PV of two stages is the time, ~2,500 cycles a tile (128 heads, 8 x 32000 keys:
+// 102 us, 700 TFLOP/s). Tried and no faster: eight softmax warps, two loading
+// threads, four more warps for the output, the parts joined by the last CTA to
+// arrive (its fences and loads in a row take 6 us and more).
 #include "latent_common.cuh"
 
 namespace nvb {
@@ -49,8 +64,8 @@ constexpr int kOCol = 128;                      // S at 0 and 64, O^T at 128 + 6
 
 // kSFull, kSFree: one per S buffer. The rows may be a tile ahead of the S issuer's look at kSFree, so the arrivals of two
 // tiles in a row must not meet in one barrier.
-enum Bar { kFull = 0, kEmpty = kFull + 2 * kUnits, kSFull = kEmpty + 2 * kUnits, kSFree = kSFull + 2, kPFull = kSFree + 2, kPVDone,
-           kQFree, kOFree, kSDrain, kPVDrain, kNumBars };
+enum Bar { kFull = 0, kEmpty = kFull + 2 * kUnits, kSFull = kEmpty + 2 * kUnits, kSFree = kSFull + 2,
+           kPFull = kSFree + 2, kPVDone, kQFree, kOFree, kSDrain, kPVDrain, kNumBars };
 constexpr int kTmemSlotOff = kNumBars * 8;
 constexpr int kPlanOff = (kTmemSlotOff + 4 + 15) & ~15;   // Plan
 constexpr int kScanOff = kPlanOff + 64;                   // long long [8] and int [8] of the warps' sums
@@ -68,7 +83,7 @@ static_assert(kSmemBytes <= 232448, "per-CTA shared memory limit");
 constexpr int kPartFloats = kRows * kLatent + 2 * kRows;
 constexpr int kCtaFloats = 2 * kPartFloats + 16;
 struct Join {
-  int first_row, rows, parts, stride;  // of the output; parts are in this CTA's scratch (1) and every stride-th CTA's behind it (0)
+  int first_row, rows, parts, stride;  // of the output; part 0 is this CTA's second, the others every stride-th CTA's first
 };
 
 // kind::f16, FP32 accumulate, BF16 A and B.

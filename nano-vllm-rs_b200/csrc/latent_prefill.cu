@@ -20,8 +20,15 @@
 // K_j leaves, K_j+2 those of V_j.
 //
 // What bounds it: the tensor core takes 2,560 cycles for a step of both tiles
-// and 128 keys, the exponentials 1,800 of the MUFU unit; the chains of softmax,
-// product and next scores of two tiles fill what is left of ~3,800 cycles.
+// and 128 keys, the exponentials 1,800 of the MUFU unit; the chain of softmax,
+// product and next scores makes it 3,900 to 4,700 (S has one buffer a tile: O and
+// S of both fill TMEM). Measured (B200, SM clock 1.65 to 1.97 GHz as the power
+// cap allows): 4 prompts of 8192 tokens, 16 heads 1.32 ms (1,040 TFLOP/s of the
+// pairs that are seen), 4 x ~506 queries behind 4000 to 8000 keys, 32 heads 250 us
+// (920), 32 prompts of 64 to 2048 255 us (720; a ragged end of a tile and the
+// masked half of the diagonal are 18 % of the work, an item's start and end ~8,000
+// cycles of ~32,000), one of 300 11.6 us. Tried and no faster: tile B started half
+// a step behind tile A, the next item looked up early, three barriers for V.
 //
 // Roles (16 warps, one CTA an SM):
 //   warp 0      claims items: a CTA that has begun takes over the indices of CTAs
