@@ -533,6 +533,9 @@ def latent_store(kv, weight, positions, slots, cache, *, rope_table, eps=1e-6, q
             q_out = q
         heads, strides, out_strides = q.shape[1], q.stride(), q_out.stride()
         q_at, out_at = q.data_ptr(), q_out.data_ptr()
+        if rows == 1 or heads == 1:  # strides of such dimensions say nothing
+            keep = (rows > 1, heads > 1, 1)
+            strides, out_strides = ([s * k for s, k in zip(x, keep)] for x in (strides, out_strides))
         shape = (rows, heads, LATENT_ROPE)
         fine = (fine and q.dtype is bf16 and q.shape == shape and strides[-1] == 1 and q.get_device() == device
                 and q_out.dtype is bf16 and q_out.shape == shape and out_strides[-1] == 1

@@ -413,12 +413,11 @@ int nvbh_rope_table(float* table, size_t positions, size_t dim, double theta, in
   const auto pair_of = [&](double turns) {
     return double(dim) * std::log(original_positions / (turns * 2.0 * pi)) / (2.0 * std::log(theta));
   };
-  std::vector<double> f(pairs);
   for (size_t i = 0; i < pairs; ++i) {
-    f[i] = std::pow(base, -2.0 * double(i) / double(dim));
+    double f = std::pow(base, -2.0 * double(i) / double(dim));
     double slowed = scaling == 1 ? 1.0 : 0.0;  // share of the pair's frequency that is divided by factor
     if (scaling == 3) {
-      const double turns = original_positions * f[i] / (2.0 * pi);
+      const double turns = original_positions * f / (2.0 * pi);
       slowed = 1.0 - std::fmin(1.0, std::fmax(0.0, (turns - slow) / (fast - slow)));
     } else if (scaling == 4) {
       const double first = std::fmax(0.0, std::floor(pair_of(fast)));
@@ -426,14 +425,12 @@ int nvbh_rope_table(float* table, size_t positions, size_t dim, double theta, in
       // where both border pairs are one, the pairs up to it keep their frequency
       slowed = std::fmin(1.0, std::fmax(0.0, (double(i) - first) / std::fmax(last - first, 1e-3)));
     }
-    f[i] *= 1.0 - slowed + slowed / (scaling ? factor : 1.0);
-  }
-  for (size_t t = 0; t < positions; ++t)
-    for (size_t i = 0; i < pairs; ++i) {
-      const double angle = double(t) * f[i];
-      table[t * dim + i] = float(std::cos(angle) * magnitude);
-      table[t * dim + pairs + i] = float(std::sin(angle) * magnitude);
+    f *= 1.0 - slowed + slowed / (scaling ? factor : 1.0);
+    for (size_t t = 0; t < positions; ++t) {
+      table[t * dim + i] = float(std::cos(double(t) * f) * magnitude);
+      table[t * dim + pairs + i] = float(std::sin(double(t) * f) * magnitude);
     }
+  }
   return 0;
 }
 

@@ -69,6 +69,7 @@ struct StoreParams {
 // loaded before it (8191 rows of 32 heads: 18.4 us, 4.8 TB/s; eight heads a warp, loaded behind the table, and CTAs of eight warps 24.9).
 __global__ void __launch_bounds__(kWarps * 32) store_kernel(const StoreParams p, const FastDiv fd_units) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the next kernel may set itself up beside this one
   const int lane = threadIdx.x & 31;
   const long long at = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (at >= (long long)p.rows * p.units) return;
@@ -189,6 +190,7 @@ constexpr int kPieces = kWidth / 8;
 
 __global__ void __launch_bounds__(kWarps * 32) gather_kernel(const GatherParams p, const FastDiv fd_bs) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the next kernel may set itself up beside this one
   const int lane = threadIdx.x & 31;
   const long long first = ((long long)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kGatherRows;
   if (first >= p.total_k) return;

@@ -28,7 +28,7 @@
 // (920), 32 prompts of 64 to 2048 255 us (720; a ragged end of a tile and the
 // masked half of the diagonal are 18 % of the work, an item's start and end ~8,000
 // cycles of ~32,000), one of 300 11.6 us. Tried and no faster: tile B started half
-// a step behind tile A, the next item looked up early, three barriers for V.
+// a step behind tile A, the next item looked up early.
 //
 // Roles (16 warps, one CTA an SM):
 //   warp 0      claims items: a CTA that has begun takes over the indices of CTAs

@@ -567,6 +567,19 @@ def test_store_in_place_queries_only_and_latents_only(nvb, interleaved):
     assert (cache[1, 1] != 0).any() and not (cache[0] != 0).any()
 
 
+def test_store_strides_of_single_rows_and_heads(nvb):
+    g, table = torch.Generator().manual_seed(2), table_of(nvb)
+    x = torch.randn(3, 5, 64, generator=g).to(torch.bfloat16).cuda()
+    positions = up(np.array([7, 8, 9], np.int32))
+    for part, at in ((x[:1], positions[:1]), (x[:, :1], positions), (x[1:2, 2:3], positions[1:2])):
+        odd = part.as_strided(part.shape, (part.stride(0) if part.shape[0] > 1 else 3,
+                                           part.stride(1) if part.shape[1] > 1 else 1, 1), part.storage_offset())
+        out = torch.zeros(part.shape, dtype=torch.bfloat16, device="cuda")
+        nvb.latent_store(None, None, at, None, None, q=odd, q_out=out, rope_table=table)
+        torch.cuda.synchronize()
+        check_rotated(ref.as64(out), ref.as64(part), table, at.cpu().numpy(), False)
+
+
 def test_store_values_at_the_ends_of_the_range(nvb):
     # zero rows (eps alone under the root), large and tiny ones; infinities and NaN stay in their row
     table = table_of(nvb)
