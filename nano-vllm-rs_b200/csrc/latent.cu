@@ -35,14 +35,14 @@
 // code, and the CTA waits for its copies and MMAs, frees TMEM and exits.
 //
 // Measured (B200, copy rate 6.55 TB/s, calls back to back in a graph): 64
-// sequences of ~4050 keys, 64 heads 74 us, of which 63 the first kernel (4.9
-// TB/s; a tile takes 2,800 to 3,300 cycles once both stages are in use, the rate
-// of HBM) and 11 the join; 16 heads 64 us; 4 of ~32400 and 32 heads 43; one of 500
-// keys 10.8. With several row tiles a sequence the chain load -> S -> softmax ->
-// PV of two stages is the time, ~2,500 cycles a tile (128 heads, 8 x 32000 keys:
-// 102 us, 700 TFLOP/s). Tried and no faster: eight softmax warps, two loading
-// threads, four more warps for the output, the parts joined by the last CTA to
-// arrive (its fences and loads in a row take 6 us and more).
+// sequences of ~4050 keys, 64 heads 68 us (4.5 TB/s over both kernels; a tile of
+// the first takes 2,800 to 3,300 cycles once both stages are in use, the rate of
+// HBM); 16 heads 60 us; 4 of ~32400 and 32 heads 41; one of 500 keys 10.9. With
+// several row tiles a sequence the chain load -> S -> softmax -> PV of two stages
+// is the time, ~2,500 cycles a tile (128 heads, 8 x 32000 keys: 100 us, 710
+// TFLOP/s). Tried and no faster: eight softmax warps, two loading threads, four
+// more warps for the output, the parts joined by the last CTA to arrive (its
+// fences and loads in a row take 6 us and more).
 #include "latent_common.cuh"
 
 namespace nvb {
@@ -139,6 +139,7 @@ struct Plan {
   long long first;  // the unit that sequence b starts at
   long long u0, u1, per;
   int b, share;
+  bool streams;  // L2 is to drop the keys first
 };
 static_assert(sizeof(Plan) <= 64, "plan's place");
 
@@ -204,7 +205,8 @@ __device__ __forceinline__ int plan_share(const LatentParams& p, long long tiles
 __device__ __forceinline__ long long units_of(const Sequence& q, int share) {
   return (long long)((q.row_tiles + share - 1) / share) * (q.tiles + 1);
 }
-__device__ __forceinline__ void plan_runs(const LatentParams& p, Plan& plan, long long total, int share, int ctas) {
+__device__ __forceinline__ void plan_runs(const LatentParams& p, Plan& plan, long long total, int share, int row_tiles,
+                                          int ctas) {
   const int groups = ctas / share, group = blockIdx.x / share;
   const long long each = total <= 0x7fffffff ? (unsigned(total) + groups - 1) / unsigned(groups)
                                              : (total + groups - 1) / groups;
@@ -212,6 +214,11 @@ __device__ __forceinline__ void plan_runs(const LatentParams& p, Plan& plan, lon
   plan.u0 = group < groups ? min(group * plan.per, total) : total;
   plan.u1 = min(plan.u0 + plan.per, total);
   plan.share = share;
+  // Keys that one CTA reads, or two at about the same time, leave L2 first, and the parts in the scratch stay there for
+  // the join: 64 sequences of ~4050 keys 74.9 -> 67.7 us, 32 of ~1000 20.8 -> 19.5, one of 32000 (16 heads) 23.8 -> 22.2.
+  // Three or four readers drift apart, and later rounds read the keys again: 16 of 500 to 8000 keys, 2 to 6 queries of
+  // 32 heads, 55.1 us without and 56.6 with it. A cache of a few MB pushes nothing out: one of 2000, 11.0 and 11.2.
+  plan.streams = (row_tiles <= 1 || share == 2) && total > p.l2_tiles / 4;
   plan.b = p.batch;  // unless a sequence has unit u0
   plan.first = total;
 }
@@ -227,7 +234,7 @@ __device__ __forceinline__ T warp_scan(T v, int lane) {
 
 // Up to 32 x kPlanEach sequences of usual sizes: every warp works the plan out for itself, in 32 bits. This stands before
 // a CTA's first load, so it has few steps that wait for one another, and few instructions to fetch for 32 sequences
-// (a batch of 32: 20.8 us, with four a lane 21.2).
+// (a batch of 32: 0.4 us less than with four a lane).
 // False where the sizes are too large for it.
 constexpr int kPlanMost = 4;
 template <int kPlanEach>
@@ -260,7 +267,7 @@ __device__ __forceinline__ bool make_plan_warp(const LatentParams& p, int ctas, 
 #pragma unroll
   for (int i = 0; i < kPlanEach; ++i) units += rounds[i] * (tiles[i] + 1);
   const int upto = warp_scan(units, lane);
-  plan_runs(p, plan, __shfl_sync(0xffffffffu, upto, 31), share, ctas);
+  plan_runs(p, plan, __shfl_sync(0xffffffffu, upto, 31), share, most, ctas);
   const int u0 = int(plan.u0);
   const unsigned has = __ballot_sync(0xffffffffu, units && upto - units <= u0 && u0 < upto);
   if (has) {
@@ -321,7 +328,7 @@ __device__ __forceinline__ void make_plan(const LatentParams& p, unsigned char* 
     total += sums[w];
   }
   Plan mine;
-  plan_runs(p, mine, total, share, ctas);
+  plan_runs(p, mine, total, share, rt, ctas);
   if (t == 0) *plan = mine;
   __syncthreads();
   if (units && upto - units <= mine.u0 && mine.u0 < upto) {
@@ -396,6 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (elect_one()) {
       tma_prefetch_desc(&qmap);
       tma_prefetch_desc(&cmap);
+      const uint64_t first_out = policy_evict_first();
       int g = 0, seg = 0;
       bool alive = true;
       while (alive && walk.next(p, plan, member, s)) {
@@ -425,8 +433,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (ok) {  // a bad page's keys are masked, whatever the tile holds
 #pragma unroll
-              for (int c = c0; c < c0 + kPieces[u]; ++c)
-                tma_load_3d_at(tile + c * kChunk, &cmap, full, c == 0 ? kLatent : (c - 1) * 64, 0, row);
+              for (int c = c0; c < c0 + kPieces[u]; ++c) {
+                const int x = c == 0 ? kLatent : (c - 1) * 64;
+                if (plan.streams)
+                  tma_load_3d_at(tile + c * kChunk, &cmap, full, x, 0, row, first_out);
+                else
+                  tma_load_3d_at(tile + c * kChunk, &cmap, full, x, 0, row);
+              }
             }
           }
           if (!alive) break;

@@ -61,6 +61,16 @@ __device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const CUtensorMap* 
       : "memory");
 }
 
+// With an L2 eviction policy.
+__device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
+                                               int c2, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+      : "memory");
+}
+
 // Whether a pair of BF16 holds an infinity or NaN: an exponent of all ones carries into the sign's place.
 __device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
   return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
