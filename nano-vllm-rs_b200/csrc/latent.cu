@@ -941,8 +941,11 @@ cudaError_t launch_latent(LatentParams p, int ctas, cudaStream_t stream) {
   p.min_units = 2;
   p.l2_tiles = (64 << 20) / kTileBytes;
   const long long rounds = ((long long)p.max_q * p.heads + kRows - 1) / kRows;
-  const long long units = (long long)p.batch * rounds * ((long long)p.table_stride * p.block_size / kKeys + 1);
-  if ((units + p.min_units - 1) / p.min_units < ctas) ctas = int((units + p.min_units - 1) / p.min_units);
+  const long long units = rounds * ((long long)p.table_stride * p.block_size / kKeys + 1);  // of one sequence, below 2^59
+  if (units < (long long)ctas * p.min_units) {
+    const long long runs = (units * p.batch + p.min_units - 1) / p.min_units;
+    if (runs < ctas) ctas = int(runs);
+  }
   // Programmatic dependents: launched while the kernel before them ends; they wait for it before any global access.
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

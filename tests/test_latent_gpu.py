@@ -190,6 +190,22 @@ def test_absorbed_max_q_only_guides(nvb, max_q):
     Absorbed([3, 1, 7], [700, 1300, 64], 32, seed=7).go(nvb, max_q=max_q)
 
 
+def test_absorbed_largest_bounds_of_a_call(nvb):
+    # the most sequences, heads and max_q and a table of a million keys: their product passes 64 bits
+    case = Absorbed([2], [700], 256, seed=17)
+    batch, page, mine = 65535, 1 << 20, 40000
+    args = case.args()
+    cache = torch.zeros(1, page, 576, dtype=torch.bfloat16, device="cuda")
+    for j in range(0, 700, case.page):
+        at, n = case.slot(0, j), min(case.page, 700 - j)
+        cache[0, j:j + n] = case.cache.view(-1, 576)[at:at + n].cuda()
+    cu, lens = torch.zeros(batch + 1, dtype=torch.int32), torch.zeros(batch, dtype=torch.int32)
+    cu[mine + 1:], lens[mine] = 2, 700
+    table = torch.zeros(batch, 1, dtype=torch.int32, device="cuda")
+    args.update(cache=cache, cu_q=cu.cuda(), kv_lens=lens.cuda(), block_table=table)
+    case.check(*case.run(nvb, args=args, max_q=2 ** 31 - 1))
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 def test_absorbed_keys_that_a_query_does_not_see(nvb, value):
     # the last two drafts' rows are not finite: the first queries' results do not change
