@@ -246,8 +246,9 @@ int nvb_cache_compact_paths(void* stream, void* const* k_layers, void* const* v_
  * and q_out are the first of `rows` x q_heads parts of 64 values, at row and
  * head strides of their own (in elements), so that they may be slices of
  * longer heads; q_out may be q itself, with the same strides, and must not
- * overlap it otherwise. kv may be null (queries only: weight, slots and cache
- * are not used), and so may q (q_heads, q_out and their strides are not used).
+ * overlap it otherwise. kv and q_out may be slices of the same rows, beside one
+ * another in each. kv may be null (queries only: weight, slots and cache are
+ * not used), and so may q (q_heads, q_out and their strides are not used).
  * Pair i of a part is its elements (i, i + 32), or (2i, 2i + 1) with
  * `interleaved`, turned by (cos, sin) = rope_table[position, i] and [position,
  * 32 + i]; rope_table is [max_positions, 64] FP32 (nvbh_rope_table, or

@@ -254,6 +254,12 @@ bool apart(long long rows, long long heads, long long row_stride, long long head
   return by_row || by_head;
 }
 
+// Whether x and y, of `x_len` and `y_len` elements a row, lie beside one another in rows that are `stride` long.
+bool beside(const void* x, long long x_len, const void* y, long long y_len, long long stride) {
+  const long long gap = (static_cast<const char*>(y) - static_cast<const char*>(x)) / 2;
+  return (gap >= x_len && gap + y_len <= stride) || (-gap >= y_len && x_len - gap <= stride);
+}
+
 }  // namespace latent_cache_detail
 }  // namespace nvb
 
@@ -300,7 +306,13 @@ int nvb_latent_store(void* stream, const void* kv, long long kv_stride, const vo
       {"positions", positions, rows * 4LL},
       {"slots", kv ? slots : nullptr, rows * 4LL},
       {"rope_table", rope_table, (long long)max_positions * kRope * 4}};
-  if (int rc = nvb::check_apart(stretches, 2)) return rc;
+  // the queries and kv may be slices of the same rows, those of one projection
+  const bool same_rows = kv && q && kv_stride == out_row_stride &&
+                         beside(kv, kWidth, q_out, (q_heads - 1) * out_head_stride + kRope, kv_stride);
+  for (int i = 0; i < 2; ++i)
+    for (int j = i + 1; j < 8; ++j)
+      if (!(i == 1 && j == 3 && same_rows) && nvb::overlap(stretches[i], stretches[j]))
+        return fail("%s overlaps %s", stretches[i].name, stretches[j].name);
   StoreParams p{};
   p.kv = static_cast<const __nv_bfloat16*>(kv);
   p.weight = static_cast<const __nv_bfloat16*>(weight);
@@ -347,9 +359,7 @@ int nvb_latent_gather(void* stream, const void* cache, const int* block_table, c
   if ((reinterpret_cast<uintptr_t>(block_table) | reinterpret_cast<uintptr_t>(cu_k)) & 3)
     return fail("block_table and cu_k must be 4-byte aligned");
   // latent and rope may be slices of the same rows, beside one another in each
-  const long long gap = (static_cast<const char*>(rope) - static_cast<const char*>(latent)) / 2;
-  const bool beside = latent_stride == rope_stride && ((gap >= kLatent && gap + kRope <= latent_stride) ||
-                                                       (-gap >= kRope && kLatent - gap <= latent_stride));
+  const bool same_rows = latent_stride == rope_stride && beside(latent, kLatent, rope, kRope, rope_stride);
   const nvb::Stretch sources[] = {{"latent", latent, ((total_k - 1) * latent_stride + kLatent) * 2},
                                   {"rope", rope, ((total_k - 1) * rope_stride + kRope) * 2},
                                   {"cache", cache, (long long)num_blocks * block_size * kWidth * 2},
@@ -357,7 +367,7 @@ int nvb_latent_gather(void* stream, const void* cache, const int* block_table, c
                                   {"cu_k", cu_k, (batch + 1) * 4LL}};
   for (int i = 0; i < 2; ++i)
     for (int j = i + 1; j < 5; ++j)
-      if (!(j == 1 && beside) && nvb::overlap(sources[i], sources[j]))
+      if (!(j == 1 && same_rows) && nvb::overlap(sources[i], sources[j]))
         return fail("%s overlaps %s", sources[i].name, sources[j].name);
   GatherParams p{};
   p.cache = static_cast<const __nv_bfloat16*>(cache);

@@ -172,6 +172,21 @@ def test_store_overlaps(nvb, bad):
     assert refused(nvb, store(nvb, **bad), overlap=True)
 
 
+# queries and latents in rows of one projection, 10 heads of 192 and the 576 of kv in either order: what fits is only
+# refused for its number of rows, looked at last
+@pytest.mark.parametrize("q, kv, stride, fits", [
+    (256, 3840, 2496, True), (1152 + 256, 0, 2496, True), (0, 3600, 2496, True), (256, 3824, 2496, False),
+    (256, 3856, 2496, True),   # kv ends at element 2504, the next row's first part begins at 2496 + 128
+    (256, 3840, 2488, True),   # 2496 and 2488 + 128
+    (256, 3840, 2368, True), (256, 3840, 2360, False),  # 2496 and 2368 + 128, 2360 + 128
+    (1152 - 16, 0, 2496, False), (1152 + 256, 0, 2488, False)])
+def test_store_of_one_projection(nvb, q, kv, stride, fits):
+    part = dict(q=at(8) + q, qr=stride, qh=192, out=at(8) + q, outr=stride, outh=192, heads=10)
+    code = store(nvb, rows=2 ** 31 - 1, kv=at(8) + kv, kv_stride=stride, **part)
+    assert refused(nvb, code, overlap=not fits)
+    assert not fits or "too many rows" in nvb.library().nvb_last_error().decode()
+
+
 @pytest.mark.parametrize("bad", [
     dict(latent=at(0)), dict(rope=at(0) + 64 * 1152 - 16), dict(rope=at(3) + 16), dict(rope=at(3) + 1008),
     dict(latent=at(4) - 16), dict(total=3, ls=576, rs=576, rope=at(3) + 1008),

@@ -583,6 +583,27 @@ def test_store_in_place_queries_only_and_latents_only(nvb, interleaved):
     assert (cache[1, 1] != 0).any() and not (cache[0] != 0).any()
 
 
+@pytest.mark.parametrize("kv_first", [False, True])
+def test_store_of_one_projection(nvb, kv_first):
+    # queries and latents are slices of the same rows, the queries turned in place
+    g, table = torch.Generator().manual_seed(3), table_of(nvb)
+    x = torch.randn(37, 5 * 192 + 576, generator=g).to(torch.bfloat16).cuda()
+    kv, q = (x[:, :576], x[:, 576:]) if kv_first else (x[:, 5 * 192:], x[:, :5 * 192])
+    q, before = q.view(37, 5, 192), ref.as64(x)
+    turned = torch.zeros(37, 5, 64, dtype=torch.bfloat16, device="cuda")
+    caches = torch.zeros(2, 1, 64, 576, dtype=torch.bfloat16, device="cuda")
+    weight, positions = torch.ones(512, dtype=torch.bfloat16, device="cuda"), up(np.arange(37, dtype=np.int32) * 5)
+    slots = up(np.arange(37, dtype=np.int32))
+    nvb.latent_store(kv.clone(), weight, positions, slots, caches[0], q=q[..., 128:].clone(), q_out=turned, rope_table=table)
+    nvb.latent_store(kv, weight, positions, slots, caches[1], q=q[..., 128:], rope_table=table)
+    torch.cuda.synchronize()
+    assert torch.equal(caches[0], caches[1]) and torch.equal(q[..., 128:], turned)
+    want = torch.from_numpy(before).to(torch.bfloat16).cuda()
+    parts = want[:, 576:] if kv_first else want[:, :5 * 192]
+    parts.view(37, 5, 192)[..., 128:] = turned
+    assert torch.equal(x, want)
+
+
 def test_store_strides_of_single_rows_and_heads(nvb):
     g, table = torch.Generator().manual_seed(2), table_of(nvb)
     x = torch.randn(3, 5, 64, generator=g).to(torch.bfloat16).cuda()
