@@ -121,7 +121,7 @@ __device__ __forceinline__ bool any_of_four_warps(bool yes) {
 // each tile, and group i takes units [i * per, (i + 1) * per). (Equal ranges of
 // each sequence, a CTA having one, were no faster where they fit: 64 sequences of
 // ~4050 keys and 64 heads on 128 of the SMs 73.5 us, by runs 74.6; 16 heads 67.5
-// and 64.)
+// and 64; all before the keys left L2 first.)
 struct Sequence {
   int begin, n, len, tiles, row_tiles;
 };
