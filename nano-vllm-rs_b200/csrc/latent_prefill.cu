@@ -88,7 +88,7 @@ constexpr int kClaimOff = (kBadOff + 16 + 15) & ~15;        // 16 bytes: the ans
 constexpr int kItemOff = kClaimOff + 16;                    // Item [2]
 constexpr int kStatsOff = (kItemOff + 2 * int(sizeof(Item)) + 15) & ~15;  // float [2][128]: 1 / l
 constexpr int kOrderOff = kStatsOff + 2 * kRows * 4;        // uint16 [kMaxOrdered]: sequences, the longest first
-constexpr int kHeadBytes = 3072;
+constexpr int kHeadBytes = 3 * 1024;
 static_assert(kOrderOff + kMaxOrdered * 2 <= kHeadBytes && 2 * kRows >= kMaxOrdered, "head layout");
 constexpr int kQOff = kHeadBytes;
 constexpr int kRingOff = kQOff + 2 * kQPieces * kPiece;
