@@ -299,7 +299,7 @@ int nvb_latent_gather(void* stream, const void* cache, const int* block_table, c
  *    cache holds there.
  *  - scores, row maxima and sums are FP32; each probability is rounded to BF16
  *    for its product with the values: up to 2^-8 of sum p |c| beside the
- *    output's own rounding.
+ *    output's own rounding. Those below 2^-125 of a row's largest may count as 0.
  *  - scratch: FP32, nvb_latent_scratch_floats(num_sms) elements for a GPU of
  *    num_sms SMs, whatever the batch (fewer make the call use fewer SMs; at
  *    least nvb_latent_scratch_floats(1)). Nothing is kept in it from one call

@@ -185,6 +185,25 @@ __device__ __forceinline__ bool take_item(uint64_t* bars, const Item* ring, int 
   return it.b >= 0;
 }
 
+// 2^x of a pair on the FMA pipe (x <= 128): x = n + f with n the nearest integer (by the rounding of 1.5 * 2^23 + x),
+// a polynomial of degree 4 for 2^f that is 1 at 0 (this file's fit, relative error below 2.9e-6), n added to its
+// exponent. From x = -127 down that gives 0 exactly, so that a masked key (-inf) has no part in the result whatever
+// finite value it has: 2^-125, as where inputs are clamped before the exponent reaches its end, is 7 with a value of
+// 3e38. Between -127 and -126 it is off by 2^-127 at most (below the normal numbers).
+__device__ __forceinline__ void exp2_to_zero_pair(float& a, float& b) {
+  const float xa = fmaxf(a, -127.0f), xb = fmaxf(b, -127.0f);
+  float ta, tb, na, nb, fa, fb, pa, pb;
+  add2(ta, tb, xa, xb, 12582912.0f, 12582912.0f);
+  add2(na, nb, ta, tb, -12582912.0f, -12582912.0f);
+  fma2(fa, fb, na, nb, -1.0f, -1.0f, xa, xb);
+  fma2(pa, pb, 0.009582852944731712f, 0.009582852944731712f, fa, fb, 0.055906426161527634f, 0.055906426161527634f);
+  fma2(pa, pb, pa, pb, fa, fb, 0.24024099111557007f, 0.24024099111557007f);
+  fma2(pa, pb, pa, pb, fa, fb, 0.6931241750717163f, 0.6931241750717163f);
+  fma2(pa, pb, pa, pb, fa, fb, 1.0f, 1.0f);
+  a = __int_as_float(__float_as_int(ta) * 8388608 + __float_as_int(pa));
+  b = __int_as_float(__float_as_int(tb) * 8388608 + __float_as_int(pb));
+}
+
 // exp2(s * sl2 + nm) for keys [C0, C0 + 32) of a row -> 16 packed BF16 pairs; row-sum partials accumulate in `sum`.
 // One pair in eight runs on the FMA pipe. BF16 is V's type: half a step of each probability; the sum keeps FP32.
 template <int C0>
@@ -195,7 +214,7 @@ __device__ __forceinline__ void exp32(const float (&s)[128], float sl2, float nm
     float e0 = s[c], e1 = s[c + 1];
     fma2(e0, e1, e0, e1, sl2, sl2, nm, nm);
     if ((c & 15) == 14) {
-      exp2_fma_pair(e0, e1);
+      exp2_to_zero_pair(e0, e1);
     } else {
       e0 = fast_exp2(e0);
       e1 = fast_exp2(e1);
@@ -321,8 +340,7 @@ __device__ __forceinline__ void softmax_role(const LatentPrefillParams& p, uint6
     }
     if (!alive) break;
     if (ix > 0 && !wait_warp(&bars[kStatsFree + x], (ix - 1) & 1)) break;
-    // no key seen: the sum holds only what exponents clamped at 2^-125 left; a row of NaN scores has a NaN sum
-    if (m_used == -INFINITY && !isnan(l)) l = 0.0f;
+    // no key seen: the sum is 0; a row of NaN scores has a NaN sum
     stats[x * kRows + r] = l == 0.0f ? 0.0f : 1.0f / l;
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars[kStatsFull + x]);
