@@ -296,7 +296,8 @@ int nvb_latent_gather(void* stream, const void* cache, const int* block_table, c
  *  - max_q (the most queries of a sequence) only guides how the work is shared
  *    out; results do not depend on the order in which CTAs run.
  *  - a key that a query does not see has no part in its result, whatever the
- *    cache holds there.
+ *    cache holds there. A seen key that is not finite makes the result NaN, or,
+ *    where its score is -inf, those of its elements that are not finite.
  *  - scores, row maxima and sums are FP32; each probability is rounded to BF16
  *    for its product with the values: up to 2^-8 of sum p |c| beside the
  *    output's own rounding. Those below 2^-125 of a row's largest may count as 0.

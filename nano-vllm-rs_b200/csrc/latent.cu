@@ -346,6 +346,37 @@ __device__ __forceinline__ void make_plan(const LatentParams& p, unsigned char* 
   __syncthreads();
 }
 
+// NaN where a row of O sees a key whose value there is not finite and was taken out of the tile. The key's score is then
+// an infinity or NaN: the row's sums are NaN, or its probability is 0 and the product 0 * inf, as in a tile that all rows
+// see whole. One warp's lanes, a dim of each 128 a lane (`cache` begins at it); keys [first, end), those that only some
+// rows see. A call, seldom made: in line its code lies between the loops and costs every segment 0.2 us of fetches.
+__device__ __noinline__ void put_back(const __nv_bfloat16* cache, const int* table, int first, int end, int ctx, int row0,
+                                      int rows, int num_blocks, int block_size, int heads, uint32_t taddr) {
+#pragma unroll 1
+  for (int d = 0; d < 4; ++d)
+#pragma unroll 1
+    for (int c = 0; c < rows; c += 16) {
+      uint32_t o[16];
+      tmem_ld16(taddr + 64 * d + c, o);
+      tmem_ld_wait();
+      reg_fence(o);
+#pragma unroll 1
+      for (int key = first; key < end; ++key) {
+        const int logical = key / block_size, page = table[logical];
+        if (!page_ok(page, num_blocks)) continue;
+        const long long row = (long long)page * block_size + (key - logical * block_size);
+        if (isfinite(__bfloat162float(cache[row * kWidth + d * 128]))) continue;
+        const int from = (key - ctx) * heads - row0;  // the first row that sees it
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (c + i >= from) o[i] = 0x7fffffffu;
+      }
+      __syncwarp();
+      tmem_st16(taddr + 64 * d + c, o);
+    }
+  tmem_st_wait();
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
     latent_kernel(const LatentParams p, const FastDiv fd_heads, const FastDiv fd_bs,
                   const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap cmap) {
@@ -552,6 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int lim_a = ctx + fd_heads.div(s.row0 + min(ra, s.rows - 1)),
                 lim_b = ctx + fd_heads.div(s.row0 + min(rb, s.rows - 1));
       float ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
+      bool taken = false;  // values that are not finite, out of keys that only some rows see
       int page = table[fd_bs.div(s.t0 * kKeys)];
       for (int t = s.t0; t < s.t1; ++t, ++g) {
         const int key0 = t * kKeys;
@@ -656,11 +688,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             return reinterpret_cast<uint4*>(v + ((i >> 3) & 7) * kChunk + (i >> 6) * 128 + (i & 7) * 16);
           };
           for (int i = 64 * real + me; i < 64 * kKeys; i += 128) *piece(i) = make_uint4(0, 0, 0, 0);
-          // What is not finite in a key that only some rows see makes the sums of those rows NaN by its score.
+          // What is not finite in a key that only some rows see counts for those at the end (put_back below).
           for (int i = 64 * min(real, max(0, seen - key0)) + me; i < 64 * real; i += 128) {
             const uint4 w = *piece(i);
-            if (nonfinite(w.x) | nonfinite(w.y) | nonfinite(w.z) | nonfinite(w.w))
+            if (nonfinite(w.x) | nonfinite(w.y) | nonfinite(w.z) | nonfinite(w.w)) {
               *piece(i) = make_uint4(finite_part(w.x), finite_part(w.y), finite_part(w.z), finite_part(w.w));
+              taken = true;
+            }
           }
         }
         fence_proxy_async_smem();
@@ -674,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         lb += __shfl_xor_sync(0xffffffffu, lb, off);
       }
       float* const mine = part + (s.t0 > 0 ? 0 : 1) * kPartFloats;
-      named_barrier(2, 128);  // nobody rescales any more
+      const bool mend = any_of_four_warps(taken);  // (and nobody rescales any more)
       if ((lane & 3) == 0) {
         if (s.whole) {
           alphas[ra] = la == 0.0f ? 0.0f : 1.0f / la;  // NaN stays NaN
@@ -691,6 +725,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       alive = alive && wait_warp(&bars[kPVDone], (g - 1) & 1);
       tc_fence_after();
       const int dim = quad * 32 + lane;
+      if (mend) {
+        const int end = min(ctx + fd_heads.div(s.row0 + s.rows - 1) + 1, min(s.len, s.t1 * kKeys));
+        put_back(p.cache + dim, table, max(max(seen, 0), s.t0 * kKeys), end, ctx, s.row0, s.rows, p.num_blocks, p.block_size,
+                 p.heads, lane_base + kOCol);
+      }
       // Loops kept as loops: a segment runs them once, and straight code would be fetched for it.
 #pragma unroll 1
       for (int d = 0; d < 4; ++d)

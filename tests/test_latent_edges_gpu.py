@@ -1,10 +1,14 @@
 """Values at the ends of their range in the latent-attention operators, on the
 GPU: what a query does not see has no part in its result, what it sees counts
 alike wherever it lies in a tile. Forms and tolerances of test_latent_gpu.py."""
+import math
+
+import numpy as np
 import pytest
 import torch
 
-from test_latent_gpu import Expanded
+import latent_ref as ref
+from test_latent_gpu import SCALE, Absorbed, Expanded
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +41,31 @@ def test_expanded_large_values_of_keys_that_weigh_nothing(nvb):
     case.kv[:400][far, :, 128:] = 3.3e38
     out, lse = case.run(nvb)
     assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+# ------------------------------------------------------------ absorbed form
+def same_where_not_finite(case, out, lse):
+    want = ref.absorbed(ref.as64(case.q), ref.as64(case.cache), case.cu, case.lens, case.table, SCALE)
+    rows = int(case.cu[-1])
+    o, s = ref.as64(out)[:rows], ref.as64(lse)[:rows]
+    assert np.array_equal(np.isnan(o), np.isnan(want[0])) and np.array_equal(np.isnan(s), np.isnan(want[1]))
+    assert np.isfinite(o[~np.isnan(o)]).all()
+    return want
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("queries, lens, heads, places", [
+    ([4, 1], [131, 90], 16, ((129, 3), (130, 100), (130, 511))),  # in the last tile, two keys of it seen in part
+    ([4, 1], [131, 90], 16, ((3, 3), (70, 200))),                 # in tiles that all rows see whole
+    ([5, 1], [131, 90], 33, ((126, 5), (127, 6), (128, 7))),      # row tiles of two queries, at a tile's end
+    ([70], [190], 1, ((125, 0), (130, 256), (189, 300))),         # a row tile over two tiles of keys
+    ([3, 1], [9000, 700], 8, ((8998, 130), (8999, 131), (10, 7))),  # joined from parts
+    ([2, 2], [3000, 2900], 130, ((2998, 1), (2999, 2)))])         # several row tiles, joined
+def test_absorbed_not_finite_in_seen_keys(nvb, queries, lens, heads, places, value):
+    # scores of either infinity or NaN: an infinite score makes the sums NaN, or has probability 0 and 0 * inf its element
+    case = Absorbed(queries, lens, heads, 64, seed=23)
+    for j, at in places:
+        case.cache.view(-1, 576)[case.slot(0, j), at] = value
+    want = same_where_not_finite(case, *case.run(nvb))
+    if math.isinf(value):  # both kinds are there
+        assert (np.isnan(want[0]).any(-1) & ~np.isnan(want[1])).any() and np.isnan(want[1]).any()
