@@ -429,6 +429,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   Walk walk(plan);
   Segment s;
   if (!aligned) {
+    // nothing to join: the second kernel goes by this whatever happened here
+    if (threadIdx.x == 128) *reinterpret_cast<Join*>(part + 2 * kPartFloats) = Join{0, 0, 0, 0};
   } else if (warp == 0) {
     // ---------------------------------------------------------- producer
     if (elect_one()) {

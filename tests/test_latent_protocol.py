@@ -4,6 +4,8 @@ test_ring_protocol.py: loads land in any order, the tensor core runs each
 thread's operations in their order, warps run at any pace. Each role's loop is
 restated with the parities of the source."""
 import random
+import re
+from pathlib import Path
 
 import pytest
 
@@ -184,6 +186,17 @@ def test_the_scores_need_a_barrier_a_buffer():
     with pytest.raises(AssertionError, match="alias|two phases past|passes early|not read|deadlock"):
         for seed in range(80):
             run_absorbed(seed, [7, 2], 2, one_free_barrier=True)
+
+
+def test_every_way_through_the_first_kernel_leaves_a_record():
+    # The second kernel goes by the record of each CTA, and the scratch holds anything before: where shared memory is not
+    # laid out as the roles need it, there is one with nothing to join.
+    source = (Path(__file__).resolve().parents[1] / "nano-vllm-rs_b200" / "csrc" / "latent.cu").read_text()
+    kernel = source[source.index("latent_kernel(const LatentParams p"):source.index("latent_join_kernel(")]
+    unused = re.search(r"if \(!aligned\) \{(.*?)\n  \} else if \(warp == 0\)", kernel, re.S).group(1)
+    record = "*reinterpret_cast<Join*>(part + 2 * kPartFloats) ="
+    assert f"if (threadIdx.x == 128) {record} Join{{0, 0, 0, 0}};" in unused
+    assert kernel.count(record) == 2  # and that of the rows' warps
 
 
 # ----------------------------------------------------------- expanded form
