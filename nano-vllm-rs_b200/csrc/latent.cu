@@ -902,7 +902,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) latent_join_kernel(const Late
         // one whose scores are all NaN has none either, its sum is NaN
         const float f = ml.y == 0.0f ? 0.0f : (ml.x == -INFINITY ? NAN : fast_exp2(ml.x - mx));
         factor[s * rows + warp] = f;
-        total += f == 0.0f ? 0.0f : f * ml.y;
+        total += f * ml.y;  // NaN of a part that otherwise weighs nothing stays; the sums are not infinite
       }
       total = warp_sum(total);
       const float inv = total == 0.0f ? 0.0f : 1.0f / total;

@@ -69,3 +69,17 @@ def test_absorbed_not_finite_in_seen_keys(nvb, queries, lens, heads, places, val
     want = same_where_not_finite(case, *case.run(nvb))
     if math.isinf(value):  # both kinds are there
         assert (np.isnan(want[0]).any(-1) & ~np.isnan(want[1])).any() and np.isnan(want[1]).any()
+
+
+@pytest.mark.parametrize("parts", [2, 40])
+def test_absorbed_nan_score_in_a_part_that_weighs_nothing(nvb, parts):
+    # all other keys of the part are 2^-400 of those of the others
+    case = Absorbed([1], [64 * parts * 4], 8, 64, seed=24)
+    flat, first = case.cache.view(-1, 576), [case.slot(0, j) for j in range(64 * 4)]
+    case.q[:, :, 0], case.cache[..., 0] = 16.0, 0.0
+    flat[first, 0] = -256.0
+    clean = case.run(nvb)
+    flat[case.slot(0, 77), 575] = math.nan
+    out, lse = case.run(nvb)
+    assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all()
+    assert torch.isfinite(clean[0]).all() and torch.isfinite(clean[1]).all()
