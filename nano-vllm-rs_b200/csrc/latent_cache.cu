@@ -205,9 +205,10 @@ __global__ void __launch_bounds__(kWarps * 32) gather_kernel(const GatherParams 
       else hi = mid - 1;
     }
     if (lo < p.batch && p.cu_k[lo] <= row) {
-      const int key = row - p.cu_k[lo], logical = fd_bs.div(key);
+      const long long key = (long long)row - p.cu_k[lo];  // past 32 bits behind an offset far below 0
+      const int logical = key <= INT_MAX ? fd_bs.div(int(key)) : p.table_stride;
       const int page = logical < p.table_stride ? p.block_table[(long long)lo * p.table_stride + logical] : -1;
-      place = page >= 0 && page < p.num_blocks ? page * p.block_size + (key - logical * p.block_size) : -1;
+      place = page >= 0 && page < p.num_blocks ? page * p.block_size + (int(key) - logical * p.block_size) : -1;
     }
   }
   constexpr int kEach = kGatherRows * kPieces / 32;

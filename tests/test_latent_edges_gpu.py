@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import latent_ref as ref
-from test_latent_gpu import SCALE, Absorbed, Expanded
+from test_latent_gpu import SCALE, Absorbed, Expanded, up
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,22 @@ def test_absorbed_nan_score_in_a_part_that_weighs_nothing(nvb, parts):
     out, lse = case.run(nvb)
     assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all()
     assert torch.isfinite(clean[0]).all() and torch.isfinite(clean[1]).all()
+
+
+# ------------------------------------------------------------ store, gather
+@pytest.mark.parametrize("first", [-2 ** 31, -2 ** 31 + 3, -2 ** 30, -2])
+@pytest.mark.parametrize("page", [1, 64])
+def test_gather_offsets_below_zero(nvb, first, page):
+    # the first sequence's rows are keys from -first on: behind its page table, as far as they are
+    cache = torch.randn(6, page, 576, device="cuda").to(torch.bfloat16)
+    table = np.array([[5, 0, 2], [1, 3, 4]], np.int32)
+    cu = np.array([first, 4, 4 + page], np.int32)
+    latent = torch.full((5 + page, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+    rope = torch.full((5 + page, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    nvb.latent_gather(cache, up(table), up(cu), latent, rope)
+    torch.cuda.synchronize()
+    want, flat = np.full((5 + page, 576), 7.0), ref.as64(cache).reshape(-1, 576)
+    for row in range(4 + page):
+        b, key = (0, row - first) if row < 4 else (1, row - 4)
+        want[row] = flat[table[b, key // page] * page + key % page] if key < 3 * page else 0.0
+    assert np.array_equal(np.concatenate([ref.as64(latent), ref.as64(rope)], 1), want)
