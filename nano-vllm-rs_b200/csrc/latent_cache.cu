@@ -146,12 +146,13 @@ __global__ void __launch_bounds__(kWarps * 32) store_kernel(const StoreParams p,
     return sum;
   };
   float sum = sum_squares();
-  if (__any_sync(0xffffffffu, isinf(sum))) {  // values from 2^59 on: their squares' sum has no FP32, that of 2^-70 of them has
+  // Values from 2^59 on: their squares' sum has no FP32, that of 2^-70 of them has.
+  if (__any_sync(0xffffffffu, isinf(sum / kLatent + eps))) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[i][e] *= 0x1p-70f;
-    eps = 0.0f;  // nothing beside them
+    eps = eps * 0x1p-70f * 0x1p-70f;
     sum = sum_squares();
   }
   const float inv = rsqrtf(sum / kLatent + eps);

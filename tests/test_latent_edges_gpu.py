@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import latent_ref as ref
-from test_latent_gpu import SCALE, Absorbed, Expanded, up
+from test_latent_gpu import BF16_HALF, SCALE, Absorbed, Expanded, table_of, up
 
 pytestmark = pytest.mark.gpu
 
@@ -86,6 +86,31 @@ def test_absorbed_nan_score_in_a_part_that_weighs_nothing(nvb, parts):
 
 
 # ------------------------------------------------------------ store, gather
+def stored(nvb, kv, weight, eps):
+    rows = kv.shape[0]
+    cache = torch.full((rows // 64 + 1, 64, 576), 7.0, dtype=torch.bfloat16, device="cuda")
+    nvb.latent_store(kv.cuda(), weight.cuda(), up(np.zeros(rows, np.int32)), up(np.arange(rows, dtype=np.int32)), cache,
+                     eps=eps, rope_table=table_of(nvb))
+    torch.cuda.synchronize()
+    got = ref.as64(cache).reshape(-1, 576)
+    assert (got[rows:] == 7.0).all()
+    return got[:rows]
+
+
+def near(got, want):
+    # half a BF16 step (2^-134 below the normal numbers), the FP32 norm as in test_latent_gpu.py
+    assert (np.abs(got - want) <= (BF16_HALF + 2.0 ** -20) * np.abs(want) + 2.0 ** -134).all()
+
+
+@pytest.mark.parametrize("eps", [1e30, 1e38, 3.4e38])
+def test_store_eps_beside_large_values(nvb, eps):
+    g = torch.Generator().manual_seed(32)
+    kv, weight = torch.randn(6, 576, generator=g), torch.ones(512, dtype=torch.bfloat16)
+    kv[1:] *= 2.0 ** torch.tensor([50.0, 60.0, 62.0, 64.0, 100.0])[:, None]
+    kv = kv.to(torch.bfloat16)
+    near(stored(nvb, kv, weight, eps)[:, :512], ref.normalise(ref.as64(kv)[:, :512], 1.0, float(np.float32(eps))))
+
+
 @pytest.mark.parametrize("first", [-2 ** 31, -2 ** 31 + 3, -2 ** 30, -2])
 @pytest.mark.parametrize("page", [1, 64])
 def test_gather_offsets_below_zero(nvb, first, page):
