@@ -30,7 +30,7 @@ def test_expanded_large_values_that_a_query_does_not_see(nvb, queries, keys, hea
 
 
 def test_expanded_large_values_of_keys_that_weigh_nothing(nvb):
-    # seen, with probabilities of 2^-150 and less: less than 2^-22 of the largest value for all 400 together
+    # seen, with probabilities of 2^-150 and less: all 400 of them together add less than 2^-13
     case = Expanded([200], [400], 2, seed=22)
     case.q[:, :, 0], case.kv[:, :, 0] = 16.0, 0.0
     keys = torch.arange(400)
@@ -109,6 +109,49 @@ def test_store_eps_beside_large_values(nvb, eps):
     kv[1:] *= 2.0 ** torch.tensor([50.0, 60.0, 62.0, 64.0, 100.0])[:, None]
     kv = kv.to(torch.bfloat16)
     near(stored(nvb, kv, weight, eps)[:, :512], ref.normalise(ref.as64(kv)[:, :512], 1.0, float(np.float32(eps))))
+
+
+def test_store_rows_of_large_and_ordinary_values(nvb):
+    # the sum of squares just below and above the largest float, huge values among ordinary ones, tiny rows
+    g = torch.Generator().manual_seed(31)
+    kv = torch.randn(40, 576, generator=g)
+    weight = (1 + 0.2 * torch.randn(512, generator=g)).to(torch.bfloat16)
+    for r in range(8):
+        kv[r, :512] *= 2.0 ** (55 + r)   # 512 of them: squares that sum to 2^(119 + 2 r)
+    kv[8:16, 5] = 2.0 ** torch.arange(60, 68).float()
+    kv[16, 17], kv[17, 511], kv[18, 0] = 2.0 ** 100, -2.0 ** 120, 3e38
+    kv[19, :512] = 3e38
+    kv[20, :256] *= 2.0 ** 64
+    kv[21, :512] = 1e-30
+    kv[22, :512] *= 1e-20
+    kv = kv.to(torch.bfloat16)
+    want = ref.normalise(ref.as64(kv)[:, :512], ref.as64(weight), 1e-6)
+    got = stored(nvb, kv, weight, 1e-6)
+    near(got[:, :512], want)
+    assert (got[21, :512] != 0).all()
+
+
+def test_store_infinities_stay_in_their_row(nvb):
+    g = torch.Generator().manual_seed(33)
+    kv, weight = torch.randn(6, 576, generator=g).to(torch.bfloat16), torch.ones(512, dtype=torch.bfloat16)
+    kv[1, 7], kv[3, 500], kv[4, 575] = math.inf, -math.inf, math.inf
+    got = stored(nvb, kv, weight, 1e-6)
+    x = ref.as64(kv)
+    for r in (0, 2, 4, 5):
+        near(got[r, :512], ref.normalise(x[r, :512], 1.0, 1e-6))
+    for r, at in ((1, 7), (3, 500)):  # inf / inf, and finite / inf
+        assert np.isnan(got[r, at]) and (np.delete(got[r, :512], at) == 0).all()
+    assert np.array_equal(np.isfinite(got[:, 512:]).all(1), [True, True, True, True, False, True])
+    assert np.isfinite(got[4, 512:543]).all()  # the pairs beside the infinity's
+
+
+@pytest.mark.parametrize("rows", [1, 33])
+def test_store_latents_alone(nvb, rows):
+    g = torch.Generator().manual_seed(34)
+    kv, weight = torch.randn(rows, 576, generator=g).to(torch.bfloat16), (torch.randn(512, generator=g)).to(torch.bfloat16)
+    got = stored(nvb, kv, weight, 1e-5)
+    near(got[:, :512], ref.normalise(ref.as64(kv)[:, :512], ref.as64(weight), 1e-5))
+    assert np.array_equal(got[:, 512:], ref.as64(kv)[:, 512:])  # position 0
 
 
 @pytest.mark.parametrize("first", [-2 ** 31, -2 ** 31 + 3, -2 ** 30, -2])
