@@ -65,6 +65,14 @@ def test_rope_table_scalings(nvb):
         assert np.array_equal(table(n, dim, theta, kind, 1.0, orig, 1.0, 32.0), table(n, dim, theta))
 
 
+@pytest.mark.parametrize("original, slow", [(4, 1.0), (60, 20.0), (4096, 5000.0)])
+def test_rope_table_by_pair_where_every_pair_is_slow(nvb, original, slow):
+    # the first pair turns original / (2 pi) times, fewer than `slow`, by more than a pair: all are divided
+    assert 64 * math.log(original / (slow * 2 * math.pi)) / (2 * math.log(10000.0)) < -1
+    got = nvb.host.rope_table(300, 64, 10000.0, "yarn", 8.0, original, slow, 2 * slow)
+    assert_table(got, angles(300, 64, 10000.0) / 8.0)
+
+
 @pytest.mark.parametrize("bad", [dict(positions=0), dict(dim=3), dict(dim=0), dict(theta=1.0), dict(theta=math.inf),
                                  dict(scaling="other"), dict(scaling="linear", factor=0.5),
                                  dict(scaling="base", factor=math.nan), dict(scaling="base", factor=2.0, dim=2),
