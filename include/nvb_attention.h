@@ -288,11 +288,11 @@ int nvb_latent_gather(void* stream, const void* cache, const int* block_table, c
  * [cu_q[b], cu_q[b + 1]) are the last of its kv_lens[b] tokens (bottom-right
  * causal mask): query i of n sees the first kv_lens[b] - n + i + 1 keys.
  *
- *  - lse (may be null) is [total_q, q_heads]. A query that sees no key has
- *    output 0 and lse -inf; so have all of a sequence whose kv_lens is
- *    negative or longer than its table. Rows before cu_q[0] and from
- *    cu_q[batch] on are left alone. Page ids outside [0, num_blocks) mask
- *    their tokens.
+ *  - lse (may be null) is [total_q, q_heads]. A query that sees no key (or
+ *    none with a score above -inf) has output 0 and lse -inf; so have all of
+ *    a sequence whose kv_lens is negative or longer than its table. Rows
+ *    before cu_q[0] and from cu_q[batch] on are left alone. Page ids outside
+ *    [0, num_blocks) mask their tokens.
  *  - max_q (the most queries of a sequence) only guides how the work is shared
  *    out; results do not depend on the order in which CTAs run.
  *  - a key that a query does not see has no part in its result, whatever the
@@ -330,8 +330,9 @@ long long nvb_latent_scratch_floats(int num_sms);
  * sees no key has output 0 and lse -inf, so have all of a sequence whose keys
  * are not within [0, total_k]; rows that belong to no sequence are left alone.
  * max_q must be at least the most queries of a sequence: rows past it are left
- * alone too. Keys a query does not see have no part in its result. Rounding as
- * nvb_paged_latent_fwd. Limits: q_heads at most 256, batch at most 65535. */
+ * alone too. Keys a query does not see have no part in its result, whatever
+ * they hold; a seen value that is not finite makes its element of the output
+ * infinite or NaN. Rounding as nvb_paged_latent_fwd. Limits: q_heads at most 256, batch at most 65535. */
 int nvb_latent_prefill_fwd(void* stream, const void* q, const void* kv, const void* k_rope,
                            long long rope_stride, void* out, const int* cu_q, const int* cu_k,
                            int batch, int total_q, int total_k, int max_q, int q_heads, float scale,

@@ -34,13 +34,14 @@
 // of each 128 dims at the end). Every wait is bounded; a timeout records an error
 // code, and the CTA waits for its copies and MMAs, frees TMEM and exits.
 //
-// Measured (B200, copy rate 6.55 TB/s, calls back to back in a graph): 64
-// sequences of ~4050 keys, 64 heads 68 us (4.5 TB/s over both kernels; a tile of
-// the first takes 2,800 to 3,300 cycles once both stages are in use, the rate of
-// HBM); 16 heads 60 us; 4 of ~32400 and 32 heads 41; one of 500 keys 10.9. With
-// several row tiles a sequence the chain load -> S -> softmax -> PV of two stages
-// is the time, ~2,500 cycles a tile (128 heads, 8 x 32000 keys: 100 us, 710
-// TFLOP/s). Tried and no faster: eight softmax warps, two loading threads, four
+// Measured (B200, copy rate 6.55 TB/s, calls back to back in a graph for seconds;
+// in brackets the best of a few calls, before the power cap takes SM clock from
+// 1.97 to ~1.73 GHz): 64 sequences of ~4050 keys, 64 heads 78 us (68), 3.9 TB/s
+// over both kernels (4.5), a tile of the first 2,800 to 3,300 cycles once both
+// stages are in use, the rate of HBM; 16 heads 65 us (61); 4 of ~32400 and 32
+// heads 41; one of 500 keys 11. With several row tiles a sequence the chain
+// load -> S -> softmax -> PV of two stages is the time, ~2,500 cycles a tile (128
+// heads, 8 x 32000 keys: 110 us, 650 TFLOP/s; 99, 720). Tried and no faster: eight softmax warps, two loading threads, four
 // more warps for the output, the parts joined by the last CTA to arrive (its
 // fences and loads in a row take 6 us and more).
 #include "latent_common.cuh"
@@ -52,6 +53,11 @@ namespace latent_detail {
 using namespace latent_common;
 
 constexpr int kLatent = 512, kWidth = 576;
+// Keys up to this size (half of this GPU's L2 of 126 MB) are in L2 when another row tile reads them, whenever that is.
+// Two row tiles a sequence, 8 and 40 sequences, apart and side by side: 64 MB of keys 40.5, 44.9 and 40.3, 44.7 us; 96 MB
+// 49.7, 54.5 and 48.8, 53.1; 384 MB 140, 142 and 122, 130. Three, 8 sequences: 64 MB 47.0 both, 96 MB 62.0 and 60.9, 384
+// MB 207 and 170. (Below it now the one, now the other is ahead, by up to 8 %, in two of 48 sizes by 11.)
+constexpr int kHeldBytes = 64 << 20;
 constexpr int kRows = 64;                       // rows of a CTA
 constexpr int kKeys = 64;                       // keys of a tile
 constexpr int kChunk = kKeys * 128;             // 64 keys (or rows) x 64 BF16, one swizzled piece
@@ -196,7 +202,7 @@ __device__ __forceinline__ T warp_sum(T v) {
 }
 
 // CTAs that read a round's keys together. Row tiles of one sequence then share them in L2 whatever the batch; that costs
-// CTAs where sequences have fewer row tiles than others, so it is for caches that L2 does not hold as a whole.
+// CTAs where sequences have fewer row tiles than others, so it is for batches whose keys L2 does not hold (kHeldBytes).
 __device__ __forceinline__ int plan_share(const LatentParams& p, long long tiles, int row_tiles, int ctas) {
   if (tiles <= p.l2_tiles || row_tiles <= 1) return 1;
   const int most = min(4, ctas), rounds = (row_tiles + most - 1) / most;
@@ -216,8 +222,11 @@ __device__ __forceinline__ void plan_runs(const LatentParams& p, Plan& plan, lon
   plan.share = share;
   // Keys that one CTA reads, or two at about the same time, leave L2 first, and the parts in the scratch stay there for
   // the join: 64 sequences of ~4050 keys 74.9 -> 67.7 us, 32 of ~1000 20.8 -> 19.5, one of 32000 (16 heads) 23.8 -> 22.2.
-  // Three or four readers drift apart, and later rounds read the keys again: 16 of 500 to 8000 keys, 2 to 6 queries of
-  // 32 heads, 55.1 us without and 56.6 with it. A cache of a few MB pushes nothing out: one of 2000, 11.0 and 11.2.
+  // By size, 8 sequences of one row tile without and with: 4 MB of keys 14.7 and 14.6 us, 16 MB 29.5 and 29.1, 96 MB 49.5
+  // and 48.3, 384 MB 95.3 and 91.2; pairs of row tiles, 96 MB 50.0 and 48.8, 384 MB 126 and 122. (From a quarter of
+  // l2_tiles on: below, one of 2000 keys had 11.0 and 11.2.) Three or four readers of sequences of one size gain 2 % (8 of
+  // three row tiles, 192 MB: 96.1 and 94.4), of mixed sizes they drift apart and read keys again: 16 of 500 to 8000 keys,
+  // 2 to 6 queries of 32 heads, 55.1 us without and 56.6 with it. So not for these.
   plan.streams = (row_tiles <= 1 || share == 2) && total > p.l2_tiles / 4;
   plan.b = p.batch;  // unless a sequence has unit u0
   plan.first = total;
@@ -980,7 +989,7 @@ cudaError_t launch_latent(LatentParams p, int ctas, cudaStream_t stream) {
   // Runs of two units at least (one chat of 500 keys 12.5 us, with four 13.6; 2000 keys of 8 heads 12.4 and 15.2), and no
   // more CTAs than that makes of the longest sequences that the table and max_q have room for.
   p.min_units = 2;
-  p.l2_tiles = (64 << 20) / kTileBytes;
+  p.l2_tiles = kHeldBytes / kTileBytes;
   const long long rounds = ((long long)p.max_q * p.heads + kRows - 1) / kRows;
   const long long units = rounds * ((long long)p.table_stride * p.block_size / kKeys + 1);  // of one sequence, below 2^59
   if (units < (long long)ctas * p.min_units) {

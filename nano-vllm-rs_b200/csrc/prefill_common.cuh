@@ -88,8 +88,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // polynomial for 2^f fitted to minimise relative error on [-1/2, 1/2] (this
 // file's own fit; max relative error 2.7e-6 in FP32), then n added to the
 // exponent field with one integer multiply-add. Inputs are clamped at -125,
-// so a masked key (-inf) gives 2^-125 rather than 0: ~1e-38 of a value that
-// the caller's V zeroing or row statistics make irrelevant.
+// so a masked key (-inf) gives 2^-125 rather than 0: ~2e-38 of a value that
+// the caller does not zero, nothing beside others unless it is 1e34 or more.
 __device__ __forceinline__ void exp2_fma_pair(float& a, float& b) {
   const float xa = fmaxf(a, -125.0f), xb = fmaxf(b, -125.0f);
   float ta, tb, na, nb, fa, fb, pa, pb;
