@@ -332,7 +332,8 @@ long long nvb_latent_scratch_floats(int num_sms);
  * max_q must be at least the most queries of a sequence: rows past it are left
  * alone too. Keys a query does not see have no part in its result, whatever
  * they hold; a seen value that is not finite makes its element of the output
- * infinite or NaN. Rounding as nvb_paged_latent_fwd. Limits: q_heads at most 256, batch at most 65535. */
+ * infinite or NaN. Rounding as nvb_paged_latent_fwd. Limits: q_heads at most
+ * 256, batch at most 65535. */
 int nvb_latent_prefill_fwd(void* stream, const void* q, const void* kv, const void* k_rope,
                            long long rope_stride, void* out, const int* cu_q, const int* cu_k,
                            int batch, int total_q, int total_k, int max_q, int q_heads, float scale,

@@ -422,7 +422,7 @@ int nvbh_rope_table(float* table, size_t positions, size_t dim, double theta, in
     } else if (scaling == 4) {
       const double first = std::fmax(0.0, std::floor(pair_of(fast)));
       const double last = std::fmin(double(dim - 1), std::ceil(pair_of(slow)));
-      // where both border pairs are one, the pairs up to it keep their frequency; where the first pair is behind both, none
+      // where both border pairs are one, the pairs up to it keep their frequency; where they lie before the first, none
       slowed = last < 0.0 ? 1.0 : std::fmin(1.0, std::fmax(0.0, (double(i) - first) / std::fmax(last - first, 1e-3)));
     }
     f *= 1.0 - slowed + slowed / (scaling ? factor : 1.0);

@@ -41,9 +41,10 @@
 // stages are in use, the rate of HBM; 16 heads 65 us (61); 4 of ~32400 and 32
 // heads 41; one of 500 keys 11. With several row tiles a sequence the chain
 // load -> S -> softmax -> PV of two stages is the time, ~2,500 cycles a tile (128
-// heads, 8 x 32000 keys: 110 us, 650 TFLOP/s; 99, 720). Tried and no faster: eight softmax warps, two loading threads, four
-// more warps for the output, the parts joined by the last CTA to arrive (its
-// fences and loads in a row take 6 us and more).
+// heads, 8 x 32000 keys: 110 us, 650 TFLOP/s; 99, 720). Tried and no faster:
+// eight softmax warps, two loading threads, four more warps for the output, the
+// parts joined by the last CTA to arrive (its fences and loads in a row take 6 us
+// and more).
 #include "latent_common.cuh"
 
 namespace nvb {
@@ -699,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             return reinterpret_cast<uint4*>(v + ((i >> 3) & 7) * kChunk + (i >> 6) * 128 + (i & 7) * 16);
           };
           for (int i = 64 * real + me; i < 64 * kKeys; i += 128) *piece(i) = make_uint4(0, 0, 0, 0);
-          // What is not finite in a key that only some rows see counts for those at the end (put_back below).
+          // What is not finite in a key that only some rows see counts for those at the end (put_back).
           for (int i = 64 * min(real, max(0, seen - key0)) + me; i < 64 * real; i += 128) {
             const uint4 w = *piece(i);
             if (nonfinite(w.x) | nonfinite(w.y) | nonfinite(w.z) | nonfinite(w.w)) {

@@ -187,7 +187,7 @@ struct GatherParams {
 // A warp takes four rows: each of four lanes finds one row's place in the
 // cache, then all 32 move their 16-byte pieces (72 a row), all loads before the
 // stores (153,692 keys, 354 MB: 56.4 us, 96 % of the copy rate; one prefix of
-// 1000 2.5, of which with eight rows a warp 0.7 more).
+// 1000 2.5; with eight rows a warp 0.7 more).
 constexpr int kGatherRows = 4;
 constexpr int kPieces = kWidth / 8;
 

@@ -23,14 +23,14 @@
 // and 128 keys, the exponentials 1,800 of the MUFU unit; the chain of softmax,
 // product and next scores makes it 3,900 to 4,700 (S has one buffer a tile: O and
 // S of both fill TMEM). Measured (B200, calls back to back for seconds, where the
-// power cap takes the SM clock from 1.97 to 1.58 to 1.71 GHz; in brackets the best
-// of a few calls; TFLOP/s of the pairs that are seen): 4 prompts of 8192 tokens, 16
+// power cap holds the SM clock between 1.58 and 1.71 GHz for 1.97; in brackets the
+// best of a few calls; TFLOP/s of the pairs that are seen): 4 prompts of 8192 tokens, 16
 // heads 1.35 ms, 1,010 TFLOP/s (1.17 ms, 1,170); 4 x ~506 queries behind 4000 to
 // 8000 keys, 32 heads 288 us, 800 (250 us, 920); 32 prompts of 64 to 2048 303 us,
 // 610 (256 us, 720; a ragged end of a tile and the masked half of the diagonal are
 // 18 % of the work, an item's start and end ~8,000 cycles of ~32,000); one of 300
-// 11.6 us. Tried and no faster: tile B started half
-// a step behind tile A, the next item looked up early.
+// 11.6 us. Tried and no faster: tile B started half a step behind tile A, the next
+// item looked up early.
 //
 // Roles (16 warps, one CTA an SM):
 //   warp 0      claims items: a CTA that has begun takes over the indices of CTAs
@@ -69,7 +69,8 @@ static_assert(2 * 128 * kSoftmaxRegs + 2 * 128 * kOtherRegs == kThreads * kLaunc
 // places that V of tile g leaves, so all that waits for tile g's has passed. [2] else: per query tile, or alternating.
 enum Bar {
   kEmpty = 0, kKFull = kEmpty + kSlots, kVFull = kKFull + 2, kVReady = kVFull + 2, kQFull = kVReady + 2,
-  kQFree = kQFull + 2, kSFull = kQFree + 2, kPFull = kSFull + 2, kPVDone = kPFull + 2, kODone = kPVDone + 2, kOFree = kODone + 2, kStatsFull = kOFree + 2,
+  kQFree = kQFull + 2, kSFull = kQFree + 2, kPFull = kSFull + 2, kPVDone = kPFull + 2, kODone = kPVDone + 2,
+  kOFree = kODone + 2, kStatsFull = kOFree + 2,
   kStatsFree = kStatsFull + 2, kItemFull = kStatsFree + 2, kItemEmpty = kItemFull + 2, kClaim = kItemEmpty + 2,
   kSDrain, kPVDrain, kNumBars
 };
